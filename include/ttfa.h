@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-#define TTFA_ABI_VERSION 7
+#define TTFA_ABI_VERSION 8
 
 enum ttfa_dtype { TTFA_BF16 = 0, TTFA_F32 = 1 };
 
@@ -51,6 +51,8 @@ enum ttfa_status {
   TTFA_E_EPS = -8,         /* eps is not in [0, 1)                               */
   TTFA_E_QROWS = -9,       /* decode: (Hq / Hkv) * Tq > 32                       */
   TTFA_E_SCRATCH = -10,    /* ttfa_bwd_static: B * Hq * T > TTFA_BWD_STATIC_MAX_ROWS */
+  TTFA_E_BITS = -11,       /* quantised cache: bits is not 4 or 8                */
+  TTFA_E_STRIDE = -12,     /* ttfa_kv_append: a stride is negative or no multiple of 16 bytes */
 };
 
 /* Library ABI version (TTFA_ABI_VERSION of the build). No reference counterpart. */
@@ -220,6 +222,56 @@ int ttfa_decode_fwd(const void *q, const void *k_cache, const void *v_cache,
                     const int *cache_seqlens, void *o, float *lse, float *workspace, int B,
                     int Hq, int Hkv, int Tq, int max_seqlen, int D, int dtype, float scale,
                     void *hip_stream);
+
+/*
+ * KV cache held in 4 or 8 bits (OCP Microscaling).  32 consecutive elements of a row share a
+ * power of two 2^e, held as the byte e + 127; the elements are e2m1 (bits = 4; two to a byte, the
+ * lower one in the low nibble) or e4m3 (bits = 8).  No reference kernel exists (README.md:158 plans
+ * a KV cache).
+ *
+ *   k_codes, v_codes   : [B, Hkv, max_seqlen, D * bits / 8] bytes, contiguous
+ *   k_scales, v_scales : [B, Hkv, max_seqlen, D / 32] bytes, contiguous
+ *   cache_seqlens      : [B] int32 in device memory, 4-byte aligned
+ *
+ * ttfa_kv_append rounds `rows` new rows of k and v, [B, Hkv, rows, D] of `dtype`, into the cache.  Row
+ * t of sequence b goes to position cache_seqlens[b] - rows + t: cache_seqlens counts the new rows
+ * already, as ttfa_decode_mx_fwd wants it.  A row whose position is outside 0 .. max_seqlen - 1
+ * (the padding of a left-padded prompt, say) is not written, and nothing else is touched.
+ *   e is the smallest integer for which the group's largest magnitude is at most 7 * 2^e (bits 4) or
+ *   464 * 2^e (bits 8): the type's largest value plus half of its last step.  It is clamped to
+ *   -125 .. 125 (bits 4) or -117 .. 119 (bits 8), so that every value is a finite normal bf16.
+ *   An element is x / 2^e rounded to nearest even, saturating.  A group with a NaN or an infinity
+ *   gets the byte 255 and codes 0; it reads back as NaN, and attention sees NaN there.
+ *   `strides`: element strides of k's, then v's first three dimensions (batch, head, row), six values in
+ *   host memory, each a multiple of 16 bytes (TTFA_E_STRIDE); NULL where both are contiguous.  The
+ *   last dimension has stride 1.
+ *
+ * ttfa_kv_read is the inverse: rows t of k and v, [B, Hkv, rows, D] of `dtype`, contiguous, from
+ * position cache_seqlens[b] - rows + t; zeros where that is outside 0 .. max_seqlen - 1.  bf16 holds
+ * every value exactly.
+ *
+ * ttfa_decode_mx_fwd is ttfa_decode_fwd (arguments, results, workspace rules) on the values that the
+ * cache stands for; q and o are bf16.
+ *
+ * Supported: bits 4 or 8 (TTFA_E_BITS), D in {64, 128}, dtype TTFA_BF16 or TTFA_F32 for the rows;
+ * pointers non-null and 16-byte aligned.  One launch each; decode one or two.
+ */
+int ttfa_kv_append(const void *k, const void *v, void *k_codes, void *k_scales, void *v_codes,
+                   void *v_scales, const int *cache_seqlens, const long long *strides, int B,
+                   int Hkv, int rows, int max_seqlen, int D, int bits, int dtype,
+                   void *hip_stream);
+
+int ttfa_kv_read(const void *k_codes, const void *k_scales, const void *v_codes,
+                 const void *v_scales, const int *cache_seqlens, void *k, void *v, int B, int Hkv,
+                 int rows, int max_seqlen, int D, int bits, int dtype, void *hip_stream);
+
+long long ttfa_decode_mx_workspace_bytes(int B, int Hq, int Hkv, int Tq, int max_seqlen, int D,
+                                         int bits);
+
+int ttfa_decode_mx_fwd(const void *q, const void *k_codes, const void *k_scales,
+                       const void *v_codes, const void *v_scales, const int *cache_seqlens,
+                       void *o, float *lse, float *workspace, int B, int Hq, int Hkv, int Tq,
+                       int max_seqlen, int D, int bits, int dtype, float scale, void *hip_stream);
 
 /*
  * Fused attention prologue (bf16 only): q/k RMSNorm + rotate-half RoPE + the layout

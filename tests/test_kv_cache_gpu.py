@@ -1,0 +1,488 @@
+"""GPU tests of the quantised KV cache against its 64-bit oracle: what appends write and reads give, to the
+bit; attention over the cache, within rounding; and the operators together, as a program uses them."""
+
+import math
+
+import pytest
+import torch
+
+from helpers import announce
+from oracle import mx_cache as mx
+from tinytrain_amd import _lib
+from tinytrain_amd.kernels import kv_cache as kv
+from tinytrain_amd.kernels.flash_attn import FlashAttnInputError, flash_attn
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def _lens(lens):
+    return torch.tensor(lens, dtype=torch.int32, device=DEV)
+
+
+def _noise_cache(B, Hkv, L, D, bits, seed=0):
+    """A cache of random bytes (CPU), so that a stray write or a missed one shows."""
+    g = torch.Generator().manual_seed(seed)
+    n = (D * bits // 8, D // 32) * 2
+    return [torch.randint(0, 255, (B, Hkv, L, m), dtype=torch.uint8, generator=g) for m in n]
+
+
+def _gpu(cache):
+    return [t.to(DEV) for t in cache]
+
+
+def _cpu(ts):
+    return [t.cpu() for t in ts]
+
+
+def _wild(shape, seed, dtype):
+    """Rows with zeros, tiny and huge groups, values on rounding borders, NaN and infinities."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(shape, generator=g).unflatten(-1, (-1, 32))
+    kind = torch.randint(0, 12, x.shape[:-1], generator=g)[..., None]
+    scale = torch.exp2(torch.randint(-30, 30, x.shape[:-1], generator=g).float())[..., None]
+    border = torch.randint(-28, 29, x.shape, generator=g) / 4.0       # every e2m1 border, many e4m3 ones
+    border[..., 0] = 7.0
+    x = torch.where(kind < 3, border * scale, x * scale)
+    x = torch.where(kind == 3, torch.zeros(()), x)
+    x = torch.where(kind == 4, x * 1e-39, x)
+    x = torch.where(kind == 5, torch.randn(x.shape, generator=g).clamp(-3, 3) * 1.1e38, x)
+    x = torch.where(kind == 6, torch.where(torch.rand(x.shape, generator=g) < 0.6, torch.zeros(()), -x), x)
+    spot = torch.randint(0, 32, x.shape[:-1], generator=g)[..., None] == torch.arange(32)
+    x = torch.where((kind == 7) & spot, math.nan, x)
+    x = torch.where((kind == 8) & spot, -math.inf, x)
+    return x.flatten(-2).to(dtype)
+
+
+# ------------------------------------------------------------------------- append and read
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("B, Hkv, T, L, D, lens", [
+    (1, 1, 1, 1, 64, [1]),
+    (3, 2, 1, 40, 128, [40, 1, 17]),
+    (4, 3, 37, 41, 64, [41, 37, 20, 0]),            # left padding, an empty sequence
+    (5, 2, 9, 12, 128, [-3, 60, 14, 9, 12]),        # nothing, all past the end, some past the end
+    (2, 1, 300, 257, 64, [257, 290]),               # more rows than the cache has
+])
+def test_append_writes_the_oracles_bytes(B, Hkv, T, L, D, lens, bits, dtype):
+    announce(f"kv append B={B} Hkv={Hkv} T={T} L={L} D={D} bits={bits} {dtype} lens={lens}")
+    k, v = _wild((B, Hkv, T, D), 1, dtype), _wild((B, Hkv, T, D), 2, dtype)
+    want = _noise_cache(B, Hkv, L, D, bits)
+    got = _gpu(want)
+    kv.kv_cache_append(k.to(DEV), v.to(DEV), *got, _lens(lens))
+    mx.append(want, k, v, lens)
+    for name, a, b in zip(kv.MXCache._fields, _cpu(got), want):
+        assert torch.equal(a, b), name
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_append_of_every_bf16_value(bits):
+    """Each finite bf16 value in a group of its own scale and in one of a larger scale."""
+    announce(f"kv append all bf16 bits={bits}")
+    x = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(BF)
+    x = x[torch.isfinite(x)]
+    k = torch.zeros(1, 1, len(x), 64, dtype=BF)
+    k[0, 0, :, 5] = x
+    k[0, 0, :, 32] = x
+    k[0, 0, :, 40] = (x.float().abs().clamp(max=1e37) * 9.5).to(BF)
+    got = _gpu(kv.mx_cache(1, 1, len(x), 64, bits, device="cpu"))
+    kv.kv_cache_append(k.to(DEV), k.to(DEV), *got, _lens([len(x)]))
+    c, s = mx.quantise(k, bits)
+    for a, b in zip(_cpu(got), (c, s, c, s)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_append_of_strided_rows(dtype):
+    """Rows as projections lay them out [B, T, H, D], slices of wider ones, an expanded batch, and K and
+    V of different strides."""
+    announce(f"kv append strides {dtype}")
+    B, Hkv, T, L, D = 3, 2, 5, 9, 64
+    lens = [9, 5, 3]
+    dense = [_wild((B, Hkv, T, D), s, dtype) for s in (3, 4)]
+    wide = torch.zeros(B, T, 2 * Hkv, D + 32, dtype=dtype, device=DEV)
+    wide[:, :, ::2, 16:16 + D] = dense[0].transpose(1, 2).to(DEV)
+    k = wide[:, :, ::2, 16:16 + D].transpose(1, 2)
+    v = dense[1].transpose(1, 2).contiguous().to(DEV).transpose(1, 2)
+    assert k.stride() != v.stride() and not k.is_contiguous()
+    want = _noise_cache(B, Hkv, L, D, 4)
+    got = _gpu(want)
+    kv.kv_cache_append(k, v, *got, _lens(lens))
+    mx.append(want, *dense, lens)
+    assert all(torch.equal(a, b) for a, b in zip(_cpu(got), want))
+    one = dense[0][:1].to(DEV)
+    got, want = _gpu(want), want
+    kv.kv_cache_append(one.expand(B, Hkv, T, D), one.expand(B, Hkv, T, D), *got, _lens(lens))
+    mx.append(want, *(dense[0][:1].expand(B, Hkv, T, D),) * 2, lens)
+    assert all(torch.equal(a, b) for a, b in zip(_cpu(got), want))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("B, Hkv, rows, L, D, lens", [
+    (1, 1, 1, 1, 64, [1]),
+    (4, 3, 37, 41, 64, [41, 37, 20, 0]),
+    (5, 2, 9, 12, 128, [-3, 60, 14, 9, 12]),
+    (2, 1, 300, 257, 128, [257, 290]),
+])
+def test_read_gives_the_oracles_values(B, Hkv, rows, L, D, lens, bits, dtype):
+    announce(f"kv read B={B} Hkv={Hkv} rows={rows} L={L} D={D} bits={bits} {dtype} lens={lens}")
+    cache = list(kv.mx_cache(B, Hkv, L, D, bits, device="cpu"))
+    mx.append(cache, _wild((B, Hkv, L, D), 5, BF), _wild((B, Hkv, L, D), 6, BF), [L] * B)
+    got = kv.kv_cache_read(*_gpu(cache), _lens(lens), rows, dtype)
+    for a, b in zip(got, mx.read(cache, lens, rows)):
+        assert a.dtype == dtype and a.is_contiguous() and torch.equal(torch.isnan(a.cpu()), torch.isnan(b))
+        assert torch.equal(a.cpu().double().nan_to_num(0.5), b.nan_to_num(0.5))
+
+
+def test_every_code_reads_as_its_value():
+    """All codes under all scales that an append can write, in both types."""
+    announce("kv read all codes")
+    for bits, lo, hi in ((4, 2, 252), (8, 10, 246)):
+        n, D = hi - lo + 1, 64
+        codes = torch.arange(256, dtype=torch.uint8)
+        if bits == 8:
+            codes[127] = codes[255] = 0
+        codes = codes.view(1, -1, 1, D * bits // 8).expand(1, -1, n, -1).contiguous()
+        scales = torch.arange(lo, hi + 1).to(torch.uint8).view(1, 1, n, 1).expand(1, codes.shape[1], n, 2).contiguous()
+        cache = [codes, scales, codes.clone(), scales.clone()]
+        for dtype in (BF, F32):
+            k, v = kv.kv_cache_read(*_gpu(cache), _lens([n]), n, dtype)
+            want = mx.values(codes, scales, bits)
+            assert torch.equal(k.cpu().double(), want) and torch.equal(v, k)
+
+
+# ------------------------------------------------------------------------------ attention
+
+def _filled(B, Hkv, L, D, bits, seed=0, device="cpu"):
+    """(cache, fp64 K, fp64 V): unit-RMS keys with uneven channels, normal values."""
+    g = torch.Generator(device).manual_seed(seed)
+    k = torch.randn(B, Hkv, L, D, generator=g, device=device)
+    k = k * torch.rsqrt(k.pow(2).mean(-1, keepdim=True)) * (1 + 0.2 * torch.randn(D, generator=g, device=device))
+    v = torch.randn(B, Hkv, L, D, generator=g, device=device)
+    cache = []
+    for x in (k, v):
+        cache += mx.quantise(x.to(BF).cpu(), bits)
+    return cache, mx.values(*cache[:2], bits), mx.values(*cache[2:], bits)
+
+
+def _queries(B, Hq, Tq, D, seed=0):
+    g = torch.Generator().manual_seed(seed + 1000)
+    q = torch.randn(B, Hq, Tq, D, generator=g)
+    return (q * torch.rsqrt(q.pow(2).mean(-1, keepdim=True))).to(BF)
+
+
+def _bounds(o, a, big, L, D):
+    """Element-wise bounds of O and LSE, from the roundings on the way.
+
+    K, V and Q enter the products exactly.  A score is a sum of D products in fp32 with the size S =
+    `big` (|error| <= D 2^-24 S), scaled and shifted by the maximum in fp32 (two roundings of at most S
+    each); exp2 and log2 are good to 2^-21; a sum of L terms in fp32 adds L 2^-24.  So a weight
+    is off by d = (D + 4) 2^-24 S + L 2^-24 + 2^-20, relatively, twice (weight and sum); rounding the
+    weights to bf16 adds 2^-8 of A = sum p |v|, rounding O to bf16 2^-8 of itself."""
+    d = (D + 4) * 2.0**-24 * big + L * 2.0**-24 + 2.0**-20
+    return (2.0**-8 + 2 * d[..., None]) * a * (1 + 2.0**-8) + 2.0**-8 * o.abs(), 2 * d + 2.0**-20
+
+
+def _check(q, cache, lens, k, v, got, L):
+    o, lse, a, big = mx.decode(q, k, v, lens)
+    tol_o, tol_lse = _bounds(o, a, big, L, q.shape[3])
+    go, gl = (t.double().cpu() for t in got)
+    assert got[0].dtype == BF and got[1].dtype == F32
+    seen = torch.isfinite(lse)
+    assert torch.equal(torch.isfinite(gl), seen) and (gl[~seen] == -math.inf).all()
+    assert ((go - o).abs() <= tol_o).all(), ((go - o).abs() / tol_o.clamp(min=1e-30)).max()
+    assert ((gl - lse)[seen].abs() <= tol_lse[seen]).all(), ((gl - lse)[seen].abs() / tol_lse[seen]).max()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("B, Hq, Hkv, Tq, L, D, lens", [
+    (1, 1, 1, 1, 1, 64, [1]),
+    (2, 8, 2, 1, 512, 128, [512, 33]),               # one launch
+    (4, 4, 4, 1, 31, 64, [31, 1, 0, -2]),            # inside one block, empty caches
+    (3, 4, 2, 3, 97, 128, [2, 97, 64]),              # rows without keys
+    (1, 16, 1, 1, 700, 128, [700]),                  # 16 columns, one tile
+    (2, 17, 1, 1, 333, 64, [333, 32]),               # 17: two tiles
+    (2, 32, 4, 4, 1500, 128, [1500, 777]),           # 32
+    (2, 6, 2, 5, 600, 64, [600, 4]),                 # 15 columns, an odd number of rows
+    (1, 12, 4, 1, 5000, 64, [4999]),                 # many chunks
+    (1, 16, 8, 1, 5001, 128, [5001]),
+    (9, 12, 12, 1, 1301, 64, [1301 - 160 * i for i in range(9)]),
+    (20, 8, 8, 2, 900, 128, [max(900 - 47 * i, 0) for i in range(20)]),
+    (3, 8, 2, 1, 600, 128, [700, 601, 600]),         # longer than the cache: clamped
+])
+def test_decode_matches_oracle(B, Hq, Hkv, Tq, L, D, lens, bits):
+    announce(f"decode_mx B={B} Hq={Hq} Hkv={Hkv} Tq={Tq} L={L} D={D} bits={bits} lens={lens[:4]}")
+    cache, k, v = _filled(B, Hkv, L, D, bits)
+    q = _queries(B, Hq, Tq, D)
+    got = kv.flash_attn_decode_mx(q.to(DEV), *_gpu(cache), _lens(lens))
+    _check(q, cache, lens, k, v, got, L)
+
+
+@pytest.mark.parametrize("bits, D", [(4, 128), (8, 64)])
+def test_decode_of_sharp_and_flat_scores(bits, D):
+    """Scores far apart (one key takes all, the maximum grows from block to block) and all equal."""
+    announce(f"decode_mx sharp bits={bits}")
+    B, Hkv, L = 2, 2, 3000
+    cache, k, v = _filled(B, Hkv, L, D, bits, seed=3)
+    q = _queries(B, 4, 1, D)
+    ramp = torch.linspace(0.1, 30, L)[:, None] * q[:, ::2, 0, None].float().sign()
+    c, s = mx.quantise(ramp.to(BF), bits)
+    for codes, scales in ((c, s), mx.quantise(torch.zeros(B, Hkv, L, D), bits)):
+        now = [codes, scales, *cache[2:]]
+        got = kv.flash_attn_decode_mx(q.to(DEV), *_gpu(now), _lens([L, 1999]))
+        _check(q, now, [L, 1999], mx.values(codes, scales, bits), v, got, L)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("B, Hkv, L, D", [(1, 2, 500, 128), (3, 2, 4000, 64), (40, 4, 1000, 128)])
+def test_decode_rows_do_not_depend_on_the_other_caches(B, Hkv, L, D, bits):
+    """A sequence's bits go by the call's shape and its own cache: whatever lies behind its last row, and
+    whatever the others hold (NaN everywhere, nothing)."""
+    announce(f"decode_mx neighbours B={B} L={L} D={D} bits={bits}")
+    cache, _, _ = _filled(B, Hkv, L, D, bits)
+    q, n = _queries(B, 2 * Hkv, 1, D).to(DEV), L - 45
+    lens = torch.full((B,), L, dtype=torch.int32)
+    lens[0] = n
+    want = kv.flash_attn_decode_mx(q, *_gpu(cache), lens.to(DEV))
+    other = _gpu(cache)
+    for t in other:
+        t[0, :, n:] = 255
+        t[1:] = 255
+    for rest in (L, 40, 0):
+        lens[1:] = rest
+        got = kv.flash_attn_decode_mx(q, *other, lens.to(DEV))
+        assert all(torch.equal(a[0], b[0]) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("L, D, lens, at", [
+    (512, 128, [512, 20], [511, 19]), (512, 64, [500, 33], [499, 32]), (512, 64, [500, 33], [250, 0]),
+    (3000, 128, [3000, 65], [2998, 64]), (3000, 64, [2999, 3], [2997, 0]), (3000, 128, [3000, 64], [2969, 62]),
+])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_decode_nan_groups_reach_the_rows_that_see_them(L, D, lens, at, which, bits):
+    """A NaN group of K makes O and LSE of exactly the rows that see its key NaN; one of V makes the 32
+    elements of O NaN that it adds to.  Every other value keeps its bits."""
+    announce(f"decode_mx NaN L={L} D={D} lens={lens} at={at} {which} bits={bits}")
+    Tq, Hkv, Hq = 3, 2, 4
+    cache, _, _ = _filled(2, Hkv, L, D, bits, seed=5)
+    q = _queries(2, Hq, Tq, D).to(DEV)
+    clean = kv.flash_attn_decode_mx(q, *_gpu(cache), _lens(lens))
+    codes, scales = (0, 1) if which == "k" else (2, 3)
+    for b in range(2):
+        cache[scales][b, 1, at[b], 1] = 255
+        cache[codes][b, 1, at[b], 4 * bits:8 * bits] = 0
+    o, lse = kv.flash_attn_decode_mx(q, *_gpu(cache), _lens(lens))
+    pos = torch.tensor(lens)[:, None] + torch.arange(-Tq, 0)
+    bad = torch.zeros(2, Hq, Tq, D, dtype=torch.bool)
+    bad[:, 2:] = (torch.tensor(at)[:, None] <= pos)[:, None, :, None]
+    rows = bad[..., 0].to(DEV) & (which == "k")
+    if which == "v":
+        bad[..., :32] = bad[..., 64:] = False
+    bad = bad.to(DEV)
+    assert torch.equal(torch.isnan(o), bad) and torch.equal(torch.isnan(lse), rows)
+    assert torch.equal(o[~bad], clean[0][~bad]) and torch.equal(lse[~rows], clean[1][~rows])
+
+
+def test_decode_agrees_with_attention_over_the_rows_read_back():
+    """The last rows of the batched forward over kv_cache_read's K and V, within both paths' roundings."""
+    announce("decode_mx vs forward over read rows")
+    B, Hq, Hkv, T, D, Tq = 2, 8, 2, 700, 128, 2
+    cache, k, v = _filled(B, Hkv, T, D, 4, seed=7)
+    q = _queries(B, Hq, T, D).to(DEV)
+    lens = _lens([T] * B)
+    dense = kv.kv_cache_read(*_gpu(cache), lens, T)
+    full = flash_attn(q, *dense)[:, :, T - Tq:]
+    qt = q[:, :, T - Tq:].contiguous()
+    o, _ = kv.flash_attn_decode_mx(qt, *_gpu(cache), lens)
+    want, _, a, big = mx.decode(qt.cpu(), k, v, [T] * B)
+    tol, _ = _bounds(want, a, big, T, D)
+    assert ((o - full).double().abs().cpu() <= 2 * tol).all()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_rows_beyond_32_bit_offsets(bits):
+    """A cache whose codes pass 4 GiB: rows of its last head, and of the last positions of a long one."""
+    announce(f"kv long cache bits={bits}")
+    D, Hkv, B = 128, 2, 3
+    L = 4_300_000_000 // (D * bits // 8 * B * Hkv) + 1
+    cache = kv.mx_cache(B, Hkv, L, D, bits)
+    assert cache.k_codes.numel() > 1 << 32
+    k, v = (_wild((B, Hkv, 70, D), s, BF) for s in (8, 9))
+    k, v = (torch.where(torch.isfinite(t.float()), t, 1.0).clamp(-4, 4) for t in (k, v))
+    lens = [L, L - 31, L]
+    kv.kv_cache_append(k.to(DEV), v.to(DEV), *cache, _lens(lens))
+    got = kv.kv_cache_read(*cache, _lens(lens), 70)
+    for x, y in zip(got, (k, v)):
+        assert torch.equal(x.cpu().double(), mx.values(*mx.quantise(y, bits), bits))
+    # keys that are zeros everywhere else: their score is 0 and they add exp(0) each
+    q = _queries(B, 4, 1, D)
+    o, lse = kv.flash_attn_decode_mx(q.to(DEV), *cache, _lens(lens))
+    kk, vv = (mx.values(*mx.quantise(y, bits), bits) for y in (k, v))
+    for h in range(4):
+        s = (kk[:, h // 2] @ q[:, h, 0].double()[..., None])[..., 0] / math.sqrt(D)
+        w = torch.exp(s)
+        total = w.sum(-1) + torch.tensor(lens) - 70
+        want = (w[:, None] @ vv[:, h // 2])[:, 0] / total[:, None]
+        size = (w[:, None] @ vv[:, h // 2].abs())[:, 0] / total[:, None]
+        # sums of up to L terms in fp32, each lane's part of at most L / 64 of them
+        tol = (2.0**-8 + L / 64 * 2.0**-24 + 2.0**-10) * size + 2.0**-8 * want.abs()
+        assert ((o[:, h, 0].cpu().double() - want).abs() <= tol).all()
+        assert ((lse[:, h, 0].cpu().double() - torch.log(total)).abs() <= L / 64 * 2.0**-24 + 2.0**-10).all()
+
+
+# ------------------------------------------------------------------------------- together
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_generation_step_by_step(bits):
+    """A left-padded batch of prompts, then tokens one at a time and two at once: after every step the
+    cache is what the oracle holds and attention over it is right."""
+    announce(f"kv generation bits={bits}")
+    B, Hq, Hkv, D, T, L = 3, 4, 2, 64, 50, 64
+    prompt = [50, 17, 1]
+    want = list(kv.mx_cache(B, Hkv, L, D, bits, device="cpu"))
+    cache = kv.mx_cache(B, Hkv, L, D, bits)
+    lens = _lens(prompt)
+    g = torch.Generator().manual_seed(4)
+    for rows in (T, 1, 1, 2, 1, 4):
+        if rows != T:
+            lens += rows
+        k, v = (torch.randn(B, Hkv, rows, D, generator=g).to(BF) for _ in range(2))
+        q = _queries(B, Hq, min(rows, 8), D, seed=rows)
+        kv.kv_cache_append(k.to(DEV), v.to(DEV), *cache, lens)
+        got = kv.flash_attn_decode_mx(q.to(DEV), *cache, lens)
+        now = lens.tolist()
+        mx.append(want, k, v, now)
+        assert all(torch.equal(a, b) for a, b in zip(_cpu(cache), want))
+        _check(q, want, now, *mx.read(want, [L] * B, L), got, L)
+
+
+def test_step_replays_in_a_graph():
+    """A step of generation captured in a HIP graph and replayed, the lengths advanced in the graph, with
+    eager work and synchronisations in between: every replay equals eager calls, bitwise."""
+    announce("kv graph replays")
+    B, Hq, Hkv, D, L = 2, 16, 8, 128, 6000
+    filled, _, _ = _filled(B, Hkv, L, D, 4, seed=11)
+    cache, eager = _gpu(filled), _gpu(filled)
+    lens = _lens([5900, 100])
+    q, k, v = (torch.empty(B, h, 1, D, dtype=BF, device=DEV) for h in (Hq, Hkv, Hkv))
+
+    def step(c, n):
+        n += 1
+        kv.kv_cache_append(k, v, *c, n)
+        return (*kv.flash_attn_decode_mx(q, *c, n), *kv.kv_cache_read(*c, n, 5))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step([t.clone() for t in cache], lens.clone())
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(cache, lens)
+    mine = lens.clone()
+    for r in range(4):
+        for t, seed in ((q, 0), (k, 1), (v, 2)):
+            t.copy_(torch.randn(t.shape, generator=torch.Generator().manual_seed(10 * r + seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(eager, mine)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), r
+        assert all(torch.equal(a, b) for a, b in zip(cache, eager)) and torch.equal(lens, mine), r
+
+
+def test_native_path_and_ops_give_the_same_bits():
+    announce("kv native path")
+    ops = torch.ops.tinytrain
+    filled, _, _ = _filled(2, 2, 300, 64, 8, seed=12)
+    a, b = _gpu(filled), _gpu(filled)
+    q, k = _queries(2, 4, 2, 64).to(DEV), _queries(2, 2, 7, 64, seed=1).to(DEV)
+    lens = torch.stack([_lens([300, 150])] * 2, 1)[:, 0]         # strided lengths
+    assert not lens.is_contiguous()
+    version = a[0]._version
+    assert kv.kv_cache_append(k, k, *a, lens) is None and a[0]._version > version
+    ops.kv_cache_append(k, k, *b, lens)
+    assert all(torch.equal(x, y) for x, y in zip(a, b)) and not torch.equal(a[0].cpu(), filled[0])
+    for x, y in zip(kv.flash_attn_decode_mx(q, *a, lens), ops.flash_attn_decode_mx(q, *b, lens)):
+        assert torch.equal(x, y)
+    for dtype in (BF, F32):
+        for x, y in zip(kv.kv_cache_read(*a, lens, 9, dtype), ops.kv_cache_read(*b, lens, 9, dtype)):
+            assert torch.equal(x, y) and x.dtype == dtype
+    with torch.inference_mode():
+        c = kv.mx_cache(2, 2, 300, 64, 8)
+        kv.kv_cache_append(k, k, *c, lens)
+        assert torch.equal(kv.kv_cache_read(*c, lens, 7)[0], kv.kv_cache_read(*a, lens, 7)[0])
+    torch.library.opcheck(kv.flash_attn_decode_mx, (q, *a, lens), test_utils=("test_schema", "test_faketensor"))
+    torch.library.opcheck(kv.kv_cache_read, (*a, lens, 5), test_utils=("test_schema", "test_faketensor"))
+    torch.library.opcheck(kv.kv_cache_append, (k, k, *a, lens), test_utils=("test_schema", "test_faketensor"))
+
+
+def test_compiled_step_mutates_the_cache():
+    announce("kv torch.compile")
+    filled, _, _ = _filled(2, 2, 100, 64, 4, seed=13)
+    a, b = _gpu(filled), _gpu(filled)
+    q, k = _queries(2, 4, 1, 64).to(DEV), _queries(2, 2, 1, 64, seed=1).to(DEV)
+
+    def step(q, k, v, c, lens):
+        kv.kv_cache_append(k * 2, v, *c, lens)
+        return kv.flash_attn_decode_mx(q, *c, lens)
+
+    torch._dynamo.reset()
+    compiled = torch.compile(step, fullgraph=True, backend="aot_eager")
+    for n in (60, 61):
+        want, got = step(q, k, k, a, _lens([n, 5])), compiled(q, k, k, b, _lens([n, 5]))
+        assert all(torch.equal(x, y) for x, y in zip(want, got))
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_calls_on_side_streams_and_determinism():
+    from concurrent.futures import ThreadPoolExecutor
+
+    announce("kv streams")
+    filled, _, _ = _filled(3, 4, 5000, 128, 4, seed=14)
+    cache = _gpu(filled)
+    q, lens = _queries(3, 8, 1, 128).to(DEV), _lens([5000, 4000, 7])
+    k = _queries(3, 4, 4, 128, seed=2).to(DEV)
+    kv.kv_cache_append(k, k, *cache, lens)
+    want = (*kv.flash_attn_decode_mx(q, *cache, lens), *kv.kv_cache_read(*cache, lens, 50))
+    torch.cuda.synchronize()
+
+    def work(_):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            mine = [t.to(DEV) for t in filled]
+            kv.kv_cache_append(k, k, *mine, lens)
+            got = (*kv.flash_attn_decode_mx(q, *mine, lens), *kv.kv_cache_read(*mine, lens, 50))
+        s.synchronize()
+        return all(torch.equal(a, b) for a, b in zip(got, want))
+
+    with ThreadPoolExecutor(4) as ex:
+        assert all(ex.map(work, range(8)))
+
+
+def test_refusals_on_the_gpu():
+    announce("kv refusals")
+    cache = kv.mx_cache(2, 2, 10, 64)
+    lens, k = _lens([3, 3]), torch.zeros(2, 2, 3, 64, dtype=BF, device=DEV)
+    with pytest.raises(FlashAttnInputError, match="four tensors"):
+        kv.kv_cache_append(k, k, cache.k_codes, cache.k_scales, cache.k_codes, cache.v_scales, lens)
+    with pytest.raises(FlashAttnInputError, match="ROCm GPU"):
+        kv.kv_cache_append(k.cpu(), k, *cache, lens)
+    with pytest.raises(FlashAttnInputError, match="ROCm GPU"):
+        kv.kv_cache_read(*cache, lens.cpu(), 3)
+    with pytest.raises(FlashAttnInputError, match="16 bytes"):
+        kv.kv_cache_append(torch.zeros(2, 2, 3, 68, dtype=BF, device=DEV)[..., :64], k, *cache, lens)
+    with pytest.raises(FlashAttnInputError, match="bfloat16"):
+        kv.flash_attn_decode_mx(k.float(), *cache, lens)
+    with pytest.raises(FlashAttnInputError, match="positive"):
+        kv.kv_cache_read(*cache, lens, 0)
+    with pytest.raises(_lib.TTFAError, match="aligned"):
+        kv.kv_cache_append(torch.zeros(2 * 2 * 3 * 64 + 1, dtype=BF, device=DEV)[1:].view(2, 2, 3, 64), k, *cache, lens)
+    with pytest.raises(_lib.TTFAError):
+        kv.kv_cache_append(k[:, :, :0], k[:, :, :0], *cache, lens)
+    assert not any(t.any() for t in cache)

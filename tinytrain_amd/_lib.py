@@ -21,18 +21,19 @@ NATIVE_PATH = _PKG / "_ttfa_torch.so"
 
 TTFA_BF16 = 0
 TTFA_F32 = 1
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 # Negative status codes of include/ttfa.h.
-E_NULL, E_HEAD_DIM, E_GROUP, E_SEQ, E_ALIGN, E_DTYPE, E_SCALE, E_EPS, E_QROWS, E_SCRATCH = (
-    -1, -2, -3, -4, -5, -6, -7, -8, -9, -10)
+(E_NULL, E_HEAD_DIM, E_GROUP, E_SEQ, E_ALIGN, E_DTYPE, E_SCALE, E_EPS, E_QROWS, E_SCRATCH, E_BITS,
+ E_STRIDE) = (-1, -2, -3, -4, -5, -6, -7, -8, -9, -10, -11, -12)
 BWD_STATIC_MAX_ROWS = 1 << 20  # TTFA_BWD_STATIC_MAX_ROWS
 EXPORTED = ("ttfa_abi_version", "ttfa_strerror", "ttfa_fwd", "ttfa_bwd", "ttfa_bwd_dq",
             "ttfa_bwd_dkdv", "ttfa_varlen_fwd", "ttfa_varlen_bwd", "ttfa_decode_workspace_bytes",
             "ttfa_decode_fwd", "ttfa_qk_prologue_fwd",
             "ttfa_qk_prologue_workspace_bytes", "ttfa_qk_prologue_bwd", "ttfa_bwd_static",
             "ttfa_d128_wide", "ttfa_qk_prologue_fwd_tables", "ttfa_qk_prologue_bwd_tables",
-            "ttfa_bwd_workspace_bytes", "ttfa_bwd_ws")
+            "ttfa_bwd_workspace_bytes", "ttfa_bwd_ws", "ttfa_kv_append", "ttfa_kv_read",
+            "ttfa_decode_mx_workspace_bytes", "ttfa_decode_mx_fwd")
 
 
 class LibraryNotBuilt(RuntimeError):
@@ -65,6 +66,10 @@ _SIGS = {
     "ttfa_varlen_bwd": ([_vp] * 11 + [_i] * 7 + [_f, _vp], _i),
     "ttfa_decode_workspace_bytes": ([_i] * 6, ctypes.c_longlong),
     "ttfa_decode_fwd": ([_vp] * 7 + [_i] * 7 + [_f, _vp], _i),
+    "ttfa_kv_append": ([_vp] * 8 + [_i] * 7 + [_vp], _i),
+    "ttfa_kv_read": ([_vp] * 7 + [_i] * 7 + [_vp], _i),
+    "ttfa_decode_mx_workspace_bytes": ([_i] * 7, ctypes.c_longlong),
+    "ttfa_decode_mx_fwd": ([_vp] * 9 + [_i] * 8 + [_f, _vp], _i),
     "ttfa_qk_prologue_fwd": ([_vp] * 12 + [_i] * 5 + [_f, _vp], _i),
     "ttfa_qk_prologue_workspace_bytes": ([_i] * 5, ctypes.c_longlong),
     "ttfa_qk_prologue_bwd": ([_vp] * 17 + [_i] * 5 + [_vp], _i),
@@ -119,6 +124,7 @@ class _OpsOnly:
         return None
 
     flash_attn = flash_attn_varlen = flash_attn_decode = qk_norm_rope = _pass
+    kv_cache_append = kv_cache_read = flash_attn_decode_mx = _pass
 
 
 _native = None

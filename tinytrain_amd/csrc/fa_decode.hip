@@ -413,6 +413,16 @@ DecodeSplit decode_split(int B, int Hkv, int Lmax, int D) {
   return {n_waves, (int)n, log2_min};
 }
 
+hipError_t launch_decode_combine(const float *part_o, const float *part_ml, void *o, float *lse,
+                                 int rows, int n_chunks, int D, hipStream_t stream) {
+  const dim3 grid((unsigned)rows), block(256);
+  if (D == 64)
+    fa_decode_combine_kernel<64><<<grid, block, 0, stream>>>(part_o, part_ml, (bf16 *)o, lse, n_chunks);
+  else
+    fa_decode_combine_kernel<128><<<grid, block, 0, stream>>>(part_o, part_ml, (bf16 *)o, lse, n_chunks);
+  return hipGetLastError();
+}
+
 template <int D, int NW, bool SPLIT>
 static hipError_t launch_decode(const void *q, const void *k_cache, const void *v_cache,
                                 const int *cache_seqlens, void *o, float *lse, float *part_o,
@@ -431,10 +441,7 @@ static hipError_t launch_decode(const void *q, const void *k_cache, const void *
       lse, part_o, part_ml, B, Hq, Hkv, Tq, Lmax, n_chunks, log2_min, scale_log2);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !SPLIT) return e;
-  const int rows = B * Hq * Tq;
-  fa_decode_combine_kernel<D><<<dim3((unsigned)rows), dim3(256), 0, stream>>>(
-      part_o, part_ml, (bf16 *)o, lse, n_chunks);
-  return hipGetLastError();
+  return launch_decode_combine(part_o, part_ml, o, lse, B * Hq * Tq, n_chunks, D, stream);
 }
 
 hipError_t launch_decode_bf16(const void *q, const void *k_cache, const void *v_cache,

@@ -66,6 +66,32 @@ hipError_t launch_decode_bf16(const void *q, const void *k_cache, const void *v_
                               int B, int Hq, int Hkv, int Tq, int Lmax, int D, float scale,
                               hipStream_t stream);
 
+// Merge pass of a split decode call: part_o [rows][n_chunks][D] unnormalised, part_ml
+// [rows][n_chunks][2] (running max in log2 units, sum) -> o, lse.
+hipError_t launch_decode_combine(const float *part_o, const float *part_ml, void *o, float *lse,
+                                 int rows, int n_chunks, int D, hipStream_t stream);
+
+// Quantised KV cache (kv_cache_mx.hip): codes [B, Hkv, Lmax, D * bits / 8] and scales
+// [B, Hkv, Lmax, D / 32], K (0) and V (1).
+struct KvCache {
+  uint8_t *codes[2];
+  uint8_t *scales[2];
+};
+// New rows k, v [B, Hkv, n_rows, D] (element strides of the first three dimensions) into the cache,
+// and rows of the cache back out, contiguous; row t at position cache_seqlens[b] - n_rows + t.
+hipError_t launch_kv_append(const void *k, const void *v, const int64_t (&stride)[2][3],
+                            const KvCache &cache, const int *cache_seqlens, int B, int Hkv,
+                            int n_rows, int Lmax, int D, int bits, bool f32, hipStream_t stream);
+hipError_t launch_kv_read(const KvCache &cache, const int *cache_seqlens, void *k, void *v, int B,
+                          int Hkv, int n_rows, int Lmax, int D, int bits, bool f32,
+                          hipStream_t stream);
+
+// launch_decode_bf16 over a quantised cache; workspace of B * Hq * Tq * n_chunks * (D + 2) floats.
+DecodeSplit decode_mx_split(int B, int Hkv, int Lmax, int D, int bits);
+hipError_t launch_decode_mx(const void *q, const KvCache &cache, const int *cache_seqlens, void *o,
+                            float *lse, float *workspace, int B, int Hq, int Hkv, int Tq, int Lmax,
+                            int D, int bits, float scale, hipStream_t stream);
+
 hipError_t launch_fwd_f32(const void *q, const void *k, const void *v, void *o, float *lse,
                           int B, int Hq, int Hkv, int T, int D, float scale, hipStream_t stream);
 hipError_t launch_bwd_dq_f32(const void *q, const void *k, const void *v, const void *o,

@@ -1,6 +1,6 @@
 // Native eager path of the public attention functions: the argument checks, the output and
 // workspace allocations, the autograd nodes and the C ABI calls of flash_attn,
-// flash_attn_varlen, flash_attn_decode and qk_norm_rope, in C++.
+// flash_attn_varlen, flash_attn_decode, qk_norm_rope and the quantised KV cache, in C++.
 //
 // Why: a training pass of the custom ops (torch.library ops whose bodies and autograd
 // formulas are Python) costs about 175 us of host time on an MI355X host, most of it in the
@@ -287,6 +287,49 @@ bool takes_decode(const Tensor &q, const Tensor &k, const Tensor &v, const Tenso
          all_int(q.sizes()) && all_int(k.sizes());
 }
 
+// --------------------------------------------------------------------- quantised KV cache
+
+struct MxCache {
+  Tensor k_codes, k_scales, v_codes, v_scales, lens;
+
+  int64_t D() const { return 32 * k_scales.size(3); }
+  int B() const { return (int)k_codes.size(0); }
+  int Hkv() const { return (int)k_codes.size(1); }
+  int L() const { return (int)k_codes.size(2); }
+  int bits() const { return k_codes.size(3) == D() ? 8 : 4; }
+
+  bool takes() const {
+    for (const Tensor *t : {&k_codes, &k_scales, &v_codes, &v_scales})
+      if (!plain_tensor(*t) || t->dim() != 4 || t->scalar_type() != at::kByte ||
+          !t->is_contiguous() || t->device() != k_codes.device() || !all_int(t->sizes()))
+        return false;
+    return k_codes.sizes() == v_codes.sizes() && k_scales.sizes() == v_scales.sizes() &&
+           k_codes.sizes().slice(0, 3) == k_scales.sizes().slice(0, 3) && (D() == 64 || D() == 128) &&
+           (2 * k_codes.size(3) == D() || k_codes.size(3) == D()) && plain_tensor(lens) &&
+           lens.dim() == 1 && lens.size(0) == k_codes.size(0) && lens.scalar_type() == at::kInt &&
+           lens.device() == k_codes.device();
+  }
+
+  bool four_tensors() const {
+    const void *p[] = {k_codes.const_data_ptr(), k_scales.const_data_ptr(), v_codes.const_data_ptr(),
+                       v_scales.const_data_ptr()};
+    for (int i = 0; i < 4; ++i)
+      for (int j = 0; j < i; ++j)
+        if (p[i] == p[j]) return false;
+    return true;
+  }
+};
+
+// Element strides of new rows [B, Hkv, T, D] for ttfa_kv_append; false where it does not take them.
+bool row_strides(const Tensor &t, long long *out) {
+  if (t.stride(3) != 1) return false;
+  for (int i = 0; i < 3; ++i) {
+    out[i] = t.size(i) > 1 ? t.stride(i) : 0;
+    if (out[i] * (int64_t)t.element_size() % 16) return false;
+  }
+  return true;
+}
+
 // ------------------------------------------------------------------------------- prologue
 
 struct Prologue {
@@ -489,6 +532,91 @@ PyObject *py_flash_attn_decode(PyObject *, PyObject *const *args, Py_ssize_t n) 
   END_HANDLE_TH_ERRORS
 }
 
+// Tells other holders of a tensor that it was written in place.
+void written(const Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+PyObject *py_kv_cache_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arity(n, 7)) return nullptr;
+  Tensor t[7];
+  if (!unpack(args, t) || !plain_mode()) Py_RETURN_NONE;
+  const Tensor &k = t[0], &v = t[1];
+  const MxCache c{t[2], t[3], t[4], t[5], t[6].defined() ? t[6].contiguous() : t[6]};
+  if (!plain_tensor(k) || !plain_tensor(v) || !c.takes() || recorded({&k, &v})) Py_RETURN_NONE;
+  long long strides[6];
+  const auto dt = k.scalar_type();
+  if (k.dim() != 4 || k.sizes() != v.sizes() || k.size(0) != c.B() || k.size(1) != c.Hkv() ||
+      k.size(3) != c.D() || (dt != at::kBFloat16 && dt != at::kFloat) || v.scalar_type() != dt ||
+      k.device() != c.k_codes.device() || v.device() != k.device() || !all_int(k.sizes()) ||
+      !row_strides(k, strides) || !row_strides(v, strides + 3) || !c.four_tensors())
+    Py_RETURN_NONE;
+  RECORD_FUNCTION("tinytrain::kv_cache_append", c10::ArrayRef<const c10::IValue>());
+  const c10::DeviceGuard on(k.device());
+  check(ttfa_kv_append(k.const_data_ptr(), v.const_data_ptr(), c.k_codes.mutable_data_ptr(),
+                       c.k_scales.mutable_data_ptr(), c.v_codes.mutable_data_ptr(),
+                       c.v_scales.mutable_data_ptr(), c.lens.const_data_ptr<int>(), strides, c.B(),
+                       c.Hkv(), (int)k.size(2), c.L(), (int)c.D(), c.bits(), dtype_of(k),
+                       stream_of(k)));
+  for (const Tensor *x : {&c.k_codes, &c.k_scales, &c.v_codes, &c.v_scales}) written(*x);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject *py_kv_cache_read(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arity(n, 7)) return nullptr;
+  Tensor t[5];
+  const int64_t rows = PyLong_AsLongLong(args[5]);
+  if (rows == -1 && PyErr_Occurred()) return nullptr;
+  const int64_t dtype = PyLong_AsLongLong(args[6]);
+  if (dtype == -1 && PyErr_Occurred()) return nullptr;
+  if (!unpack(args, t) || !plain_mode() || rows < 1 || rows > kIntMax) Py_RETURN_NONE;
+  const MxCache c{t[0], t[1], t[2], t[3], t[4].defined() ? t[4].contiguous() : t[4]};
+  if (!c.takes()) Py_RETURN_NONE;
+  RECORD_FUNCTION("tinytrain::kv_cache_read", c10::ArrayRef<const c10::IValue>());
+  const c10::DeviceGuard on(c.k_codes.device());
+  const auto opt = c.k_codes.options().dtype(dtype == TTFA_F32 ? at::kFloat : at::kBFloat16);
+  Tensor k = at::empty({c.B(), c.Hkv(), rows, c.D()}, opt), v = at::empty(k.sizes(), opt);
+  check(ttfa_kv_read(c.k_codes.const_data_ptr(), c.k_scales.const_data_ptr(),
+                     c.v_codes.const_data_ptr(), c.v_scales.const_data_ptr(),
+                     c.lens.const_data_ptr<int>(), k.mutable_data_ptr(), v.mutable_data_ptr(), c.B(),
+                     c.Hkv(), (int)rows, c.L(), (int)c.D(), c.bits(), (int)dtype,
+                     stream_of(c.k_codes)));
+  return pack({k, v});
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject *py_flash_attn_decode_mx(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arity(n, 6)) return nullptr;
+  Tensor t[6];
+  if (!unpack(args, t) || !plain_mode()) Py_RETURN_NONE;
+  const Tensor &q = t[0];
+  const MxCache c{t[1], t[2], t[3], t[4], t[5].defined() ? t[5].contiguous() : t[5]};
+  if (!plain_tensor(q) || !c.takes() || recorded({&q})) Py_RETURN_NONE;
+  if (q.dim() != 4 || q.size(0) != c.B() || q.size(3) != c.D() || c.Hkv() < 1 ||
+      q.size(1) % c.Hkv() != 0 || (q.size(1) / c.Hkv()) * q.size(2) > 32 ||
+      q.scalar_type() != at::kBFloat16 || !q.is_contiguous() || q.device() != c.k_codes.device() ||
+      !all_int(q.sizes()))
+    Py_RETURN_NONE;
+  const int B = c.B(), Hq = (int)q.size(1), Tq = (int)q.size(2), D = (int)c.D();
+  const long long bytes = ttfa_decode_mx_workspace_bytes(B, Hq, c.Hkv(), Tq, c.L(), D, c.bits());
+  if (bytes < 0) Py_RETURN_NONE;
+  RECORD_FUNCTION("tinytrain::flash_attn_decode_mx", c10::ArrayRef<const c10::IValue>());
+  const c10::DeviceGuard on(q.device());
+  Tensor ws = f32(q, {bytes / 4 + 4}), o = same(q), lse = f32(q, {B, Hq, Tq});
+  check(ttfa_decode_mx_fwd(q.const_data_ptr(), c.k_codes.const_data_ptr(),
+                           c.k_scales.const_data_ptr(), c.v_codes.const_data_ptr(),
+                           c.v_scales.const_data_ptr(), c.lens.const_data_ptr<int>(),
+                           o.mutable_data_ptr(), lse.mutable_data_ptr<float>(),
+                           ws.mutable_data_ptr<float>(), B, Hq, c.Hkv(), Tq, c.L(), D, c.bits(),
+                           TTFA_BF16, scale_of(D), stream_of(q)));
+  return pack({o, lse});
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject *py_qk_norm_rope(PyObject *, PyObject *const *args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!arity(n, 8)) return nullptr;
@@ -516,6 +644,12 @@ PyMethodDef methods[] = {
      "(o, lse) of flash_attn_decode(q, k_cache, v_cache, cache_seqlens), or None."},
     {"qk_norm_rope", (PyCFunction)(void (*)(void))py_qk_norm_rope, METH_FASTCALL,
      "(q, k, v) of qk_norm_rope(q, k, v, wq, wk, cos, sin, eps), or None."},
+    {"kv_cache_append", (PyCFunction)(void (*)(void))py_kv_cache_append, METH_FASTCALL,
+     "True once kv_cache_append(k, v, *cache, cache_seqlens) is done, or None."},
+    {"kv_cache_read", (PyCFunction)(void (*)(void))py_kv_cache_read, METH_FASTCALL,
+     "(k, v) of kv_cache_read(*cache, cache_seqlens, rows, ttfa dtype), or None."},
+    {"flash_attn_decode_mx", (PyCFunction)(void (*)(void))py_flash_attn_decode_mx, METH_FASTCALL,
+     "(o, lse) of flash_attn_decode_mx(q, *cache, cache_seqlens), or None."},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ttfa_torch",

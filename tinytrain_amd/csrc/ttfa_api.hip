@@ -66,6 +66,44 @@ int check_decode(int B, int Hq, int Hkv, int Tq, int Lmax, int D, int dtype, flo
   return TTFA_OK;
 }
 
+// Quantised KV cache of rows of D elements: extents of one head within 32-bit byte offsets.
+int check_kv(int B, int Hkv, int max_seqlen, int D, int bits) {
+  if (bits != 4 && bits != 8) return TTFA_E_BITS;
+  if (D != 64 && D != 128) return TTFA_E_HEAD_DIM;
+  if (Hkv < 1) return TTFA_E_GROUP;
+  if (B < 1 || max_seqlen < 1) return TTFA_E_SEQ;
+  if ((int64_t)max_seqlen * D > (int64_t)0x7fffffff) return TTFA_E_SEQ;
+  if ((int64_t)B * Hkv > (int64_t)0x7fffffff / 4) return TTFA_E_SEQ;
+  return TTFA_OK;
+}
+
+// Rows moved in or out of it: one 16th of a workgroup at least each, numbered in 32 bits.
+int check_kv_rows(int B, int Hkv, int rows, int max_seqlen, int D, int bits, int dtype) {
+  if (dtype != TTFA_BF16 && dtype != TTFA_F32) return TTFA_E_DTYPE;
+  const int rc = check_kv(B, Hkv, max_seqlen, D, bits);
+  if (rc) return rc;
+  if (rows < 1 || (int64_t)rows > ((int64_t)0x7fffffff - 64) / ((int64_t)B * Hkv)) return TTFA_E_SEQ;
+  return TTFA_OK;
+}
+
+int check_decode_mx(int B, int Hq, int Hkv, int Tq, int max_seqlen, int D, int bits, int dtype,
+                    float scale) {
+  const int rc = check_kv(B, Hkv, max_seqlen, D, bits);
+  // a length of 1 in place of max_seqlen, which check_kv holds to bytes of fewer bits
+  return rc ? rc : check_decode(B, Hq, Hkv, Tq, 1, D, dtype, scale);
+}
+
+int check_seqlens(const int *cache_seqlens) {
+  if (cache_seqlens == nullptr) return TTFA_E_NULL;
+  return reinterpret_cast<uintptr_t>(cache_seqlens) & 3u ? TTFA_E_ALIGN : TTFA_OK;
+}
+
+ttfa::KvCache kv_cache(const void *k_codes, const void *k_scales, const void *v_codes,
+                       const void *v_scales) {
+  auto p = [](const void *x) { return const_cast<uint8_t *>(static_cast<const uint8_t *>(x)); };
+  return {{p(k_codes), p(v_codes)}, {p(k_scales), p(v_scales)}};
+}
+
 // Device address of `scratch` on the current device, resolved once per device (the first
 // ttfa_bwd_static call on it) and cached; *out stays null on failure.
 hipError_t static_scratch_ptr(float **out) {
@@ -130,6 +168,8 @@ const char *ttfa_strerror(int code) {
     case TTFA_E_SCALE: return "ttfa: scale must be finite and > 0";
     case TTFA_E_EPS: return "ttfa: eps must be in [0, 1)";
     case TTFA_E_QROWS: return "ttfa: decode needs (Hq / Hkv) * Tq <= 32 query rows per KV head";
+    case TTFA_E_BITS: return "ttfa: a quantised cache holds elements of 4 or 8 bits";
+    case TTFA_E_STRIDE: return "ttfa: strides must be multiples of 16 bytes and not negative";
     case TTFA_E_SCRATCH:
       return "ttfa: ttfa_bwd_static needs B * Hq * T <= TTFA_BWD_STATIC_MAX_ROWS (1048576)";
     default: break;
@@ -229,6 +269,58 @@ int ttfa_decode_fwd(const void *q, const void *k_cache, const void *v_cache,
   return static_cast<int>(ttfa::launch_decode_bf16(q, k_cache, v_cache, cache_seqlens, o, lse,
                                                    workspace, B, Hq, Hkv, Tq, max_seqlen, D,
                                                    scale, static_cast<hipStream_t>(hip_stream)));
+}
+
+int ttfa_kv_append(const void *k, const void *v, void *k_codes, void *k_scales, void *v_codes,
+                   void *v_scales, const int *cache_seqlens, const long long *strides, int B, int Hkv,
+                   int rows, int max_seqlen, int D, int bits, int dtype, void *hip_stream) {
+  int rc = check_kv_rows(B, Hkv, rows, max_seqlen, D, bits, dtype);
+  if (rc) return rc;
+  const void *ptrs[] = {k, v, k_codes, k_scales, v_codes, v_scales};
+  if ((rc = check_ptrs(ptrs, 6)) || (rc = check_seqlens(cache_seqlens))) return rc;
+  const int64_t most = (int64_t)1 << 40, unit = dtype == TTFA_BF16 ? 8 : 4;
+  int64_t st[2][3];
+  const int64_t dense[3] = {(int64_t)Hkv * rows * D, (int64_t)rows * D, D};
+  for (int i = 0; i < 6; ++i) {
+    const int64_t x = strides ? strides[i] : dense[i % 3];
+    if (x < 0 || x % unit || x > most) return TTFA_E_STRIDE;
+    st[i / 3][i % 3] = x;
+  }
+  return static_cast<int>(ttfa::launch_kv_append(
+      k, v, st, kv_cache(k_codes, k_scales, v_codes, v_scales), cache_seqlens, B, Hkv, rows,
+      max_seqlen, D, bits, dtype == TTFA_F32, static_cast<hipStream_t>(hip_stream)));
+}
+
+int ttfa_kv_read(const void *k_codes, const void *k_scales, const void *v_codes, const void *v_scales,
+                 const int *cache_seqlens, void *k, void *v, int B, int Hkv, int rows, int max_seqlen,
+                 int D, int bits, int dtype, void *hip_stream) {
+  int rc = check_kv_rows(B, Hkv, rows, max_seqlen, D, bits, dtype);
+  if (rc) return rc;
+  const void *ptrs[] = {k_codes, k_scales, v_codes, v_scales, k, v};
+  if ((rc = check_ptrs(ptrs, 6)) || (rc = check_seqlens(cache_seqlens))) return rc;
+  return static_cast<int>(ttfa::launch_kv_read(
+      kv_cache(k_codes, k_scales, v_codes, v_scales), cache_seqlens, k, v, B, Hkv, rows, max_seqlen, D,
+      bits, dtype == TTFA_F32, static_cast<hipStream_t>(hip_stream)));
+}
+
+long long ttfa_decode_mx_workspace_bytes(int B, int Hq, int Hkv, int Tq, int max_seqlen, int D,
+                                         int bits) {
+  if (check_decode_mx(B, Hq, Hkv, Tq, max_seqlen, D, bits, TTFA_BF16, 1.f)) return -1;
+  const ttfa::DecodeSplit sp = ttfa::decode_mx_split(B, Hkv, max_seqlen, D, bits);
+  return (long long)B * Hq * Tq * sp.n_chunks * (D + 2) * (long long)sizeof(float);
+}
+
+int ttfa_decode_mx_fwd(const void *q, const void *k_codes, const void *k_scales, const void *v_codes,
+                       const void *v_scales, const int *cache_seqlens, void *o, float *lse,
+                       float *workspace, int B, int Hq, int Hkv, int Tq, int max_seqlen, int D,
+                       int bits, int dtype, float scale, void *hip_stream) {
+  int rc = check_decode_mx(B, Hq, Hkv, Tq, max_seqlen, D, bits, dtype, scale);
+  if (rc) return rc;
+  const void *ptrs[] = {q, k_codes, k_scales, v_codes, v_scales, o, lse, workspace};
+  if ((rc = check_ptrs(ptrs, 8)) || (rc = check_seqlens(cache_seqlens))) return rc;
+  return static_cast<int>(ttfa::launch_decode_mx(
+      q, kv_cache(k_codes, k_scales, v_codes, v_scales), cache_seqlens, o, lse, workspace, B, Hq, Hkv,
+      Tq, max_seqlen, D, bits, scale, static_cast<hipStream_t>(hip_stream)));
 }
 
 int ttfa_bwd(const void *q, const void *k, const void *v, const void *o, const void *dout,
