@@ -48,6 +48,7 @@
 //   B 64, Hkv 12, D 64, lengths 200..2000 of 2000       49.5   44.8   43.0
 //   B 1, Hkv 8, D 128, 16384 keys                       17.0   17.0   16.9
 //   B 1, Hkv 2, D 128, 512 keys                         11.6    9.1    9.1  (one launch)
+#include "decode_split.h"
 #include "fa_bwd.h"  // allow_lds
 #include "fa_common.h"
 #include "fa_kernels.h"
@@ -136,22 +137,6 @@ __device__ __forceinline__ void decode_block(const bf16 *Kt, const bf16 *Vt,
 #pragma unroll
     for (int db = 0; db < P::DB; ++db) oacc[db] = mfma32(vf[db], pb[m], oacc[db]);
   }
-}
-
-// Workgroups of a unit that have work: its nb blocks, 2^log2_min each at least (a power of two:
-// a quotient would stand between the length's load and the first block's).
-__device__ __forceinline__ int used_chunks(int nb, int n_chunks, int log2_min) {
-  return max(min((nb + (1 << log2_min) - 1) >> log2_min, n_chunks), 1);
-}
-
-// Places by which chunk `chunk` turns its units (n_units >= 8).  Consecutive workgroups go to the
-// XCDs in turn, and those of an XCD to its 32 CUs: 37 = 4 * 8 + 5 moves a unit's chunks to
-// other XCDs and other CUs.  Fewer units have more chunks, whose own numbers do that.
-__device__ __forceinline__ int chunk_turn(int chunk, int n_units) {
-  int turn = chunk * (n_units >= 64 ? 37 : 5);
-  if (n_units < 32) turn &= 7;
-  while (turn >= n_units) turn -= n_units;  // at most five times
-  return turn;
 }
 
 }  // namespace

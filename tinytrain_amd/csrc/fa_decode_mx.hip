@@ -4,27 +4,41 @@
 // values the cache stands for, and so are the split over keys and the merge pass.
 //
 // Layout: a wave takes 32 keys at a time and 16 or 32 query columns (R = G * Tq <= 32 of them are
-// real; the others repeat them) through v_mfma_f32_16x16x32_bf16,
-//      A[i][k] in lane i + 16 * (k / 8), slot k % 8      (16 rows, 32 deep)
-//      B[k][j] in lane j + 16 * (k / 8), slot k % 8
-//      D[i][j] in lane j + 16 * (i / 4), register i % 4,
-// chosen over the 32x32 shape because a lane then holds a quarter of a K row: at D = 128 exactly one
-// group of 32 with its one scale, loaded straight into registers.  S^T = K Q^T is formed as two
-// tiles t whose row 4q + r is key 8q + 4t + r of the block.  Lane (j, q) then ends up with the
-// scores of keys 8q .. 8q + 7 of column j, which is the B operand of O^T += V^T P^T as it stands.
-// Its A operand has keys 8q .. 8q + 7 of one d in lane (i, q): the lane loads D / 16 consecutive
-// elements of each of the eight rows, converts each row's with that row's scale, and pairs up
-// rows with v_perm, giving D / 16 tiles whose row i is d = D / 16 * i + tile.  No LDS in the loop.
+// real; the others repeat them).  S^T = K Q^T is formed as two tiles of 16 keys, tile t's row 4q + r
+// being key q + 16t + 4r of the block, so that the result (D[i][j] in lane j + 16 * (i / 4), register
+// i % 4) leaves lane (j, q) with the scores of keys q + 4e, e = 4t + r, of column j: the B operand of
+// O^T += V^T P^T through v_mfma_f32_16x16x32_bf16 as it stands, and every load instruction reads
+// whole consecutive rows.
+//  * K stays as it lies in the cache: v_mfma_scale_f32_16x16x128_f8f6f4 takes e2m1 or e4m3 elements
+//    with one power of two per 32.  Its k index runs, for e2m1, 32 elements in lane i + 16 * (k / 32);
+//    for e4m3 the elements 16c .. 16c + 15 and 64 + 16c .. of lane i + 16 c; the scale of elements
+//    32c .. 32c + 31 comes from lane i + 16 c (checked element by element on gfx950).  Q is split
+//    once into two e4m3 terms, q = hi + lo: a bf16 has 8 significant bits and each term 4, so the sum
+//    is exact but for elements below 2^-13 of the row's largest, which lose at most 2^-21 of that.
+//    At D = 64 both terms share one product: k = 0..63 are hi, 64..127 lo, and K is given twice.
+//    (K through bf16 conversions took 32 more of about 200 vector instructions a block.)
+//  * V: lane (i, q) loads D / 16 consecutive elements of each of the rows q + 4e, converts each
+//    row's to bf16 with that row's scale, and pairs up rows with v_perm, giving the A operands of
+//    D / 16 tiles whose row i is d = D / 16 * i + tile.  The scale goes by row, so it cannot move into
+//    the product, whose scales go along the keys.
+// No LDS in the loop.
+#include "decode_split.h"
+#include "fa_bwd.h"  // allow_lds
 #include "fa_common.h"
 #include "fa_kernels.h"
 #include "mx.h"
+
+#include <algorithm>
 
 namespace ttfa {
 
 namespace {
 
 constexpr float kMxSlack = 8.0f;
-constexpr int kMxBlock = 32;  // keys per block
+// Running maximum before any key: finite, so that differences from it are no NaN.
+constexpr float kMxLowest = -3.402823466e38f;
+constexpr int kMxBlock = 64;  // keys per block: two halves of 32
+constexpr int kMxMerged = 16;  // partials of a row that one wave merges
 
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -43,78 +57,102 @@ __device__ __forceinline__ float quarters_sum(float x) {
 template <int D, int BITS>
 struct MxShape {
   static constexpr int CODE = D * BITS / 8, GR = D / 32;  // bytes of a row: codes, scales
-  static constexpr int KS = D / 32;                       // products of a score tile
   static constexpr int DT = D / 16;                       // output tiles; V elements of a lane's row
-  static constexpr int KW = CODE / 16;                    // words of a lane's K quarter row
-  static constexpr int VB = CODE / 16;                    // bytes of a lane's V row piece
+  static constexpr bool PAIRED = D == 64 && BITS == 4;    // a lane's load serves two K tiles / V rows
+  static constexpr int KW = D == 128 && BITS == 8 ? 8 : 4;  // words of a lane's K piece
+  static constexpr int KL = PAIRED ? 1 : 2, VL = PAIRED ? 4 : 8;  // loads of a half: K tiles, V rows
+  static constexpr int VW = D == 128 && BITS == 8 ? 2 : 1;  // words of a V load
 };
 
-// What a lane holds of one block: its quarter row of each K tile and its piece of eight V rows, as
-// they lie in the cache.
+// What a lane holds of a half block, as it lies in the cache.
+//  * K: for tile t its 16 or 32 bytes of row q' + 4 r' + 16 t, where i = 4 q' + r'.  e2m1 at D = 64
+//    needs the same two pieces of a row in lanes q and q + 2: the lower half of the wave loads tile
+//    0, the upper one tile 1, and they are exchanged at use.
+//  * V: D / 16 elements of each of the rows q + 4e; those 2 bytes of e2m1 at D = 64 come as words,
+//    an even lane's from row e = 2r, an odd lane's from row 2r + 1, and neighbours exchange halves.
 template <int D, int BITS>
-struct MxBlock {
+struct MxCodes {
   using P = MxShape<D, BITS>;
-  uint32_t k[2][P::KW];
-  uint32_t v[8][P::VB > 4 ? 2 : 1];
-  uint32_t ks[2];  // scale byte of the K piece
-  uint32_t vs;     // scale bytes of V row 8q + (i & 7)
+  uint32_t k[P::KL][P::KW];
+  uint32_t v[P::VL][P::VW];
 };
 
-// This lane's byte offsets within a block.
+// Scale bytes of a block: of K row q' + 4 r' + 16 q (tile q of the block's four) and of V row
+// q + 4 (i & 7) + 32 (i >> 3).  A block's scales come in two loads of 64 rows each: loads of 32 rows
+// at a time took 2 to 4 of 20 us at 64 x 12 caches of D = 64.
+struct MxScales {
+  uint32_t k, v;
+};
+
+// This lane's byte offsets within a half (codes) or a block (scales).
 template <int D, int BITS>
 struct MxLane {
   using P = MxShape<D, BITS>;
-  uint32_t k, ks, v, vs;
+  uint32_t k, v, ks, vs;
   __device__ explicit MxLane(int lane) {
-    const int i = lane & 15, q = lane >> 4, row = 8 * (i >> 2) + (i & 3);
-    k = row * P::CODE + q * (P::CODE / 4);
-    ks = row * P::GR + q * P::GR / 4;
-    v = 8 * q * P::CODE + i * P::VB;
-    vs = (8 * q + (i & 7)) * P::GR;
-  }
-};
-
-struct MxSrc {  // one (batch, KV head) of the cache, L rows of it
-  const uint8_t *kc, *ks, *vc, *vs;
-  int L;
-};
-
-// Loads past row L give zeros (codes 0 of scale 2^-127: exact zeros), so no block needs a bound.
-template <int D, int BITS>
-__device__ __forceinline__ void load_block(MxBlock<D, BITS> &x, const MxSrc &s,
-                                           const MxLane<D, BITS> &o, int k0) {
-  using P = MxShape<D, BITS>;
-  const uint32_t left = (uint32_t)max(s.L - k0, 0);
-  const auto kc = make_rsrc(s.kc + (int64_t)k0 * P::CODE, left * P::CODE);
-  const auto ks = make_rsrc(s.ks + (int64_t)k0 * P::GR, left * P::GR);
-  const auto vc = make_rsrc(s.vc + (int64_t)k0 * P::CODE, left * P::CODE);
-  const auto vs = make_rsrc(s.vs + (int64_t)k0 * P::GR, left * P::GR);
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const uint32_t at = o.k + 4 * t * P::CODE;
-    if constexpr (P::KW == 2) {
-      const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(kc, at, 0, 0);
-      x.k[t][0] = w[0], x.k[t][1] = w[1];
+    const int i = lane & 15, q = lane >> 4, row = (i >> 2) + 4 * (i & 3);
+    if constexpr (P::PAIRED) {
+      k = (row + 16 * (q >> 1)) * P::CODE + 16 * (q & 1);
+      v = (q + 4 * (i & 1)) * P::CODE + 4 * (i >> 1);
     } else {
-#pragma unroll
-      for (int c = 0; c < P::KW / 4; ++c) {
-        const u32x4 w = buf_load16(kc, at + 16 * c);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x.k[t][4 * c + e] = w[e];
-      }
+      k = row * P::CODE + 16 * q;
+      v = q * P::CODE + i * (P::CODE / 16);
     }
-    x.ks[t] = __builtin_amdgcn_raw_buffer_load_b8(ks, o.ks + 4 * t * P::GR, 0, 0);
+    ks = (row + 16 * q) * P::GR;
+    vs = (q + 4 * (i & 7) + 32 * (i >> 3)) * P::GR;
   }
-  x.vs = P::GR == 4 ? buf_load4(vs, o.vs) : (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(vs, o.vs, 0, 0);
+};
+
+struct MxSrc {  // one (batch, KV head) of the cache
+  const uint8_t *kc, *ks, *vc, *vs;
+};
+
+// Loads of rows past `end` read nothing and give zeros (codes 0 of scale 2^-127: exact zeros).
+template <int D, int BITS>
+__device__ __forceinline__ void load_codes(MxCodes<D, BITS> &x, const MxSrc &s,
+                                           const MxLane<D, BITS> &o, int k0, int end) {
+  using P = MxShape<D, BITS>;
+  const uint32_t bytes = (uint32_t)max(end - k0, 0) * P::CODE;
+  const auto kc = make_rsrc(s.kc + (int64_t)k0 * P::CODE, bytes);
+  const auto vc = make_rsrc(s.vc + (int64_t)k0 * P::CODE, bytes);
 #pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    const uint32_t at = o.v + r * P::CODE;
-    if constexpr (P::VB == 2) x.v[r][0] = __builtin_amdgcn_raw_buffer_load_b16(vc, at, 0, 0);
-    else if constexpr (P::VB == 4) x.v[r][0] = buf_load4(vc, at);
+  for (int t = 0; t < P::KL; ++t)
+#pragma unroll
+    for (int c = 0; c < P::KW / 4; ++c) {  // e4m3, D = 128: elements 16q .. and 64 + 16q ..
+      const u32x4 w = buf_load16(kc, o.k + 16 * t * P::CODE + 64 * c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x.k[t][4 * c + e] = w[e];
+    }
+#pragma unroll
+  for (int r = 0; r < P::VL; ++r) {
+    const uint32_t at = o.v + (32 / P::VL) * r * P::CODE;
+    if constexpr (P::VW == 1) x.v[r][0] = buf_load4(vc, at);
     else {
       const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(vc, at, 0, 0);
       x.v[r][0] = w[0], x.v[r][1] = w[1];
     }
+  }
+}
+
+template <int D, int BITS>
+__device__ __forceinline__ MxScales load_scales(const MxSrc &s, const MxLane<D, BITS> &o, int k0, int end) {
+  using P = MxShape<D, BITS>;
+  const uint32_t bytes = (uint32_t)max(end - k0, 0) * P::GR;
+  const auto ks = make_rsrc(s.ks + (int64_t)k0 * P::GR, bytes);
+  const auto vs = make_rsrc(s.vs + (int64_t)k0 * P::GR, bytes);
+  if constexpr (P::GR == 4) return {buf_load4(ks, o.ks), buf_load4(vs, o.vs)};
+  else
+    return {(uint32_t)__builtin_amdgcn_raw_buffer_load_b16(ks, o.ks, 0, 0),
+            (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(vs, o.vs, 0, 0)};
+}
+
+// x of row (of 16 lanes) T of the wave, in every row, for T = 0..3
+__device__ __forceinline__ void spread_rows(uint32_t (&out)[4], uint32_t x) {
+  const auto h = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const auto p = __builtin_amdgcn_permlane16_swap(h[u], h[u], false, false);
+    out[2 * u] = p[0], out[2 * u + 1] = p[1];
   }
 }
 
@@ -124,60 +162,133 @@ __device__ __forceinline__ uint32_t row_bcast(uint32_t x) {
   return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x150 + S, 0xF, 0xF, true);
 }
 
-// Scale of V row S for this lane's group, on the exponent bits (the conversions look at nothing
-// else): `turn` rotates the byte of the group there.
-template <int S, class Block>
-__device__ __forceinline__ uint32_t v_scale(const Block &x, uint32_t turn) {
-  const uint32_t sc = row_bcast<S>(x.vs);
-  return __builtin_amdgcn_alignbit(sc, sc, turn);
+// Scales of this lane's group in its eight V rows of half U, on the exponent bits (the conversions
+// look at nothing else): `turn` rotates the group's byte of a row's there.
+template <int U>
+__device__ __forceinline__ void v_scales(uint32_t (&sc)[8], uint32_t vs, uint32_t turn) {
+  sc[0] = row_bcast<8 * U>(vs), sc[1] = row_bcast<8 * U + 1>(vs);
+  sc[2] = row_bcast<8 * U + 2>(vs), sc[3] = row_bcast<8 * U + 3>(vs);
+  sc[4] = row_bcast<8 * U + 4>(vs), sc[5] = row_bcast<8 * U + 5>(vs);
+  sc[6] = row_bcast<8 * U + 6>(vs), sc[7] = row_bcast<8 * U + 7>(vs);
+#pragma unroll
+  for (int r = 0; r < 8; ++r) sc[r] = __builtin_amdgcn_alignbit(sc[r], sc[r], turn);
 }
 
-// The lane's V piece of row S as bf16 pairs (DT / 2 of them).  CLEAN: values of a NaN group are
-// zeros, and mark[S] is 1 for one.
-template <int D, int BITS, bool CLEAN, int S>
-__device__ __forceinline__ void v_row(bf16x2 (&out)[D / 32], const MxBlock<D, BITS> &x, uint32_t turn,
-                                      bf16x8 &mark) {
-  uint32_t sc = v_scale<S>(x, turn);
-  if constexpr (CLEAN) {
-    const bool nan = (sc & 0x7f800000u) == 0x7f800000u;
-    mark[S] = (bf16)(nan ? 1.f : 0.f);
-    sc = nan ? 0 : sc;
+// 1 in the slot of every row whose group is NaN, whose scale becomes 2^-127 (its codes are zeros).
+__device__ __forceinline__ bf16x8 take_out_nans(uint32_t (&sc)[8]) {
+  bf16x8 mark;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    const bool nan = (sc[r] & 0x7f800000u) == 0x7f800000u;
+    mark[r] = (bf16)(nan ? 1.f : 0.f);
+    sc[r] = nan ? 0 : sc[r];
   }
-  const float scale = __uint_as_float(sc);
-  if constexpr (BITS == 4) {
-    out[0] = mx_values2<4, 0>(x.v[S][0], scale);
-    out[1] = mx_values2<4, 1>(x.v[S][0], scale);
-    if constexpr (D == 128) {
-      out[2] = mx_values2<4, 2>(x.v[S][0], scale);
-      out[3] = mx_values2<4, 3>(x.v[S][0], scale);
-    }
-  } else {
-    out[0] = mx_values2<8, 0>(x.v[S][0], scale);
-    out[1] = mx_values2<8, 1>(x.v[S][0], scale);
-    if constexpr (D == 128) {
-      out[2] = mx_values2<8, 0>(x.v[S][1], scale);
-      out[3] = mx_values2<8, 1>(x.v[S][1], scale);
-    }
+  return mark;
+}
+
+// A operands of output tiles 2W and 2W + 1: slot r = V[key q + 4r][d = DT * i + 2W, + 1]
+template <int D, int BITS, int W>
+__device__ __forceinline__ void v_pair(bf16x8 &even, bf16x8 &odd,
+                                       const uint32_t (&v)[MxShape<D, BITS>::VL][MxShape<D, BITS>::VW],
+                                       const uint32_t (&sc)[8]) {
+  using P = MxShape<D, BITS>;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    const float scale = __uint_as_float(sc[r]);
+    bf16x2 y;
+    if constexpr (P::PAIRED)
+      y = r & 1 ? mx_values2<4, W + 2>(v[r / 2][0], scale) : mx_values2<4, W>(v[r / 2][0], scale);
+    else if constexpr (BITS == 4) y = mx_values2<4, W>(v[r % P::VL][0], scale);
+    else y = mx_values2<8, W & 1>(v[r % P::VL][W >> 1], scale);
+    even[r] = y[0], odd[r] = y[1];
   }
 }
 
-// A operands of all output tiles: tile[n] slot s = V[key 8q + s][d = DT * i + n]
-template <int D, int BITS, bool CLEAN>
-__device__ __forceinline__ void v_tiles(bf16x8 (&tile)[D / 16], const MxBlock<D, BITS> &x, uint32_t turn,
-                                        bf16x8 &mark) {
-  bf16x2 a[8][D / 32];
-  v_row<D, BITS, CLEAN, 0>(a[0], x, turn, mark);
-  v_row<D, BITS, CLEAN, 1>(a[1], x, turn, mark);
-  v_row<D, BITS, CLEAN, 2>(a[2], x, turn, mark);
-  v_row<D, BITS, CLEAN, 3>(a[3], x, turn, mark);
-  v_row<D, BITS, CLEAN, 4>(a[4], x, turn, mark);
-  v_row<D, BITS, CLEAN, 5>(a[5], x, turn, mark);
-  v_row<D, BITS, CLEAN, 6>(a[6], x, turn, mark);
-  v_row<D, BITS, CLEAN, 7>(a[7], x, turn, mark);
+// One column's query row as a lane holds it: e4m3 terms hi and lo of its 32 elements (D = 64: 16 of
+// each), and the bytes of their powers of two.
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+template <int D>
+struct MxQuery {
+  i32x8 t[D == 128 ? 2 : 1];
+  int scale[D == 128 ? 2 : 1];
+
+  // The row's elements as they come: runs of 16 from 16 q and (D = 128) 64 + 16 q.
+  u32x4 raw[D / 32];
+
+  __device__ __forceinline__ void load(const bf16 *row, int q4) {
 #pragma unroll
-  for (int n = 0; n < D / 16; ++n)
+    for (int c = 0; c < D / 32; ++c)
+      raw[c] = *reinterpret_cast<const u32x4 *>(row + 64 * (c >> 1) + 16 * q4 + 8 * (c & 1));
+  }
+
+  __device__ __forceinline__ void split(int q4) {
+    u16x2 m{};
 #pragma unroll
-    for (int s = 0; s < 8; ++s) tile[n][s] = a[s][n >> 1][n & 1];
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, raw[c][w] & 0x7fff7fffu));
+    uint32_t top = (uint32_t)max(m[0], m[1]) << 16;
+    auto p = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+    top = max(p[0], p[1]);
+    p = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+    top = max(p[0], p[1]);
+    const uint32_t byte = mx_scale_byte<8>(top);
+    const int b_lo = byte == 255 ? 255 : (int)byte - 4;  // NaN and infinity: the whole row is NaN
+    // x 2^-e is at most 464, or 511 next to the largest bf16, where hi is 448 and lo at most 63
+    const float inv = __uint_as_float((254 - min(byte, 253u)) << 23);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      u32x2 hi{}, lo{};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t w = raw[c][e];
+        const f32x2 y{__uint_as_float(w << 16) * inv, __uint_as_float(w & 0xffff0000u) * inv};
+        hi = mx_pack<8>(hi, e, y, 1.f, 448.f);
+        const uint32_t code = hi[e >> 1];
+        const f32x2 h = e & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(code, 1.f, 1)
+                              : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(code, 1.f, 0);
+        lo = mx_pack<8>(lo, e, f32x2{y[0] - h[0], y[1] - h[1]}, 0x1p-4f, 28.f);
+      }
+      // D = 128: run c / 2 of both terms; D = 64: hi is run 0 and lo run 1 of one operand
+      if constexpr (D == 128) {
+        t[0][2 * c] = (int)hi[0], t[0][2 * c + 1] = (int)hi[1];
+        t[1][2 * c] = (int)lo[0], t[1][2 * c + 1] = (int)lo[1];
+      } else {
+        t[0][2 * c] = (int)hi[0], t[0][2 * c + 1] = (int)hi[1];
+        t[0][4 + 2 * c] = (int)lo[0], t[0][4 + 2 * c + 1] = (int)lo[1];
+      }
+    }
+    if constexpr (D == 128) scale[0] = (int)byte, scale[1] = b_lo;
+    else scale[0] = q4 < 2 ? (int)byte : b_lo;
+  }
+};
+
+// A operand of a K tile
+template <int D, int BITS>
+__device__ __forceinline__ i32x8 k_operand(const uint32_t (&k)[MxShape<D, BITS>::KW]) {
+  i32x8 a{};
+#pragma unroll
+  for (int w = 0; w < MxShape<D, BITS>::KW; ++w) a[w] = (int)k[w];
+  if constexpr (D == 64 && BITS == 8) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) a[4 + w] = (int)k[w];
+  }
+  return a;
+}
+
+// S^T tile of one column tile; `scale`: byte 0 is that of the row's group q (D = 64: q & 1)
+template <int D, int BITS>
+__device__ __forceinline__ f32x4 scores(i32x8 a, uint32_t scale, const MxQuery<D> &q) {
+  constexpr int type = BITS == 4 ? 4 : 0;  // e2m1, e4m3
+  f32x4 s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q.t[0], f32x4{}, type, 0, 0, (int)scale, 0,
+                                                             q.scale[0]);
+  if constexpr (D == 128)
+    s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q.t[1], s, type, 0, 0, (int)scale, 0,
+                                                         q.scale[1]);
+  return s;
 }
 
 // Whether one of the row's scale bytes is 255 (a NaN group)
@@ -191,87 +302,108 @@ __device__ __forceinline__ bool any_nan_scale(uint32_t bytes) {
 // Grid: (B * Hkv units, n_chunks), workgroups of NW waves; NC tiles of 16 query columns.  Partial rows
 // are indexed (b * Hq + h) * Tq + i, each with n_chunks slots.
 template <int D, int BITS, int NW, int NC, bool SPLIT>
-__global__ __launch_bounds__(64 * NW) void fa_decode_mx_kernel(
+__global__ __launch_bounds__(64 * NW, 2) void fa_decode_mx_kernel(
     const bf16 *__restrict__ Q, KvCache cache, const int *__restrict__ cache_seqlens,
     bf16 *__restrict__ O, float *__restrict__ LSE, float *__restrict__ part_o,
     float *__restrict__ part_ml, int B, int Hq, int Hkv, int Tq, int Lmax, int n_chunks, int log2_min,
     float scale_log2) {
   using P = MxShape<D, BITS>;
-  constexpr int KS = P::KS, DT = P::DT, COLS = 16 * NC;
-  __shared__ __attribute__((aligned(16))) float stage[NW][16 * D];
+  constexpr int DT = P::DT, COLS = 16 * NC;
+  // per wave the partial rows of min(R, 16) columns
+  extern __shared__ __attribute__((aligned(16))) float stage[];
   __shared__ float wm[NW][COLS], wsum[NW][COLS];
   const int chunk = SPLIT ? blockIdx.y : 0;
-  const int bhk = blockIdx.x;
+  int bhk = blockIdx.x;
+  // B * Hkv is the grid's width (gridDim would put hidden arguments on every launch)
+  if (const int n_units = B * Hkv; SPLIT && n_units >= 8) {
+    bhk -= chunk_turn(chunk, n_units);
+    if (bhk < 0) bhk += n_units;
+  }
   const int b = bhk / Hkv, hk = bhk - b * Hkv;
   const int G = Hq / Hkv, R = G * Tq;
   const int wave = wave_id(), lane = threadIdx.x & 63;
   const int i16 = lane & 15, q4 = lane >> 4;
-  const int L = min(max(cache_seqlens[b], 0), Lmax);
+  const int64_t slab = (int64_t)bhk * Lmax;
+  const MxSrc src{cache.codes[0] + slab * P::CODE, cache.scales[0] + slab * P::GR,
+                  cache.codes[1] + slab * P::CODE, cache.scales[1] + slab * P::GR};
+  const MxLane<D, BITS> off(lane);
+  const int blk0 = chunk * NW + wave;
 
-  const int nb = (L + kMxBlock - 1) / kMxBlock;
-  const int used = SPLIT ? max(min((nb + (1 << log2_min) - 1) >> log2_min, n_chunks), 1) : 1;
-  const int step = used * NW, blk0 = chunk < used ? chunk * NW + wave : nb;
-
-  // the query columns of this lane, one per tile
-  int pos[NC];  // last visible key
-  const bf16 *qp[NC];
+  MxQuery<D> query[NC];
+  int last[NC];  // this lane's query column of a tile sees keys up to L + last
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int col = (16 * c + i16) % R, g = col / Tq, i = col - g * Tq;
-    pos[c] = L - Tq + i;
-    qp[c] = Q + (((int64_t)b * Hq + hk * G + g) * Tq + i) * D;
+    last[c] = i - Tq;
+    query[c].load(Q + (((int64_t)b * Hq + hk * G + g) * Tq + i) * D, q4);
   }
+
+  // A half is loaded into the registers of the one just used: the wave's next block is on its way
+  // while it works on this one.
+  MxCodes<D, BITS> x[2];
+  MxScales sc;
+
+  const int L = min(max(cache_seqlens[b], 0), Lmax);
+  const int nb = (L + kMxBlock - 1) / kMxBlock;
+  const int used = SPLIT ? used_chunks(nb, n_chunks, log2_min) : 1, step = used * NW;
 
   f32x4 oacc[NC][DT];
   float m_t[NC], l_part[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    m_t[c] = -INFINITY, l_part[c] = 0.f;
+    m_t[c] = kMxLowest, l_part[c] = 0.f;
 #pragma unroll
     for (int n = 0; n < DT; ++n) oacc[c][n] = f32x4{};
   }
 
-  if (blk0 < nb) {
-    bf16x8 qf[NC][KS];
+  if (chunk < used && blk0 < nb) {
+    sc = load_scales(src, off, blk0 * kMxBlock, L);
+    load_codes(x[0], src, off, blk0 * kMxBlock, L);
+    __builtin_amdgcn_sched_barrier(0);  // in this order: the waits in the loop count on it
+    load_codes(x[1], src, off, blk0 * kMxBlock + 32, L);
+    __builtin_amdgcn_sched_barrier(0);
+    int pos[NC];  // last visible key
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int kk = 0; kk < KS; ++kk)
-        qf[c][kk] = *reinterpret_cast<const bf16x8 *>(qp[c] + q4 * (D / 4) + 8 * kk);
-    const int64_t slab = (int64_t)bhk * Lmax;
-    const MxSrc src{cache.codes[0] + slab * P::CODE, cache.scales[0] + slab * P::GR,
-                    cache.codes[1] + slab * P::CODE, cache.scales[1] + slab * P::GR, L};
-    const MxLane<D, BITS> off(lane);
+    for (int c = 0; c < NC; ++c) {
+      pos[c] = L + last[c];
+      query[c].split(q4);
+    }
     // rotates byte g of a row's scale bytes to bits 30:23
     const uint32_t turn = (8 * (i16 * P::GR / 16) + 9) & 31;
     const int first_masked = L - Tq;  // keys past this need the mask for some column
 
-#pragma unroll 1
-    for (int blk = blk0; blk < nb; blk += step) {
-      const int k0 = blk * kMxBlock;
-      MxBlock<D, BITS> x;
-      load_block(x, src, off, k0);
+    // selects bytes of (neighbour's word, own word) = bytes (7..4, 3..0)
+    const uint32_t halves = lane & 1 ? 0x03020706u : 0x05040100u;
+    const uint32_t kshift = 8 * (q4 & (P::GR - 1));  // brings the byte of this lane's K group down
+    // Half U of a block: keys k0 .. k0 + 31
+    auto attend = [&](auto u, const MxCodes<D, BITS> &x, const uint32_t (&ks)[4], uint32_t vs, int k0) {
+      constexpr int U = decltype(u)::value;
       f32x4 s[NC][2];
+      i32x8 ka[2];
+      if constexpr (P::PAIRED) {
+        uint32_t k[2][P::KW];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const float scale = __uint_as_float(x.ks[t] << 23);
-#pragma unroll
-        for (int kk = 0; kk < KS; ++kk) {
-          const u32x2 w = BITS == 4 ? u32x2{x.k[t][kk], 0}
-                                    : u32x2{x.k[t][2 * kk % P::KW], x.k[t][(2 * kk + 1) % P::KW]};
-          const bf16x8 kf = mx_values8<BITS>(w, scale);
-#pragma unroll
-          for (int c = 0; c < NC; ++c) s[c][t] = mfma16(kf, qf[c][kk], kk ? s[c][t] : f32x4{});
+        for (int w = 0; w < P::KW; ++w) {
+          const auto p = __builtin_amdgcn_permlane32_swap(x.k[0][w], x.k[0][w], false, false);
+          k[0][w] = p[0], k[1][w] = p[1];
         }
+        ka[0] = k_operand<D, BITS>(k[0]), ka[1] = k_operand<D, BITS>(k[1]);
+      } else {
+        ka[0] = k_operand<D, BITS>(x.k[0]), ka[1] = k_operand<D, BITS>(x.k[P::KL - 1]);
       }
-      const bool masked = k0 + kMxBlock - 1 > first_masked;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          s[c][t] = scores<D, BITS>(ka[t], ks[2 * U + t] >> kshift, query[c]);
+      const bool masked = k0 + 31 > first_masked;
       bf16x8 pb[NC];
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         if (masked) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (k0 + 8 * q4 + e > pos[c]) s[c][e >> 2][e & 3] = -INFINITY;
+            if (k0 + q4 + 4 * e > pos[c]) s[c][e >> 2][e & 3] = -INFINITY;
         }
         float mx = fmax2(s[c][0][0], s[c][0][1]);
 #pragma unroll
@@ -280,52 +412,89 @@ __global__ __launch_bounds__(64 * NW) void fa_decode_mx_kernel(
         if (__builtin_amdgcn_ballot_w64(mx > m_t[c] + kMxSlack)) {
           // each column by itself: its bits do not depend on when others rescale
           const float m_new = mx > m_t[c] + kMxSlack ? mx : m_t[c];
-          // 0 when m_t is still -inf; 1 for a column that stays all-masked (m_new = -inf; its
-          // sums are still 0), where exp2(-inf - -inf) would be NaN
-          const float alpha = m_new == -INFINITY ? 1.f : exp2f_fast(m_t[c] - m_new);
+          const float alpha = exp2f_fast(m_t[c] - m_new);  // 0 from the lowest; 1 if unchanged
           m_t[c] = m_new;
           l_part[c] *= alpha;
 #pragma unroll
           for (int n = 0; n < DT; ++n) oacc[c][n] *= alpha;
         }
-        const float m_use = m_t[c] == -INFINITY ? 0.f : m_t[c];
         float p[8], rs = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          p[e] = exp2f_fast(__builtin_fmaf(s[c][e >> 2][e & 3], scale_log2, -m_use));
+          p[e] = exp2f_fast(__builtin_fmaf(s[c][e >> 2][e & 3], scale_log2, -m_t[c]));
           rs += p[e];
         }
         l_part[c] += rs;
         const bf16x4 lo = pack4(p[0], p[1], p[2], p[3]), hi = pack4(p[4], p[5], p[6], p[7]);
         pb[c] = bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
       }
-      bf16x8 vt[DT], mark;
+      uint32_t sc[8];
+      v_scales<U>(sc, vs, turn);
       // Where rows see different keys (several new rows), a NaN group of a key that a row does not
-      // see must not reach it through 0 * NaN: those blocks count the NaN keys that each row sees.
-      const bool nans = masked && Tq > 1 && __builtin_amdgcn_ballot_w64(any_nan_scale(x.vs));
-      if (!nans) {
-        v_tiles<D, BITS, false>(vt, x, turn, mark);
-#pragma unroll
-        for (int n = 0; n < DT; ++n)
-#pragma unroll
-          for (int c = 0; c < NC; ++c) oacc[c][n] = mfma16(vt[n], pb[c], oacc[c][n]);
-      } else {
-        v_tiles<D, BITS, true>(vt, x, turn, mark);
+      // see must not reach it through 0 * NaN: those blocks count the NaN keys that each row sees,
+      // make NaN what they add to, and go on without them.
+      if (masked && Tq > 1 && __builtin_amdgcn_ballot_w64(any_nan_scale(vs))) {
+        const bf16x8 mark = take_out_nans(sc);
+        int key = k0 + q4;
+        asm volatile("" : "+v"(key));  // keeps this block's comparisons in it
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           bf16x8 seen;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) seen[e] = (bf16)(k0 + 8 * q4 + e > pos[c] ? 0.f : 1.f);
+          for (int e = 0; e < 8; ++e) seen[e] = (bf16)(key + 4 * e > pos[c] ? 0.f : 1.f);
           const f32x4 count = mfma16(mark, seen, f32x4{});
 #pragma unroll
-          for (int n = 0; n < DT; ++n) {
-            oacc[c][n] = mfma16(vt[n], pb[c], oacc[c][n]);
+          for (int n = 0; n < DT; ++n)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
               if (count[r] > 0.f) oacc[c][n][r] = __builtin_nanf("");
-          }
         }
       }
+      uint32_t v[P::VL][P::VW];
+#pragma unroll
+      for (int r = 0; r < P::VL; ++r)
+#pragma unroll
+        for (int w = 0; w < P::VW; ++w) v[r][w] = x.v[r][w];
+      if constexpr (P::PAIRED) {
+        // even lanes take the low halves of their own row's word and their neighbour's, odd lanes
+        // the high halves of the neighbour's and their own: row 2r's elements, then row 2r + 1's
+#pragma unroll
+        for (int r = 0; r < P::VL; ++r) {
+          const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v[r][0], 0xB1, 0xF, 0xF, true);
+          v[r][0] = __builtin_amdgcn_perm(other, v[r][0], halves);
+        }
+      }
+      auto add = [&](auto w) {
+        constexpr int W = decltype(w)::value;
+        bf16x8 even, odd;
+        v_pair<D, BITS, W>(even, odd, v, sc);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) oacc[c][2 * W] = mfma16(even, pb[c], oacc[c][2 * W]);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) oacc[c][2 * W + 1] = mfma16(odd, pb[c], oacc[c][2 * W + 1]);
+      };
+      add(std::integral_constant<int, 0>{});
+      add(std::integral_constant<int, 1>{});
+      if constexpr (D == 128) {
+        add(std::integral_constant<int, 2>{});
+        add(std::integral_constant<int, 3>{});
+      }
+    };
+#pragma unroll 1
+    for (int blk = blk0; blk < nb; blk += step) {
+      const int k0 = blk * kMxBlock, kn = k0 + step * kMxBlock;
+      uint32_t ks[4];
+      spread_rows(ks, sc.k);
+      const uint32_t vs = sc.v;
+      sc = load_scales(src, off, kn, L);
+      attend(std::integral_constant<int, 0>{}, x[0], ks, vs, k0);
+      __builtin_amdgcn_sched_barrier(0);
+      load_codes(x[0], src, off, kn, L);
+      __builtin_amdgcn_sched_barrier(0);
+      if (k0 + 32 < L) attend(std::integral_constant<int, 1>{}, x[1], ks, vs, k0 + 32);
+      __builtin_amdgcn_sched_barrier(0);
+      load_codes(x[1], src, off, kn + 32, L);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
@@ -344,9 +513,9 @@ __global__ __launch_bounds__(64 * NW) void fa_decode_mx_kernel(
   for (int c = 0; c < NC; ++c) {
     const float l = quarters_sum(l_part[c]);
     if (q4 == 0) {
-      // A wave without visible keys (l exactly 0) weighs nothing.  A NaN sum is no empty one: its
-      // max may still be -inf (no score compares greater), and then the sum is relative to 0.
-      wm[wave][16 * c + i16] = l == 0.f ? -INFINITY : m_t[c] == -INFINITY ? 0.f : m_t[c];
+      // A wave without visible keys (l exactly 0) weighs nothing; the NaN of one that saw a NaN score
+      // goes on through the maximum and the weights.
+      wm[wave][16 * c + i16] = l == 0.f ? -INFINITY : l == l ? m_t[c] : l;
       wsum[wave][16 * c + i16] = l;
     }
   }
@@ -354,6 +523,7 @@ __global__ __launch_bounds__(64 * NW) void fa_decode_mx_kernel(
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int col = 16 * c + i16, cols = min(R - 16 * c, 16);  // cols > 0: R > 16 where NC is 2
+    const int rows = min(R, 16);
     if (c) __syncthreads();  // the first tile's rows are read
     float M = wm[0][col];
 #pragma unroll
@@ -366,7 +536,7 @@ __global__ __launch_bounds__(64 * NW) void fa_decode_mx_kernel(
 #pragma unroll
         for (int n = 0; n < DT; n += 4) {
           const int ch = (DT * (4 * q4 + r) + n) / 4;
-          *reinterpret_cast<f32x4 *>(&stage[wave][i16 * D + ((ch ^ (i16 & 7)) << 2)]) =
+          *reinterpret_cast<f32x4 *>(&stage[(wave * rows + i16) * D + ((ch ^ (i16 & 7)) << 2)]) =
               alpha != 0.f ? f32x4{oacc[c][n][r] * alpha, oacc[c][n + 1][r] * alpha,
                                    oacc[c][n + 2][r] * alpha, oacc[c][n + 3][r] * alpha}
                            : f32x4{};
@@ -381,7 +551,7 @@ __global__ __launch_bounds__(64 * NW) void fa_decode_mx_kernel(
       for (int w = 1; w < NW; ++w) mx = fmax2(mx, wm[w][k]);
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        t += *reinterpret_cast<const f32x4 *>(&stage[w][j * D + ((ch ^ (j & 7)) << 2)]);
+        t += *reinterpret_cast<const f32x4 *>(&stage[(w * rows + j) * D + ((ch ^ (j & 7)) << 2)]);
         ls += wm[w][k] == -INFINITY ? 0.f : wsum[w][k] * exp2f_fast(wm[w][k] - mx);
       }
       const int g = k / Tq;
@@ -400,55 +570,144 @@ __global__ __launch_bounds__(64 * NW) void fa_decode_mx_kernel(
   }
 }
 
-// Workgroups per unit, waves per workgroup, and the blocks a workgroup takes at least (see
-// decode_split).
-DecodeSplit decode_mx_split(int B, int Hkv, int Lmax, int D, int bits) {
+// Merge of up to kMxMerged partials per query row (fa_decode_combine_kernel's rule), a wave per row: lane c
+// sums D / 64 columns over the partials in order, all of whose loads go out at once.
+template <int D>
+__global__ __launch_bounds__(256) void fa_decode_mx_merge_kernel(const float *__restrict__ part_o,
+                                                                 const float *__restrict__ part_ml,
+                                                                 bf16 *__restrict__ O,
+                                                                 float *__restrict__ LSE, int rows,
+                                                                 int n_splits) {
+  typedef float vec __attribute__((ext_vector_type(D / 64)));
+  const int row = blockIdx.x * 4 + wave_id(), lane = threadIdx.x & 63;
+  if (row >= rows) return;
+  const f32x2 *ml = reinterpret_cast<const f32x2 *>(part_ml) + (int64_t)row * n_splits;
+  const vec *po = reinterpret_cast<const vec *>(part_o + (int64_t)row * n_splits * D) + lane;
+  const f32x2 mine = lane < n_splits ? ml[lane] : f32x2{-INFINITY, 0.f};
+  vec x[kMxMerged];
+#pragma unroll
+  for (int s = 0; s < kMxMerged; ++s)
+    if (s < n_splits) x[s] = po[s * 64];
+  float M = mine[1] != 0.f ? mine[0] : -INFINITY;
+#pragma unroll
+  for (int m = 1; m < kMxMerged; m <<= 1) M = fmax2(M, __shfl_xor(M, m));
+  M = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(M)));
+  const float w = mine[1] != 0.f ? exp2f_fast(mine[0] - M) : 0.f;
+  float sum = w * mine[1];
+#pragma unroll
+  for (int m = 1; m < kMxMerged; m <<= 1) sum += __shfl_xor(sum, m);
+  sum = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(sum)));
+  vec acc{};
+#pragma unroll
+  for (int s = 0; s < kMxMerged; ++s) {
+    const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), s));
+    // an unused chunk wrote no O
+    if (s < n_splits && ws != 0.f) {
+#pragma unroll
+      for (int e = 0; e < D / 64; ++e) acc[e] = __builtin_fmaf(x[s][e], ws, acc[e]);
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e) O[(int64_t)row * D + lane * (D / 64) + e] = (bf16)(acc[e] * inv);
+  if (lane == 0) LSE[row] = sum == 0.f ? -INFINITY : (M + __log2f(sum)) * kLn2;
+}
+
+// Workgroups per unit, waves per workgroup, and the blocks a workgroup takes at least.  Times in us
+// back to back, D 128 and 4 bits unless said; "uneven" is lengths from a tenth of the capacity up.
+//  * One chunk, and one launch, up to 512 keys (512 keys, 2 heads: 6.1; two launches 7.6).
+//  * Otherwise as many as stay within 256 workgroups, one per CU (96 units of 3000 keys: 2 chunks 14.7, 1
+//    15.8, 3 17.0; 160 units: 1 17.2, 3 18.7; 256 of 4096: 1 27.4, 2 31.1; 8 units of 16384: 32 chunks 10.8, 16 12.4, 64 12.2; of 131072:
+//    30.9, 43.0, 32.4; 48 units of 3000: 5 chunks 11.4, 2 14.1, 11 13.7), of at least a block per wave.
+//    More than kMxMerged chunks need the slower merge, which pays from 32768 elements a chunk (8 units
+//    of 8192: 32 chunks 9.1, 16 9.7; 12 units of 8000, D 64: 9.7, 8.1).
+//  * A long cache among short ones: with several sequences and a capacity over 4096, chunks of about
+//    2048 keys, up to 4096 workgroups (16 caches of 8 heads, one of 16384, the others of 300: 8 chunks
+//    19.2, 2 38.6; full and uneven calls lose nothing: 64 x 8 of up to 16384: 8 chunks 130, 1 133).
+//  * Waves of a one-chunk call: eight for 129 to 447 units, whose four-wave workgroups leave CUs
+//    unevenly filled (uneven caches: 320 units 19.5 against 21.3, 384 of 8 bits 34.5 against 39.9; full ones
+//    34.3 against 32.0), else four (448 units: 24.2 and 23.8, full 35.7 against 37.6; 1024: 25.7, 31.9).
+//  * A chunk's least is its share of a full cache, so that short caches cost one workgroup each; with up
+//    to 32 units, which leave the device idle, a block for every wave.
+DecodeSplit decode_mx_split(int B, int Hkv, int Lmax, int D) {
   const int64_t units = (int64_t)B * Hkv;
   const int64_t blocks = ((int64_t)Lmax + kMxBlock - 1) / kMxBlock;
-  if (blocks <= 16) return {4, 1, 0};
-  int64_t n = 1024 / units;
-  if (n < 1) n = 1;
-  const int64_t most = (blocks + 3) / 4;
-  n = n > most ? most : n > 512 ? 512 : n;
+  if (blocks <= 8) return {4, 1, 0};
+  int64_t n = std::max<int64_t>(256 / units, 1);
+  if (n > kMxMerged && (int64_t)Lmax * D < n * 32768) n = kMxMerged;
+  if (B > 1 && Lmax > 4096) {
+    const int64_t even = std::min(blocks / 32, 4096 / units);  // chunks of 2048 keys
+    n = std::max(n, even);
+  }
+  n = std::min(n, (blocks + 3) / 4);
+  n = std::min<int64_t>(n, 512);
+  if (n <= 1) return {units > 128 && units < 448 ? 8 : 4, 1, 0};
   const int64_t least = units <= 32 ? 4 : (blocks + n - 1) / n;
   int log2_min = 0;
   while (least >> (log2_min + 1)) ++log2_min;
   return {4, (int)n, log2_min};
 }
 
-template <int D, int BITS, int NC>
-static hipError_t launch_shape(const void *q, const KvCache &cache, const int *cache_seqlens, void *o,
-                               float *lse, float *workspace, int B, int Hq, int Hkv, int Tq, int Lmax,
-                               const DecodeSplit &sp, float scale_log2, hipStream_t stream) {
-  const int rows = B * Hq * Tq;
-  float *part_o = workspace, *part_ml = workspace + (int64_t)rows * sp.n_chunks * D;
-  const dim3 grid((unsigned)((int64_t)B * Hkv), (unsigned)sp.n_chunks), block(256);
-  auto go = [&](auto kernel) {
-    kernel<<<grid, block, 0, stream>>>((const bf16 *)q, cache, cache_seqlens, (bf16 *)o, lse, part_o,
-                                       part_ml, B, Hq, Hkv, Tq, Lmax, sp.n_chunks, sp.log2_min,
-                                       scale_log2);
-    return hipGetLastError();
-  };
-  if (sp.n_chunks == 1) return go(fa_decode_mx_kernel<D, BITS, 4, NC, false>);
-  const hipError_t e = go(fa_decode_mx_kernel<D, BITS, 4, NC, true>);
-  return e != hipSuccess ? e : launch_decode_combine(part_o, part_ml, o, lse, rows, sp.n_chunks, D, stream);
+namespace {
+
+struct MxCall {
+  const bf16 *q;
+  KvCache cache;
+  const int *cache_seqlens;
+  bf16 *o;
+  float *lse, *workspace;
+  int B, Hq, Hkv, Tq, Lmax;
+  DecodeSplit sp;
+  float scale_log2;
+  hipStream_t stream;
+};
+
+template <int D, int BITS, int NW, int NC, bool SPLIT>
+hipError_t launch_waves(const MxCall &a) {
+  const int rows = a.B * a.Hq * a.Tq, cols = a.Hq / a.Hkv * a.Tq, n = a.sp.n_chunks;
+  float *part_o = a.workspace, *part_ml = a.workspace + (int64_t)rows * n * D;
+  constexpr size_t most = NW * 16 * D * sizeof(float);
+  const size_t lds = most * (cols < 16 ? cols : 16) / 16;
+  // the kernel's static arrays come on top of the dynamic stages
+  if (lds + 2 * NW * 16 * NC * sizeof(float) > 65536) {
+    hipError_t e = allow_lds<fa_decode_mx_kernel<D, BITS, NW, NC, SPLIT>>(most);
+    if (e != hipSuccess) return e;
+  }
+  const dim3 grid((unsigned)((int64_t)a.B * a.Hkv), (unsigned)n), block(64 * NW);
+  fa_decode_mx_kernel<D, BITS, NW, NC, SPLIT><<<grid, block, lds, a.stream>>>(
+      a.q, a.cache, a.cache_seqlens, a.o, a.lse, part_o, part_ml, a.B, a.Hq, a.Hkv, a.Tq, a.Lmax, n,
+      a.sp.log2_min, a.scale_log2);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !SPLIT) return e;
+  if (n > kMxMerged) return launch_decode_combine(part_o, part_ml, a.o, a.lse, rows, n, D, a.stream);
+  fa_decode_mx_merge_kernel<D><<<dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, a.stream>>>(
+      part_o, part_ml, a.o, a.lse, rows, n);
+  return hipGetLastError();
 }
+
+template <int D, int BITS, int NC>
+hipError_t launch_shape(const MxCall &a) {
+  if (a.sp.n_chunks > 1) {
+    return launch_waves<D, BITS, 4, NC, true>(a);
+  }
+  if (a.sp.n_waves == 8) return launch_waves<D, BITS, 8, NC, false>(a);
+  return launch_waves<D, BITS, 4, NC, false>(a);
+}
+
+}  // namespace
 
 hipError_t launch_decode_mx(const void *q, const KvCache &cache, const int *cache_seqlens, void *o,
                             float *lse, float *workspace, int B, int Hq, int Hkv, int Tq, int Lmax,
                             int D, int bits, float scale, hipStream_t stream) {
-  const DecodeSplit sp = decode_mx_split(B, Hkv, Lmax, D, bits);
-  auto go = [&](auto launch) {
-    return launch(q, cache, cache_seqlens, o, lse, workspace, B, Hq, Hkv, Tq, Lmax, sp,
-                  scale * kLog2e, stream);
-  };
+  const MxCall a{(const bf16 *)q, cache, cache_seqlens, (bf16 *)o, lse, workspace, B, Hq, Hkv, Tq,
+                 Lmax, decode_mx_split(B, Hkv, Lmax, D), scale * kLog2e, stream};
   const bool wide = Hq / Hkv * Tq > 16;
   if (D == 64) {
-    if (bits == 4) return wide ? go(launch_shape<64, 4, 2>) : go(launch_shape<64, 4, 1>);
-    return wide ? go(launch_shape<64, 8, 2>) : go(launch_shape<64, 8, 1>);
+    if (bits == 4) return wide ? launch_shape<64, 4, 2>(a) : launch_shape<64, 4, 1>(a);
+    return wide ? launch_shape<64, 8, 2>(a) : launch_shape<64, 8, 1>(a);
   }
-  if (bits == 4) return wide ? go(launch_shape<128, 4, 2>) : go(launch_shape<128, 4, 1>);
-  return wide ? go(launch_shape<128, 8, 2>) : go(launch_shape<128, 8, 1>);
+  if (bits == 4) return wide ? launch_shape<128, 4, 2>(a) : launch_shape<128, 4, 1>(a);
+  return wide ? launch_shape<128, 8, 2>(a) : launch_shape<128, 8, 1>(a);
 }
 
 }  // namespace ttfa

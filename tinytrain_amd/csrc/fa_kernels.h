@@ -87,7 +87,7 @@ hipError_t launch_kv_read(const KvCache &cache, const int *cache_seqlens, void *
                           hipStream_t stream);
 
 // launch_decode_bf16 over a quantised cache; workspace of B * Hq * Tq * n_chunks * (D + 2) floats.
-DecodeSplit decode_mx_split(int B, int Hkv, int Lmax, int D, int bits);
+DecodeSplit decode_mx_split(int B, int Hkv, int Lmax, int D);
 hipError_t launch_decode_mx(const void *q, const KvCache &cache, const int *cache_seqlens, void *o,
                             float *lse, float *workspace, int B, int Hq, int Hkv, int Tq, int Lmax,
                             int D, int bits, float scale, hipStream_t stream);

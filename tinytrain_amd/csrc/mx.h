@@ -30,12 +30,13 @@ __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t top) {
 
 // Elements 2i, 2i + 1 of eight, divided by `scale` (a power of two) and rounded to nearest even,
 // into their place among the codes c.  The e2m1 conversion saturates; the e4m3 one gives NaN past
-// 464, which only a clamped scale (magnitudes of 2^127 and more) can leave: hence the clamp to the
-// largest value 448 * 2^119.
+// 464, which only a clamped scale (magnitudes of 2^127 and more) can leave: hence the clamp to
+// `most`, at first the largest value 448 * 2^119.
 constexpr float kMx8Top = 448.0f * 0x1p119f;
 
 template <int BITS>
-__device__ __forceinline__ u32x2 mx_pack(u32x2 c, int i, f32x2 x, float scale) {
+__device__ __forceinline__ u32x2 mx_pack(u32x2 c, int i, f32x2 x, float scale,
+                                           float most = kMx8Top) {
   if constexpr (BITS == 4) {
     uint32_t w = c[0];
     switch (i) {
@@ -46,8 +47,8 @@ __device__ __forceinline__ u32x2 mx_pack(u32x2 c, int i, f32x2 x, float scale) {
     }
     c[0] = w;
   } else {
-    const float a = __builtin_amdgcn_fmed3f(x[0], -kMx8Top, kMx8Top);
-    const float b = __builtin_amdgcn_fmed3f(x[1], -kMx8Top, kMx8Top);
+    const float a = __builtin_amdgcn_fmed3f(x[0], -most, most);
+    const float b = __builtin_amdgcn_fmed3f(x[1], -most, most);
     const uint32_t old = c[i >> 1];  // a copy: __builtin_bit_cast of a vector's element reads element 0
     s16x2 w = __builtin_bit_cast(s16x2, old);
     w = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, a, b, scale, 1)

@@ -306,7 +306,7 @@ int ttfa_kv_read(const void *k_codes, const void *k_scales, const void *v_codes,
 long long ttfa_decode_mx_workspace_bytes(int B, int Hq, int Hkv, int Tq, int max_seqlen, int D,
                                          int bits) {
   if (check_decode_mx(B, Hq, Hkv, Tq, max_seqlen, D, bits, TTFA_BF16, 1.f)) return -1;
-  const ttfa::DecodeSplit sp = ttfa::decode_mx_split(B, Hkv, max_seqlen, D, bits);
+  const ttfa::DecodeSplit sp = ttfa::decode_mx_split(B, Hkv, max_seqlen, D);
   return (long long)B * Hq * Tq * sp.n_chunks * (D + 2) * (long long)sizeof(float);
 }
 
