@@ -81,62 +81,107 @@ struct Eight<float> {
 
 }  // namespace
 
-// A lane takes eight elements, D / 8 lanes a row; blockIdx.y picks K or V.  Row t of T goes to
-// position cache_seqlens[b] - T + t; one outside the cache is not written.
-template <int D, int BITS, class T>
+namespace {
+
+// Rows moved by a call, numbered (b, h, t): b * Hkv + h and t by a multiplication with the divisor's
+// reciprocal, rounded up at 2^(31 + bits of the divisor): exact for dividends below 2^31.
+struct Divisor {
+  uint32_t n, mul, shift;
+  explicit Divisor(int d) : n((uint32_t)d), shift(0) {
+    while ((1u << shift) < n) ++shift;
+    mul = (uint32_t)((((uint64_t)1 << (31 + shift)) + n - 1) / n);
+  }
+  __device__ __forceinline__ uint32_t quotient(uint32_t x) const {
+    return (uint32_t)(((uint64_t)x * mul) >> 31) >> shift;
+  }
+};
+
+}  // namespace
+
+// A lane takes eight elements, D / 8 lanes a row, U rows of a lane at once; blockIdx.y picks K or V.
+// Row t of T goes to position cache_seqlens[b] - T + t; one outside the cache is not written.
+// Bound by memory: 16 x 8 rows of up to 4000, D 128, bf16 to 4 bits 51 us (copy rate: 45).
+template <int D, int BITS, class T, int U>
 __global__ __launch_bounds__(256) void kv_append_mx_kernel(KvRows<T> in, KvCache cache,
                                                            const int *__restrict__ cache_seqlens,
-                                                           int rows, int Hkv, int n_rows, int Lmax) {
-  constexpr int LPR = D / 8, CODE = D * BITS / 8;
+                                                           int rows, Divisor heads, Divisor per_head,
+                                                           int Lmax) {
+  constexpr int LPR = D / 8, CODE = D * BITS / 8, STEP = 256 / LPR;
   const int which = blockIdx.y;
-  const int row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR, ln = threadIdx.x % LPR;
-  if (row >= rows) return;  // whole rows, so whole groups of lanes
-  const int bh = row / n_rows, t = row - bh * n_rows;
-  const int b = bh / Hkv, h = bh - b * Hkv;
-  const int64_t pos = (int64_t)cache_seqlens[b] - n_rows + t;
-  if (pos < 0 || pos >= Lmax) return;
+  const int row0 = blockIdx.x * (STEP * U) + threadIdx.x / LPR, ln = threadIdx.x % LPR;
   const int64_t *st = in.stride[which];
-  Eight<T> x;
-  x.load(in.x[which] + b * st[0] + h * st[1] + t * st[2] + 8 * ln);
-  const uint32_t byte = mx_scale_byte<BITS>(quad_max(x.top()));
-  u32x2 c = x.template codes<BITS>(__uint_as_float(byte << 23));
-  if (byte == 255) c = u32x2{};
-  const int64_t at = (int64_t)bh * Lmax + pos;
-  uint8_t *out = cache.codes[which] + at * CODE;
-  if constexpr (BITS == 4) reinterpret_cast<uint32_t *>(out)[ln] = c[0];
-  else reinterpret_cast<u32x2 *>(out)[ln] = c;
-  if (ln % 4 == 0) cache.scales[which][at * (D / 32) + ln / 4] = (uint8_t)byte;
+  Eight<T> x[U];
+  int64_t at[U];  // position in the cache, over all heads; -1: not written
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t row = row0 + u * STEP;
+    at[u] = -1;
+    if (row < (uint32_t)rows) {  // whole rows, so whole groups of lanes
+      const uint32_t bh = per_head.quotient(row), t = row - bh * per_head.n;
+      const uint32_t b = heads.quotient(bh), h = bh - b * heads.n;
+      const int64_t pos = (int64_t)cache_seqlens[b] - per_head.n + t;
+      if (pos >= 0 && pos < Lmax) {
+        at[u] = (int64_t)bh * Lmax + pos;
+        x[u].load(in.x[which] + b * st[0] + h * st[1] + t * st[2] + 8 * ln);
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (at[u] < 0) continue;
+    const uint32_t byte = mx_scale_byte<BITS>(quad_max(x[u].top()));
+    u32x2 c = x[u].template codes<BITS>(__uint_as_float(byte << 23));
+    if (byte == 255) c = u32x2{};
+    uint8_t *out = cache.codes[which] + at[u] * CODE;
+    if constexpr (BITS == 4) reinterpret_cast<uint32_t *>(out)[ln] = c[0];
+    else reinterpret_cast<u32x2 *>(out)[ln] = c;
+    if (ln % 4 == 0) cache.scales[which][at[u] * (D / 32) + ln / 4] = (uint8_t)byte;
+  }
 }
 
 // The inverse: row t of n_rows comes from position cache_seqlens[b] - n_rows + t, zeros where that
-// lies outside the cache.
-template <int D, int BITS, class T>
+// lies outside the cache.  A lane writes 16 bytes, so that every store instruction writes whole lines, past
+// the L2 (the rows are read by another kernel, mostly after more of them than it holds): 16 x 8 x 4000
+// rows of D 128 in 4 bits 60 us, through the L2 76 (copy rate: 63).
+template <int D, int BITS, class T, int U>
 __global__ __launch_bounds__(256) void kv_read_mx_kernel(KvCache cache,
                                                          const int *__restrict__ cache_seqlens,
                                                          T *__restrict__ k, T *__restrict__ v, int rows,
-                                                         int Hkv, int n_rows, int Lmax) {
-  constexpr int LPR = D / 8, CODE = D * BITS / 8;
+                                                         Divisor heads, Divisor per_head, int Lmax) {
+  constexpr int E = 16 / sizeof(T), LPR = D / E, CODE = D * BITS / 8, STEP = 256 / LPR;
+  constexpr int BYTES = E * BITS / 8;  // of a lane's codes: 2, 4 or 8
   const int which = blockIdx.y;
-  const int row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR, ln = threadIdx.x % LPR;
-  if (row >= rows) return;
-  const int bh = row / n_rows, t = row - bh * n_rows;
-  const int64_t pos = (int64_t)cache_seqlens[bh / Hkv] - n_rows + t;
-  u32x2 c{};
-  uint32_t byte = 0;
-  if (pos >= 0 && pos < Lmax) {
-    const int64_t at = (int64_t)bh * Lmax + pos;
-    const uint8_t *src = cache.codes[which] + at * CODE;
-    if constexpr (BITS == 4) c[0] = reinterpret_cast<const uint32_t *>(src)[ln];
-    else c = reinterpret_cast<const u32x2 *>(src)[ln];
-    byte = cache.scales[which][at * (D / 32) + ln / 4];
+  const int row0 = blockIdx.x * (STEP * U) + threadIdx.x / LPR, ln = threadIdx.x % LPR;
+  u32x2 c[U];
+  uint32_t byte[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t row = row0 + u * STEP;
+    c[u] = u32x2{};
+    byte[u] = 0;
+    if (row < (uint32_t)rows) {
+      const uint32_t bh = per_head.quotient(row), t = row - bh * per_head.n;
+      const int64_t pos = (int64_t)cache_seqlens[heads.quotient(bh)] - per_head.n + t;
+      if (pos >= 0 && pos < Lmax) {
+        const int64_t at = (int64_t)bh * Lmax + pos;
+        const uint8_t *src = cache.codes[which] + at * CODE;
+        if constexpr (BYTES == 2) c[u][0] = reinterpret_cast<const uint16_t *>(src)[ln];
+        else if constexpr (BYTES == 4) c[u][0] = reinterpret_cast<const uint32_t *>(src)[ln];
+        else c[u] = reinterpret_cast<const u32x2 *>(src)[ln];
+        byte[u] = cache.scales[which][at * (D / 32) + ln * E / 32];
+      }
+    }
   }
-  const float scale = __uint_as_float(byte << 23);
-  T *out = (which ? v : k) + (int64_t)row * D + 8 * ln;
-  if constexpr (sizeof(T) == 2) {
-    *reinterpret_cast<bf16x8 *>(out) = mx_values8<BITS>(c, scale);
-  } else {
-    reinterpret_cast<f32x4 *>(out)[0] = mx_values4_f32<BITS>(c, 0, scale);
-    reinterpret_cast<f32x4 *>(out)[1] = mx_values4_f32<BITS>(c, 1, scale);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int row = row0 + u * STEP;
+    if (row >= rows) continue;
+    const float scale = __uint_as_float(byte[u] << 23);
+    T *out = (which ? v : k) + (int64_t)row * D + E * ln;
+    if constexpr (sizeof(T) == 2)
+      __builtin_nontemporal_store(mx_values8<BITS>(c[u], scale), reinterpret_cast<bf16x8 *>(out));
+    else
+      __builtin_nontemporal_store(mx_values4_f32<BITS>(c[u], 0, scale), reinterpret_cast<f32x4 *>(out));
   }
 }
 
@@ -155,6 +200,23 @@ hipError_t kv_dispatch(int D, int bits, bool f32, F f) {
   return D == 64 ? by_bits(integral_constant<int, 64>{}) : by_bits(integral_constant<int, 128>{});
 }
 
+// f(rows of a lane at once, grid) for `rows` rows of `lanes` lanes each.  Two rows at once keep more
+// loads on the way, which pays for 2^24 elements or more whose lanes load little each (TWO: appends of
+// bf16 81.7 -> 74.0 us at 16 x 8 x 4000 rows of D 128 in 8 bits, reads of 8 bits 74.4 -> 66.1; appends of
+// fp32 lose, 28.2 -> 29.5 at 2 x 8 x 8192, and reads of 4 bits, 19.6 -> 21.3 at 8 x 16384; so do small calls,
+// which leave CUs idle, 2.5 -> 2.8 at 32 x 8 rows).
+template <bool TWO, class F>
+hipError_t kv_launch(int rows, int lanes, F f) {
+  auto go = [&](auto u) {
+    const int64_t per = 256 / lanes * decltype(u)::value;
+    f(u, dim3((unsigned)((rows + per - 1) / per), 2));
+    return hipGetLastError();
+  };
+  if constexpr (TWO)
+    if ((int64_t)rows * lanes >= 1 << 21) return go(std::integral_constant<int, 2>{});
+  return go(std::integral_constant<int, 1>{});
+}
+
 }  // namespace
 
 hipError_t launch_kv_append(const void *k, const void *v, const int64_t (&stride)[2][3],
@@ -166,10 +228,10 @@ hipError_t launch_kv_append(const void *k, const void *v, const int64_t (&stride
     constexpr int kD = decltype(d)::value, kBits = decltype(b)::value;
     KvRows<T> in{{(const T *)k, (const T *)v}, {}};
     for (int i = 0; i < 6; ++i) in.stride[i / 3][i % 3] = stride[i / 3][i % 3];
-    const dim3 grid((unsigned)(((int64_t)rows * (kD / 8) + 255) / 256), 2);
-    kv_append_mx_kernel<kD, kBits, T><<<grid, dim3(256), 0, stream>>>(in, cache, cache_seqlens, rows,
-                                                                     Hkv, n_rows, Lmax);
-    return hipGetLastError();
+    return kv_launch<sizeof(T) == 2>(rows, kD / 8, [&](auto u, dim3 grid) {
+      kv_append_mx_kernel<kD, kBits, T, decltype(u)::value><<<grid, dim3(256), 0, stream>>>(
+          in, cache, cache_seqlens, rows, Divisor(Hkv), Divisor(n_rows), Lmax);
+    });
   });
 }
 
@@ -180,10 +242,10 @@ hipError_t launch_kv_read(const KvCache &cache, const int *cache_seqlens, void *
   return kv_dispatch(D, bits, f32, [&](auto d, auto b, auto t) {
     using T = decltype(t);
     constexpr int kD = decltype(d)::value, kBits = decltype(b)::value;
-    const dim3 grid((unsigned)(((int64_t)rows * (kD / 8) + 255) / 256), 2);
-    kv_read_mx_kernel<kD, kBits, T><<<grid, dim3(256), 0, stream>>>(cache, cache_seqlens, (T *)k, (T *)v,
-                                                                   rows, Hkv, n_rows, Lmax);
-    return hipGetLastError();
+    return kv_launch<kBits == 8>(rows, kD * (int)sizeof(T) / 16, [&](auto u, dim3 grid) {
+      kv_read_mx_kernel<kD, kBits, T, decltype(u)::value><<<grid, dim3(256), 0, stream>>>(
+          cache, cache_seqlens, (T *)k, (T *)v, rows, Divisor(Hkv), Divisor(n_rows), Lmax);
+    });
   });
 }
 
