@@ -251,7 +251,8 @@ int ttfa_decode_fwd(const void *q, const void *k_cache, const void *v_cache,
  * every value exactly.
  *
  * ttfa_decode_mx_fwd is ttfa_decode_fwd (arguments, results, workspace rules) on the values that the
- * cache stands for; q and o are bf16.
+ * cache stands for; q and o are bf16.  Where ttfa_decode_mx_workspace_bytes gives 0 (calls of one
+ * launch) the workspace is not used and may be NULL.
  *
  * Supported: bits 4 or 8 (TTFA_E_BITS), D in {64, 128}, dtype TTFA_BF16 or TTFA_F32 for the rows;
  * pointers non-null and 16-byte aligned.  One launch each; decode one or two.

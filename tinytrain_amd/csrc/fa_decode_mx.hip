@@ -71,10 +71,14 @@ struct MxShape {
 //  * V: D / 16 elements of each of the rows q + 4e; those 2 bytes of e2m1 at D = 64 come as words,
 //    an even lane's from row e = 2r, an odd lane's from row 2r + 1, and neighbours exchange halves.
 template <int D, int BITS>
-struct MxCodes {
+struct MxK {
   using P = MxShape<D, BITS>;
-  uint32_t k[P::KL][P::KW];
-  uint32_t v[P::VL][P::VW];
+  uint32_t x[P::KL][P::KW];
+};
+template <int D, int BITS>
+struct MxV {
+  using P = MxShape<D, BITS>;
+  uint32_t x[P::VL][P::VW];
 };
 
 // Scale bytes of a block: of K row q' + 4 r' + 16 q (tile q of the block's four) and of V row
@@ -109,27 +113,32 @@ struct MxSrc {  // one (batch, KV head) of the cache
 
 // Loads of rows past `end` read nothing and give zeros (codes 0 of scale 2^-127: exact zeros).
 template <int D, int BITS>
-__device__ __forceinline__ void load_codes(MxCodes<D, BITS> &x, const MxSrc &s,
-                                           const MxLane<D, BITS> &o, int k0, int end) {
+__device__ __forceinline__ void load_k(MxK<D, BITS> &k, const MxSrc &s, const MxLane<D, BITS> &o,
+                                       int k0, int end) {
   using P = MxShape<D, BITS>;
-  const uint32_t bytes = (uint32_t)max(end - k0, 0) * P::CODE;
-  const auto kc = make_rsrc(s.kc + (int64_t)k0 * P::CODE, bytes);
-  const auto vc = make_rsrc(s.vc + (int64_t)k0 * P::CODE, bytes);
+  const auto kc = make_rsrc(s.kc + (int64_t)k0 * P::CODE, (uint32_t)max(end - k0, 0) * P::CODE);
 #pragma unroll
   for (int t = 0; t < P::KL; ++t)
 #pragma unroll
     for (int c = 0; c < P::KW / 4; ++c) {  // e4m3, D = 128: elements 16q .. and 64 + 16q ..
       const u32x4 w = buf_load16(kc, o.k + 16 * t * P::CODE + 64 * c);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x.k[t][4 * c + e] = w[e];
+      for (int e = 0; e < 4; ++e) k.x[t][4 * c + e] = w[e];
     }
+}
+
+template <int D, int BITS>
+__device__ __forceinline__ void load_v(MxV<D, BITS> &v, const MxSrc &s, const MxLane<D, BITS> &o,
+                                       int k0, int end) {
+  using P = MxShape<D, BITS>;
+  const auto vc = make_rsrc(s.vc + (int64_t)k0 * P::CODE, (uint32_t)max(end - k0, 0) * P::CODE);
 #pragma unroll
   for (int r = 0; r < P::VL; ++r) {
     const uint32_t at = o.v + (32 / P::VL) * r * P::CODE;
-    if constexpr (P::VW == 1) x.v[r][0] = buf_load4(vc, at);
+    if constexpr (P::VW == 1) v.x[r][0] = buf_load4(vc, at);
     else {
       const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(vc, at, 0, 0);
-      x.v[r][0] = w[0], x.v[r][1] = w[1];
+      v.x[r][0] = w[0], v.x[r][1] = w[1];
     }
   }
 }
@@ -186,10 +195,33 @@ __device__ __forceinline__ bf16x8 take_out_nans(uint32_t (&sc)[8]) {
   return mark;
 }
 
+// The words v_pair takes.  PAIRED: even lanes take the low halves of their own row's word and their
+// neighbour's, odd lanes the high halves of the neighbour's and their own: row 2r's elements, then
+// row 2r + 1's.
+template <int D, int BITS>
+__device__ __forceinline__ MxV<D, BITS> v_words(const MxV<D, BITS> &v, int lane) {
+  using P = MxShape<D, BITS>;
+  MxV<D, BITS> out;
+  // bytes of (neighbour's word, own word) = bytes (7..4, 3..0)
+  const uint32_t halves = lane & 1 ? 0x03020706u : 0x05040100u;
+#pragma unroll
+  for (int r = 0; r < P::VL; ++r)
+#pragma unroll
+    for (int w = 0; w < P::VW; ++w) {
+      const uint32_t own = v.x[r][w];
+      if constexpr (P::PAIRED) {
+        const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)own, 0xB1, 0xF, 0xF, true);
+        out.x[r][w] = __builtin_amdgcn_perm(other, own, halves);
+      } else {
+        out.x[r][w] = own;
+      }
+    }
+  return out;
+}
+
 // A operands of output tiles 2W and 2W + 1: slot r = V[key q + 4r][d = DT * i + 2W, + 1]
 template <int D, int BITS, int W>
-__device__ __forceinline__ void v_pair(bf16x8 &even, bf16x8 &odd,
-                                       const uint32_t (&v)[MxShape<D, BITS>::VL][MxShape<D, BITS>::VW],
+__device__ __forceinline__ void v_pair(bf16x8 &even, bf16x8 &odd, const MxV<D, BITS> &v,
                                        const uint32_t (&sc)[8]) {
   using P = MxShape<D, BITS>;
 #pragma unroll
@@ -197,86 +229,117 @@ __device__ __forceinline__ void v_pair(bf16x8 &even, bf16x8 &odd,
     const float scale = __uint_as_float(sc[r]);
     bf16x2 y;
     if constexpr (P::PAIRED)
-      y = r & 1 ? mx_values2<4, W + 2>(v[r / 2][0], scale) : mx_values2<4, W>(v[r / 2][0], scale);
-    else if constexpr (BITS == 4) y = mx_values2<4, W>(v[r % P::VL][0], scale);
-    else y = mx_values2<8, W & 1>(v[r % P::VL][W >> 1], scale);
+      y = r & 1 ? mx_values2<4, W + 2>(v.x[r / 2][0], scale) : mx_values2<4, W>(v.x[r / 2][0], scale);
+    else if constexpr (BITS == 4) y = mx_values2<4, W>(v.x[r % P::VL][0], scale);
+    else y = mx_values2<8, W & 1>(v.x[r % P::VL][W >> 1], scale);
     even[r] = y[0], odd[r] = y[1];
   }
 }
 
-// One column's query row as a lane holds it: e4m3 terms hi and lo of its 32 elements (D = 64: 16 of
-// each), and the bytes of their powers of two.
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
+// The query rows of a workgroup in LDS: per row D bytes of hi, then D bytes of lo, in 16-byte pieces
+// whose place is turned by the row (a fragment read takes the same piece of 16 rows), and the bytes
+// of the rows' powers of two.
 template <int D>
-struct MxQuery {
-  i32x8 t[D == 128 ? 2 : 1];
-  int scale[D == 128 ? 2 : 1];
+__device__ __forceinline__ uint8_t *query_piece(uint8_t *rows, int row, int piece) {
+  return rows + row * 2 * D + ((piece ^ (row & (D / 8 - 1))) << 4);
+}
 
-  // The row's elements as they come: runs of 16 from 16 q and (D = 128) 64 + 16 q.
-  u32x4 raw[D / 32];
-
-  __device__ __forceinline__ void load(const bf16 *row, int q4) {
+// Splits the workgroup's query rows into e4m3 terms; a lane takes eight elements, N times.
+template <int D, int N>
+__device__ __forceinline__ void split_queries(const u32x4 (&q)[N], int n_rows, uint8_t *rows,
+                                              uint8_t *bytes, int threads) {
+  constexpr int LPR = D / 8;
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c)
-      raw[c] = *reinterpret_cast<const u32x4 *>(row + 64 * (c >> 1) + 16 * q4 + 8 * (c & 1));
-  }
-
-  __device__ __forceinline__ void split(int q4) {
+  for (int j = 0; j < N; ++j) {
+    const int at = threadIdx.x + j * threads;
+    if (at >= n_rows * LPR) break;  // whole rows, so whole groups of lanes
+    const u32x4 w = q[j];
     u16x2 m{};
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-        m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, raw[c][w] & 0x7fff7fffu));
+    for (int i = 0; i < 4; ++i)
+      m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
     uint32_t top = (uint32_t)max(m[0], m[1]) << 16;
-    auto p = __builtin_amdgcn_permlane16_swap(top, top, false, false);
-    top = max(p[0], p[1]);
-    p = __builtin_amdgcn_permlane32_swap(top, top, false, false);
-    top = max(p[0], p[1]);
-    const uint32_t byte = mx_scale_byte<8>(top);
-    const int b_lo = byte == 255 ? 255 : (int)byte - 4;  // NaN and infinity: the whole row is NaN
-    // x 2^-e is at most 464, or 511 next to the largest bf16, where hi is 448 and lo at most 63
-    const float inv = __uint_as_float((254 - min(byte, 253u)) << 23);
+    auto with = [&](auto dpp) {
+      top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, decltype(dpp)::value, 0xF, 0xF, true));
+    };
+    with(std::integral_constant<int, 0xB1>{});   // lane ^ 1
+    with(std::integral_constant<int, 0x4E>{});   // lane ^ 2
+    with(std::integral_constant<int, 0x141>{});  // mirrored in eight
+    if constexpr (LPR == 16) with(std::integral_constant<int, 0x140>{});  // in sixteen
+    // As mx_scale_byte<8>, not clamped above: no cache value has to hold these.
+    const int e = (int)((top + (0x7fffff - 0x680000)) >> 23) - 8;
+    const int byte = top >= 0x7f800000u ? 255 : max(e, 10);
+    const float inv = __uint_as_float((uint32_t)(254 - min(byte, 253)) << 23);
+    u32x2 hi{}, lo{};
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-      u32x2 hi{}, lo{};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t w = raw[c][e];
-        const f32x2 y{__uint_as_float(w << 16) * inv, __uint_as_float(w & 0xffff0000u) * inv};
-        hi = mx_pack<8>(hi, e, y, 1.f, 448.f);
-        const uint32_t code = hi[e >> 1];
-        const f32x2 h = e & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(code, 1.f, 1)
-                              : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(code, 1.f, 0);
-        lo = mx_pack<8>(lo, e, f32x2{y[0] - h[0], y[1] - h[1]}, 0x1p-4f, 28.f);
-      }
-      // D = 128: run c / 2 of both terms; D = 64: hi is run 0 and lo run 1 of one operand
-      if constexpr (D == 128) {
-        t[0][2 * c] = (int)hi[0], t[0][2 * c + 1] = (int)hi[1];
-        t[1][2 * c] = (int)lo[0], t[1][2 * c + 1] = (int)lo[1];
-      } else {
-        t[0][2 * c] = (int)hi[0], t[0][2 * c + 1] = (int)hi[1];
-        t[0][4 + 2 * c] = (int)lo[0], t[0][4 + 2 * c + 1] = (int)lo[1];
-      }
+    for (int i = 0; i < 4; ++i) {
+      const float y0 = __uint_as_float(w[i] << 16) * inv, y1 = __uint_as_float(w[i] & 0xffff0000u) * inv;
+      const uint32_t h_old = hi[i >> 1], l_old = lo[i >> 1];
+      const s16x2 h = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(__builtin_bit_cast(s16x2, h_old), y0, y1, 1.f, 1)
+                            : __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(__builtin_bit_cast(s16x2, h_old), y0, y1, 1.f, 0);
+      hi[i >> 1] = __builtin_bit_cast(uint32_t, h);
+      const uint32_t code = hi[i >> 1];
+      const f32x2 v = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(code, 1.f, 1)
+                            : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(code, 1.f, 0);
+      const s16x2 l = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(__builtin_bit_cast(s16x2, l_old), y0 - v[0], y1 - v[1], 0x1p-4f, 1)
+                            : __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(__builtin_bit_cast(s16x2, l_old), y0 - v[0], y1 - v[1], 0x1p-4f, 0);
+      lo[i >> 1] = __builtin_bit_cast(uint32_t, l);
     }
-    if constexpr (D == 128) scale[0] = (int)byte, scale[1] = b_lo;
-    else scale[0] = q4 < 2 ? (int)byte : b_lo;
+    const int row = at / LPR, part = at % LPR;
+    *reinterpret_cast<u32x2 *>(query_piece<D>(rows, row, part >> 1) + 8 * (part & 1)) = hi;
+    *reinterpret_cast<u32x2 *>(query_piece<D>(rows, row, D / 16 + (part >> 1)) + 8 * (part & 1)) = lo;
+    if (part == 0) bytes[row] = (uint8_t)byte;
+  }
+}
+
+// One column's query row as a lane holds it: the B operands (D = 64: hi and lo in one) and the bytes of
+// their powers of two.
+template <int D>
+struct MxQuery {
+  static constexpr int N = D / 64;
+  i32x8 t[N];
+  int scale[N];
+
+  __device__ __forceinline__ void read(uint8_t *rows, const uint8_t *bytes, int row, int q4) {
+    // D = 128: elements 16 q .. and 64 + 16 q .. of each term; D = 64: 16 q .. of both
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(query_piece<D>(rows, row, 8 * n + 4 * r + q4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[n][4 * r + e] = (int)w[e];
+      }
+    const int hi = bytes[row], lo = hi == 255 ? 255 : hi - 4;  // NaN and infinity: the whole row is NaN
+    if constexpr (D == 128) scale[0] = hi, scale[1] = lo;
+    else scale[0] = q4 < 2 ? hi : lo;
   }
 };
 
-// A operand of a K tile
+// A operands of a half's two K tiles
 template <int D, int BITS>
-__device__ __forceinline__ i32x8 k_operand(const uint32_t (&k)[MxShape<D, BITS>::KW]) {
-  i32x8 a{};
+__device__ __forceinline__ void k_operands(i32x8 (&a)[2], const MxK<D, BITS> &k) {
+  using P = MxShape<D, BITS>;
 #pragma unroll
-  for (int w = 0; w < MxShape<D, BITS>::KW; ++w) a[w] = (int)k[w];
-  if constexpr (D == 64 && BITS == 8) {
+  for (int t = 0; t < 2; ++t) {
+    a[t] = i32x8{};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) a[4 + w] = (int)k[w];
+    for (int w = 0; w < P::KW; ++w) a[t][w] = (int)k.x[t % P::KL][w];
+    if constexpr (D == 64 && BITS == 8) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) a[t][4 + w] = (int)k.x[t][w];
+    }
   }
-  return a;
+  if constexpr (P::PAIRED) {
+#pragma unroll
+    for (int w = 0; w < P::KW; ++w) {
+      const auto p = __builtin_amdgcn_permlane32_swap(k.x[0][w], k.x[0][w], false, false);
+      a[0][w] = (int)p[0], a[1][w] = (int)p[1];
+    }
+  }
 }
 
 // S^T tile of one column tile; `scale`: byte 0 is that of the row's group q (D = 64: q & 1)
@@ -300,52 +363,67 @@ __device__ __forceinline__ bool any_nan_scale(uint32_t bytes) {
 }  // namespace
 
 // Grid: (B * Hkv units, n_chunks), workgroups of NW waves; NC tiles of 16 query columns.  Partial rows
-// are indexed (b * Hq + h) * Tq + i, each with n_chunks slots.
+// are indexed as q's, each with n_chunks slots.
 template <int D, int BITS, int NW, int NC, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, 2) void fa_decode_mx_kernel(
-    const bf16 *__restrict__ Q, KvCache cache, const int *__restrict__ cache_seqlens,
+    const bf16 *Q, KvCache cache, const int *__restrict__ cache_seqlens,
     bf16 *__restrict__ O, float *__restrict__ LSE, float *__restrict__ part_o,
-    float *__restrict__ part_ml, int B, int Hq, int Hkv, int Tq, int Lmax, int n_chunks, int log2_min,
-    float scale_log2) {
+    float *__restrict__ part_ml, Divisor units, Divisor heads, int G, Divisor new_rows, int Lmax,
+    int n_chunks, int log2_min, int turn_units, float scale_log2) {
   using P = MxShape<D, BITS>;
   constexpr int DT = P::DT, COLS = 16 * NC;
-  // per wave the partial rows of min(R, 16) columns
+  // first the query rows' terms, in the end per wave the partial rows of min(R, 16) columns
   extern __shared__ __attribute__((aligned(16))) float stage[];
   __shared__ float wm[NW][COLS], wsum[NW][COLS];
+  __shared__ uint8_t query_bytes[COLS];
+  uint8_t *query_rows = reinterpret_cast<uint8_t *>(stage);
+  // The way to the first loads has no branches, and neither have they: a load behind one would have to
+  // be waited for before the query rows, which come first.
   const int chunk = SPLIT ? blockIdx.y : 0;
-  int bhk = blockIdx.x;
-  // B * Hkv is the grid's width (gridDim would put hidden arguments on every launch)
-  if (const int n_units = B * Hkv; SPLIT && n_units >= 8) {
-    bhk -= chunk_turn(chunk, n_units);
-    if (bhk < 0) bhk += n_units;
+  uint32_t bhk = blockIdx.x;
+  if (SPLIT) {
+    bhk += chunk * turn_units;
+    bhk -= units.quotient(bhk) * units.n;
   }
-  const int b = bhk / Hkv, hk = bhk - b * Hkv;
-  const int G = Hq / Hkv, R = G * Tq;
+  const int b = (int)heads.quotient(bhk), Tq = (int)new_rows.n, R = G * Tq;
   const int wave = wave_id(), lane = threadIdx.x & 63;
   const int i16 = lane & 15, q4 = lane >> 4;
-  const int64_t slab = (int64_t)bhk * Lmax;
-  const MxSrc src{cache.codes[0] + slab * P::CODE, cache.scales[0] + slab * P::GR,
-                  cache.codes[1] + slab * P::CODE, cache.scales[1] + slab * P::GR};
-  const MxLane<D, BITS> off(lane);
-  const int blk0 = chunk * NW + wave;
-
-  MxQuery<D> query[NC];
-  int last[NC];  // this lane's query column of a tile sees keys up to L + last
+  const int64_t row0 = (int64_t)bhk * R;  // the unit's rows of q, O and the partials follow each other
+  constexpr int NQ = (COLS * D / 8 + 64 * NW - 1) / (64 * NW);
+  const auto q_rows = make_rsrc(Q + row0 * D, (uint32_t)(R * D) * sizeof(bf16));
+  u32x4 q[NQ];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int col = (16 * c + i16) % R, g = col / Tq, i = col - g * Tq;
-    last[c] = i - Tq;
-    query[c].load(Q + (((int64_t)b * Hq + hk * G + g) * Tq + i) * D, q4);
-  }
-
-  // A half is loaded into the registers of the one just used: the wave's next block is on its way
-  // while it works on this one.
-  MxCodes<D, BITS> x[2];
-  MxScales sc;
+  for (int j = 0; j < NQ; ++j) q[j] = buf_load16(q_rows, 16 * (threadIdx.x + j * 64 * NW));
+  asm volatile("" ::: "memory");  // keeps them here: they are used behind a branch
 
   const int L = min(max(cache_seqlens[b], 0), Lmax);
   const int nb = (L + kMxBlock - 1) / kMxBlock;
   const int used = SPLIT ? used_chunks(nb, n_chunks, log2_min) : 1, step = used * NW;
+  const int blk0 = chunk * NW + wave, end = !SPLIT || chunk < used ? L : 0;
+  // The next block's K is loaded into the registers of this one's once its scores are formed, its V
+  // once this one's is added, its scales before both.
+  const int64_t slab = (int64_t)bhk * Lmax;
+  const MxSrc src{cache.codes[0] + slab * P::CODE, cache.scales[0] + slab * P::GR,
+                  cache.codes[1] + slab * P::CODE, cache.scales[1] + slab * P::GR};
+  const MxLane<D, BITS> off(lane);
+  MxK<D, BITS> kx[2];
+  MxV<D, BITS> vx[2];
+  __builtin_amdgcn_sched_barrier(0);  // in this order: the waits count on it
+  MxScales sc = load_scales(src, off, blk0 * kMxBlock, end);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) load_k(kx[u], src, off, blk0 * kMxBlock + 32 * u, end);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) load_v(vx[u], src, off, blk0 * kMxBlock + 32 * u, end);
+  __builtin_amdgcn_sched_barrier(0);
+  if (SPLIT && chunk >= used) {  // an empty partial, whose O the merge does not read
+    if (threadIdx.x < R)
+      *reinterpret_cast<f32x2 *>(part_ml + ((row0 + threadIdx.x) * n_chunks + chunk) * 2) =
+          f32x2{-INFINITY, 0.f};
+    return;
+  }
+  split_queries<D>(q, R, query_rows, query_bytes, 64 * NW);
+  __syncthreads();
 
   f32x4 oacc[NC][DT];
   float m_t[NC], l_part[NC];
@@ -356,58 +434,56 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_decode_mx_kernel(
     for (int n = 0; n < DT; ++n) oacc[c][n] = f32x4{};
   }
 
-  if (chunk < used && blk0 < nb) {
-    sc = load_scales(src, off, blk0 * kMxBlock, L);
-    load_codes(x[0], src, off, blk0 * kMxBlock, L);
-    __builtin_amdgcn_sched_barrier(0);  // in this order: the waits in the loop count on it
-    load_codes(x[1], src, off, blk0 * kMxBlock + 32, L);
-    __builtin_amdgcn_sched_barrier(0);
-    int pos[NC];  // last visible key
+  if (blk0 < nb) {
+    MxQuery<D> query[NC];
+    int pos[NC];  // last key that this lane's query column of a tile sees
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      pos[c] = L + last[c];
-      query[c].split(q4);
+      const int col = min(16 * c + i16, R - 1);  // columns past the last repeat it
+      pos[c] = L - Tq + col - (int)new_rows.quotient((uint32_t)col) * Tq;
+      query[c].read(query_rows, query_bytes, col, q4);
     }
     // rotates byte g of a row's scale bytes to bits 30:23
     const uint32_t turn = (8 * (i16 * P::GR / 16) + 9) & 31;
     const int first_masked = L - Tq;  // keys past this need the mask for some column
 
-    // selects bytes of (neighbour's word, own word) = bytes (7..4, 3..0)
-    const uint32_t halves = lane & 1 ? 0x03020706u : 0x05040100u;
     const uint32_t kshift = 8 * (q4 & (P::GR - 1));  // brings the byte of this lane's K group down
-    // Half U of a block: keys k0 .. k0 + 31
-    auto attend = [&](auto u, const MxCodes<D, BITS> &x, const uint32_t (&ks)[4], uint32_t vs, int k0) {
-      constexpr int U = decltype(u)::value;
-      f32x4 s[NC][2];
-      i32x8 ka[2];
-      if constexpr (P::PAIRED) {
-        uint32_t k[2][P::KW];
+
+#pragma unroll 1
+    for (int blk = blk0; blk < nb; blk += step) {
+      const int k0 = blk * kMxBlock, kn = k0 + step * kMxBlock;
+      uint32_t ks[4];
+      spread_rows(ks, sc.k);
+      const uint32_t vs = sc.v;
+      sc = load_scales(src, off, kn, L);
+      f32x4 s[NC][4];  // of keys k0 + q + 4 (4t + r)
 #pragma unroll
-        for (int w = 0; w < P::KW; ++w) {
-          const auto p = __builtin_amdgcn_permlane32_swap(x.k[0][w], x.k[0][w], false, false);
-          k[0][w] = p[0], k[1][w] = p[1];
-        }
-        ka[0] = k_operand<D, BITS>(k[0]), ka[1] = k_operand<D, BITS>(k[1]);
-      } else {
-        ka[0] = k_operand<D, BITS>(x.k[0]), ka[1] = k_operand<D, BITS>(x.k[P::KL - 1]);
+      for (int u = 0; u < 2; ++u) {
+        i32x8 a[2];
+        k_operands<D, BITS>(a, kx[u]);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+            s[c][2 * u + t] = scores<D, BITS>(a[t], ks[2 * u + t] >> kshift, query[c]);
       }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-          s[c][t] = scores<D, BITS>(ka[t], ks[2 * U + t] >> kshift, query[c]);
-      const bool masked = k0 + 31 > first_masked;
-      bf16x8 pb[NC];
+      for (int u = 0; u < 2; ++u) load_k(kx[u], src, off, kn + 32 * u, L);
+      __builtin_amdgcn_sched_barrier(0);
+
+      const bool masked = k0 + kMxBlock - 1 > first_masked;
+      bf16x8 pb[NC][2];
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         if (masked) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
+          for (int e = 0; e < 16; ++e)
             if (k0 + q4 + 4 * e > pos[c]) s[c][e >> 2][e & 3] = -INFINITY;
         }
-        float mx = fmax2(s[c][0][0], s[c][0][1]);
-#pragma unroll
-        for (int e = 2; e < 8; e += 2) mx = fmax3(mx, s[c][e >> 2][e & 3], s[c][e >> 2][(e + 1) & 3]);
+        float mx = max16(f32x16{s[c][0][0], s[c][0][1], s[c][0][2], s[c][0][3], s[c][1][0], s[c][1][1],
+                                s[c][1][2], s[c][1][3], s[c][2][0], s[c][2][1], s[c][2][2], s[c][2][3],
+                                s[c][3][0], s[c][3][1], s[c][3][2], s[c][3][3]}, -INFINITY);
         mx = quarters_max(mx) * scale_log2;
         if (__builtin_amdgcn_ballot_w64(mx > m_t[c] + kMxSlack)) {
           // each column by itself: its bits do not depend on when others rescale
@@ -418,93 +494,67 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_decode_mx_kernel(
 #pragma unroll
           for (int n = 0; n < DT; ++n) oacc[c][n] *= alpha;
         }
-        float p[8], rs = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          p[e] = exp2f_fast(__builtin_fmaf(s[c][e >> 2][e & 3], scale_log2, -m_t[c]));
-          rs += p[e];
+        for (int u = 0; u < 2; ++u) {
+          float p[8], rs = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            p[e] = exp2f_fast(__builtin_fmaf(s[c][2 * u + (e >> 2)][e & 3], scale_log2, -m_t[c]));
+            rs += p[e];
+          }
+          l_part[c] += rs;
+          const bf16x4 lo = pack4(p[0], p[1], p[2], p[3]), hi = pack4(p[4], p[5], p[6], p[7]);
+          pb[c][u] = bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         }
-        l_part[c] += rs;
-        const bf16x4 lo = pack4(p[0], p[1], p[2], p[3]), hi = pack4(p[4], p[5], p[6], p[7]);
-        pb[c] = bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
       }
-      uint32_t sc[8];
-      v_scales<U>(sc, vs, turn);
       // Where rows see different keys (several new rows), a NaN group of a key that a row does not
       // see must not reach it through 0 * NaN: those blocks count the NaN keys that each row sees,
       // make NaN what they add to, and go on without them.
-      if (masked && Tq > 1 && __builtin_amdgcn_ballot_w64(any_nan_scale(vs))) {
-        const bf16x8 mark = take_out_nans(sc);
-        int key = k0 + q4;
-        asm volatile("" : "+v"(key));  // keeps this block's comparisons in it
+      const bool nans = masked && Tq > 1 && __builtin_amdgcn_ballot_w64(any_nan_scale(vs));
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          bf16x8 seen;
+      for (int u = 0; u < 2; ++u) {
+        uint32_t vsc[8];
+        if (u == 0) v_scales<0>(vsc, vs, turn);
+        else v_scales<1>(vsc, vs, turn);
+        if (nans) {
+          int key = k0 + 32 * u + q4;
+          asm volatile("" : "+v"(key));  // keeps this block's comparisons in it
+          const bf16x8 mark = take_out_nans(vsc);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) seen[e] = (bf16)(key + 4 * e > pos[c] ? 0.f : 1.f);
-          const f32x4 count = mfma16(mark, seen, f32x4{});
+          for (int c = 0; c < NC; ++c) {
+            bf16x8 seen;
 #pragma unroll
-          for (int n = 0; n < DT; ++n)
+            for (int e = 0; e < 8; ++e) seen[e] = (bf16)(key + 4 * e > pos[c] ? 0.f : 1.f);
+            const f32x4 count = mfma16(mark, seen, f32x4{});
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (count[r] > 0.f) oacc[c][n][r] = __builtin_nanf("");
+            for (int n = 0; n < DT; ++n)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (count[r] > 0.f) oacc[c][n][r] = __builtin_nanf("");
+          }
+        }
+        const MxV<D, BITS> v = v_words(vx[u], lane);
+        auto add = [&](auto w) {
+          constexpr int W = decltype(w)::value;
+          bf16x8 even, odd;
+          v_pair<D, BITS, W>(even, odd, v, vsc);
+#pragma unroll
+          for (int c = 0; c < NC; ++c) oacc[c][2 * W] = mfma16(even, pb[c][u], oacc[c][2 * W]);
+#pragma unroll
+          for (int c = 0; c < NC; ++c) oacc[c][2 * W + 1] = mfma16(odd, pb[c][u], oacc[c][2 * W + 1]);
+        };
+        add(std::integral_constant<int, 0>{});
+        add(std::integral_constant<int, 1>{});
+        if constexpr (D == 128) {
+          add(std::integral_constant<int, 2>{});
+          add(std::integral_constant<int, 3>{});
         }
       }
-      uint32_t v[P::VL][P::VW];
-#pragma unroll
-      for (int r = 0; r < P::VL; ++r)
-#pragma unroll
-        for (int w = 0; w < P::VW; ++w) v[r][w] = x.v[r][w];
-      if constexpr (P::PAIRED) {
-        // even lanes take the low halves of their own row's word and their neighbour's, odd lanes
-        // the high halves of the neighbour's and their own: row 2r's elements, then row 2r + 1's
-#pragma unroll
-        for (int r = 0; r < P::VL; ++r) {
-          const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v[r][0], 0xB1, 0xF, 0xF, true);
-          v[r][0] = __builtin_amdgcn_perm(other, v[r][0], halves);
-        }
-      }
-      auto add = [&](auto w) {
-        constexpr int W = decltype(w)::value;
-        bf16x8 even, odd;
-        v_pair<D, BITS, W>(even, odd, v, sc);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) oacc[c][2 * W] = mfma16(even, pb[c], oacc[c][2 * W]);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) oacc[c][2 * W + 1] = mfma16(odd, pb[c], oacc[c][2 * W + 1]);
-      };
-      add(std::integral_constant<int, 0>{});
-      add(std::integral_constant<int, 1>{});
-      if constexpr (D == 128) {
-        add(std::integral_constant<int, 2>{});
-        add(std::integral_constant<int, 3>{});
-      }
-    };
-#pragma unroll 1
-    for (int blk = blk0; blk < nb; blk += step) {
-      const int k0 = blk * kMxBlock, kn = k0 + step * kMxBlock;
-      uint32_t ks[4];
-      spread_rows(ks, sc.k);
-      const uint32_t vs = sc.v;
-      sc = load_scales(src, off, kn, L);
-      attend(std::integral_constant<int, 0>{}, x[0], ks, vs, k0);
       __builtin_amdgcn_sched_barrier(0);
-      load_codes(x[0], src, off, kn, L);
-      __builtin_amdgcn_sched_barrier(0);
-      if (k0 + 32 < L) attend(std::integral_constant<int, 1>{}, x[1], ks, vs, k0 + 32);
-      __builtin_amdgcn_sched_barrier(0);
-      load_codes(x[1], src, off, kn + 32, L);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) load_v(vx[u], src, off, kn + 32 * u, L);
       __builtin_amdgcn_sched_barrier(0);
     }
-  }
-
-  if (SPLIT && chunk >= used) {  // an empty partial, whose O the merge does not read
-    if (threadIdx.x < R) {
-      const int g = threadIdx.x / Tq;
-      const int64_t row = ((int64_t)b * Hq + hk * G + g) * Tq + (threadIdx.x - g * Tq);
-      *reinterpret_cast<f32x2 *>(part_ml + (row * n_chunks + chunk) * 2) = f32x2{-INFINITY, 0.f};
-    }
-    return;
   }
 
   // Merge of the workgroup's waves, as in fa_decode.hip: every wave scales its partial to the
@@ -554,8 +604,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_decode_mx_kernel(
         t += *reinterpret_cast<const f32x4 *>(&stage[(w * rows + j) * D + ((ch ^ (j & 7)) << 2)]);
         ls += wm[w][k] == -INFINITY ? 0.f : wsum[w][k] * exp2f_fast(wm[w][k] - mx);
       }
-      const int g = k / Tq;
-      const int64_t row = ((int64_t)b * Hq + hk * G + g) * Tq + (k - g * Tq);
+      const int64_t row = row0 + k;
       if (!SPLIT) {
         const float inv = ls == 0.f ? 0.f : 1.f / ls;  // NaN sums reach O and LSE
         *reinterpret_cast<bf16x4 *>(O + row * D + 4 * ch) =
@@ -650,6 +699,13 @@ DecodeSplit decode_mx_split(int B, int Hkv, int Lmax, int D) {
 
 namespace {
 
+// Places by which a chunk turns its units against the chunk before it (units are the grid's width, its
+// chunks follow each other).  Consecutive workgroups go to the XCDs in turn, and those of an XCD to its
+// 32 CUs: without a turn every chunk of a unit would share an XCD, or a CU, where the number of units is
+// a multiple of 8 (or 256), and a long cache would be read by few (16 caches of 8 heads, one of 16384
+// keys: 52 us without, 23 with).  37 = 4 * 8 + 5 moves a unit's chunks to other XCDs and other CUs.
+int chunk_turn(int units) { return (units >= 64 ? 37 : 5) % units; }
+
 struct MxCall {
   const bf16 *q;
   KvCache cache;
@@ -673,10 +729,11 @@ hipError_t launch_waves(const MxCall &a) {
     hipError_t e = allow_lds<fa_decode_mx_kernel<D, BITS, NW, NC, SPLIT>>(most);
     if (e != hipSuccess) return e;
   }
-  const dim3 grid((unsigned)((int64_t)a.B * a.Hkv), (unsigned)n), block(64 * NW);
+  const int units = a.B * a.Hkv;
+  const dim3 grid((unsigned)units, (unsigned)n), block(64 * NW);
   fa_decode_mx_kernel<D, BITS, NW, NC, SPLIT><<<grid, block, lds, a.stream>>>(
-      a.q, a.cache, a.cache_seqlens, a.o, a.lse, part_o, part_ml, a.B, a.Hq, a.Hkv, a.Tq, a.Lmax, n,
-      a.sp.log2_min, a.scale_log2);
+      a.q, a.cache, a.cache_seqlens, a.o, a.lse, part_o, part_ml, Divisor(units), Divisor(a.Hkv),
+      a.Hq / a.Hkv, Divisor(a.Tq), a.Lmax, n, a.sp.log2_min, units - chunk_turn(units), a.scale_log2);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !SPLIT) return e;
   if (n > kMxMerged) return launch_decode_combine(part_o, part_ml, a.o, a.lse, rows, n, D, a.stream);

@@ -81,23 +81,8 @@ struct Eight<float> {
 
 }  // namespace
 
-namespace {
-
-// Rows moved by a call, numbered (b, h, t): b * Hkv + h and t by a multiplication with the divisor's
-// reciprocal, rounded up at 2^(31 + bits of the divisor): exact for dividends below 2^31.
-struct Divisor {
-  uint32_t n, mul, shift;
-  explicit Divisor(int d) : n((uint32_t)d), shift(0) {
-    while ((1u << shift) < n) ++shift;
-    mul = (uint32_t)((((uint64_t)1 << (31 + shift)) + n - 1) / n);
-  }
-  __device__ __forceinline__ uint32_t quotient(uint32_t x) const {
-    return (uint32_t)(((uint64_t)x * mul) >> 31) >> shift;
-  }
-};
-
-}  // namespace
-
+// Rows moved by a call are numbered (b, h, t).
+//
 // A lane takes eight elements, D / 8 lanes a row, U rows of a lane at once; blockIdx.y picks K or V.
 // Row t of T goes to position cache_seqlens[b] - T + t; one outside the cache is not written.
 // Bound by memory: 16 x 8 rows of up to 4000, D 128, bf16 to 4 bits 51 us (copy rate: 45).

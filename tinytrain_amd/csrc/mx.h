@@ -10,6 +10,19 @@ namespace ttfa {
 
 typedef short s16x2 __attribute__((ext_vector_type(2)));
 
+// Division of numbers below 2^31 by a number that the launch knows: a multiplication with its
+// reciprocal, rounded up at 2^(31 + bits of the divisor), which is exact for them.
+struct Divisor {
+  uint32_t n, mul, shift;
+  explicit Divisor(int d) : n((uint32_t)d), shift(0) {
+    while ((1u << shift) < n) ++shift;
+    mul = (uint32_t)((((uint64_t)1 << (31 + shift)) + n - 1) / n);
+  }
+  __device__ __forceinline__ uint32_t quotient(uint32_t x) const {
+    return (uint32_t)(((uint64_t)x * mul) >> 31) >> shift;
+  }
+};
+
 // New rows of K (0) and V (1): [B, H, T, D] with the strides of the first three in elements.
 template <class T>
 struct KvRows {

@@ -606,13 +606,14 @@ PyObject *py_flash_attn_decode_mx(PyObject *, PyObject *const *args, Py_ssize_t 
   if (bytes < 0) Py_RETURN_NONE;
   RECORD_FUNCTION("tinytrain::flash_attn_decode_mx", c10::ArrayRef<const c10::IValue>());
   const c10::DeviceGuard on(q.device());
-  Tensor ws = f32(q, {bytes / 4 + 4}), o = same(q), lse = f32(q, {B, Hq, Tq});
+  Tensor ws, o = same(q), lse = f32(q, {B, Hq, Tq});
+  if (bytes) ws = f32(q, {bytes / 4});
   check(ttfa_decode_mx_fwd(q.const_data_ptr(), c.k_codes.const_data_ptr(),
                            c.k_scales.const_data_ptr(), c.v_codes.const_data_ptr(),
                            c.v_scales.const_data_ptr(), c.lens.const_data_ptr<int>(),
                            o.mutable_data_ptr(), lse.mutable_data_ptr<float>(),
-                           ws.mutable_data_ptr<float>(), B, Hq, c.Hkv(), Tq, c.L(), D, c.bits(),
-                           TTFA_BF16, scale_of(D), stream_of(q)));
+                           bytes ? ws.mutable_data_ptr<float>() : nullptr, B, Hq, c.Hkv(), Tq,
+                           c.L(), D, c.bits(), TTFA_BF16, scale_of(D), stream_of(q)));
   return pack({o, lse});
   END_HANDLE_TH_ERRORS
 }

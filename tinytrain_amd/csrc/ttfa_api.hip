@@ -307,6 +307,7 @@ long long ttfa_decode_mx_workspace_bytes(int B, int Hq, int Hkv, int Tq, int max
                                          int bits) {
   if (check_decode_mx(B, Hq, Hkv, Tq, max_seqlen, D, bits, TTFA_BF16, 1.f)) return -1;
   const ttfa::DecodeSplit sp = ttfa::decode_mx_split(B, Hkv, max_seqlen, D);
+  if (sp.n_chunks == 1) return 0;
   return (long long)B * Hq * Tq * sp.n_chunks * (D + 2) * (long long)sizeof(float);
 }
 
@@ -316,8 +317,9 @@ int ttfa_decode_mx_fwd(const void *q, const void *k_codes, const void *k_scales,
                        int bits, int dtype, float scale, void *hip_stream) {
   int rc = check_decode_mx(B, Hq, Hkv, Tq, max_seqlen, D, bits, dtype, scale);
   if (rc) return rc;
+  const bool one = ttfa::decode_mx_split(B, Hkv, max_seqlen, D).n_chunks == 1;
   const void *ptrs[] = {q, k_codes, k_scales, v_codes, v_scales, o, lse, workspace};
-  if ((rc = check_ptrs(ptrs, 8)) || (rc = check_seqlens(cache_seqlens))) return rc;
+  if ((rc = check_ptrs(ptrs, one ? 7 : 8)) || (rc = check_seqlens(cache_seqlens))) return rc;
   return static_cast<int>(ttfa::launch_decode_mx(
       q, kv_cache(k_codes, k_scales, v_codes, v_scales), cache_seqlens, o, lse, workspace, B, Hq, Hkv,
       Tq, max_seqlen, D, bits, scale, static_cast<hipStream_t>(hip_stream)));

@@ -173,14 +173,15 @@ def flash_attn_decode_mx(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch
     nbytes = lib.ttfa_decode_mx_workspace_bytes(B, Hq, Hkv, Tq, L, D, bits)
     if nbytes < 0:
         _lib.check(_lib.E_SEQ)
-    ws = torch.empty((nbytes // 4 + 4,), device=q.device, dtype=torch.float32)
+    ws = torch.empty((nbytes // 4,), device=q.device, dtype=torch.float32) if nbytes else None
     o = torch.empty_like(q)
     lse = torch.empty((B, Hq, Tq), device=q.device, dtype=torch.float32)
     seqlens = cache_seqlens.contiguous()
     with torch.cuda.device(q.device):
         _lib.check(lib.ttfa_decode_mx_fwd(
             q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
-            v_scales.data_ptr(), seqlens.data_ptr(), o.data_ptr(), lse.data_ptr(), ws.data_ptr(), B, Hq,
+            v_scales.data_ptr(), seqlens.data_ptr(), o.data_ptr(), lse.data_ptr(),
+            ws.data_ptr() if nbytes else None, B, Hq,
             Hkv, Tq, L, D, bits, _lib.TTFA_BF16, 1.0 / math.sqrt(D),
             torch.cuda.current_stream(q.device).cuda_stream))
     return o, lse
