@@ -435,13 +435,17 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_decode_mx_kernel(
   }
 
   if (blk0 < nb) {
+    // 32 columns of 8 bits at D = 128 read their query rows again for every block, one tile's at a
+    // time: held, those 36 registers push others to scratch (16 x 4 units of 5000 keys 28.6 us, read
+    // again 23.7; 64 x 4 uneven ones 64.7 and 54.4).
+    constexpr bool kReread = NC == 2 && D == 128 && BITS == 8;
     MxQuery<D> query[NC];
     int pos[NC];  // last key that this lane's query column of a tile sees
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int col = min(16 * c + i16, R - 1);  // columns past the last repeat it
       pos[c] = L - Tq + col - (int)new_rows.quotient((uint32_t)col) * Tq;
-      query[c].read(query_rows, query_bytes, col, q4);
+      if (!kReread) query[c].read(query_rows, query_bytes, col, q4);
     }
     // rotates byte g of a row's scale bytes to bits 30:23
     const uint32_t turn = (8 * (i16 * P::GR / 16) + 9) & 31;
@@ -457,15 +461,33 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_decode_mx_kernel(
       const uint32_t vs = sc.v;
       sc = load_scales(src, off, kn, L);
       f32x4 s[NC][4];  // of keys k0 + q + 4 (4t + r)
+      if constexpr (kReread) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        i32x8 a[2];
-        k_operands<D, BITS>(a, kx[u]);
+        for (int c = 0; c < NC; ++c) {
+          asm volatile("" ::: "memory");  // keeps the reads inside the loop, one tile's at a time
+          query[0].read(query_rows, query_bytes, min(16 * c + i16, R - 1), q4);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+          for (int u = 0; u < 2; ++u) {
+            i32x8 a[2];
+            k_operands<D, BITS>(a, kx[u]);
 #pragma unroll
-          for (int c = 0; c < NC; ++c)
-            s[c][2 * u + t] = scores<D, BITS>(a[t], ks[2 * u + t] >> kshift, query[c]);
+            for (int t = 0; t < 2; ++t)
+              s[c][2 * u + t] = scores<D, BITS>(a[t], ks[2 * u + t] >> kshift, query[0]);
+          }
+#pragma unroll
+          for (int t = 0; t < 4; ++t) asm volatile("" : "+v"(s[c][t]));  // formed here, not at first use
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          i32x8 a[2];
+          k_operands<D, BITS>(a, kx[u]);
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+              s[c][2 * u + t] = scores<D, BITS>(a[t], ks[2 * u + t] >> kshift, query[c]);
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
