@@ -241,7 +241,9 @@ int ttfa_decode_fwd(const void *q, const void *k_cache, const void *v_cache,
  *   464 * 2^e (bits 8): the type's largest value plus half of its last step.  It is clamped to
  *   -125 .. 125 (bits 4) or -117 .. 119 (bits 8), so that every value is a finite normal bf16.
  *   An element is x / 2^e rounded to nearest even, saturating.  A group with a NaN or an infinity
- *   gets the byte 255 and codes 0; it reads back as NaN, and attention sees NaN there.
+ *   gets the byte 255 and codes 0; it reads back as NaN.  Attention over one of K makes O and LSE of the
+ *   rows that see its key NaN; one of V the elements of O to which its key adds a weight of 2^-126 of
+ *   the row's largest or more.  Rows that do not see the key are not touched by either.
  *   `strides`: element strides of k's, then v's first three dimensions (batch, head, row), six values in
  *   host memory, each a multiple of 16 bytes (TTFA_E_STRIDE); NULL where both are contiguous.  The
  *   last dimension has stride 1.
@@ -255,7 +257,8 @@ int ttfa_decode_fwd(const void *q, const void *k_cache, const void *v_cache,
  * launch) the workspace is not used and may be NULL.
  *
  * Supported: bits 4 or 8 (TTFA_E_BITS), D in {64, 128}, dtype TTFA_BF16 or TTFA_F32 for the rows;
- * pointers non-null and 16-byte aligned.  One launch each; decode one or two.
+ * pointers non-null and 16-byte aligned; max_seqlen * D < 2^31; B * Hkv * rows * D up to 2^34 - 2^13,
+ * B * Hkv of a decode below 2^24 (TTFA_E_SEQ).  One launch each; decode one or two.
  */
 int ttfa_kv_append(const void *k, const void *v, void *k_codes, void *k_scales, void *v_codes,
                    void *v_scales, const int *cache_seqlens, const long long *strides, int B,

@@ -265,3 +265,24 @@ def test_fullgraph_trace_of_a_step_is_its_ops():
     assert o.shape == (2, 4, 1, 64) and lse.shape == (2, 4, 1) and k.shape == v.shape == (2, 2, 4, 64)
     schema = torch.ops.tinytrain.kv_cache_append.default._schema
     assert [a.name for a in schema.arguments if a.is_write] == ["k_codes", "k_scales", "v_codes", "v_scales"]
+
+
+@needs_lib
+def test_largest_calls():
+    """Launches of 2^32 threads or more are refused; the calls below them get as far as the pointers."""
+    null = [None] * 7
+    for rows in (_append, _read):
+        for dtype in (_lib.TTFA_BF16, _lib.TTFA_F32):
+            most = ((1 << 34) - (1 << 13)) // (4 * 128)
+            assert rows(ptrs=null, B=2, Hkv=2, T=most, D=128, dtype=dtype) == _lib.E_NULL
+            assert rows(ptrs=null, B=2, Hkv=2, T=most + 1, D=128, dtype=dtype) == _lib.E_SEQ
+    assert _decode(ptrs=[None] * 9, B=(1 << 22) - 1, Hq=4, Hkv=4, T=1) == _lib.E_NULL
+    assert _decode(ptrs=[None] * 9, B=1 << 22, Hq=4, Hkv=4, T=1) == _lib.E_SEQ
+    w = _lib.load().ttfa_decode_mx_workspace_bytes
+    assert w(1 << 22, 4, 4, 1, 128, 64, 4) == -1 and w((1 << 22) - 1, 4, 4, 1, 128, 64, 4) == 0
+
+
+def test_lengths_past_32_bits_are_refused():
+    cache = [torch.empty(1, 1, 1 << 32, n, dtype=torch.uint8, device="meta") for n in (32, 2, 32, 2)]
+    with pytest.raises(FlashAttnInputError, match="too large"):
+        kv._check_cache(*cache, torch.zeros(1, dtype=torch.int32))

@@ -77,18 +77,20 @@ int check_kv(int B, int Hkv, int max_seqlen, int D, int bits) {
   return TTFA_OK;
 }
 
-// Rows moved in or out of it: one 16th of a workgroup at least each, numbered in 32 bits.
+// Rows moved in or out of it: a launch has fewer than 2^32 threads, of four elements at least each,
+// and a last workgroup that may be part empty.
 int check_kv_rows(int B, int Hkv, int rows, int max_seqlen, int D, int bits, int dtype) {
   if (dtype != TTFA_BF16 && dtype != TTFA_F32) return TTFA_E_DTYPE;
   const int rc = check_kv(B, Hkv, max_seqlen, D, bits);
   if (rc) return rc;
-  if (rows < 1 || (int64_t)rows > ((int64_t)0x7fffffff - 64) / ((int64_t)B * Hkv)) return TTFA_E_SEQ;
-  return TTFA_OK;
+  const int64_t most = (((int64_t)1 << 34) - (1 << 13)) / D;
+  return rows < 1 || (int64_t)rows > most / ((int64_t)B * Hkv) ? TTFA_E_SEQ : TTFA_OK;
 }
 
 int check_decode_mx(int B, int Hq, int Hkv, int Tq, int max_seqlen, int D, int bits, int dtype,
                     float scale) {
-  const int rc = check_kv(B, Hkv, max_seqlen, D, bits);
+  int rc = check_kv(B, Hkv, max_seqlen, D, bits);
+  if (!rc && (int64_t)B * Hkv >= 1 << 24) rc = TTFA_E_SEQ;  // workgroups of 256 threads, 2^32 in all
   // a length of 1 in place of max_seqlen, which check_kv holds to bytes of fewer bits
   return rc ? rc : check_decode(B, Hq, Hkv, Tq, 1, D, dtype, scale);
 }

@@ -75,6 +75,8 @@ def _check_cache(k_codes, k_scales, v_codes, v_scales, cache_seqlens):
             f"codes {tuple(k_codes.shape)}, {tuple(v_codes.shape)} and scales {tuple(k_scales.shape)}, "
             f"{tuple(v_scales.shape)} do not make one cache")
     B, Hkv, L, n = k_codes.shape
+    if max(B, Hkv, L) > 0x7fffffff:
+        raise FlashAttnInputError(f"a cache of {B} x {Hkv} x {L} rows is too large")
     D = GROUP * k_scales.shape[3]
     if D not in (64, 128):
         raise FlashAttnInputError(f"head dim D={D} is not supported (64 or 128)")
