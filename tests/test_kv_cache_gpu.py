@@ -174,21 +174,39 @@ def _queries(B, Hq, Tq, D, seed=0):
     return (q * torch.rsqrt(q.pow(2).mean(-1, keepdim=True))).to(BF)
 
 
-def _bounds(o, a, big, L, D):
+def _cut(q, k):
+    """The largest sum over eights of |q_d k_d|'s maximum, over a row's keys, / sqrt(D)."""
+    G, D = q.shape[1] // k.shape[1], q.shape[3]
+    q, k = q.double().abs().nan_to_num(0, 0, 0), k.abs().nan_to_num(0)
+    rows = torch.zeros(*q.shape[:3], k.shape[2], dtype=torch.float64)
+    for d in range(0, D, 8):
+        top = 0.0
+        for j in range(d, d + 8):
+            x = q[..., j].unflatten(1, (-1, G))[..., None] * k[:, :, None, None, :, j]
+            top = x if j == d else torch.maximum(top, x)
+        rows += top.flatten(1, 2)
+    return rows.amax(-1) / math.sqrt(D)
+
+
+def _bounds(o, a, big, cut, L, D):
     """Element-wise bounds of O and LSE, from the roundings on the way.
 
-    K, V and Q enter the products exactly.  A score is a sum of D products in fp32 with the size S =
+    K, V and Q enter the products exactly, but for elements of Q below 2^-13 of the row's largest, which
+    may lose 2^-21 of that.  Of eight consecutive products of a score the matrix unit cuts every bit
+    below 2^-13 of the largest: less than 7 2^-13 of it for Q's first term, 2^-4 of that for its
+    second.  7 (1 + 2^-4) < 7.5: the cuts, and what such small elements lose, stay within 2^-10 of `cut`, the
+    sum of the eights' largest products.  The sums of the eights are fp32, of size S =
     `big` (|error| <= D 2^-24 S), scaled and shifted by the maximum in fp32 (two roundings of at most S
     each); exp2 and log2 are good to 2^-21; a sum of L terms in fp32 adds L 2^-24.  So a weight
-    is off by d = (D + 4) 2^-24 S + L 2^-24 + 2^-20, relatively, twice (weight and sum); rounding the
-    weights to bf16 adds 2^-8 of A = sum p |v|, rounding O to bf16 2^-8 of itself."""
-    d = (D + 4) * 2.0**-24 * big + L * 2.0**-24 + 2.0**-20
+    is off by d = 2^-10 cut + (D + 4) 2^-24 S + L 2^-24 + 2^-20, relatively, twice (weight and sum);
+    rounding the weights to bf16 adds 2^-8 of A = sum p |v|, rounding O to bf16 2^-8 of itself."""
+    d = 2.0**-10 * cut + (D + 4) * 2.0**-24 * big + L * 2.0**-24 + 2.0**-20
     return (2.0**-8 + 2 * d[..., None]) * a * (1 + 2.0**-8) + 2.0**-8 * o.abs(), 2 * d + 2.0**-20
 
 
 def _check(q, cache, lens, k, v, got, L):
     o, lse, a, big = mx.decode(q, k, v, lens)
-    tol_o, tol_lse = _bounds(o, a, big, L, q.shape[3])
+    tol_o, tol_lse = _bounds(o, a, big, _cut(q, k), L, q.shape[3])
     go, gl = (t.double().cpu() for t in got)
     assert got[0].dtype == BF and got[1].dtype == F32
     seen = torch.isfinite(lse)
@@ -299,7 +317,7 @@ def test_decode_agrees_with_attention_over_the_rows_read_back():
     qt = q[:, :, T - Tq:].contiguous()
     o, _ = kv.flash_attn_decode_mx(qt, *_gpu(cache), lens)
     want, _, a, big = mx.decode(qt.cpu(), k, v, [T] * B)
-    tol, _ = _bounds(want, a, big, T, D)
+    tol, _ = _bounds(want, a, big, _cut(qt.cpu(), k), T, D)
     assert ((o - full).double().abs().cpu() <= 2 * tol).all()
 
 
@@ -486,3 +504,157 @@ def test_refusals_on_the_gpu():
     with pytest.raises(_lib.TTFAError):
         kv.kv_cache_append(k[:, :, :0], k[:, :, :0], *cache, lens)
     assert not any(t.any() for t in cache)
+
+
+# ------------------------------------------------------- both sides of the rules on sizes
+
+def _decode_tiled(B, Hq, Hkv, Tq, L, D, bits, lens):
+    """Attention of a batch that repeats three sequences (caches, queries, lengths) B times in turn; every
+    repeat is checked."""
+    cache, k, v = _filled(3, Hkv, L, D, bits, seed=L + B)
+    q = _queries(3, Hq, Tq, D)
+    turn = torch.arange(B) % 3
+    got = kv.flash_attn_decode_mx(q.to(DEV)[turn], *(t[turn.to(DEV)] for t in _gpu(cache)),
+                                  _lens(lens)[turn.to(DEV)])
+    for b in range(0, B, 3):
+        part = [t[b:b + 3] for t in got]
+        n = len(part[0])
+        _check(q[:n], cache, lens[:n], k[:n], v[:n], part, L)
+
+
+def _chunks(B, Hq, Hkv, Tq, L, D, bits):
+    n = _lib.load().ttfa_decode_mx_workspace_bytes(B, Hq, Hkv, Tq, L, D, bits)
+    return n // (B * Hq * Tq * (D + 2) * 4) or 1
+
+
+@pytest.mark.parametrize("B, Hq, Hkv, Tq, L, D, bits, chunks", [
+    (3, 4, 2, 1, 512, 64, 4, 1), (3, 4, 2, 1, 513, 64, 4, 3),               # one launch, or two
+    (32, 8, 4, 1, 600, 128, 8, 2), (33, 8, 4, 2, 600, 128, 8, 1),           # 128 and 132 units
+    (33, 16, 4, 8, 600, 128, 8, 1), (33, 20, 4, 5, 600, 128, 4, 1),         # eight waves, two tiles
+    (149, 6, 3, 1, 580, 64, 8, 1), (150, 3, 3, 6, 580, 64, 4, 1),           # 447 and 450
+    (1, 8, 8, 1, 8191, 128, 4, 16), (1, 8, 8, 1, 8192, 128, 4, 32),         # the two merges
+    (1, 8, 8, 3, 16383, 64, 8, 16), (1, 8, 8, 3, 16384, 64, 8, 32),
+    (66, 4, 4, 1, 4096, 64, 4, 1), (66, 4, 4, 1, 4097, 64, 4, 2),           # chunks for long among short
+    (2, 32, 1, 1, 32768, 128, 8, 128), (2, 1, 1, 32, 32767, 64, 4, 16),
+])
+def test_decode_on_both_sides_of_every_bound(B, Hq, Hkv, Tq, L, D, bits, chunks):
+    announce(f"decode_mx bounds B={B} Hq={Hq} Hkv={Hkv} Tq={Tq} L={L} D={D} bits={bits}")
+    assert _chunks(B, Hq, Hkv, Tq, L, D, bits) == chunks
+    _decode_tiled(B, Hq, Hkv, Tq, L, D, bits, [L, 70, Tq - 1] if L % 2 else [L - 1, 300, 1])
+
+
+@pytest.mark.parametrize("D, B, Hkv, T", [(128, 3, 5, 8738), (128, 3, 5, 8739), (64, 2, 7, 18725)])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_moves_of_many_rows(D, B, Hkv, T, bits):
+    """One and two rows at a time (2^21 lanes on), with a last workgroup that is part empty, rows before the
+    cache's first and past its last."""
+    announce(f"kv large moves D={D} B={B} Hkv={Hkv} T={T} bits={bits}")
+    L, lens = T - 100, ([T - 100, T // 3, T - 90][:B])
+    g = torch.Generator().manual_seed(T)
+    k = torch.randn(B, Hkv, T, D, generator=g).to(BF)
+    codes, scales = mx.quantise(k, bits)
+    want = _noise_cache(B, Hkv, L, D, bits)
+    got = _gpu(want)
+    kv.kv_cache_append(k.to(DEV), -k.to(DEV), *got, _lens(lens))
+    sign = 0x88 if bits == 4 else 0x80
+    for b, n in enumerate(lens):
+        lo, hi = max(n - T, 0), min(n, L)
+        rows = slice(lo - n + T, hi - n + T)
+        for c, m in ((0, 0), (2, sign)):
+            want[c][b, :, lo:hi], want[c + 1][b, :, lo:hi] = codes[b, :, rows] ^ m, scales[b, :, rows]
+    assert all(torch.equal(a, b) for a, b in zip(_cpu(got), want))
+    plain = mx.values(codes, scales, bits).float()
+    for dtype in (BF, F32):
+        rk, rv = kv.kv_cache_read(*got, _lens(lens), T, dtype)
+        assert torch.equal(rv, -rk)
+        for b, n in enumerate(lens):
+            lo, hi = max(T - n, 0), min(L - n + T, T)
+            assert torch.equal(rk[b, :, lo:hi].cpu().float(), plain[b, :, lo:hi])
+            assert not rk[b, :, :lo].any() and not rk[b, :, hi:].any()
+
+
+# ------------------------------------------------------------------------- unusual queries
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("B, Hkv, L, D", [(1, 1, 200, 64), (2, 1, 3000, 128), (33, 4, 600, 128)])
+def test_unusual_queries(B, Hkv, L, D, bits):
+    """Rows of zeros, tiny and huge rows, elements far below the row's largest, subnormal rows, and rows
+    with a NaN or an infinity, which alone come out NaN."""
+    announce(f"decode_mx queries B={B} Hkv={Hkv} L={L} D={D} bits={bits}")
+    G = 12
+    cache, k, v = _filled(B, Hkv, L, D, bits, seed=21)
+    q = _queries(B, G * Hkv, 1, D).unflatten(1, (Hkv, G))
+    q[:, :, 1] = 0
+    q[:, :, 2] *= 2.0**-100
+    q[:, :, 3] = (q[:, :, 3].float() * 2.0**-131).to(BF)
+    q[:, :, 4] *= 2.0**100
+    q[:, :, 5] = q[:, :, 5] * torch.exp2(-torch.arange(D) % 23.0).to(BF)
+    q[:, :, 6, 0, D // 2:] *= 2.0**-18
+    q[:, :, 7] *= 100
+    q[:, :, 8, 0, 5] = math.nan
+    q[:, :, 9, 0, D - 1] = math.inf
+    q[:, :, 10, 0, 0] = -math.inf
+    q = q.flatten(1, 2)
+    lens = [L - i for i in range(B)]
+    o, lse = kv.flash_attn_decode_mx(q.to(DEV), *_gpu(cache), _lens(lens))
+    bad = torch.zeros(B, Hkv, G, 1, dtype=torch.bool)
+    bad[:, :, 8:11] = True
+    bad = bad.flatten(1, 2)
+    assert torch.equal(torch.isnan(lse).cpu(), bad)
+    assert torch.equal(torch.isnan(o).cpu(), bad[..., None].expand_as(o))
+    clean = torch.where(bad[..., None], 0.0, q.float()).to(BF)
+    wo, wl, a, big = mx.decode(clean, k, v, lens)
+    # elements of q far below the row's largest may each lose 2^-21 of that
+    kk = k.abs().sum(-1).amax(-1).repeat_interleave(G, 1)[..., None]
+    lost = 2.0**-21 * clean.double().abs().amax(-1) * kk / math.sqrt(D)
+    tol, tol_lse = _bounds(wo, a, big, _cut(clean, k) + 2.0**10 * lost, L, D)
+    # weights below 2^-126 of the largest are 0 in fp32: each of L keys may miss that much of its value
+    most = v.abs().amax((2, 3)).repeat_interleave(G, 1)[..., None, None]
+    tol = tol + 2.0**-126 * L * most
+    err = (o.cpu().double() - wo).abs()
+    assert (err <= tol)[~bad].all(), (err / tol)[~bad].max()
+    # a huge row keeps to the largest score, relatively
+    assert ((lse.cpu().double() - wl).abs() <= tol_lse)[~bad].all()
+    # its O stays a mixture of the values (weights and O rounded to bf16)
+    assert (o.cpu().double().abs() <= most * (1 + 2.0**-6))[~bad].all()
+
+
+def test_inputs_that_require_grad_are_read_alike():
+    """The operators have no backward; under autograd they give what they give without."""
+    announce("kv requires_grad")
+    filled, _, _ = _filled(2, 2, 90, 64, 4, seed=31)
+    a, b = _gpu(filled), _gpu(filled)
+    q, k = _queries(2, 4, 1, 64).to(DEV), _queries(2, 2, 3, 64, seed=1).to(DEV)
+    lens = _lens([90, 40])
+    kv.kv_cache_append(k, k, *a, lens)
+    want = kv.flash_attn_decode_mx(q, *a, lens)
+    leaf = k.clone().requires_grad_()
+    kv.kv_cache_append(leaf, leaf * 1, *b, lens)
+    got = kv.flash_attn_decode_mx(q.clone().requires_grad_(), *b, lens)
+    assert all(torch.equal(x, y) for x, y in zip((*a, *want), (*b, *got)))
+    assert not any(t.requires_grad for t in b) and leaf.grad is None
+
+
+def test_two_graphs_of_one_cache_keep_apart():
+    """Two captured calls over one cache, replayed at once on two streams with new queries each time."""
+    announce("kv two graphs")
+    filled, _, _ = _filled(2, 4, 9000, 128, 4, seed=32)
+    cache, lens = _gpu(filled), _lens([9000, 4500])
+    qs = [_queries(2, 8, 1, 128, seed=s).to(DEV) for s in (0, 1)]
+    kv.flash_attn_decode_mx(qs[0], *cache, lens)
+    torch.cuda.synchronize()
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in qs]
+    for q in qs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(kv.flash_attn_decode_mx(q, *cache, lens))
+    for r in range(4):
+        for q, s in zip(qs, (2 * r, 2 * r + 1)):
+            q.copy_(_queries(2, 8, 1, 128, seed=50 + s))
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for q, out in zip(qs, outs):
+            assert all(torch.equal(x, y) for x, y in zip(out, kv.flash_attn_decode_mx(q, *cache, lens))), r

@@ -17,6 +17,11 @@
 //    is exact but for elements below 2^-13 of the row's largest, which lose at most 2^-21 of that.
 //    At D = 64 both terms share one product: k = 0..63 are hi, 64..127 lo, and K is given twice.
 //    (K through bf16 conversions took 32 more of about 200 vector instructions a block.)
+//    The instruction adds in fp32, but within every eight consecutive products it drops the bits below
+//    2^-13 of the largest (seen with single pairs of products).  A score is off by less than
+//    2^-10 of the sum of those largest ones; measured, relative to sum |q k|, 2^-22 on average and
+//    2^-16.4 at most of 4096 random scores in 4 bits, 2^-19 and 2^-14.9 in 8 bits.  At scores of a few tens
+//    that is below the 2^-9 to which the weights are rounded, and far below what 4 or 8 bits left of K.
 //  * V: lane (i, q) loads D / 16 consecutive elements of each of the rows q + 4e, converts each
 //    row's to bf16 with that row's scale, and pairs up rows with v_perm, giving the A operands of
 //    D / 16 tiles whose row i is d = D / 16 * i + tile.  The scale goes by row, so it cannot move into
@@ -354,6 +359,12 @@ __device__ __forceinline__ f32x4 scores(i32x8 a, uint32_t scale, const MxQuery<D
   return s;
 }
 
+// x - y, not fused with the product that x comes from
+__device__ __forceinline__ float minus(float x, float y) {
+#pragma clang fp contract(off)
+  return x - y;
+}
+
 // Whether one of the row's scale bytes is 255 (a NaN group)
 __device__ __forceinline__ bool any_nan_scale(uint32_t bytes) {
   const uint32_t x = ~bytes;  // has a zero byte?
@@ -498,6 +509,11 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_decode_mx_kernel(
       bf16x8 pb[NC][2];
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
+        // Scaled before the maximum is taken off, each with its own rounding: fused, the largest
+        // score's rounding error would be left there, an exponent of any size for scores past 2^30
+        // (0 to 1% of a call's time).
+#pragma unroll
+        for (int t = 0; t < 4; ++t) s[c][t] *= scale_log2;
         if (masked) {
 #pragma unroll
           for (int e = 0; e < 16; ++e)
@@ -506,7 +522,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_decode_mx_kernel(
         float mx = max16(f32x16{s[c][0][0], s[c][0][1], s[c][0][2], s[c][0][3], s[c][1][0], s[c][1][1],
                                 s[c][1][2], s[c][1][3], s[c][2][0], s[c][2][1], s[c][2][2], s[c][2][3],
                                 s[c][3][0], s[c][3][1], s[c][3][2], s[c][3][3]}, -INFINITY);
-        mx = quarters_max(mx) * scale_log2;
+        mx = quarters_max(mx);
         if (__builtin_amdgcn_ballot_w64(mx > m_t[c] + kMxSlack)) {
           // each column by itself: its bits do not depend on when others rescale
           const float m_new = mx > m_t[c] + kMxSlack ? mx : m_t[c];
@@ -521,7 +537,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_decode_mx_kernel(
           float p[8], rs = 0.f;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            p[e] = exp2f_fast(__builtin_fmaf(s[c][2 * u + (e >> 2)][e & 3], scale_log2, -m_t[c]));
+            p[e] = exp2f_fast(minus(s[c][2 * u + (e >> 2)][e & 3], m_t[c]));
             rs += p[e];
           }
           l_part[c] += rs;
