@@ -509,17 +509,15 @@ def test_refusals_on_the_gpu():
 # ------------------------------------------------------- both sides of the rules on sizes
 
 def _decode_tiled(B, Hq, Hkv, Tq, L, D, bits, lens):
-    """Attention of a batch that repeats three sequences (caches, queries, lengths) B times in turn; every
-    repeat is checked."""
+    """Attention of a batch that repeats three sequences (caches, queries, lengths) B times in turn: the first
+    three against the oracle, every repeat bit by bit against its first."""
     cache, k, v = _filled(3, Hkv, L, D, bits, seed=L + B)
     q = _queries(3, Hq, Tq, D)
-    turn = torch.arange(B) % 3
-    got = kv.flash_attn_decode_mx(q.to(DEV)[turn], *(t[turn.to(DEV)] for t in _gpu(cache)),
-                                  _lens(lens)[turn.to(DEV)])
-    for b in range(0, B, 3):
-        part = [t[b:b + 3] for t in got]
-        n = len(part[0])
-        _check(q[:n], cache, lens[:n], k[:n], v[:n], part, L)
+    turn = torch.arange(B, device=DEV) % 3
+    got = kv.flash_attn_decode_mx(q.to(DEV)[turn], *(t[turn] for t in _gpu(cache)), _lens(lens)[turn])
+    n = min(B, 3)
+    _check(q[:n], cache, lens[:n], k[:n], v[:n], [t[:n] for t in got], L)
+    assert all(torch.equal(t, t[:3][turn]) for t in got)
 
 
 def _chunks(B, Hq, Hkv, Tq, L, D, bits):
@@ -528,13 +526,19 @@ def _chunks(B, Hq, Hkv, Tq, L, D, bits):
 
 
 @pytest.mark.parametrize("B, Hq, Hkv, Tq, L, D, bits, chunks", [
-    (3, 4, 2, 1, 512, 64, 4, 1), (3, 4, 2, 1, 513, 64, 4, 3),               # one launch, or two
-    (32, 8, 4, 1, 600, 128, 8, 2), (33, 8, 4, 2, 600, 128, 8, 1),           # 128 and 132 units
-    (33, 16, 4, 8, 600, 128, 8, 1), (33, 20, 4, 5, 600, 128, 4, 1),         # eight waves, two tiles
-    (149, 6, 3, 1, 580, 64, 8, 1), (150, 3, 3, 6, 580, 64, 4, 1),           # 447 and 450
+    (3, 4, 2, 1, 768, 64, 4, 1), (3, 4, 2, 1, 769, 64, 4, 4),               # one launch, or two
+    (32, 8, 4, 1, 1024, 128, 8, 1), (32, 8, 4, 1, 1025, 128, 8, 2),
+    (9, 8, 8, 1, 1024, 64, 8, 3), (33, 8, 4, 2, 1025, 128, 8, 1),           # 72 and 132 units
+    (33, 8, 4, 2, 1472, 128, 4, 1), (33, 8, 4, 2, 1473, 128, 4, 1),         # four waves, eight
+    (33, 16, 4, 8, 512, 128, 4, 1), (33, 20, 4, 5, 513, 64, 4, 1),          # two tiles: four, eight
+    (33, 4, 4, 3, 1473, 64, 8, 1), (33, 20, 4, 4, 1500, 128, 8, 1),         # rows of 64 and 128 bytes
+    (65, 8, 4, 1, 1984, 64, 8, 1), (65, 8, 4, 2, 1985, 128, 8, 1),          # 260 units: four, eight
+    (65, 20, 4, 4, 1985, 128, 8, 1), (65, 16, 4, 8, 1985, 64, 4, 1),
+    (149, 6, 3, 1, 2000, 64, 8, 1), (112, 4, 4, 6, 2000, 64, 4, 1),         # 447 and 448
     (1, 8, 8, 1, 8191, 128, 4, 16), (1, 8, 8, 1, 8192, 128, 4, 32),         # the two merges
     (1, 8, 8, 3, 16383, 64, 8, 16), (1, 8, 8, 3, 16384, 64, 8, 32),
     (66, 4, 4, 1, 4096, 64, 4, 1), (66, 4, 4, 1, 4097, 64, 4, 2),           # chunks for long among short
+    (2, 17, 1, 1, 1333, 64, 8, 6), (2, 6, 2, 5, 1600, 64, 4, 7), (3, 11, 1, 2, 1100, 128, 4, 5),
     (2, 32, 1, 1, 32768, 128, 8, 128), (2, 1, 1, 32, 32767, 64, 4, 16),
 ])
 def test_decode_on_both_sides_of_every_bound(B, Hq, Hkv, Tq, L, D, bits, chunks):

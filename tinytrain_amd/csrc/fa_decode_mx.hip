@@ -26,7 +26,12 @@
 //    row's to bf16 with that row's scale, and pairs up rows with v_perm, giving the A operands of
 //    D / 16 tiles whose row i is d = D / 16 * i + tile.  The scale goes by row, so it cannot move into
 //    the product, whose scales go along the keys.
-// No LDS in the loop.
+// No LDS in the loop, but for the one case that reads its queries there (below).
+//
+// What bounds it: up to 16 query columns, memory (1.5 GB of caches in turn: 64 x 8 heads of up to 16384
+// keys, 678 MB, 131 us, 5.2 TB/s; 32 x 8 of 4096, 143 MB, 27.8 us, where a kernel of nothing but these loads
+// takes 26.8); 17 to 32 columns on few heads, the vector instructions of a block, about 1.2 us for a wave
+// (16 x 4 heads of 5000 keys, 32 columns: 18.8 us, 16 columns 15.0, and 8.3 without keys).
 #include "decode_split.h"
 #include "fa_bwd.h"  // allow_lds
 #include "fa_common.h"
@@ -252,6 +257,12 @@ __device__ __forceinline__ uint8_t *query_piece(uint8_t *rows, int row, int piec
   return rows + row * 2 * D + ((piece ^ (row & (D / 8 - 1))) << 4);
 }
 
+// x / scale, y / scale as e4m3 in half H of a word
+template <int H>
+__device__ __forceinline__ s16x2 put_fp8(uint32_t word, float x, float y, float scale) {
+  return __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(__builtin_bit_cast(s16x2, word), x, y, scale, H);
+}
+
 // Splits the workgroup's query rows into e4m3 terms; a lane takes eight elements, N times.
 template <int D, int N>
 __device__ __forceinline__ void split_queries(const u32x4 (&q)[N], int n_rows, uint8_t *rows,
@@ -268,7 +279,8 @@ __device__ __forceinline__ void split_queries(const u32x4 (&q)[N], int n_rows, u
       m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
     uint32_t top = (uint32_t)max(m[0], m[1]) << 16;
     auto with = [&](auto dpp) {
-      top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, decltype(dpp)::value, 0xF, 0xF, true));
+      top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, decltype(dpp)::value, 0xF, 0xF,
+                                                           true));
     };
     with(std::integral_constant<int, 0xB1>{});   // lane ^ 1
     with(std::integral_constant<int, 0x4E>{});   // lane ^ 2
@@ -283,14 +295,13 @@ __device__ __forceinline__ void split_queries(const u32x4 (&q)[N], int n_rows, u
     for (int i = 0; i < 4; ++i) {
       const float y0 = __uint_as_float(w[i] << 16) * inv, y1 = __uint_as_float(w[i] & 0xffff0000u) * inv;
       const uint32_t h_old = hi[i >> 1], l_old = lo[i >> 1];
-      const s16x2 h = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(__builtin_bit_cast(s16x2, h_old), y0, y1, 1.f, 1)
-                            : __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(__builtin_bit_cast(s16x2, h_old), y0, y1, 1.f, 0);
+      const s16x2 h = i & 1 ? put_fp8<1>(h_old, y0, y1, 1.f) : put_fp8<0>(h_old, y0, y1, 1.f);
       hi[i >> 1] = __builtin_bit_cast(uint32_t, h);
       const uint32_t code = hi[i >> 1];
       const f32x2 v = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(code, 1.f, 1)
                             : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(code, 1.f, 0);
-      const s16x2 l = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(__builtin_bit_cast(s16x2, l_old), y0 - v[0], y1 - v[1], 0x1p-4f, 1)
-                            : __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(__builtin_bit_cast(s16x2, l_old), y0 - v[0], y1 - v[1], 0x1p-4f, 0);
+      const s16x2 l = i & 1 ? put_fp8<1>(l_old, y0 - v[0], y1 - v[1], 0x1p-4f)
+                            : put_fp8<0>(l_old, y0 - v[0], y1 - v[1], 0x1p-4f);
       lo[i >> 1] = __builtin_bit_cast(uint32_t, l);
     }
     const int row = at / LPR, part = at % LPR;
@@ -700,26 +711,26 @@ __global__ __launch_bounds__(256) void fa_decode_mx_merge_kernel(const float *__
   if (lane == 0) LSE[row] = sum == 0.f ? -INFINITY : (M + __log2f(sum)) * kLn2;
 }
 
-// Workgroups per unit, waves per workgroup, and the blocks a workgroup takes at least.  Times in us
-// back to back, D 128 and 4 bits unless said; "uneven" is lengths from a tenth of the capacity up.
-//  * One chunk, and one launch, up to 512 keys (512 keys, 2 heads: 6.1; two launches 7.6).
-//  * Otherwise as many as stay within 256 workgroups, one per CU (96 units of 3000 keys: 2 chunks 14.7, 1
-//    15.8, 3 17.0; 160 units: 1 17.2, 3 18.7; 256 of 4096: 1 27.4, 2 31.1; 8 units of 16384: 32 chunks 10.8, 16 12.4, 64 12.2; of 131072:
-//    30.9, 43.0, 32.4; 48 units of 3000: 5 chunks 11.4, 2 14.1, 11 13.7), of at least a block per wave.
+// Workgroups per unit and the blocks that one takes at least; four waves each.  Times in us
+// back to back, caches rotated through 1.5 GB, D 128, 4 bits and full caches unless said; "uneven" is
+// lengths from a tenth of the capacity up.
+//  * One chunk, and one launch, up to 768 keys, or 1024 where there would be two chunks (8 units of 768
+//    keys: 6.9, two launches 7.6; of 1000: 8.0, 7.6; 64 of 768: 7.3, 8.0; 128 of 1000: 8.4, 9.2; of 1500:
+//    11.0, 10.9; 32 columns, 8 units of 768: 10.2, 9.8).  A call by itself gains 3 us more on the host.
+//  * Otherwise as many as stay within 256 workgroups, one per CU, of at least a block per wave:
+//      96 units of 3000 keys: 2 chunks 14.3, 1 17.1, 3 16.1; 160 units: 1 16.6, 2 20.8, 3 18.6;
+//      256 of 4096: 1 27.8, 2 30.6; 48 of 3000: 5 chunks 10.8, 2 13.5, 11 12.9;
+//      8 of 16384: 32 chunks 10.3, 16 11.7, 64 11.5; 8 of 131072: 32 32.6, 16 43.4, 64 32.7.
 //    More than kMxMerged chunks need the slower merge, which pays from 32768 elements a chunk (8 units
-//    of 8192: 32 chunks 9.1, 16 9.7; 12 units of 8000, D 64: 9.7, 8.1).
+//    of 8192: 32 chunks 8.6, 16 9.3; 12 units of 8000, D 64: 21 chunks 9.0, 16 7.6).
 //  * A long cache among short ones: with several sequences and a capacity over 4096, chunks of about
 //    2048 keys, up to 4096 workgroups (16 caches of 8 heads, one of 16384, the others of 300: 8 chunks
-//    19.2, 2 38.6; full and uneven calls lose nothing: 64 x 8 of up to 16384: 8 chunks 130, 1 133).
-//  * Waves of a one-chunk call: eight for 129 to 447 units, whose four-wave workgroups leave CUs
-//    unevenly filled (uneven caches: 320 units 19.5 against 21.3, 384 of 8 bits 34.5 against 39.9; full ones
-//    34.3 against 32.0), else four (448 units: 24.2 and 23.8, full 35.7 against 37.6; 1024: 25.7, 31.9).
+//    19.5, 2 38.4; full and uneven calls lose nothing: 64 x 8 of up to 16384: 8 chunks 131, 1 133).
 //  * A chunk's least is its share of a full cache, so that short caches cost one workgroup each; with up
 //    to 32 units, which leave the device idle, a block for every wave.
 DecodeSplit decode_mx_split(int B, int Hkv, int Lmax, int D) {
   const int64_t units = (int64_t)B * Hkv;
   const int64_t blocks = ((int64_t)Lmax + kMxBlock - 1) / kMxBlock;
-  if (blocks <= 8) return {4, 1, 0};
   int64_t n = std::max<int64_t>(256 / units, 1);
   if (n > kMxMerged && (int64_t)Lmax * D < n * 32768) n = kMxMerged;
   if (B > 1 && Lmax > 4096) {
@@ -728,7 +739,8 @@ DecodeSplit decode_mx_split(int B, int Hkv, int Lmax, int D) {
   }
   n = std::min(n, (blocks + 3) / 4);
   n = std::min<int64_t>(n, 512);
-  if (n <= 1) return {units > 128 && units < 448 ? 8 : 4, 1, 0};
+  if (blocks <= 12 || (n == 2 && blocks <= 16)) n = 1;
+  if (n <= 1) return {4, 1, 0};
   const int64_t least = units <= 32 ? 4 : (blocks + n - 1) / n;
   int log2_min = 0;
   while (least >> (log2_min + 1)) ++log2_min;
@@ -736,6 +748,23 @@ DecodeSplit decode_mx_split(int B, int Hkv, int Lmax, int D) {
 }
 
 namespace {
+
+// Waves of a one-chunk call: four, or eight, which halve a long cache's time where a CU has one
+// workgroup, and keep fewer caches on the device at once where it has several.  Times of eight waves
+// against four, uneven caches, then full ones:
+//  * up to 256 units, rows of 64 bytes or less: from 24 blocks on (192 units, D 128, 4 bits: 600 keys 0.94,
+//    1.01; 1000 1.01, 0.97; 1500 0.98, 0.94; 4000 0.89, 0.94), with 32 columns from 9 on (64 units, 512
+//    keys 0.94; 768 0.91; 192, 600 0.92), whose vector instructions then come in shorter runs.  Rows
+//    of 128 bytes have enough on the way with four (192 units: 1500 1.09, 1.09; 4000 1.05, 1.03).
+//  * up to 447 units: from 32 blocks on (320 units: 600 keys 1.29, 1.25; 1000 1.11, 1.16; 2000 0.90, 1.08;
+//    4000 0.88, 1.05; 8 bits: 1000 1.01, 1.15; 2000 0.89, 1.06; 4000 0.87, 1.03; 32 columns: 600 1.38,
+//    2000 1.03, 4000 0.86).
+//  * more: four (448 units of 3000: 0.94, 1.03; 1024 of 1500: 1.17, 1.08; 512 of 2000, 32 columns 1.11).
+int one_chunk_waves(int64_t units, int Lmax, int row_bytes, bool wide) {
+  const int blocks = (Lmax + kMxBlock - 1) / kMxBlock;
+  if (units <= 256) return row_bytes <= 64 && blocks >= (wide ? 9 : 24) ? 8 : 4;
+  return units < 448 && blocks >= 32 ? 8 : 4;
+}
 
 // Places by which a chunk turns its units against the chunk before it (units are the grid's width, its
 // chunks follow each other).  Consecutive workgroups go to the XCDs in turn, and those of an XCD to its
@@ -782,9 +811,7 @@ hipError_t launch_waves(const MxCall &a) {
 
 template <int D, int BITS, int NC>
 hipError_t launch_shape(const MxCall &a) {
-  if (a.sp.n_chunks > 1) {
-    return launch_waves<D, BITS, 4, NC, true>(a);
-  }
+  if (a.sp.n_chunks > 1) return launch_waves<D, BITS, 4, NC, true>(a);
   if (a.sp.n_waves == 8) return launch_waves<D, BITS, 8, NC, false>(a);
   return launch_waves<D, BITS, 4, NC, false>(a);
 }
@@ -794,9 +821,10 @@ hipError_t launch_shape(const MxCall &a) {
 hipError_t launch_decode_mx(const void *q, const KvCache &cache, const int *cache_seqlens, void *o,
                             float *lse, float *workspace, int B, int Hq, int Hkv, int Tq, int Lmax,
                             int D, int bits, float scale, hipStream_t stream) {
-  const MxCall a{(const bf16 *)q, cache, cache_seqlens, (bf16 *)o, lse, workspace, B, Hq, Hkv, Tq,
-                 Lmax, decode_mx_split(B, Hkv, Lmax, D), scale * kLog2e, stream};
+  MxCall a{(const bf16 *)q, cache, cache_seqlens, (bf16 *)o, lse, workspace, B, Hq, Hkv, Tq,
+           Lmax, decode_mx_split(B, Hkv, Lmax, D), scale * kLog2e, stream};
   const bool wide = Hq / Hkv * Tq > 16;
+  if (a.sp.n_chunks == 1) a.sp.n_waves = one_chunk_waves((int64_t)B * Hkv, Lmax, D * bits / 8, wide);
   if (D == 64) {
     if (bits == 4) return wide ? launch_shape<64, 4, 2>(a) : launch_shape<64, 4, 1>(a);
     return wide ? launch_shape<64, 8, 2>(a) : launch_shape<64, 8, 1>(a);
