@@ -243,7 +243,8 @@ int ttfa_decode_fwd(const void *q, const void *k_cache, const void *v_cache,
  *   An element is x / 2^e rounded to nearest even, saturating.  A group with a NaN or an infinity
  *   gets the byte 255 and codes 0; it reads back as NaN.  Attention over one of K makes O and LSE of the
  *   rows that see its key NaN; one of V the elements of O to which its key adds a weight of 2^-126 of
- *   the row's largest or more.  Rows that do not see the key are not touched by either.
+ *   the row's largest or more.  Rows that do not see the key are not touched by either.  That holds for
+ *   caches written here: no group of theirs has e4m3's own NaN among its codes (0x7f, 0xff).
  *   `strides`: element strides of k's, then v's first three dimensions (batch, head, row), six values in
  *   host memory, each a multiple of 16 bytes (TTFA_E_STRIDE); NULL where both are contiguous.  The
  *   last dimension has stride 1.

@@ -662,3 +662,26 @@ def test_two_graphs_of_one_cache_keep_apart():
         torch.cuda.synchronize()
         for q, out in zip(qs, outs):
             assert all(torch.equal(x, y) for x, y in zip(out, kv.flash_attn_decode_mx(q, *cache, lens))), r
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_moves_of_more_than_31_bits_of_elements(bits):
+    """One call that writes, and one that reads, over 2^31 elements of K and of V: every 2^20th row and the last
+    ones differ from the rest, in a batch of two."""
+    announce(f"kv large calls bits={bits}")
+    B, Hkv, D, T = 2, 1, 128, (1 << 23) + 77
+    rows = torch.randn(2, D, generator=torch.Generator().manual_seed(3)).to(BF).to(DEV)
+    k = rows[0].expand(B, Hkv, T, D)                      # strides 0: one row stands for all
+    cache = kv.mx_cache(B, Hkv, T, D, bits)
+    lens = _lens([T, T])
+    kv.kv_cache_append(k, k, *cache, lens)
+    odd = torch.arange(1 << 20, T, 1 << 20)
+    for n in (*odd.tolist(), T):
+        kv.kv_cache_append(rows[1].expand(B, Hkv, 1, D), rows[1].expand(B, Hkv, 1, D), *cache, _lens([n, n]))
+    want = mx.values(*mx.quantise(rows.cpu(), bits), bits).to(BF).to(DEV)
+    for x in kv.kv_cache_read(*cache, lens, T):
+        assert x.numel() > 1 << 31
+        one = torch.zeros(T, dtype=torch.bool, device=DEV)
+        one[odd.to(DEV) - 1] = one[T - 1] = True
+        for b in range(B):
+            assert torch.equal((x[b, 0] == want[0]).all(-1), ~one) and torch.equal((x[b, 0] == want[1]).all(-1), one)
