@@ -685,3 +685,21 @@ def test_moves_of_more_than_31_bits_of_elements(bits):
         one[odd.to(DEV) - 1] = one[T - 1] = True
         for b in range(B):
             assert torch.equal((x[b, 0] == want[0]).all(-1), ~one) and torch.equal((x[b, 0] == want[1]).all(-1), one)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("ek, ev", [(110, 100), (-105, -100)])
+def test_decode_of_scales_far_from_one(bits, ek, ev):
+    """Keys scaled up or down by powers of two that the queries take back, values of 2^100 and 2^-100: the
+    bits of the unscaled call, LSE and all, since only exponents differ."""
+    announce(f"decode_mx exponents ek={ek} ev={ev} bits={bits}")
+    B, Hq, Hkv, Tq, L, D = 2, 6, 2, 2, 1500, 128
+    cache, k, v = _filled(B, Hkv, L, D, bits, seed=41)
+    q = _queries(B, Hq, Tq, D)
+    want = kv.flash_attn_decode_mx(q.to(DEV), *_gpu(cache), _lens([L, 70]))
+    far = [t.clone() for t in cache]
+    far[1] = (far[1].int() + ek).to(torch.uint8)
+    far[3] = (far[3].int() + ev).to(torch.uint8)
+    o, lse = kv.flash_attn_decode_mx((q.float() * 2.0**-ek).to(BF).to(DEV), *_gpu(far), _lens([L, 70]))
+    assert torch.equal(lse, want[1]) and torch.equal(o.float(), want[0].float() * 2.0**ev)
+    _check(q, cache, [L, 70], k, v, want, L)

@@ -166,7 +166,7 @@ __global__ __launch_bounds__(256) void kv_read_mx_kernel(KvCache cache,
     if constexpr (sizeof(T) == 2)
       __builtin_nontemporal_store(mx_values8<BITS>(c[u], scale), reinterpret_cast<bf16x8 *>(out));
     else
-      __builtin_nontemporal_store(mx_values4_f32<BITS>(c[u], 0, scale), reinterpret_cast<f32x4 *>(out));
+      __builtin_nontemporal_store(mx_values4_f32<BITS>(c[u][0], scale), reinterpret_cast<f32x4 *>(out));
   }
 }
 

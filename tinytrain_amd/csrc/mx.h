@@ -43,13 +43,12 @@ __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t top) {
 
 // Elements 2i, 2i + 1 of eight, divided by `scale` (a power of two) and rounded to nearest even,
 // into their place among the codes c.  The e2m1 conversion saturates; the e4m3 one gives NaN past
-// 464, which only a clamped scale (magnitudes of 2^127 and more) can leave: hence the clamp to
-// `most`, at first the largest value 448 * 2^119.
+// 464, which only a clamped scale (magnitudes of 2^127 and more) can leave: hence the clamp to the
+// largest value.
 constexpr float kMx8Top = 448.0f * 0x1p119f;
 
 template <int BITS>
-__device__ __forceinline__ u32x2 mx_pack(u32x2 c, int i, f32x2 x, float scale,
-                                           float most = kMx8Top) {
+__device__ __forceinline__ u32x2 mx_pack(u32x2 c, int i, f32x2 x, float scale) {
   if constexpr (BITS == 4) {
     uint32_t w = c[0];
     switch (i) {
@@ -60,8 +59,8 @@ __device__ __forceinline__ u32x2 mx_pack(u32x2 c, int i, f32x2 x, float scale,
     }
     c[0] = w;
   } else {
-    const float a = __builtin_amdgcn_fmed3f(x[0], -most, most);
-    const float b = __builtin_amdgcn_fmed3f(x[1], -most, most);
+    const float a = __builtin_amdgcn_fmed3f(x[0], -kMx8Top, kMx8Top);
+    const float b = __builtin_amdgcn_fmed3f(x[1], -kMx8Top, kMx8Top);
     const uint32_t old = c[i >> 1];  // a copy: __builtin_bit_cast of a vector's element reads element 0
     s16x2 w = __builtin_bit_cast(s16x2, old);
     w = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, a, b, scale, 1)
@@ -114,18 +113,16 @@ __device__ __forceinline__ bf16x8 mx_values8(u32x2 c, float scale) {
   return bf16x8{x[0][0], x[0][1], x[1][0], x[1][1], x[2][0], x[2][1], x[3][0], x[3][1]};
 }
 
-// Elements 4i .. 4i + 3 of eight, as fp32.
+// Four fp32 values of the codes w (BITS 4: in its low half).
 template <int BITS>
-__device__ __forceinline__ f32x4 mx_values4_f32(u32x2 c, int i, float scale) {
+__device__ __forceinline__ f32x4 mx_values4_f32(uint32_t w, float scale) {
   f32x2 x, y;
   if constexpr (BITS == 4) {
-    x = i ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[0], scale, 2)
-          : __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[0], scale, 0);
-    y = i ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[0], scale, 3)
-          : __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[0], scale, 1);
+    x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 0);
+    y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 1);
   } else {
-    x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[i], scale, 0);
-    y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[i], scale, 1);
+    x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, 0);
+    y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, 1);
   }
   return f32x4{x[0], x[1], y[0], y[1]};
 }

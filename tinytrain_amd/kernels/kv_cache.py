@@ -26,7 +26,8 @@ prompts padded on the left to T rows needs no mask, and ``cache_seqlens`` filled
     o, lse = flash_attn_decode_mx(q, *cache, cache_seqlens)
 
 Supported: D in {64, 128}; rows in bf16 or fp32 with any strides that are multiples of 16 bytes and
-a dense last dimension; q in bf16, with the limits of ``flash_attn_decode``.
+a dense last dimension; q in bf16, with the limits of ``flash_attn_decode``; tensors that start at a
+multiple of 16 bytes; max_seqlen * D below 2^31.
 """
 
 from __future__ import annotations
