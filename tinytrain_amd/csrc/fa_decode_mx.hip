@@ -3,9 +3,9 @@
 // of fa_decode.hip (the last Tq rows of the reference's causal attention, model.py:94-98) on the
 // values the cache stands for, and so are the split over keys and the merge pass.
 //
-// Layout: a wave takes 32 keys at a time and 16 or 32 query columns (R = G * Tq <= 32 of them are
-// real; the others repeat them).  S^T = K Q^T is formed as two tiles of 16 keys, tile t's row 4q + r
-// being key q + 16t + 4r of the block, so that the result (D[i][j] in lane j + 16 * (i / 4), register
+// Layout: a wave takes blocks of 64 keys, in halves of 32, and 16 or 32 query columns (R = G * Tq <= 32
+// of them are real; the others repeat them).  S^T = K Q^T is formed as two tiles of 16 keys a half, tile
+// t's row 4q + r being key q + 16t + 4r of it, so that the result (D[i][j] in lane j + 16 * (i / 4), register
 // i % 4) leaves lane (j, q) with the scores of keys q + 4e, e = 4t + r, of column j: the B operand of
 // O^T += V^T P^T through v_mfma_f32_16x16x32_bf16 as it stands, and every load instruction reads
 // whole consecutive rows.
@@ -16,9 +16,9 @@
 //    once into two e4m3 terms, q = hi + lo: a bf16 has 8 significant bits and each term 4, so the sum
 //    is exact but for elements below 2^-13 of the row's largest, which lose at most 2^-21 of that.
 //    At D = 64 both terms share one product: k = 0..63 are hi, 64..127 lo, and K is given twice.
-//    (K through bf16 conversions took 32 more of about 200 vector instructions a block.)
+//    (K through bf16 conversions took 32 more of about 200 vector instructions a half.)
 //    The instruction adds in fp32, but within every eight consecutive products it drops the bits below
-//    2^-13 of the largest (seen with single pairs of products).  A score is off by less than
+//    2^-13 of the largest (seen with pairs of products, in one eight and in two).  A score is off by less than
 //    2^-10 of the sum of those largest ones; measured, relative to sum |q k|, 2^-22 on average and
 //    2^-16.4 at most of 4096 random scores in 4 bits, 2^-19 and 2^-14.9 in 8 bits.  At scores of a few tens
 //    that is below the 2^-9 to which the weights are rounded, and far below what 4 or 8 bits left of K.
