@@ -254,7 +254,9 @@ int ttfa_decode_fwd(const void *q, const void *k_cache, const void *v_cache,
  * every value exactly.
  *
  * ttfa_decode_mx_fwd is ttfa_decode_fwd (arguments, results, workspace rules) on the values that the
- * cache stands for; q and o are bf16.  A score is within 2^-10 (on average 2^-19) of its sum of
+ * cache stands for; q and o are bf16.  Query row t sits at position cache_seqlens[b] - Tq + t, also
+ * where that is past the capacity (ttfa_decode_fwd clamps the length first), and sees the keys up to it
+ * that the cache holds.  A score is within 2^-10 (on average 2^-19) of its sum of
  * |q_d k_d| * scale: the matrix unit cuts products of these types before it adds them in fp32.  Where
  * ttfa_decode_mx_workspace_bytes gives 0 (calls of one launch) the workspace is not used and may be NULL.
  *

@@ -85,7 +85,8 @@ def read(cache, cache_seqlens, rows):
 
 def decode(q, k, v, cache_seqlens):
     """Attention of the newest rows q [B, Hq, Tq, D] over fp64 values k, v [B, Hkv, L, D], each row over the
-    keys it sees and no others (a NaN elsewhere does not matter).
+    keys it sees and no others (a NaN elsewhere does not matter): row i sits at position
+    cache_seqlens[b] - Tq + i and sees those up to it that the cache holds.
 
     Returns (O, LSE, A, S): A = sum p |v| and S = the row's largest sum |q_d k_d| / sqrt(D), the sizes
     that rounding errors of O and of the scores go by."""
@@ -96,9 +97,8 @@ def decode(q, k, v, cache_seqlens):
     lse = torch.full((B, Hq, Tq), -math.inf, dtype=torch.float64, device=dev)
     big = torch.zeros(B, Hq, Tq, dtype=torch.float64, device=dev)
     for b in range(B):
-        L = min(max(int(cache_seqlens[b]), 0), Lmax)
         for i in range(Tq):
-            n = L - Tq + i + 1
+            n = min(int(cache_seqlens[b]) - Tq + i + 1, Lmax)
             if n < 1:
                 continue
             x = q[b, :, i].double().view(Hkv, G, D)

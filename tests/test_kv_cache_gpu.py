@@ -703,3 +703,60 @@ def test_decode_of_scales_far_from_one(bits, ek, ev):
     o, lse = kv.flash_attn_decode_mx((q.float() * 2.0**-ek).to(BF).to(DEV), *_gpu(far), _lens([L, 70]))
     assert torch.equal(lse, want[1]) and torch.equal(o.float(), want[0].float() * 2.0**ev)
     _check(q, cache, [L, 70], k, v, want, L)
+
+
+# ------------------------------------------------------------------ lengths past the capacity
+
+def _check_sharp(q, cache, lens, k, v, got, L):
+    """_check where scores lie so far apart that weights underflow: a weight below 2^-126 of the row's largest
+    is 0 or a subnormal of few bits in fp32, off by 2^-126 at most, so O misses up to 2^-126 |v| for each of L
+    keys (which covers half a step, 2^-134, of O's own subnormals)."""
+    o, lse, a, big = mx.decode(q, k, v, lens)
+    tol_o, tol_lse = _bounds(o, a, big, _cut(q, k), L, q.shape[3])
+    tol_o = tol_o + 2.0**-126 * L * v.abs().amax((2, 3)).repeat_interleave(q.shape[1] // k.shape[1], 1)[..., None, None]
+    go, gl = (t.double().cpu() for t in got)
+    assert torch.isfinite(lse).all() and ((gl - lse).abs() <= tol_lse).all(), ((gl - lse).abs() / tol_lse).max()
+    assert ((go - o).abs() <= tol_o).all(), ((go - o).abs() / tol_o).max()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("B, Hq, Hkv, Tq, L, D, over", [
+    (4, 8, 2, 4, 64, 64, [1, 3, 4, 70]),                 # one launch, a whole number of blocks
+    (3, 4, 2, 3, 97, 128, [1, 2, 2**31 - 1 - 97]),
+    (2, 32, 4, 4, 333, 128, [2, 0]),                     # two tiles
+    (3, 4, 4, 5, 5000, 128, [1, 4, 200]),                # several chunks
+    (2, 3, 3, 6, 4992, 64, [5, 6]),
+])
+def test_queries_past_the_capacity_keep_their_positions(B, Hq, Hkv, Tq, L, D, over, bits):
+    """Rows that no longer fit are not written, and every query still sees the keys up to its own position
+    that the cache holds, its own among them."""
+    announce(f"decode_mx past the capacity B={B} Tq={Tq} L={L} D={D} bits={bits} over={over}")
+    want, _, _ = _filled(B, Hkv, L, D, bits, seed=51)
+    cache, lens = _gpu(want), [L + n for n in over]
+    g = torch.Generator().manual_seed(52)
+    # keys far above the others, along the queries: a row that misses one is off by its whole weight
+    q = _queries(B, Hq, Tq, D)
+    k = (8 * q[:, ::Hq // Hkv].float()).to(BF)
+    v = torch.randn(B, Hkv, Tq, D, generator=g).to(BF)
+    kv.kv_cache_append(k.to(DEV), v.to(DEV), *cache, _lens(lens))
+    mx.append(want, k, v, lens)
+    assert all(torch.equal(a, b) for a, b in zip(_cpu(cache), want))
+    got = kv.flash_attn_decode_mx(q.to(DEV), *cache, _lens(lens))
+    _check_sharp(q, want, lens, *mx.read(want, [L] * B, L), got, L)
+
+
+@pytest.mark.parametrize("L", [64, 333, 5000])
+def test_nan_groups_past_the_capacity_reach_the_rows_that_see_them(L):
+    """A NaN group of the cache's last V row, lengths one and two past the capacity: rows before it stay clean."""
+    announce(f"decode_mx NaN past the capacity L={L}")
+    B, Hq, Hkv, Tq, D = 2, 4, 2, 4, 64
+    cache, _, _ = _filled(B, Hkv, L, D, 4, seed=53)
+    q, lens = _queries(B, Hq, Tq, D).to(DEV), _lens([L + 1, L + 2])
+    clean = kv.flash_attn_decode_mx(q, *_gpu(cache), lens)
+    cache[3][:, :, L - 1, 1] = 255
+    cache[2][:, :, L - 1, 16:] = 0
+    o, lse = kv.flash_attn_decode_mx(q, *_gpu(cache), lens)
+    bad = torch.zeros(B, Hq, Tq, D, dtype=torch.bool, device=DEV)
+    bad[0, :, 2:, 32:] = bad[1, :, 1:, 32:] = True
+    assert torch.equal(torch.isnan(o), bad) and torch.equal(lse, clean[1])
+    assert torch.equal(o[~bad], clean[0][~bad])

@@ -286,3 +286,11 @@ def test_lengths_past_32_bits_are_refused():
     cache = [torch.empty(1, 1, 1 << 32, n, dtype=torch.uint8, device="meta") for n in (32, 2, 32, 2)]
     with pytest.raises(FlashAttnInputError, match="too large"):
         kv._check_cache(*cache, torch.zeros(1, dtype=torch.int32))
+
+
+def test_oracle_positions_past_the_capacity():
+    """Queries keep their positions where the newest rows no longer fit: row i of three sees
+    len - 3 + i + 1 keys, or all that there are."""
+    k = torch.zeros(5, 1, 6, 64, dtype=torch.float64)
+    _, lse, _, _ = mx.decode(torch.zeros(5, 1, 3, 64), k, k, [6, 7, 8, 2**31 - 1, 1])
+    assert lse.exp().round().view(5, 3).tolist() == [[4, 5, 6], [5, 6, 6], [6, 6, 6], [6, 6, 6], [0, 0, 1]]

@@ -418,7 +418,8 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_decode_mx_kernel(
   for (int j = 0; j < NQ; ++j) q[j] = buf_load16(q_rows, 16 * (threadIdx.x + j * 64 * NW));
   asm volatile("" ::: "memory");  // keeps them here: they are used behind a branch
 
-  const int L = min(max(cache_seqlens[b], 0), Lmax);
+  // Rows past the capacity were dropped: their keys are missing, the queries' positions stay.
+  const int len = max(cache_seqlens[b], 0), L = min(len, Lmax);
   const int nb = (L + kMxBlock - 1) / kMxBlock;
   const int used = SPLIT ? used_chunks(nb, n_chunks, log2_min) : 1, step = used * NW;
   const int blk0 = chunk * NW + wave, end = !SPLIT || chunk < used ? L : 0;
@@ -462,16 +463,16 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_decode_mx_kernel(
     // again 23.7; 64 x 4 uneven ones 64.7 and 54.4).
     constexpr bool kReread = NC == 2 && D == 128 && BITS == 8;
     MxQuery<D> query[NC];
-    int pos[NC];  // last key that this lane's query column of a tile sees
+    int pos[NC];  // last key that this lane's query column of a tile sees; none past the cache
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int col = min(16 * c + i16, R - 1);  // columns past the last repeat it
-      pos[c] = L - Tq + col - (int)new_rows.quotient((uint32_t)col) * Tq;
+      pos[c] = min(len - Tq + col - (int)new_rows.quotient((uint32_t)col) * Tq, L - 1);
       if (!kReread) query[c].read(query_rows, query_bytes, col, q4);
     }
     // rotates byte g of a row's scale bytes to bits 30:23
     const uint32_t turn = (8 * (i16 * P::GR / 16) + 9) & 31;
-    const int first_masked = L - Tq;  // keys past this need the mask for some column
+    const int first_masked = min(len - Tq, L - 1);  // keys past this need the mask for some column
 
     const uint32_t kshift = 8 * (q4 & (P::GR - 1));  // brings the byte of this lane's K group down
 

@@ -16,7 +16,8 @@ group's largest magnitude is at most 7 * 2^e (bits 4) or 464 * 2^e (bits 8), an 
 rounded to nearest even.  A group with a NaN or an infinity reads back as NaN.
 
 ``cache_seqlens`` [B] int32 counts the new rows already, in every one of these calls: row t of T new (or
-wanted) ones of sequence b sits at position cache_seqlens[b] - T + t.  Rows at positions outside
+wanted) ones of sequence b sits at position cache_seqlens[b] - T + t.  A length past max_seqlen
+shifts none of them: a query attends to the keys up to its own position that the cache holds.  Rows at positions outside
 0 .. max_seqlen - 1 are not written by ``kv_cache_append`` and are zeros from ``kv_cache_read``, so a batch of
 prompts padded on the left to T rows needs no mask, and ``cache_seqlens`` filled with n makes
 ``kv_cache_read(..., rows=n)`` the first n rows.  A step of generation:
