@@ -760,3 +760,42 @@ def test_nan_groups_past_the_capacity_reach_the_rows_that_see_them(L):
     bad[0, :, 2:, 32:] = bad[1, :, 1:, 32:] = True
     assert torch.equal(torch.isnan(o), bad) and torch.equal(lse, clean[1])
     assert torch.equal(o[~bad], clean[0][~bad])
+
+
+# --------------------------------------------------------------------- queries next to zero
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("D", [64, 128])
+def test_queries_next_to_the_smallest_normal(D, bits):
+    """Queries of 2^-124 against keys scaled up by as much: the bits of the same mantissas at size one."""
+    announce(f"decode_mx queries of 2^-124 D={D} bits={bits}")
+    B, Hq, Hkv, Tq, L, ek = 2, 6, 2, 2, 1500, 124
+    cache, k, v = _filled(B, Hkv, L, D, bits, seed=54)
+    tiny = (_queries(B, Hq, Tq, D).float() * 2.0**-ek).to(BF)
+    q = (tiny.float() * 2.0**ek).to(BF)                  # exact: the subnormal ones have fewer bits
+    far = [t.clone() for t in cache]
+    far[1] = (far[1].int() + ek).to(torch.uint8)
+    assert cache[1].int().max() + ek <= mx.LIMITS[bits][2] + 127 and (tiny.float().abs().amax(-1) >= 2.0**-126).all()
+    want = kv.flash_attn_decode_mx(q.to(DEV), *_gpu(cache), _lens([L, 70]))
+    got = kv.flash_attn_decode_mx(tiny.to(DEV), *_gpu(far), _lens([L, 70]))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    _check(q, cache, [L, 70], k, v, want, L)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("Hq, Hkv, L, D", [(6, 1, 700, 64), (6, 1, 700, 128), (24, 1, 2000, 128)])
+def test_queries_of_few_bits_left(Hq, Hkv, L, D, bits):
+    """Rows whose elements all have one magnitude, from 2^-108 down to subnormals, over keys of up to 2^126
+    along their signs: an error of the query's terms adds up over the row."""
+    announce(f"decode_mx tiny queries Hq={Hq} L={L} D={D} bits={bits}")
+    g = torch.Generator().manual_seed(55)
+    sign = torch.randint(0, 2, (D,), generator=g) * 2 - 1
+    size = torch.tensor([1.2109375 * 2.0**-124, 113 * 2.0**-133, 1.9921875 * 2.0**-117, 1.1484375 * 2.0**-120,
+                         1.6796875 * 2.0**-126, 1.2109375 * 2.0**-109], dtype=torch.float64).repeat(Hq // 6)
+    q = (size[:, None] * sign).view(1, Hq, 1, D).to(BF)
+    assert torch.equal(q.double(), (size[:, None] * sign).view(1, Hq, 1, D))
+    ramp = torch.linspace(0.1, 1, L).double()[:, None] * 2.0**126 * sign * (1 + 0.1 * torch.rand(D, generator=g))
+    v = torch.randn(1, Hkv, L, D, generator=g).to(BF)
+    cache = [*mx.quantise(ramp.view(1, 1, L, D).to(BF), bits), *mx.quantise(v, bits)]
+    got = kv.flash_attn_decode_mx(q.to(DEV), *_gpu(cache), _lens([L]))
+    _check_sharp(q, cache, [L], mx.values(*cache[:2], bits), mx.values(*cache[2:], bits), got, L)

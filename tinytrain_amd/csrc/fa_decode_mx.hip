@@ -15,6 +15,8 @@
 //    32c .. 32c + 31 comes from lane i + 16 c (checked element by element on gfx950).  Q is split
 //    once into two e4m3 terms, q = hi + lo: a bf16 has 8 significant bits and each term 4, so the sum
 //    is exact but for elements below 2^-13 of the row's largest, which lose at most 2^-21 of that.
+//    Rows of less than 2^-108, whose powers of two the instruction's scales would not reach, enter it
+//    scaled up, and their scores are scaled down with the softmax scale.
 //    At D = 64 both terms share one product: k = 0..63 are hi, 64..127 lo, and K is given twice.
 //    (K through bf16 conversions took 32 more of about 200 vector instructions a half.)
 //    The instruction adds in fp32, but within every eight consecutive products it drops the bits below
@@ -250,8 +252,11 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 // The query rows of a workgroup in LDS: per row D bytes of hi, then D bytes of lo, in 16-byte pieces
-// whose place is turned by the row (a fragment read takes the same piece of 16 rows), and the bytes
-// of the rows' powers of two.
+// whose place is turned by the row (a fragment read takes the same piece of 16 rows), and the rows'
+// exponents e + 127: -8 (subnormals) to 247, or 255 for a row with a NaN or an infinity.  The product
+// takes a lower one than kLeastExp as that, whose lo term, 4 below, is then in reach too.
+constexpr int kLeastExp = 10;
+
 template <int D>
 __device__ __forceinline__ uint8_t *query_piece(uint8_t *rows, int row, int piece) {
   return rows + row * 2 * D + ((piece ^ (row & (D / 8 - 1))) << 4);
@@ -266,7 +271,7 @@ __device__ __forceinline__ s16x2 put_fp8(uint32_t word, float x, float y, float 
 // Splits the workgroup's query rows into e4m3 terms; a lane takes eight elements, N times.
 template <int D, int N>
 __device__ __forceinline__ void split_queries(const u32x4 (&q)[N], int n_rows, uint8_t *rows,
-                                              uint8_t *bytes, int threads) {
+                                              int16_t *exps, int threads) {
   constexpr int LPR = D / 8;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
@@ -286,14 +291,14 @@ __device__ __forceinline__ void split_queries(const u32x4 (&q)[N], int n_rows, u
     with(std::integral_constant<int, 0x4E>{});   // lane ^ 2
     with(std::integral_constant<int, 0x141>{});  // mirrored in eight
     if constexpr (LPR == 16) with(std::integral_constant<int, 0x140>{});  // in sixteen
-    // As mx_scale_byte<8>, not clamped above: no cache value has to hold these.
+    // As mx_scale_byte<8>, not clamped: no cache value has to hold these.
     const int e = (int)((top + (0x7fffff - 0x680000)) >> 23) - 8;
-    const int byte = top >= 0x7f800000u ? 255 : max(e, 10);
-    const float inv = __uint_as_float((uint32_t)(254 - min(byte, 253)) << 23);
+    const int exp = top >= 0x7f800000u ? 255 : e;
     u32x2 hi{}, lo{};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float y0 = __uint_as_float(w[i] << 16) * inv, y1 = __uint_as_float(w[i] & 0xffff0000u) * inv;
+      const float y0 = __builtin_ldexpf(__uint_as_float(w[i] << 16), 127 - exp);
+      const float y1 = __builtin_ldexpf(__uint_as_float(w[i] & 0xffff0000u), 127 - exp);
       const uint32_t h_old = hi[i >> 1], l_old = lo[i >> 1];
       const s16x2 h = i & 1 ? put_fp8<1>(h_old, y0, y1, 1.f) : put_fp8<0>(h_old, y0, y1, 1.f);
       hi[i >> 1] = __builtin_bit_cast(uint32_t, h);
@@ -307,7 +312,7 @@ __device__ __forceinline__ void split_queries(const u32x4 (&q)[N], int n_rows, u
     const int row = at / LPR, part = at % LPR;
     *reinterpret_cast<u32x2 *>(query_piece<D>(rows, row, part >> 1) + 8 * (part & 1)) = hi;
     *reinterpret_cast<u32x2 *>(query_piece<D>(rows, row, D / 16 + (part >> 1)) + 8 * (part & 1)) = lo;
-    if (part == 0) bytes[row] = (uint8_t)byte;
+    if (part == 0) exps[row] = (int16_t)exp;
   }
 }
 
@@ -319,7 +324,7 @@ struct MxQuery {
   i32x8 t[N];
   int scale[N];
 
-  __device__ __forceinline__ void read(uint8_t *rows, const uint8_t *bytes, int row, int q4) {
+  __device__ __forceinline__ void read(uint8_t *rows, const int16_t *exps, int row, int q4) {
     // D = 128: elements 16 q .. and 64 + 16 q .. of each term; D = 64: 16 q .. of both
 #pragma unroll
     for (int n = 0; n < N; ++n)
@@ -329,7 +334,7 @@ struct MxQuery {
 #pragma unroll
         for (int e = 0; e < 4; ++e) t[n][4 * r + e] = (int)w[e];
       }
-    const int hi = bytes[row], lo = hi == 255 ? 255 : hi - 4;  // NaN and infinity: the whole row is NaN
+    const int hi = max((int)exps[row], kLeastExp), lo = hi == 255 ? 255 : hi - 4;  // 255: the row is NaN
     if constexpr (D == 128) scale[0] = hi, scale[1] = lo;
     else scale[0] = q4 < 2 ? hi : lo;
   }
@@ -397,7 +402,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_decode_mx_kernel(
   // first the query rows' terms, in the end per wave the partial rows of min(R, 16) columns
   extern __shared__ __attribute__((aligned(16))) float stage[];
   __shared__ float wm[NW][COLS], wsum[NW][COLS];
-  __shared__ uint8_t query_bytes[COLS];
+  __shared__ int16_t query_exps[COLS];
   uint8_t *query_rows = reinterpret_cast<uint8_t *>(stage);
   // The way to the first loads has no branches, and neither have they: a load behind one would have to
   // be waited for before the query rows, which come first.
@@ -445,7 +450,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_decode_mx_kernel(
           f32x2{-INFINITY, 0.f};
     return;
   }
-  split_queries<D>(q, R, query_rows, query_bytes, 64 * NW);
+  split_queries<D>(q, R, query_rows, query_exps, 64 * NW);
   __syncthreads();
 
   f32x4 oacc[NC][DT];
@@ -464,11 +469,13 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_decode_mx_kernel(
     constexpr bool kReread = NC == 2 && D == 128 && BITS == 8;
     MxQuery<D> query[NC];
     int pos[NC];  // last key that this lane's query column of a tile sees; none past the cache
+    float scale[NC];  // of its scores, in log2 units
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int col = min(16 * c + i16, R - 1);  // columns past the last repeat it
       pos[c] = min(len - Tq + col - (int)new_rows.quotient((uint32_t)col) * Tq, L - 1);
-      if (!kReread) query[c].read(query_rows, query_bytes, col, q4);
+      scale[c] = __builtin_ldexpf(scale_log2, min((int)query_exps[col] - kLeastExp, 0));
+      if (!kReread) query[c].read(query_rows, query_exps, col, q4);
     }
     // rotates byte g of a row's scale bytes to bits 30:23
     const uint32_t turn = (8 * (i16 * P::GR / 16) + 9) & 31;
@@ -488,7 +495,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_decode_mx_kernel(
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           asm volatile("" ::: "memory");  // keeps the reads inside the loop, one tile's at a time
-          query[0].read(query_rows, query_bytes, min(16 * c + i16, R - 1), q4);
+          query[0].read(query_rows, query_exps, min(16 * c + i16, R - 1), q4);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             i32x8 a[2];
@@ -525,7 +532,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_decode_mx_kernel(
         // score's rounding error would be left there, an exponent of any size for scores past 2^30
         // (0 to 1% of a call's time).
 #pragma unroll
-        for (int t = 0; t < 4; ++t) s[c][t] *= scale_log2;
+        for (int e = 0; e < 16; ++e) s[c][e >> 2][e & 3] *= scale[c];
         if (masked) {
 #pragma unroll
           for (int e = 0; e < 16; ++e)
