@@ -294,3 +294,14 @@ def test_oracle_positions_past_the_capacity():
     k = torch.zeros(5, 1, 6, 64, dtype=torch.float64)
     _, lse, _, _ = mx.decode(torch.zeros(5, 1, 3, 64), k, k, [6, 7, 8, 2**31 - 1, 1])
     assert lse.exp().round().view(5, 3).tolist() == [[4, 5, 6], [5, 6, 6], [6, 6, 6], [6, 6, 6], [0, 0, 1]]
+
+
+@pytest.mark.parametrize("rows", [1 << 31, (1 << 32) + 1])
+def test_row_counts_past_32_bits_are_refused(rows):
+    """Expanded rows take no memory, so that such a call can be made: (1 << 32) + 1 rows are not one row."""
+    k = _rows(1, 1, 1, 64).expand(1, 1, rows, 64)
+    lens = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(FlashAttnInputError, match="too many"):
+        kv.kv_cache_append(k, k, *_cpu_cache(1, 1), lens)
+    with pytest.raises(FlashAttnInputError, match="too many"):
+        kv.kv_cache_read(*_cpu_cache(1, 1), lens, rows)

@@ -89,6 +89,11 @@ def _check_cache(k_codes, k_scales, v_codes, v_scales, cache_seqlens):
     return B, Hkv, L, D, 8 * n // D
 
 
+def _check_rows(n):
+    if n > 0x7fffffff:  # the C ABI's int
+        raise FlashAttnInputError(f"{n} rows are too many for one call")
+
+
 def _check_device(*tensors):
     for t in tensors:
         if t.device.type != "cuda" or t.device != tensors[0].device:
@@ -115,6 +120,7 @@ def kv_cache_append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_s
                                   f"{tuple(k.shape)} and {tuple(v.shape)}")
     if k.dtype not in _DTYPES or v.dtype != k.dtype:
         raise FlashAttnInputError("k and v must both be bfloat16 or float32")
+    _check_rows(k.shape[2])
     strides = (ctypes.c_longlong * 6)(*_strides(k), *_strides(v))
     _check_device(k_codes, k_scales, v_codes, v_scales, cache_seqlens, k, v)
     if len({t.data_ptr() for t in (k_codes, k_scales, v_codes, v_scales)}) != 4:
@@ -139,6 +145,7 @@ def kv_cache_read(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.
     B, Hkv, L, D, bits = _check_cache(k_codes, k_scales, v_codes, v_scales, cache_seqlens)
     if rows < 1:
         raise FlashAttnInputError(f"rows must be positive, not {rows}")
+    _check_rows(rows)
     if dtype not in _DTYPES:
         raise FlashAttnInputError("rows are read as bfloat16 or float32")
     _check_device(k_codes, k_scales, v_codes, v_scales, cache_seqlens)
