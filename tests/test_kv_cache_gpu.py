@@ -799,3 +799,18 @@ def test_queries_of_few_bits_left(Hq, Hkv, L, D, bits):
     cache = [*mx.quantise(ramp.view(1, 1, L, D).to(BF), bits), *mx.quantise(v, bits)]
     got = kv.flash_attn_decode_mx(q.to(DEV), *_gpu(cache), _lens([L]))
     _check_sharp(q, cache, [L], mx.values(*cache[:2], bits), mx.values(*cache[2:], bits), got, L)
+
+
+# ---------------------------------------------------------------------------- large reads
+
+@pytest.mark.parametrize("D, B, Hkv, T", [(128, 3, 5, 4369), (128, 3, 5, 4370), (64, 2, 7, 9362), (64, 2, 7, 9363),
+                                          (128, 3, 5, 8738), (128, 3, 5, 8739)])
+def test_large_reads_of_8_bits_in_fp32(D, B, Hkv, T):
+    """Sizes around 2^21 lanes of four elements and around 2^24 elements, with a last workgroup that is part
+    empty."""
+    announce(f"kv large fp32 reads D={D} B={B} Hkv={Hkv} T={T}")
+    codes = torch.randint(0, 256, (B, Hkv, T, D), dtype=torch.uint8, generator=torch.Generator().manual_seed(T))
+    codes[(codes & 127) == 127] = 0
+    scales = (120 + codes[..., ::32] % 15).to(torch.uint8)
+    k, v = kv.kv_cache_read(*_gpu([codes, scales, codes ^ 0x80, scales]), _lens([T] * B), T, F32)
+    assert torch.equal(k.cpu(), mx.values(codes, scales, 8).float()) and torch.equal(v, -k)

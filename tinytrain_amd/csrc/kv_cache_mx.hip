@@ -186,10 +186,11 @@ hipError_t kv_dispatch(int D, int bits, bool f32, F f) {
 }
 
 // f(rows of a lane at once, grid) for `rows` rows of `lanes` lanes each.  Two rows at once keep more
-// loads on the way, which pays for 2^24 elements or more whose lanes load little each (TWO: appends of
-// bf16 81.7 -> 74.0 us at 16 x 8 x 4000 rows of D 128 in 8 bits, reads of 8 bits 74.4 -> 66.1; appends of
-// fp32 lose, 28.2 -> 29.5 at 2 x 8 x 8192, and reads of 4 bits, 19.6 -> 21.3 at 8 x 16384; so do small calls,
-// which leave CUs idle, 2.5 -> 2.8 at 32 x 8 rows).
+// loads on the way, which pays for some moves (TWO) of 2^21 lanes, of eight elements there, or more: appends
+// of bf16 81.7 -> 74.0 us at 16 x 8 x 4000 rows of D 128 in 8 bits, reads of 8 bits as bf16 74.4 -> 66.1, and
+// 22.4 -> 20.4 at 2^21 lanes; small calls, which leave CUs idle, lose (2.5 -> 2.8 at 32 x 8 rows).  The others
+// lose: appends of fp32 28.2 -> 29.5 at 2 x 8 x 8192, reads of 4 bits 19.6 -> 21.3 at 8 x 16384, reads of 8
+// bits as fp32, of four elements a lane, 15.7 -> 16.1 at 2^21 lanes and 67.0 -> 68.5 at 2^23.
 template <bool TWO, class F>
 hipError_t kv_launch(int rows, int lanes, F f) {
   auto go = [&](auto u) {
@@ -227,7 +228,7 @@ hipError_t launch_kv_read(const KvCache &cache, const int *cache_seqlens, void *
   return kv_dispatch(D, bits, f32, [&](auto d, auto b, auto t) {
     using T = decltype(t);
     constexpr int kD = decltype(d)::value, kBits = decltype(b)::value;
-    return kv_launch<kBits == 8>(rows, kD * (int)sizeof(T) / 16, [&](auto u, dim3 grid) {
+    return kv_launch<kBits == 8 && sizeof(T) == 2>(rows, kD * (int)sizeof(T) / 16, [&](auto u, dim3 grid) {
       kv_read_mx_kernel<kD, kBits, T, decltype(u)::value><<<grid, dim3(256), 0, stream>>>(
           cache, cache_seqlens, (T *)k, (T *)v, rows, Divisor(Hkv), Divisor(n_rows), Lmax);
     });
