@@ -814,3 +814,38 @@ def test_large_reads_of_8_bits_in_fp32(D, B, Hkv, T):
     scales = (120 + codes[..., ::32] % 15).to(torch.uint8)
     k, v = kv.kv_cache_read(*_gpu([codes, scales, codes ^ 0x80, scales]), _lens([T] * B), T, F32)
     assert torch.equal(k.cpu(), mx.values(codes, scales, 8).float()) and torch.equal(v, -k)
+
+
+# ------------------------------------------------------------------------- fp32 roundings
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_append_of_fp32_values_next_to_every_border(bits):
+    """The borders between neighbouring values of the type, under every power of two that a group may
+    have, with the fp32 values just below and above them; and groups whose largest magnitude lies just below,
+    at and above the border between two powers."""
+    announce(f"kv append fp32 borders bits={bits}")
+    top, lo, hi = mx.LIMITS[bits]
+    v, inf = mx.magnitudes(bits), torch.tensor(math.inf)
+    unit = torch.exp2(torch.arange(lo, hi + 1).double())[:, None]
+
+    def near(x):
+        x32 = x.float()
+        assert torch.equal(x32.double(), x)
+        return torch.stack([torch.nextafter(x32, -inf), x32, torch.nextafter(x32, inf)], -1)
+
+    mids = near((v[1:] + v[:-1]) / 2 * unit).flatten(1)                                  # [powers, 3 borders]
+    mids = torch.nn.functional.pad(mids, (0, -mids.shape[1] % 31)).unflatten(1, (-1, 31))
+    largest = (v[-1] * unit).float()[:, None].expand(-1, mids.shape[1], 1)               # fixes the power
+    groups = torch.cat([largest, mids], -1).flatten(0, 1)
+    assert mx.quantise(groups, bits)[1].view(-1, mids.shape[1])[:, 0].tolist() == list(range(lo + 127, hi + 128))
+    g = torch.Generator().manual_seed(56)
+    tops = near(top * unit).flatten()[:, None]
+    groups = torch.cat([groups, torch.cat([tops, tops * torch.rand(len(tops), 31, generator=g)], -1)])
+    groups = groups * (torch.randint(0, 2, groups.shape, generator=g) * 2 - 1)
+    groups = torch.nn.functional.pad(groups, (0, 0, 0, len(groups) % 2))
+    k = groups.view(1, 1, -1, 64)
+    T = k.shape[2]
+    got = _gpu(kv.mx_cache(1, 1, T, 64, bits, device="cpu"))
+    kv.kv_cache_append(k.to(DEV), -k.to(DEV), *got, _lens([T]))
+    for a, b in zip(_cpu(got), (*mx.quantise(k, bits), *mx.quantise(-k, bits))):
+        assert torch.equal(a, b)

@@ -8,8 +8,8 @@
 // a <= M 2^e, M the type's largest value plus half of its last step (6 + 1, 448 + 16): the
 // largest element then rounds down by no more than half a step, and on normal data the 4-bit
 // error is 3% below that of M = 6.  An element is x 2^-e rounded to nearest even, which the
-// hardware conversions do in one step (checked against the definition for every bf16 value and
-// a million fp32 values next to the rounding borders).  x 2^-e is exact, so the cache is defined
+// hardware conversions do in one step (tested against the definition with every bf16 value, and
+// with every rounding border and its fp32 neighbours under every e).  x 2^-e is exact, so the cache is defined
 // to the bit.  e is clamped so that every value is a finite normal bf16; a group with a NaN or an
 // infinity gets the byte 255, which the conversions read back as NaN.
 #include "fa_common.h"
