@@ -849,3 +849,33 @@ def test_append_of_fp32_values_next_to_every_border(bits):
     kv.kv_cache_append(k.to(DEV), -k.to(DEV), *got, _lens([T]))
     for a, b in zip(_cpu(got), (*mx.quantise(k, bits), *mx.quantise(-k, bits))):
         assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------ transforms
+
+def test_function_transforms():
+    """Under vmap attention and reads are loops of their calls; what has no rule (writing a cache under vmap,
+    tangents of recorded inputs) raises."""
+    import torch.autograd.forward_ad as fw
+
+    announce("kv transforms")
+    filled, _, _ = _filled(2, 2, 90, 64, 8, seed=57)
+    cache, lens = _gpu(filled), _lens([90, 40])
+    qs = torch.stack([_queries(2, 4, 1, 64, seed=s) for s in (0, 1, 2)]).to(DEV)
+    ks = torch.stack([_queries(2, 2, 1, 64, seed=s) for s in (3, 4)]).to(DEV)
+    got = torch.vmap(lambda q: kv.flash_attn_decode_mx(q, *cache, lens))(qs)
+    for i, q in enumerate(qs):
+        assert all(torch.equal(x[i], y) for x, y in zip(got, kv.flash_attn_decode_mx(q, *cache, lens)))
+    many = torch.stack([lens, lens - 30])
+    got = torch.vmap(lambda n: kv.kv_cache_read(*cache, n, 9, F32))(many)
+    for i, n in enumerate(many):
+        assert all(torch.equal(x[i], y) for x, y in zip(got, kv.kv_cache_read(*cache, n, 9, F32)))
+    with pytest.raises(RuntimeError, match="[Bb]atching rule"):
+        torch.vmap(lambda k: kv.kv_cache_append(k, k, *cache, lens))(ks)
+    assert all(torch.equal(a, b) for a, b in zip(_cpu(cache), filled))
+    want = kv.flash_attn_decode_mx(qs[0], *cache, lens)
+    with fw.dual_level():
+        got = kv.flash_attn_decode_mx(fw.make_dual(qs[0], torch.ones_like(qs[0])), *cache, lens)
+        assert all(torch.equal(fw.unpack_dual(x).primal, y) for x, y in zip(got, want))
+        with pytest.raises(NotImplementedError, match="forward mode AD"):
+            kv.flash_attn_decode_mx(fw.make_dual(qs[0].clone().requires_grad_(), torch.ones_like(qs[0])), *cache, lens)
