@@ -139,6 +139,16 @@ __device__ __forceinline__ void decode_block(const bf16 *Kt, const bf16 *Vt,
   }
 }
 
+// Places by which chunk `chunk` turns its units (n_units >= 8).  Consecutive workgroups go to the
+// XCDs in turn, and those of an XCD to its 32 CUs: 37 = 4 * 8 + 5 moves a unit's chunks to
+// other XCDs and other CUs.  Fewer units have more chunks, whose own numbers do that.
+__device__ __forceinline__ int chunk_turn(int chunk, int n_units) {
+  int turn = chunk * (n_units >= 64 ? 37 : 5);
+  if (n_units < 32) turn &= 7;
+  while (turn >= n_units) turn -= n_units;  // at most five times
+  return turn;
+}
+
 }  // namespace
 
 // Grid: (B * Hkv units, n_chunks), workgroups of NW waves.  Partial rows are indexed
