@@ -257,7 +257,8 @@ int ttfa_decode_fwd(const void *q, const void *k_cache, const void *v_cache,
  * cache stands for; q and o are bf16.  Query row t sits at position cache_seqlens[b] - Tq + t, also
  * where that is past the capacity (ttfa_decode_fwd clamps the length first), and sees the keys up to it
  * that the cache holds.  A score is within 2^-10 (on average 2^-19) of its sum of
- * |q_d k_d| * scale: the matrix unit cuts products of these types before it adds them in fp32.  Where
+ * |q_d k_d| * scale: the matrix unit cuts products of these types before it adds them in fp32.  LSE
+ * follows the scores: it is fp32, but no closer than they are.  Where
  * ttfa_decode_mx_workspace_bytes gives 0 (calls of one launch) the workspace is not used and may be NULL.
  *
  * Supported: bits 4 or 8 (TTFA_E_BITS), D in {64, 128}, dtype TTFA_BF16 or TTFA_F32 for the rows;

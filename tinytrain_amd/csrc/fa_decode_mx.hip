@@ -21,9 +21,10 @@
 //    (K through bf16 conversions took 32 more of about 200 vector instructions a half.)
 //    The instruction adds in fp32, but within every eight consecutive products it drops the bits below
 //    2^-13 of the largest (seen with pairs of products, in one eight and in two).  A score is off by less than
-//    2^-10 of the sum of those largest ones; measured, relative to sum |q k|, 2^-22 on average and
-//    2^-16.4 at most of 4096 random scores in 4 bits, 2^-19 and 2^-14.9 in 8 bits.  At scores of a few tens
-//    that is below the 2^-9 to which the weights are rounded, and far below what 4 or 8 bits left of K.
+//    2^-10 of the sum of those largest ones (at a sum of 30, by 0.03 at worst, and LSE by as much), most where
+//    one product outweighs its eight; measured, relative to sum |q k|, 2^-22 on average and 2^-16.4 at most
+//    of 4096 random scores in 4 bits, 2^-19 and 2^-14.9 in 8 bits.  At sums of a few hundred that is on average
+//    below the 2^-8 to which the weights are rounded, and far below what 4 or 8 bits left of K.
 //  * V: lane (i, q) loads D / 16 consecutive elements of each of the rows q + 4e, converts each
 //    row's to bf16 with that row's scale, and pairs up rows with v_perm, giving the A operands of
 //    D / 16 tiles whose row i is d = D / 16 * i + tile.  The scale goes by row, so it cannot move into
@@ -560,6 +561,8 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_decode_mx_kernel(
             rs += p[e];
           }
           l_part[c] += rs;
+          // The weights are rounded to bf16, as the product takes them beside V, whose values are bf16
+          // exactly: up to 2^-8 of each, which averages out over the keys; their sum is fp32 of the unrounded.
           const bf16x4 lo = pack4(p[0], p[1], p[2], p[3]), hi = pack4(p[4], p[5], p[6], p[7]);
           pb[c][u] = bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         }
@@ -760,10 +763,12 @@ namespace {
 // Waves of a one-chunk call: four, or eight, which halve a long cache's time where a CU has one
 // workgroup, and keep fewer caches on the device at once where it has several.  Times of eight waves
 // against four, uneven caches, then full ones:
-//  * up to 256 units, rows of 64 bytes or less: from 24 blocks on (192 units, D 128, 4 bits: 600 keys 0.94,
-//    1.01; 1000 1.01, 0.97; 1500 0.98, 0.94; 4000 0.89, 0.94), with 32 columns from 9 on (64 units, 512
-//    keys 0.94; 768 0.91; 192, 600 0.92), whose vector instructions then come in shorter runs.  Rows
-//    of 128 bytes have enough on the way with four (192 units: 1500 1.09, 1.09; 4000 1.05, 1.03).
+//  * up to 256 units, rows of 64 bytes or less: from 24 blocks on, which calls of 129 units or more have in
+//    one chunk (192 units, D 128, 4 bits: 600 keys 0.94, 1.01; 1000 1.01, 0.97; 1500 0.98, 0.94; 4000 0.89,
+//    0.94; 132, 144 and 256 units, uneven: 1536 0.97; 2000 0.94 to 0.95; 4000 0.90 to 0.93); with 32 columns
+//    from 9 on, whose vector instructions then come in shorter runs (64 units, 512 keys 0.94; 768 0.91; 192,
+//    600 0.92; 520 to 768 keys of 1 to 128 units: D 128, 4 bits 0.89 to 0.92, D 64 0.94 to 0.97).  Rows of 128
+//    bytes have enough on the way with four (192 units: 1500 1.09, 1.09; 4000 1.05, 1.03).
 //  * up to 447 units: from 32 blocks on (320 units: 600 keys 1.29, 1.25; 1000 1.11, 1.16; 2000 0.90, 1.08;
 //    4000 0.88, 1.05; 8 bits: 1000 1.01, 1.15; 2000 0.89, 1.06; 4000 0.87, 1.03; 32 columns: 600 1.38,
 //    2000 1.03, 4000 0.86).
@@ -779,6 +784,7 @@ int one_chunk_waves(int64_t units, int Lmax, int row_bytes, bool wide) {
 // 32 CUs: without a turn every chunk of a unit would share an XCD, or a CU, where the number of units is
 // a multiple of 8 (or 256), and a long cache would be read by few (16 caches of 8 heads, one of 16384
 // keys: 52 us without, 23 with).  37 = 4 * 8 + 5 moves a unit's chunks to other XCDs and other CUs.
+// fa_decode.hip turns by the chunk's number, fewer than 32 units by its last three bits.
 int chunk_turn(int units) { return (units >= 64 ? 37 : 5) % units; }
 
 struct MxCall {

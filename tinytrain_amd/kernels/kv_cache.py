@@ -18,9 +18,10 @@ rounded to nearest even.  A group with a NaN or an infinity reads back as NaN.
 ``cache_seqlens`` [B] int32 counts the new rows already, in every one of these calls: row t of T new (or
 wanted) ones of sequence b sits at position cache_seqlens[b] - T + t.  A length past max_seqlen
 shifts none of them: a query attends to the keys up to its own position that the cache holds.  Rows at positions outside
-0 .. max_seqlen - 1 are not written by ``kv_cache_append`` and are zeros from ``kv_cache_read``, so a batch of
-prompts padded on the left to T rows needs no mask, and ``cache_seqlens`` filled with n makes
-``kv_cache_read(..., rows=n)`` the first n rows.  A step of generation:
+0 .. max_seqlen - 1 are not written by ``kv_cache_append`` and are zeros from ``kv_cache_read``, so appending a batch
+of prompts padded on the left to T rows needs no mask, and ``cache_seqlens`` filled with n makes
+``kv_cache_read(..., rows=n)`` the first n rows.  (Zero rows are keys of score 0 to ``flash_attn``, which has no mask:
+attention over padded prompts takes the real rows, as ``flash_attn_varlen`` does.)  A step of generation:
 
     cache_seqlens += 1
     kv_cache_append(k, v, *cache, cache_seqlens)          # k, v [B, Hkv, 1, D]
