@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-#define TTFA_ABI_VERSION 8
+#define TTFA_ABI_VERSION 9
 
 enum ttfa_dtype { TTFA_BF16 = 0, TTFA_F32 = 1 };
 
@@ -51,8 +51,10 @@ enum ttfa_status {
   TTFA_E_EPS = -8,         /* eps is not in [0, 1)                               */
   TTFA_E_QROWS = -9,       /* decode: (Hq / Hkv) * Tq > 32                       */
   TTFA_E_SCRATCH = -10,    /* ttfa_bwd_static: B * Hq * T > TTFA_BWD_STATIC_MAX_ROWS */
-  TTFA_E_BITS = -11,       /* quantised cache: bits is not 4 or 8                */
+  TTFA_E_BITS = -11,       /* quantised cache or weight: bits is not 4 or 8      */
   TTFA_E_STRIDE = -12,     /* ttfa_kv_append: a stride is negative or no multiple of 16 bytes */
+  TTFA_E_COLS = -13,       /* block operators: a row length is no multiple of 8 (32 where rows are
+                              quantised), or out of range                        */
 };
 
 /* Library ABI version (TTFA_ABI_VERSION of the build). No reference counterpart. */
@@ -345,6 +347,67 @@ int ttfa_qk_prologue_bwd(const void *dq, const void *dk, const void *dv, const v
                          const float *rstd_k, void *dq_raw, void *dk_raw, void *dv_raw,
                          float *dq_norm_w, float *dk_norm_w, float *workspace, int B, int T,
                          int Hq, int Hkv, int D, void *hip_stream);
+
+/*
+ * Around attention in a block (model.py:128-139): rows of C (or K) elements, M of them, contiguous.
+ *
+ * RMSNorm with the residual's addition before it (model.py:24-35):
+ *   h = x + residual, in fp32, rounded to r_dtype;  y = h w / sqrt(mean(h^2) + eps), from that h
+ *   x [M, C] x_dtype, residual and h [M, C] r_dtype, w [C] fp32, y [M, C] y_dtype (each TTFA_BF16 or
+ *   TTFA_F32).  residual and h both NULL: h is x (r_dtype is not looked at).
+ * ttfa_rms_norm_mx gives y in 8 bits, rounded once from fp64: codes [M, C] and scales [M, C / 32], the
+ *   format of the quantised KV cache.
+ * ttfa_rms_norm_bwd: dy [M, C] y_dtype, dh [M, C] r_dtype or NULL (zeros), h (of the forward; x where it
+ *   had no residual) -> dr [M, C] r_dtype, the gradient of x and of residual, and dw [C] fp32.  dx, if
+ *   not NULL, gets the same in the other type (where x is of that type).  workspace:
+ *   ttfa_rms_norm_workspace_bytes (0: may be NULL).  One launch, or two; sums in a fixed order.
+ * C a multiple of 8 (32 for _mx) up to 16384; eps in [0, 1).
+ */
+int ttfa_rms_norm_fwd(const void *x, const void *residual, const float *w, void *y, void *h,
+                      long long M, int C, int x_dtype, int r_dtype, int y_dtype, double eps,
+                      void *hip_stream);
+
+int ttfa_rms_norm_mx(const void *x, const void *residual, const float *w, void *codes, void *scales,
+                     void *h, long long M, int C, int x_dtype, int r_dtype, double eps,
+                     void *hip_stream);
+
+long long ttfa_rms_norm_workspace_bytes(long long M, int C);
+
+int ttfa_rms_norm_bwd(const void *dy, const void *dh, const void *h, const float *w, void *dx, void *dr,
+                      float *dw, float *workspace, long long M, int C, int r_dtype, int y_dtype,
+                      double eps, void *hip_stream);
+
+/*
+ * Gated feed-forward input (model.py:111-125), bf16 with fp32 sums:
+ *   a = silu(x w_gate^T) * (x w_up^T):  x [M, K], w_gate and w_up [N, K], a [M, N]
+ * ttfa_swiglu_bwd: da [M, N] -> dx [M, K], dw_gate and dw_up [N, K]; dx, or both weight gradients, may be
+ * NULL (not computed).  The products are formed again, nothing of the forward is kept but its inputs.
+ * K and N multiples of 8, up to 2^20.  workspace: ttfa_swiglu_workspace_bytes of the pass (backward 0 or
+ * 1), or NULL where that is 0.
+ */
+long long ttfa_swiglu_workspace_bytes(int M, int K, int N, int backward);
+
+int ttfa_swiglu_fwd(const void *x, const void *w_gate, const void *w_up, void *a, void *workspace, int M,
+                    int K, int N, void *hip_stream);
+
+int ttfa_swiglu_bwd(const void *da, const void *x, const void *w_gate, const void *w_up, void *dx,
+                    void *dw_gate, void *dw_up, void *workspace, int M, int K, int N,
+                    void *hip_stream);
+
+/*
+ * Products with a quantised weight: y [M, N] bf16 = x W^T with W [N, K] in 4 or 8 bits, codes
+ * [N, K * bits / 8] and scales [N, K / 32] (uint8), the format of the quantised KV cache, and x [M, K]
+ * in bf16 (x_scales NULL) or in 8 bits (codes [M, K] and x_scales [M, K / 32], what ttfa_rms_norm_mx
+ * gives).  Exact products, fp32 sums.  K a multiple of 32 and N of 8, up to 2^20.
+ * ttfa_mx_quantize rounds rows x [M, K], `dtype`, into that format.
+ */
+int ttfa_mx_quantize(const void *x, void *codes, void *scales, long long M, int K, int bits, int dtype,
+                     void *hip_stream);
+
+long long ttfa_linear_mx_workspace_bytes(int M, int K, int N, int bits, int x_quantised);
+
+int ttfa_linear_mx(const void *x, const void *x_scales, const void *codes, const void *scales, void *y,
+                   void *workspace, int M, int K, int N, int bits, void *hip_stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,450 @@
+"""GPU tests of the block's operators (RMSNorm with the residual, gated feed-forward, products with quantised
+weights) against the 64-bit oracle.
+
+Tolerances count roundings.  u = 2^-24 for fp32, and half a step of the result's type at the end
+(bf16 2^-8, fp32 2^-24 of the value).
+* Norm: a lane adds at most 64 squares and the rows' lanes are joined in at most 8 steps, so the mean is off
+  by at most 72 u, its root by half of that, and five more roundings follow: 48 u with room.  Gradients:
+  two such sums and ten roundings on the terms: 160 u of the terms' sizes.  dw adds at most 5 rows a lane
+  (1024 workgroups), 32 lane groups and 64 + 16 partials, each term off by 48 u: 170 u with the sizes of
+  these tests.
+* Products: n terms in fp32, each addition off by at most 2 u (the matrix unit may cut instead of round):
+  2 n u of the sum of magnitudes.  The activation (an exponential and a reciprocal of one step each, the
+  argument of the exponential rounded) adds 2^-20 with |g| < 8.  dg and du are rounded to bf16 before the
+  last products: 2^-8 of their magnitudes.
+"""
+
+import math
+import random
+
+import pytest
+import torch
+
+from helpers import announce
+from oracle import block, mx_cache
+from tinytrain_amd import _lib
+from tinytrain_amd.kernels.linear_mx import linear_mx, mx_quantize
+from tinytrain_amd.kernels.rms_norm import add_rms_norm, add_rms_norm_mx, rms_norm, rms_norm_fwd
+from tinytrain_amd.kernels.swiglu import swiglu, swiglu_fwd
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+U = 2.0**-24
+
+
+def _rand(*shape, seed=0, dtype=F32, scale=1.0):
+    g = torch.Generator("cuda").manual_seed(seed)
+    return (scale * torch.randn(*shape, generator=g, device="cuda")).to(dtype)
+
+
+def _half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _within(name, got, want, tol):
+    """|got - want| <= tol + half a step of got's type, everywhere; NaN where the oracle has NaN."""
+    err = (got.double() - want).abs()
+    tol = tol + want.abs() * _half(got.dtype) * (1 + 2.0**-7) + 1e-37
+    bad = ~(err <= tol) & ~(torch.isnan(want) & torch.isnan(got.double())) & ~(got.double() == want)
+    assert not bad.any(), f"{name}: {int(bad.sum())} of {bad.numel()} off, worst {(err / tol).nan_to_num(0).max():.3g} of the tolerance"
+
+
+# ----------------------------------------------------------------------------------- norm
+
+NORM_SHAPES = [(1, 8), (3, 64), (37, 72), (5, 256), (130, 768), (33, 1000), (9, 2048), (7, 2056), (6, 4096), (5, 8200),
+               (3, 16384), (5000, 96), (4100, 768)]
+
+
+@pytest.mark.parametrize("M, C", NORM_SHAPES)
+@pytest.mark.parametrize("xt, rt", [(BF, BF), (BF, F32), (F32, BF), (F32, F32)])
+def test_add_rms_norm(M, C, xt, rt):
+    announce(f"add_rms_norm M={M} C={C} {xt} {rt}")
+    x, r = _rand(M, C, seed=1, dtype=xt), _rand(M, C, seed=2, dtype=rt, scale=3.0)
+    w = 1 + 0.3 * _rand(C, seed=3)
+    t = [v.requires_grad_() for v in (x, r, w)]
+    yt = F32 if (M + C) % 3 == 0 else BF
+    y, h = add_rms_norm(*t, 1e-6, yt)
+    assert y.dtype == yt and h.dtype == rt
+    want, stored = block.add_rms_norm(x.detach(), r.detach(), w.detach(), 1e-6)
+    assert torch.equal(h, stored)
+    _within("y", y.detach(), want, 48 * U * want.abs())
+    dy, dh = _rand(M, C, seed=4, dtype=yt), _rand(M, C, seed=5, dtype=rt)
+    dx, dr, dw = torch.autograd.grad((y, h), t, (dy, dh))
+    assert (dx.dtype, dr.dtype, dw.dtype) == (xt, rt, F32)
+    d, size, wantw, sizew = block.add_rms_norm_grads(dy, dh, stored, w.detach(), 1e-6)
+    _within("dx", dx, d, 160 * U * size)
+    _within("dr", dr, d, 160 * U * size)
+    _within("dw", dw, wantw, 170 * U * sizew)
+
+
+@pytest.mark.parametrize("xt", [BF, F32])
+@pytest.mark.parametrize("shape", [(7, 64), (2, 3, 1000), (4096,)])
+def test_rms_norm_alone(shape, xt):
+    announce(f"rms_norm {shape} {xt}")
+    x, w = _rand(*shape, seed=1, dtype=xt).requires_grad_(), (1 + 0.3 * _rand(shape[-1], seed=2)).to(BF).requires_grad_()
+    y = rms_norm(x, w, 1e-5, BF)
+    want, _ = block.add_rms_norm(x.detach(), None, w.detach(), 1e-5)
+    _within("y", y.detach(), want, 48 * U * want.abs())
+    dy = _rand(*shape, seed=3, dtype=BF)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    d, size, wantw, sizew = block.add_rms_norm_grads(dy, None, x.detach(), w.detach(), 1e-5)
+    _within("dx", dx, d, 160 * U * size)
+    assert dw.dtype == BF
+    _within("dw", dw, wantw, 170 * U * sizew)
+
+
+def test_norm_unused_outputs_and_strided_gradients():
+    """A gradient through h alone or y alone, expanded and transposed gradients."""
+    x, r, w = _rand(40, 72, seed=1, dtype=BF), _rand(40, 72, seed=2), _rand(72, seed=3)
+    t = [v.requires_grad_() for v in (x, r, w)]
+    g = _rand(72, 40, seed=4).t()
+    y, h = add_rms_norm(*t)
+    dx, dr, dw = torch.autograd.grad(h, t, g, allow_unused=True, retain_graph=True)
+    assert torch.equal(dr, g) and torch.equal(dx, g.to(BF)) and (dw is None or not dw.any())
+    gy = torch.ones(1, 1, device="cuda", dtype=BF).expand(40, 72)
+    dx, dr, dw = torch.autograd.grad(y, t, gy)
+    d, size, wantw, sizew = block.add_rms_norm_grads(gy, None, h.detach(), w.detach(), 1e-6)
+    _within("dr", dr, d, 160 * U * size)
+    _within("dx", dx, d, 160 * U * size)
+    _within("dw", dw, wantw, 170 * U * sizew)
+
+
+def test_norm_special_rows():
+    """A row of zeros, rows with NaN and infinity, and their neighbours."""
+    x, r, w = _rand(6, 96, seed=1, dtype=BF), _rand(6, 96, seed=2, dtype=BF), _rand(96, seed=3)
+    x[1] = 0
+    r[1] = 0
+    x[2, 5] = math.nan
+    r[4, 7] = math.inf
+    want, stored = block.add_rms_norm(x, r, w, 1e-6)
+    y, h = add_rms_norm(x, r, w)
+    assert torch.equal(h.nan_to_num(-1), stored.nan_to_num(-1)) and not y[1].any()
+    for row in (0, 1, 3, 5):
+        _within("y", y[row], want[row], 48 * U * want[row].abs())
+    assert torch.isnan(y[2]).all() and torch.isnan(y[4, 7])
+    codes, scales, _ = add_rms_norm_mx(x, r, w)
+    assert (scales[2] == 255).all() and not codes[2].any()
+    assert not (codes[1] & 127).any()  # zeros, of the weights' signs
+    assert (scales[[0, 1, 3, 5]] != 255).all()
+    y0, _ = add_rms_norm(x * 0, r * 0, w, 0.0)   # 0 / 0, as the formula has it
+    assert torch.isnan(y0).all()
+
+
+@pytest.mark.parametrize("M, C", [(1, 32), (33, 96), (130, 768), (9, 2048), (7, 2080), (6, 4096), (3, 16384)])
+@pytest.mark.parametrize("xt, rt", [(BF, BF), (F32, F32), (BF, F32), (F32, None)])
+def test_add_rms_norm_mx(M, C, xt, rt):
+    """Bytes equal to the definition's: y in 64 bits, rounded once."""
+    announce(f"add_rms_norm_mx M={M} C={C} {xt} {rt}")
+    x = _rand(M, C, seed=1, dtype=xt)
+    r = None if rt is None else _rand(M, C, seed=2, dtype=rt, scale=3.0)
+    w = 1 + 0.3 * _rand(C, seed=3)
+    codes, scales, h = add_rms_norm_mx(x, r, w, 1e-6)
+    want, stored = block.add_rms_norm(x, r, w, 1e-6)
+    assert torch.equal(h, stored)
+    c, s = mx_cache.quantise(want.cpu(), 8)
+    assert torch.equal(scales.cpu(), s) and torch.equal(codes.cpu(), c)
+
+
+def test_norm_empty_and_other_ranks():
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    for shape in ((0, 64), (2, 0, 64)):
+        x, r = torch.empty(shape, device="cuda", dtype=BF, requires_grad=True), torch.empty(shape, device="cuda")
+        y, h = add_rms_norm(x, r, w)
+        assert y.shape == h.shape == shape
+        dx, dw = torch.autograd.grad((y.float() + h).sum(), (x, w))
+        assert dx.shape == shape and not dw.any()
+        codes, scales, _ = add_rms_norm_mx(x.detach(), r, w.detach())
+        assert codes.shape == shape and scales.shape == (*shape[:-1], 2)
+
+
+# --------------------------------------------------------------------------------- swiglu
+
+SWIGLU_SHAPES = [(1, 8, 8), (1, 768, 2304), (5, 64, 72), (16, 104, 200), (33, 768, 328), (100, 40, 136), (128, 32, 128),
+                 (129, 200, 264), (300, 1000, 520), (1000, 136, 1032), (2051, 72, 128)]
+
+
+def _check_swiglu(M, K, N):
+    x = _rand(M, K, seed=1, dtype=BF).requires_grad_()
+    wg, wu = (_rand(N, K, seed=s, dtype=BF, scale=1 / math.sqrt(K)).requires_grad_() for s in (2, 3))
+    a = swiglu(x, wg, wu)
+    want, unit = block.swiglu(*(t.detach() for t in (x, wg, wu)))
+    _within("a", a.detach(), want, 2 * K * U * unit + 2.0**-20 * want.abs())
+    da = _rand(M, N, seed=4, dtype=BF)
+    grads = torch.autograd.grad(a, (x, wg, wu), da)
+    oracle = block.swiglu_grads(da, *(t.detach() for t in (x, wg, wu)))
+    for g, (name, (want, size, unit)) in zip(grads, oracle.items()):
+        n = 2 * N if name == "dx" else M
+        _within(name, g, want, (2.0**-8 + 2.0**-20 + 2 * n * U) * size + 2 * K * U * 1.01 * unit)
+    return a, grads
+
+
+@pytest.mark.parametrize("M, K, N", SWIGLU_SHAPES)
+def test_swiglu(M, K, N):
+    announce(f"swiglu M={M} K={K} N={N}")
+    a, grads = _check_swiglu(M, K, N)
+    again, grads2 = _check_swiglu(M, K, N)
+    assert torch.equal(a, again) and all(torch.equal(p, q) for p, q in zip(grads, grads2))
+
+
+def test_swiglu_random_sizes():
+    rng = random.Random(7)
+    for _ in range(12):
+        M, K, N = rng.randint(1, 700), 8 * rng.randint(1, 90), 8 * rng.randint(1, 120)
+        announce(f"swiglu M={M} K={K} N={N}")
+        _check_swiglu(M, K, N)
+
+
+def test_swiglu_needs_and_strides():
+    """Frozen inputs get no gradient, the others the same bits; gradients with other strides; 3-D rows."""
+    x, wg, wu = _rand(6, 7, 64, seed=1, dtype=BF), _rand(48, 64, seed=2, dtype=BF), _rand(48, 64, seed=3, dtype=BF)
+    da = _rand(6, 48, 7, seed=4, dtype=BF).transpose(1, 2)
+    full = torch.autograd.grad(swiglu(*(t.requires_grad_() for t in (x, wg, wu))), (x, wg, wu), da)
+    for need in ((1, 0, 0), (0, 1, 1), (0, 0, 1)):
+        t = [v.detach().clone().requires_grad_(bool(n)) for v, n in zip((x, wg, wu), need)]
+        got = torch.autograd.grad(swiglu(*t), [v for v, n in zip(t, need) if n], da)
+        for g, w in zip(got, [f for f, n in zip(full, need) if n]):
+            assert torch.equal(g, w)
+    flat = torch.autograd.grad(swiglu(x.view(42, 64), wg, wu), x, da.contiguous().view(42, 48))
+    assert torch.equal(flat[0], full[0])
+    e = torch.empty(0, 64, device="cuda", dtype=BF, requires_grad=True)
+    a = swiglu(e, wg, wu)
+    ge, gg = torch.autograd.grad(a.sum(), (e, wg))
+    assert a.shape == (0, 48) and ge.shape == e.shape and not gg.any()
+
+
+@pytest.mark.parametrize("M", [3, 200])
+def test_swiglu_keeps_nan_and_infinity_in_place(M):
+    """A NaN in a row of x reaches that row of a and of dx and its columns of the weights' gradients; one in a
+    row of a weight reaches that column of a."""
+    K, N = 104, 136
+    x, wg, wu = _rand(M, K, seed=1, dtype=BF), _rand(N, K, seed=2, dtype=BF), _rand(N, K, seed=3, dtype=BF)
+    da = _rand(M, N, seed=4, dtype=BF)
+    clean = swiglu(x, wg, wu)
+    t = [v.clone().requires_grad_() for v in (x, wg, wu)]
+    cgrads = torch.autograd.grad(swiglu(*t), t, da)
+    bad = x.clone()
+    bad[1, K - 1] = math.nan
+    t = [bad.requires_grad_(), wg.clone().requires_grad_(), wu.clone().requires_grad_()]
+    a = swiglu(*t)
+    dx, dwg, _ = torch.autograd.grad(a, t, da)
+    rows = [m for m in range(M) if m != 1]
+    assert torch.isnan(a[1]).all() and torch.equal(a[rows], clean[rows])
+    assert torch.isnan(dx[1]).all() and torch.equal(dx[rows], cgrads[0][rows]) and torch.isnan(dwg).all()
+    bad = wu.clone()
+    bad[N - 1, 0] = math.inf
+    a = swiglu(x, wg, bad)
+    assert torch.equal(a[:, :N - 1], clean[:, :N - 1]) and not torch.isfinite(a[:, N - 1]).any()
+
+
+def test_swiglu_activation_at_its_ends():
+    """Large gates of either sign: silu is g, or 0."""
+    g = torch.tensor([0.0, 1.0, -1.0, 20.0, -20.0, 80.0, -80.0, 200.0, -200.0, 3e4, -3e4], device="cuda")
+    x = torch.zeros(len(g), 8, device="cuda", dtype=BF)
+    x[:, 0], x[:, 1] = g, 1.0
+    wg, wu = torch.zeros(8, 8, device="cuda", dtype=BF), torch.zeros(8, 8, device="cuda", dtype=BF)
+    wg[:, 0], wu[:, 1] = 1.0, 1.0
+    x.requires_grad_()
+    a = swiglu(x, wg, wu)
+    want, _ = block.swiglu(x.detach(), wg, wu)
+    # sig = 1 / (1 + 2^(-g log2 e)): the exponent's rounding is 2^-23 |g|
+    _within("a", a.detach(), want, want.abs() * (2.0**-20 + 2.0**-22 * g.abs().double().clamp(max=130))[:, None] + 1e-36)
+    assert torch.isfinite(torch.autograd.grad(a, x, torch.ones_like(a))[0]).all()
+
+
+# -------------------------------------------------------------------------- quantised weights
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("shape", [(8, 32), (3, 5, 96), (40, 4096), (0, 64)])
+def test_mx_quantize(shape, dtype, bits):
+    announce(f"mx_quantize {shape} {dtype} {bits}")
+    x = _rand(*shape, seed=1, dtype=dtype) * torch.exp2(torch.arange(shape[-1], device="cuda") % 40 - 20).to(dtype)
+    codes, scales = mx_quantize(x, bits)
+    c, s = mx_cache.quantise(x.cpu(), bits) if x.numel() else (codes.cpu(), scales.cpu())
+    assert torch.equal(codes.cpu(), c) and torch.equal(scales.cpu(), s)
+
+
+LINEAR_SHAPES = [(1, 32, 8), (1, 4096, 520), (2, 96, 40), (7, 736, 104), (16, 128, 64), (17, 1024, 72), (32, 160, 136),
+                 (33, 512, 264), (64, 2048, 48), (65, 288, 128), (150, 640, 328), (520, 256, 392), (1027, 96, 136)]
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("x8", [False, True])
+@pytest.mark.parametrize("M, K, N", LINEAR_SHAPES)
+def test_linear_mx(M, K, N, x8, bits):
+    announce(f"linear_mx M={M} K={K} N={N} bits={bits} x8={x8}")
+    x = _rand(M, K, seed=1, dtype=BF)
+    codes, scales = mx_quantize(_rand(N, K, seed=2, scale=1 / math.sqrt(K)), bits)
+    xs = None
+    if x8:
+        x, xs = mx_quantize(x, 8)
+    y = linear_mx(x, codes, scales, xs)
+    want, size = block.linear_mx(x, xs, codes, scales)
+    _within("y", y.cpu(), want, 2 * K * U * size)
+    assert torch.equal(y, linear_mx(x, codes, scales, xs))
+
+
+@pytest.mark.parametrize("M", [2, 300])
+def test_linear_mx_keeps_nan_in_place_and_takes_odd_scales(M):
+    """A group of NaN in x reaches its row, one in W its column; groups of very different powers of two."""
+    K, N = 192, 72
+    x = _rand(M, K, seed=1, dtype=BF)
+    x[:, 32:64] *= 2.0**40
+    w = _rand(N, K, seed=2)
+    w[:, 32:64] *= 2.0**-40
+    w[5, 64:96] *= 2.0**60
+    for bits in (4, 8):
+        codes, scales = mx_quantize(w, bits)
+        for xs in (None, True):
+            xx, xx_s = (x, None) if xs is None else mx_quantize(x, 8)
+            want, size = block.linear_mx(xx, xx_s, codes, scales)
+            y = linear_mx(xx, codes, scales, xx_s)
+            _within("y", y.cpu(), want, 2 * K * U * size)
+            bad = scales.clone()
+            bad[3, 5] = 255
+            got = linear_mx(xx, codes, bad, xx_s)
+            keep = [n for n in range(N) if n != 3]
+            assert torch.isnan(got[:, 3]).all() and torch.equal(got[:, keep], y[:, keep])
+            rows = [m for m in range(M) if m != 1]
+            if xs is None:
+                xb = xx.clone()
+                xb[1, K - 1] = math.nan
+                got = linear_mx(xb, codes, scales)
+            else:
+                sb = xx_s.clone()
+                sb[1, 0] = 255
+                got = linear_mx(xx, codes, scales, sb)
+            assert torch.isnan(got[1]).all() and torch.equal(got[rows], y[rows])
+
+
+# ------------------------------------------------------------------- paths, streams, graphs
+
+def test_rows_behind_the_last_are_left():
+    """Outputs are written up to their last row and no further (C ABI, buffers with rows to spare)."""
+    lib, s = _lib.load(), torch.cuda.current_stream().cuda_stream
+    for M in (1, 5, 37, 130, 513):
+        K, N = 96, 136
+        x, r = _rand(M, K, seed=1, dtype=BF), _rand(M, K, seed=2, dtype=BF)
+        w, wg, wu = _rand(K, seed=3), _rand(N, K, seed=4, dtype=BF), _rand(N, K, seed=5, dtype=BF)
+        codes, scales = mx_quantize(wg, 4)
+        out = {n: torch.full((M + 2, c), 7.0, device="cuda", dtype=BF)
+               for n, c in (("y", K), ("h", K), ("a", N), ("lin", N), ("dx", K), ("dr", K))}
+        dw = torch.full((K + 8,), 7.0, device="cuda")
+        dwg, dwu = (torch.full((N + 2, K), 7.0, device="cuda", dtype=BF) for _ in range(2))
+        p = {n: t.data_ptr() for n, t in out.items()}
+        ws = torch.empty(max(lib.ttfa_swiglu_workspace_bytes(M, K, N, 1), lib.ttfa_swiglu_workspace_bytes(M, K, N, 0),
+                             lib.ttfa_rms_norm_workspace_bytes(M, K),
+                             lib.ttfa_linear_mx_workspace_bytes(M, K, N, 4, 0), 16), device="cuda", dtype=torch.uint8)
+        da = _rand(M, N, seed=6, dtype=BF)
+        assert lib.ttfa_rms_norm_fwd(x.data_ptr(), r.data_ptr(), w.data_ptr(), p["y"], p["h"], M, K, 0, 0, 0, 1e-6, s) == 0
+        assert lib.ttfa_rms_norm_bwd(x.data_ptr(), None, r.data_ptr(), w.data_ptr(), None, p["dr"], dw.data_ptr(),
+                                     ws.data_ptr(), M, K, 0, 0, 1e-6, s) == 0
+        assert lib.ttfa_swiglu_fwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), p["a"], ws.data_ptr(), M, K, N, s) == 0
+        assert lib.ttfa_swiglu_bwd(da.data_ptr(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), p["dx"], dwg.data_ptr(),
+                                   dwu.data_ptr(), ws.data_ptr(), M, K, N, s) == 0
+        assert lib.ttfa_linear_mx(x.data_ptr(), None, codes.data_ptr(), scales.data_ptr(), p["lin"], ws.data_ptr(), M, K,
+                                  N, 4, s) == 0
+        torch.cuda.synchronize()
+        for n, t in out.items():
+            assert (t[M:] == 7).all() and not (t[:M] == 7).all(), n
+        assert (dw[K:] == 7).all() and (dwg[N:] == 7).all() and (dwu[N:] == 7).all()
+
+
+def test_native_path_equals_the_ops():
+    """The extension's calls and the custom ops: equal bits, forward and backward."""
+    x, r, w = _rand(37, 96, seed=1, dtype=BF), _rand(37, 96, seed=2), _rand(96, seed=3)
+    wg, wu = _rand(72, 96, seed=4, dtype=BF), _rand(72, 96, seed=5, dtype=BF)
+    def grads(y, ts):
+        return torch.autograd.grad(y, ts, [torch.ones_like(v) for v in y])
+    t = [v.requires_grad_() for v in (x, r, w)]
+    a, b = add_rms_norm(*t, 1e-6, BF), rms_norm_fwd(*t, 1e-6, BF)
+    assert type(a[0].grad_fn).__name__ != type(b[0].grad_fn).__name__  # two paths
+    for p, q in zip((*a, *grads(a, t)), (*b, *grads(b, t))):
+        assert torch.equal(p, q)
+    t = [v.requires_grad_() for v in (x.detach(), wg, wu)]
+    a, b = swiglu(*t), swiglu_fwd(*t)
+    for p, q in zip((a, *grads([a], t)), (b, *grads([b], t))):
+        assert torch.equal(p, q)
+    torch.library.opcheck(rms_norm_fwd, (x.detach(), r.detach(), w.detach(), 1e-6, BF))
+    torch.library.opcheck(swiglu_fwd, (x.detach(), wg.detach(), wu.detach()))
+
+
+def test_saved_tensor_hooks():
+    """A backward whose saved tensors come back elsewhere or in another layout."""
+    x, r, w = (_rand(37, 96, seed=1, dtype=BF).requires_grad_(), _rand(37, 96, seed=2).requires_grad_(),
+               _rand(96, seed=3).requires_grad_())
+    wg, wu = _rand(72, 96, seed=4, dtype=BF).requires_grad_(), _rand(72, 96, seed=5, dtype=BF).requires_grad_()
+
+    def run():
+        y, h = add_rms_norm(x, r, w)
+        return torch.autograd.grad(swiglu(y, wg, wu).float().sum() + h.sum(), (x, r, w, wg, wu))
+    plain = run()
+    with torch.autograd.graph.save_on_cpu():
+        for p, q in zip(plain, run()):
+            assert torch.equal(p, q)
+
+
+def test_other_stream():
+    s = torch.cuda.Stream()
+    x, r, w = _rand(500, 768, seed=1, dtype=BF), _rand(500, 768, seed=2, dtype=BF), _rand(768, seed=3)
+    wg, wu = _rand(520, 768, seed=4, dtype=BF), _rand(520, 768, seed=5, dtype=BF)
+    codes, scales = mx_quantize(wg, 4)
+    want = (*add_rms_norm(x, r, w), swiglu(x, wg, wu), linear_mx(x, codes, scales), *add_rms_norm_mx(x, r, w))
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = (*add_rms_norm(x, r, w), swiglu(x, wg, wu), linear_mx(x, codes, scales), *add_rms_norm_mx(x, r, w))
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_captured_step_replays():
+    """A training step of norm and feed-forward and a serving step over quantised rows in one graph, replayed with
+    new inputs and eager work between, bitwise the eager results."""
+    M, C, N = 130, 96, 136
+    x, r, w = _rand(M, C, seed=1, dtype=BF), _rand(M, C, seed=2), _rand(C, seed=3)
+    wg, wu = _rand(N, C, seed=4, dtype=BF), _rand(N, C, seed=5, dtype=BF)
+    da, weight = _rand(M, N, seed=6, dtype=BF), mx_quantize(wg, 4)
+    t = [v.requires_grad_() for v in (x, r, w, wg, wu)]
+
+    def step():
+        y, h = add_rms_norm(x, r, w)
+        a = swiglu(y, wg, wu)
+        out = [a.detach(), h.detach(), *torch.autograd.grad((a, h), t, (da, torch.ones_like(h)))]
+        codes, scales, h2 = add_rms_norm_mx(x.detach(), r.detach(), w.detach())
+        return out + [codes, scales, h2, linear_mx(codes, *weight, scales), linear_mx(a.detach()[:, :C].contiguous(), *weight)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for i in range(4):
+        with torch.no_grad():
+            x.copy_(_rand(M, C, seed=20 + i, dtype=BF))
+            da.copy_(_rand(M, N, seed=30 + i, dtype=BF))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [v.clone() for v in captured]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
+        torch.cuda.synchronize()
+
+
+def test_serving_step_as_used():
+    """Norm to 8 bits, gate and up projections in 4 bits, activation, norm again: the run against one in 64 bits
+    over the values that the bytes stand for."""
+    M, C, N = 5, 256, 512
+    x, h0, w = _rand(M, C, seed=1, dtype=BF), _rand(M, C, seed=2, dtype=BF), 1 + 0.2 * _rand(C, seed=3)
+    wg, wu, wd = (mx_quantize(_rand(*s, seed=i, scale=1 / 16), 4) for i, s in ((4, (N, C)), (5, (N, C)), (6, (C, N))))
+    codes, scales, h = add_rms_norm_mx(x, h0, w)
+    g, u = linear_mx(codes, *wg, scales), linear_mx(codes, *wu, scales)
+    y = linear_mx((torch.nn.functional.silu(g) * u), *wd)
+    out, _ = add_rms_norm(y, h, w)
+    v = mx_cache.values(codes.cpu(), scales.cpu(), 8)
+    W = [mx_cache.values(c.cpu(), s.cpu(), 4) for c, s in (wg, wu, wd)]
+    a = torch.nn.functional.silu(v @ W[0].t()) * (v @ W[1].t())
+    want, _ = block.add_rms_norm((a @ W[2].t()).float(), h.cpu().float(), w.cpu(), 1e-6)
+    # four roundings to bf16 on the branch and two on the way out, each 2^-8 at most
+    assert (out.cpu().double() - want).norm() <= 6 * 2.0**-8 * want.norm()

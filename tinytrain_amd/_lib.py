@@ -21,11 +21,11 @@ NATIVE_PATH = _PKG / "_ttfa_torch.so"
 
 TTFA_BF16 = 0
 TTFA_F32 = 1
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 # Negative status codes of include/ttfa.h.
 (E_NULL, E_HEAD_DIM, E_GROUP, E_SEQ, E_ALIGN, E_DTYPE, E_SCALE, E_EPS, E_QROWS, E_SCRATCH, E_BITS,
- E_STRIDE) = (-1, -2, -3, -4, -5, -6, -7, -8, -9, -10, -11, -12)
+ E_STRIDE, E_COLS) = (-1, -2, -3, -4, -5, -6, -7, -8, -9, -10, -11, -12, -13)
 BWD_STATIC_MAX_ROWS = 1 << 20  # TTFA_BWD_STATIC_MAX_ROWS
 EXPORTED = ("ttfa_abi_version", "ttfa_strerror", "ttfa_fwd", "ttfa_bwd", "ttfa_bwd_dq",
             "ttfa_bwd_dkdv", "ttfa_varlen_fwd", "ttfa_varlen_bwd", "ttfa_decode_workspace_bytes",
@@ -33,7 +33,10 @@ EXPORTED = ("ttfa_abi_version", "ttfa_strerror", "ttfa_fwd", "ttfa_bwd", "ttfa_b
             "ttfa_qk_prologue_workspace_bytes", "ttfa_qk_prologue_bwd", "ttfa_bwd_static",
             "ttfa_d128_wide", "ttfa_qk_prologue_fwd_tables", "ttfa_qk_prologue_bwd_tables",
             "ttfa_bwd_workspace_bytes", "ttfa_bwd_ws", "ttfa_kv_append", "ttfa_kv_read",
-            "ttfa_decode_mx_workspace_bytes", "ttfa_decode_mx_fwd")
+            "ttfa_decode_mx_workspace_bytes", "ttfa_decode_mx_fwd", "ttfa_rms_norm_fwd",
+            "ttfa_rms_norm_mx", "ttfa_rms_norm_workspace_bytes", "ttfa_rms_norm_bwd",
+            "ttfa_swiglu_workspace_bytes", "ttfa_swiglu_fwd", "ttfa_swiglu_bwd", "ttfa_mx_quantize",
+            "ttfa_linear_mx_workspace_bytes", "ttfa_linear_mx")
 
 
 class LibraryNotBuilt(RuntimeError):
@@ -53,6 +56,7 @@ _lock = threading.Lock()
 _lib = None
 
 _vp, _i, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+_ll, _d = ctypes.c_longlong, ctypes.c_double
 _SIGS = {
     "ttfa_abi_version": ([], _i),
     "ttfa_strerror": ([_i], ctypes.c_char_p),
@@ -76,6 +80,16 @@ _SIGS = {
     "ttfa_qk_prologue_fwd_tables": ([_vp] * 7 + [_i] + [_vp] * 5 + [_i] * 5 + [_f, _vp], _i),
     "ttfa_qk_prologue_bwd_tables": ([_vp] * 9 + [_i] + [_vp] * 8 + [_i] * 5 + [_vp], _i),
     "ttfa_bwd_static": ([_vp] * 9 + [_i] * 6 + [_f, _vp], _i),
+    "ttfa_rms_norm_fwd": ([_vp] * 5 + [_ll] + [_i] * 4 + [_d, _vp], _i),
+    "ttfa_rms_norm_mx": ([_vp] * 6 + [_ll] + [_i] * 3 + [_d, _vp], _i),
+    "ttfa_rms_norm_workspace_bytes": ([_ll, _i], _ll),
+    "ttfa_rms_norm_bwd": ([_vp] * 8 + [_ll] + [_i] * 3 + [_d, _vp], _i),
+    "ttfa_swiglu_workspace_bytes": ([_i] * 4, _ll),
+    "ttfa_swiglu_fwd": ([_vp] * 5 + [_i] * 3 + [_vp], _i),
+    "ttfa_swiglu_bwd": ([_vp] * 8 + [_i] * 3 + [_vp], _i),
+    "ttfa_mx_quantize": ([_vp] * 3 + [_ll] + [_i] * 3 + [_vp], _i),
+    "ttfa_linear_mx_workspace_bytes": ([_i] * 5, _ll),
+    "ttfa_linear_mx": ([_vp] * 6 + [_i] * 4 + [_vp], _i),
     "ttfa_d128_wide": ([_i] * 3 + [ctypes.POINTER(_i)] * 2, _i),
 }
 
@@ -125,6 +139,7 @@ class _OpsOnly:
 
     flash_attn = flash_attn_varlen = flash_attn_decode = qk_norm_rope = _pass
     kv_cache_append = kv_cache_read = flash_attn_decode_mx = _pass
+    add_rms_norm = add_rms_norm_mx = swiglu = linear_mx = _pass
 
 
 _native = None

@@ -92,6 +92,36 @@ hipError_t launch_decode_mx(const void *q, const KvCache &cache, const int *cach
                             float *lse, float *workspace, int B, int Hq, int Hkv, int Tq, int Lmax,
                             int D, int bits, float scale, hipStream_t stream);
 
+// `elements` (a multiple of 32) of rows into the same format.
+hipError_t launch_mx_quantize(const void *x, void *codes, void *scales, int64_t elements, int bits,
+                              bool f32, hipStream_t stream);
+
+// y [M, N] bf16 = x W^T: x [M, K] bf16 (x_scales null) or in 8 bits, W [N, K] in `bits` (linear_mx.hip).
+hipError_t launch_linear_mx(const void *x, const void *x_scales, const void *codes, const void *scales,
+                            void *y, int M, int K, int N, int bits, hipStream_t stream);
+
+// RMSNorm of x + r over rows of C (rms_norm.hip); r and h null: of x.  Types by ttfa_dtype.
+hipError_t launch_rms_norm_fwd(const void *x, const void *r, const float *w, void *y, void *h,
+                               int64_t M, int C, int x_dtype, int r_dtype, int y_dtype, double eps,
+                               hipStream_t stream);
+hipError_t launch_rms_norm_mx(const void *x, const void *r, const float *w, void *codes, void *scales,
+                              void *h, int64_t M, int C, int x_dtype, int r_dtype, double eps,
+                              hipStream_t stream);
+// dr in h's type; dx, if not null, the same in the other type.  dh may be null (zeros).  part: C floats
+// for each of rms_norm_bwd_parts, unused if that is 1.
+int rms_norm_bwd_parts(int64_t M, int C);
+hipError_t launch_rms_norm_bwd(const void *dy, const void *dh, const void *h, const float *w, void *dx,
+                               void *dr, float *dw, float *part, int64_t M, int C, int r_dtype,
+                               int y_dtype, double eps, hipStream_t stream);
+
+// a [M, N] = silu(x Wg^T) (x Wu^T), bf16, and its backward (swiglu.hip).  dx, or both weight
+// gradients, may be null.  workspace: 2 M N bf16.
+hipError_t launch_swiglu_fwd(const void *x, const void *w_gate, const void *w_up, void *a, int M, int K,
+                             int N, hipStream_t stream);
+hipError_t launch_swiglu_bwd(const void *da, const void *x, const void *w_gate, const void *w_up, void *dx,
+                             void *dw_gate, void *dw_up, void *workspace, int M, int K, int N,
+                             hipStream_t stream);
+
 hipError_t launch_fwd_f32(const void *q, const void *k, const void *v, void *o, float *lse,
                           int B, int Hq, int Hkv, int T, int D, float scale, hipStream_t stream);
 hipError_t launch_bwd_dq_f32(const void *q, const void *k, const void *v, const void *o,

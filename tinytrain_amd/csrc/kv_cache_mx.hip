@@ -22,12 +22,6 @@ namespace {
 
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
-// Largest of the group's 32 magnitudes: over the four lanes that hold it.
-__device__ __forceinline__ uint32_t quad_max(uint32_t x) {
-  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xF, 0xF, true));  // lane ^ 1
-  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, true));  // lane ^ 2
-}
-
 // Eight elements of a row, as a lane holds them.
 template <class T>
 struct Eight;
@@ -172,6 +166,23 @@ __global__ __launch_bounds__(256) void kv_read_mx_kernel(KvCache cache,
   }
 }
 
+// Plain rows into the format (weights, activations): a lane takes eight elements, one after the other over
+// all rows, whose length is a multiple of a group.
+template <int BITS, class T>
+__global__ __launch_bounds__(256) void mx_quantize_kernel(const T *__restrict__ x, uint8_t *__restrict__ codes,
+                                                          uint8_t *__restrict__ scales, int64_t lanes) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= lanes) return;  // whole groups of lanes
+  Eight<T> v;
+  v.load(x + 8 * i);
+  const uint32_t byte = mx_scale_byte<BITS>(quad_max(v.top()));
+  u32x2 c = v.template codes<BITS>(__uint_as_float(byte << 23));
+  if (byte == 255) c = u32x2{};
+  if constexpr (BITS == 4) reinterpret_cast<uint32_t *>(codes)[i] = c[0];
+  else reinterpret_cast<u32x2 *>(codes)[i] = c;
+  if (i % 4 == 0) scales[i / 4] = (uint8_t)byte;
+}
+
 namespace {
 
 // f(kernel tag): the instantiation of (D, bits, dtype)
@@ -235,6 +246,20 @@ hipError_t launch_kv_read(const KvCache &cache, const int *cache_seqlens, void *
           cache, cache_seqlens, (T *)k, (T *)v, rows, Divisor(Hkv), Divisor(n_rows), Lmax);
     });
   });
+}
+
+hipError_t launch_mx_quantize(const void *x, void *codes, void *scales, int64_t elements, int bits,
+                              bool f32, hipStream_t stream) {
+  const int64_t lanes = elements / 8;
+  auto go = [&](auto b, auto t) {
+    using T = decltype(t);
+    mx_quantize_kernel<decltype(b)::value, T><<<dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, stream>>>(
+        (const T *)x, (uint8_t *)codes, (uint8_t *)scales, lanes);
+    return hipGetLastError();
+  };
+  using std::integral_constant;
+  if (bits == 4) return f32 ? go(integral_constant<int, 4>{}, float{}) : go(integral_constant<int, 4>{}, bf16{});
+  return f32 ? go(integral_constant<int, 8>{}, float{}) : go(integral_constant<int, 8>{}, bf16{});
 }
 
 }  // namespace ttfa

@@ -1,5 +1,5 @@
-// Device-side conversions of the quantised KV cache's element types (kv_cache_mx.hip describes the
-// format): e2m1 (BITS 4) and e4m3 (BITS 8) with a shared power of two per 32 elements.
+// Device-side conversions of the quantised element types of the KV cache and of weights (kv_cache_mx.hip
+// describes the format): e2m1 (BITS 4) and e4m3 (BITS 8) with a shared power of two per 32 elements.
 #pragma once
 
 #include <type_traits>
@@ -29,6 +29,12 @@ struct KvRows {
   const T *x[2];
   int64_t stride[2][3];
 };
+
+// Largest of the group's 32 magnitudes: over the four lanes that hold it.
+__device__ __forceinline__ uint32_t quad_max(uint32_t x) {
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xF, 0xF, true));  // lane ^ 1
+  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, true));  // lane ^ 2
+}
 
 // Byte e + 127 of a group whose largest magnitude has the fp32 bits `top`: the smallest e with
 // top <= M 2^e, M = 7 = 1.75 * 2^2 or 464 = 1.8125 * 2^8 (the exponent goes up by one where the

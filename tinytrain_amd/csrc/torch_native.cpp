@@ -1,6 +1,7 @@
 // Native eager path of the public attention functions: the argument checks, the output and
 // workspace allocations, the autograd nodes and the C ABI calls of flash_attn,
-// flash_attn_varlen, flash_attn_decode, qk_norm_rope and the quantised KV cache, in C++.
+// flash_attn_varlen, flash_attn_decode, qk_norm_rope, the quantised KV cache and the block's
+// other operators (norms, swiglu, linear_mx), in C++.
 //
 // Why: a training pass of the custom ops (torch.library ops whose bodies and autograd
 // formulas are Python) costs about 175 us of host time on an MI355X host, most of it in the
@@ -459,6 +460,198 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
   }
 };
 
+// ---------------------------------------------------------------- norms around the branches
+
+constexpr int64_t kMaxNormCols = 16384, kMaxCols = 1 << 20;
+
+bool is_f(const Tensor &t) {
+  return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat;
+}
+
+// Rows of a multiple of `unit` elements, at least one of them (the custom op takes empty calls).
+bool rows_of(const Tensor &t, int64_t unit, int64_t most) {
+  return t.dim() >= 1 && t.numel() > 0 && t.size(-1) % unit == 0 && t.size(-1) <= most && t.is_contiguous();
+}
+
+Tensor workspace(const Tensor &like, long long bytes) {
+  if (bytes < 0) check(TTFA_E_SEQ);
+  return bytes ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
+}
+
+void *ptr(const Tensor &t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+const void *cptr(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+
+struct NormIn {
+  Tensor x, r, w;  // r may be undefined
+
+  int64_t C() const { return x.size(-1); }
+  int64_t M() const { return x.numel() / x.size(-1); }
+  const Tensor &h_like() const { return r.defined() ? r : x; }
+
+  bool takes(int64_t unit) const {
+    if (!plain_tensor(x) || !plain_tensor(w) || !rows_of(x, unit, kMaxNormCols) || !is_f(x)) return false;
+    if (r.defined() && (!plain_tensor(r) || r.sizes() != x.sizes() || !is_f(r) || !r.is_contiguous() ||
+                        r.device() != x.device()))
+      return false;
+    return w.dim() == 1 && w.size(0) == C() && w.is_floating_point() && w.device() == x.device();
+  }
+};
+
+std::pair<Tensor, Tensor> norm_fwd(const NormIn &n, double eps, at::ScalarType y_type) {
+  RECORD_FUNCTION("tinytrain::rms_norm_fwd", c10::ArrayRef<const c10::IValue>());
+  const c10::DeviceGuard on(n.x.device());
+  const Tensor w = weight(n.w);
+  Tensor y = at::empty(n.x.sizes(), n.x.options().dtype(y_type)), h;
+  if (n.r.defined()) h = same(n.r);
+  check(ttfa_rms_norm_fwd(n.x.const_data_ptr(), cptr(n.r), w.const_data_ptr<float>(), y.mutable_data_ptr(),
+                          ptr(h), n.M(), (int)n.C(), dtype_of(n.x), dtype_of(n.h_like()), dtype_of(y), eps,
+                          stream_of(n.x)));
+  return {y, h};
+}
+
+// {d in h's type, d in x's type (the same tensor if that is h's), dw}
+Grads3 norm_bwd(const Tensor &gy, const Tensor &gh, const Tensor &h, const Tensor &w0, double eps,
+                at::ScalarType x_type) {
+  RECORD_FUNCTION("tinytrain::rms_norm_bwd", c10::ArrayRef<const c10::IValue>());
+  const c10::DeviceGuard on(h.device());
+  const Tensor dy = gy.contiguous(), dh = gh.defined() ? gh.contiguous() : gh, w = weight(w0);
+  const int64_t C = h.size(-1), M = h.numel() / C;
+  Tensor dr = same(h), dx, dw = f32(h, {C});
+  if (x_type != h.scalar_type()) dx = at::empty(h.sizes(), h.options().dtype(x_type));
+  Tensor ws = workspace(h, ttfa_rms_norm_workspace_bytes(M, (int)C));
+  check(ttfa_rms_norm_bwd(dy.const_data_ptr(), cptr(dh), h.const_data_ptr(), w.const_data_ptr<float>(),
+                          ptr(dx), dr.mutable_data_ptr(), dw.mutable_data_ptr<float>(), (float *)ptr(ws), M,
+                          (int)C, dtype_of(h), dtype_of(dy), eps, stream_of(h)));
+  return {dr, dx.defined() ? dx : dr, dw.to(w0.scalar_type())};
+}
+
+Grads3 norm_grads(AutogradContext *ctx, const variable_list &grads) {
+  const auto s = ctx->get_saved_variables();
+  const Tensor &h = s[0], &w = s[1];
+  const double eps = ctx->saved_data["eps"].toDouble();
+  const auto x_type = (at::ScalarType)ctx->saved_data["x_type"].toInt();
+  const auto y_type = (at::ScalarType)ctx->saved_data["y_type"].toInt();
+  const Tensor dh = grads.size() > 1 ? grads[1] : Tensor();
+  const Tensor dy = grads[0].defined() ? grads[0] : at::zeros(h.sizes(), h.options().dtype(y_type));
+  if (plain_backward() && NormIn{h, {}, w}.takes(8) && grad_of(dy, h, h.sizes(), y_type) &&
+      (!dh.defined() || grad_of(dh, h, h.sizes(), h.scalar_type())))
+    return norm_bwd(dy, dh, h, w, eps, x_type);
+  auto [dr, dx, dw] = op<Grads3(const Tensor &, const std::optional<Tensor> &, const Tensor &, const Tensor &,
+                                double, at::ScalarType)>("tinytrain::rms_norm_bwd")
+                          .call(dy, dh.defined() ? std::optional<Tensor>(dh) : std::nullopt, h, w, eps, x_type);
+  return {dr, x_type == h.scalar_type() ? dr : dx, dw};
+}
+
+void keep_norm(AutogradContext *ctx, const Tensor &h, const Tensor &w, double eps, at::ScalarType x_type,
+               at::ScalarType y_type) {
+  ctx->set_materialize_grads(false);
+  ctx->save_for_backward({h, w});
+  ctx->saved_data["eps"] = eps;
+  ctx->saved_data["x_type"] = (int64_t)x_type;
+  ctx->saved_data["y_type"] = (int64_t)y_type;
+}
+
+struct RmsNorm : torch::autograd::Function<RmsNorm> {
+  static constexpr bool is_traceable = true;
+
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, double eps, int64_t y_type) {
+    keep_norm(ctx, x, w, eps, x.scalar_type(), (at::ScalarType)y_type);
+    return norm_fwd({x, {}, w}, eps, (at::ScalarType)y_type).first;
+  }
+
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    auto [dr, dx, dw] = norm_grads(ctx, grads);
+    return {dr, dw, Tensor(), Tensor()};
+  }
+};
+
+struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
+  static constexpr bool is_traceable = true;
+
+  static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &r, const Tensor &w,
+                               double eps, int64_t y_type) {
+    auto [y, h] = norm_fwd({x, r, w}, eps, (at::ScalarType)y_type);
+    keep_norm(ctx, h, w, eps, x.scalar_type(), (at::ScalarType)y_type);
+    return {y, h};
+  }
+
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    auto [dr, dx, dw] = norm_grads(ctx, grads);
+    return {dx, dr, dw, Tensor(), Tensor()};
+  }
+};
+
+// -------------------------------------------------------------------------- gated feed-forward
+
+struct SwigluIn {
+  Tensor x, wg, wu;
+
+  int64_t K() const { return x.size(-1); }
+  int64_t M() const { return x.numel() / x.size(-1); }
+  int64_t N() const { return wg.size(0); }
+
+  bool takes() const {
+    for (const Tensor *t : {&x, &wg, &wu})
+      if (!plain_tensor(*t) || t->scalar_type() != at::kBFloat16 || !rows_of(*t, 8, kMaxCols) ||
+          t->device() != x.device())
+        return false;
+    return wg.dim() == 2 && wg.sizes() == wu.sizes() && wg.size(1) == K() && N() % 8 == 0 && N() <= kMaxCols &&
+           M() <= kIntMax;
+  }
+  std::vector<int64_t> out_sizes() const {
+    auto v = x.sizes().vec();
+    v.back() = N();
+    return v;
+  }
+};
+
+Tensor swiglu_fwd(const SwigluIn &i) {
+  RECORD_FUNCTION("tinytrain::swiglu_fwd", c10::ArrayRef<const c10::IValue>());
+  const c10::DeviceGuard on(i.x.device());
+  const int M = (int)i.M(), K = (int)i.K(), N = (int)i.N();
+  Tensor a = at::empty(i.out_sizes(), i.x.options());
+  Tensor ws = workspace(i.x, ttfa_swiglu_workspace_bytes(M, K, N, 0));
+  check(ttfa_swiglu_fwd(i.x.const_data_ptr(), i.wg.const_data_ptr(), i.wu.const_data_ptr(),
+                        a.mutable_data_ptr(), ptr(ws), M, K, N, stream_of(i.x)));
+  return a;
+}
+
+Grads3 swiglu_bwd(const Tensor &da, const SwigluIn &i, bool need_dx, bool need_dw) {
+  RECORD_FUNCTION("tinytrain::swiglu_bwd", c10::ArrayRef<const c10::IValue>());
+  const c10::DeviceGuard on(i.x.device());
+  const Tensor g = da.contiguous();
+  const int M = (int)i.M(), K = (int)i.K(), N = (int)i.N();
+  Tensor dx, dwg, dwu;
+  if (need_dx) dx = same(i.x);
+  if (need_dw) dwg = same(i.wg), dwu = same(i.wu);
+  Tensor ws = workspace(i.x, ttfa_swiglu_workspace_bytes(M, K, N, 1));
+  check(ttfa_swiglu_bwd(g.const_data_ptr(), i.x.const_data_ptr(), i.wg.const_data_ptr(),
+                        i.wu.const_data_ptr(), ptr(dx), ptr(dwg), ptr(dwu), ptr(ws), M, K, N, stream_of(i.x)));
+  return {dx, dwg, dwu};
+}
+
+struct Swiglu : torch::autograd::Function<Swiglu> {
+  static constexpr bool is_traceable = true;
+
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &wg, const Tensor &wu) {
+    ctx->save_for_backward({x, wg, wu});
+    return swiglu_fwd({x, wg, wu});
+  }
+
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const SwigluIn i{s[0], s[1], s[2]};
+    const Tensor &g = grads[0];
+    const bool nx = ctx->needs_input_grad(0), ng = ctx->needs_input_grad(1), nu = ctx->needs_input_grad(2);
+    const bool native = plain_backward() && i.takes() && grad_of(g, s[0], i.out_sizes(), at::kBFloat16);
+    Grads3 d = native ? swiglu_bwd(g, i, nx, ng || nu)
+                      : op<Grads3(const Tensor &, const Tensor &, const Tensor &, const Tensor &, bool, bool)>(
+                            "tinytrain::swiglu_bwd")
+                            .call(g, s[0], s[1], s[2], nx, ng || nu);
+    return {nx ? std::get<0>(d) : Tensor(), ng ? std::get<1>(d) : Tensor(), nu ? std::get<2>(d) : Tensor()};
+  }
+};
+
 // ------------------------------------------------------------------------ Python bindings
 
 // The first n arguments as tensors; false when one of them is not an exact Tensor.
@@ -636,6 +829,117 @@ PyObject *py_qk_norm_rope(PyObject *, PyObject *const *args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// args[i] as a tensor, or undefined for None; false when it is neither.
+bool unpack_optional(PyObject *arg, Tensor &out) {
+  if (arg == Py_None) return true;
+  if (!THPVariable_CheckExact(arg)) return false;
+  out = THPVariable_Unpack(arg);
+  return true;
+}
+
+// add_rms_norm(x, residual or None, weight, eps, ttfa dtype of y or -1 for x's)
+PyObject *py_add_rms_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arity(n, 5)) return nullptr;
+  NormIn in;
+  const double eps = PyFloat_AsDouble(args[3]);
+  if (eps == -1.0 && PyErr_Occurred()) return nullptr;
+  const int64_t dtype = PyLong_AsLongLong(args[4]);
+  if (dtype == -1 && PyErr_Occurred()) return nullptr;
+  if (!THPVariable_CheckExact(args[0]) || !unpack_optional(args[1], in.r) || !THPVariable_CheckExact(args[2]) ||
+      !plain_mode())
+    Py_RETURN_NONE;
+  in.x = THPVariable_Unpack(args[0]);
+  in.w = THPVariable_Unpack(args[2]);
+  if (!in.takes(8)) Py_RETURN_NONE;
+  const auto y_type = dtype < 0 ? in.x.scalar_type() : dtype == TTFA_F32 ? at::kFloat : at::kBFloat16;
+  if (!in.r.defined())
+    return THPVariable_Wrap(recorded({&in.x, &in.w}) ? RmsNorm::apply(in.x, in.w, eps, (int64_t)y_type)
+                                                     : norm_fwd(in, eps, y_type).first);
+  if (recorded({&in.x, &in.r, &in.w})) {
+    const auto o = AddRmsNorm::apply(in.x, in.r, in.w, eps, (int64_t)y_type);
+    return pack({o[0], o[1]});
+  }
+  const auto o = norm_fwd(in, eps, y_type);
+  return pack({o.first, o.second});
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject *py_add_rms_norm_mx(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arity(n, 4)) return nullptr;
+  NormIn in;
+  const double eps = PyFloat_AsDouble(args[3]);
+  if (eps == -1.0 && PyErr_Occurred()) return nullptr;
+  if (!THPVariable_CheckExact(args[0]) || !unpack_optional(args[1], in.r) || !THPVariable_CheckExact(args[2]) ||
+      !plain_mode())
+    Py_RETURN_NONE;
+  in.x = THPVariable_Unpack(args[0]);
+  in.w = THPVariable_Unpack(args[2]);
+  if (!in.takes(32) || recorded({&in.x, &in.w}) || (in.r.defined() && recorded({&in.r}))) Py_RETURN_NONE;
+  RECORD_FUNCTION("tinytrain::rms_norm_mx", c10::ArrayRef<const c10::IValue>());
+  const c10::DeviceGuard on(in.x.device());
+  const Tensor w = weight(in.w);
+  auto sizes = in.x.sizes().vec();
+  const auto bytes = in.x.options().dtype(at::kByte);
+  Tensor codes = at::empty(sizes, bytes), h;
+  sizes.back() /= 32;
+  Tensor scales = at::empty(sizes, bytes);
+  if (in.r.defined()) h = same(in.r);
+  check(ttfa_rms_norm_mx(in.x.const_data_ptr(), cptr(in.r), w.const_data_ptr<float>(),
+                         codes.mutable_data_ptr(), scales.mutable_data_ptr(), ptr(h), in.M(), (int)in.C(),
+                         dtype_of(in.x), dtype_of(in.h_like()), eps, stream_of(in.x)));
+  return pack({codes, scales, h.defined() ? h : in.x});
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject *py_swiglu(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arity(n, 3)) return nullptr;
+  Tensor t[3];
+  if (!unpack(args, t) || !plain_mode()) Py_RETURN_NONE;
+  const SwigluIn in{t[0], t[1], t[2]};
+  if (!in.takes()) Py_RETURN_NONE;
+  return THPVariable_Wrap(recorded({&t[0], &t[1], &t[2]}) ? Swiglu::apply(t[0], t[1], t[2]) : swiglu_fwd(in));
+  END_HANDLE_TH_ERRORS
+}
+
+// linear_mx(x, codes, scales, x_scales or None)
+PyObject *py_linear_mx(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arity(n, 4)) return nullptr;
+  Tensor t[3], xs;
+  if (!unpack(args, t) || !unpack_optional(args[3], xs) || !plain_mode()) Py_RETURN_NONE;
+  const Tensor &x = t[0], &codes = t[1], &scales = t[2];
+  for (const Tensor *c : {&codes, &scales})
+    if (!plain_tensor(*c) || c->dim() != 2 || c->scalar_type() != at::kByte || !c->is_contiguous() ||
+        c->device() != codes.device())
+      Py_RETURN_NONE;
+  const int64_t N = scales.size(0), K = 32 * scales.size(1);
+  if (codes.size(0) != N || (2 * codes.size(1) != K && codes.size(1) != K) || K > kMaxCols || N < 8 || N % 8 ||
+      N > kMaxCols || !plain_tensor(x) || !rows_of(x, 32, kMaxCols) || x.size(-1) != K ||
+      x.scalar_type() != (xs.defined() ? at::kByte : at::kBFloat16) || x.device() != codes.device() ||
+      x.numel() / K > kIntMax || recorded({&x}))
+    Py_RETURN_NONE;
+  auto sizes = x.sizes().vec();
+  if (xs.defined()) {
+    sizes.back() = K / 32;
+    if (!plain_tensor(xs) || xs.sizes() != at::IntArrayRef(sizes) || xs.scalar_type() != at::kByte ||
+        !xs.is_contiguous() || xs.device() != x.device())
+      Py_RETURN_NONE;
+  }
+  RECORD_FUNCTION("tinytrain::linear_mx", c10::ArrayRef<const c10::IValue>());
+  const c10::DeviceGuard on(x.device());
+  sizes.back() = N;
+  Tensor y = at::empty(sizes, x.options().dtype(at::kBFloat16));
+  const int M = (int)(x.numel() / K), bits = (int)(8 * codes.size(1) / K);
+  Tensor ws = workspace(x, ttfa_linear_mx_workspace_bytes(M, (int)K, (int)N, bits, xs.defined()));
+  check(ttfa_linear_mx(x.const_data_ptr(), cptr(xs), codes.const_data_ptr(), scales.const_data_ptr(),
+                       y.mutable_data_ptr(), ptr(ws), M, (int)K, (int)N, bits, stream_of(x)));
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"flash_attn", (PyCFunction)(void (*)(void))py_flash_attn, METH_FASTCALL,
      "o of flash_attn(q, k, v), or None where the custom op has to take the call."},
@@ -651,6 +955,14 @@ PyMethodDef methods[] = {
      "(k, v) of kv_cache_read(*cache, cache_seqlens, rows, ttfa dtype), or None."},
     {"flash_attn_decode_mx", (PyCFunction)(void (*)(void))py_flash_attn_decode_mx, METH_FASTCALL,
      "(o, lse) of flash_attn_decode_mx(q, *cache, cache_seqlens), or None."},
+    {"add_rms_norm", (PyCFunction)(void (*)(void))py_add_rms_norm, METH_FASTCALL,
+     "(y, h) of add_rms_norm(x, residual, weight, eps, ttfa dtype or -1), y without a residual, or None."},
+    {"add_rms_norm_mx", (PyCFunction)(void (*)(void))py_add_rms_norm_mx, METH_FASTCALL,
+     "(codes, scales, h) of add_rms_norm_mx(x, residual or None, weight, eps), or None."},
+    {"swiglu", (PyCFunction)(void (*)(void))py_swiglu, METH_FASTCALL,
+     "a of swiglu(x, w_gate, w_up), or None."},
+    {"linear_mx", (PyCFunction)(void (*)(void))py_linear_mx, METH_FASTCALL,
+     "y of linear_mx(x, codes, scales, x_scales or None), or None."},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ttfa_torch",

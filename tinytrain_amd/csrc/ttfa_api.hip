@@ -136,6 +136,49 @@ int check_ptrs(const void *const *ptrs, int n) {
   return TTFA_OK;
 }
 
+bool is_dtype(int dtype) { return dtype == TTFA_BF16 || dtype == TTFA_F32; }
+
+// M rows of C elements, C a multiple of `unit` up to `most`; total elements within int64 with margin.
+int check_rows(int64_t M, int C, int unit, int most) {
+  if (C < unit || C % unit || C > most) return TTFA_E_COLS;
+  return M < 1 || M > ((int64_t)1 << 40) / C ? TTFA_E_SEQ : TTFA_OK;
+}
+
+int check_norm(int64_t M, int C, int unit, int x_dtype, int r_dtype, int y_dtype, double eps) {
+  if (!is_dtype(x_dtype) || !is_dtype(r_dtype) || !is_dtype(y_dtype)) return TTFA_E_DTYPE;
+  if (!(eps >= 0.0) || !(eps < 1.0)) return TTFA_E_EPS;
+  return check_rows(M, C, unit, 16384);
+}
+
+// The residual and its sum, which come together or not at all, after the other pointers.
+int check_residual(const void *const *ptrs, int n, const void *residual, const void *h) {
+  const int rc = check_ptrs(ptrs, n);
+  if (rc || (!residual && !h)) return rc;
+  const void *pair[] = {residual, h};
+  return check_ptrs(pair, 2);
+}
+
+constexpr int kMostCols = 1 << 20;  // of a product: a tile's byte offsets stay within 31 bits
+
+// Tiles of tm x tn of a result: workgroups of 256 threads, 2^32 in all.
+int check_tiles(int64_t M, int64_t N, int tm, int tn) {
+  return (M + tm - 1) / tm * ((N + tn - 1) / tn) < 1 << 23 ? TTFA_OK : TTFA_E_SEQ;
+}
+
+int check_swiglu(int M, int K, int N) {
+  int rc = check_rows(M, K, 8, kMostCols);
+  if (rc || (rc = check_rows(M, N, 8, kMostCols))) return rc;
+  if ((rc = check_tiles(M, N, 128, 128)) || (rc = check_tiles(M, K, 128, 128))) return rc;
+  return check_tiles(2ll * N, K, 128, 128);
+}
+
+int check_linear_mx(int M, int K, int N, int bits) {
+  if (bits != 4 && bits != 8) return TTFA_E_BITS;
+  int rc = check_rows(M, K, 32, kMostCols);
+  if (rc || (rc = check_rows(M, N, 8, kMostCols))) return rc;
+  return check_tiles(M, N, 64, 16);
+}
+
 // The workspace of ttfa_bwd_ws: Delta rows, padded to 16 bytes, then the dK/dV partials.
 int64_t delta_floats(int B, int Hq, int T) { return ((int64_t)B * Hq * T + 3) / 4 * 4; }
 
@@ -170,8 +213,10 @@ const char *ttfa_strerror(int code) {
     case TTFA_E_SCALE: return "ttfa: scale must be finite and > 0";
     case TTFA_E_EPS: return "ttfa: eps must be in [0, 1)";
     case TTFA_E_QROWS: return "ttfa: decode needs (Hq / Hkv) * Tq <= 32 query rows per KV head";
-    case TTFA_E_BITS: return "ttfa: a quantised cache holds elements of 4 or 8 bits";
+    case TTFA_E_BITS: return "ttfa: a quantised cache or weight holds elements of 4 or 8 bits";
     case TTFA_E_STRIDE: return "ttfa: strides must be multiples of 16 bytes and not negative";
+    case TTFA_E_COLS:
+      return "ttfa: row lengths must be multiples of 8 (32 where rows are quantised) and in range";
     case TTFA_E_SCRATCH:
       return "ttfa: ttfa_bwd_static needs B * Hq * T <= TTFA_BWD_STATIC_MAX_ROWS (1048576)";
     default: break;
@@ -390,6 +435,103 @@ int ttfa_bwd_static(const void *q, const void *k, const void *v, const void *o,
   // them, so nothing left by an earlier call is ever read and nothing needs clearing.
   return ttfa_bwd(q, k, v, o, dout, lse, delta, dq, dk, dv, B, Hq, Hkv, T, D, dtype, scale,
                   hip_stream);
+}
+
+int ttfa_rms_norm_fwd(const void *x, const void *residual, const float *w, void *y, void *h,
+                      long long M, int C, int x_dtype, int r_dtype, int y_dtype, double eps,
+                      void *hip_stream) {
+  int rc = check_norm(M, C, 8, x_dtype, residual ? r_dtype : x_dtype, y_dtype, eps);
+  if (rc) return rc;
+  const void *ptrs[] = {x, w, y};
+  if ((rc = check_residual(ptrs, 3, residual, h))) return rc;
+  return static_cast<int>(ttfa::launch_rms_norm_fwd(x, residual, w, y, h, M, C, x_dtype, r_dtype, y_dtype,
+                                                    eps, static_cast<hipStream_t>(hip_stream)));
+}
+
+int ttfa_rms_norm_mx(const void *x, const void *residual, const float *w, void *codes, void *scales,
+                     void *h, long long M, int C, int x_dtype, int r_dtype, double eps,
+                     void *hip_stream) {
+  int rc = check_norm(M, C, 32, x_dtype, residual ? r_dtype : x_dtype, TTFA_BF16, eps);
+  if (rc) return rc;
+  const void *ptrs[] = {x, w, codes, scales};
+  if ((rc = check_residual(ptrs, 4, residual, h))) return rc;
+  return static_cast<int>(ttfa::launch_rms_norm_mx(x, residual, w, codes, scales, h, M, C, x_dtype, r_dtype,
+                                                   eps, static_cast<hipStream_t>(hip_stream)));
+}
+
+long long ttfa_rms_norm_workspace_bytes(long long M, int C) {
+  if (check_rows(M, C, 8, 16384)) return -1;
+  const int parts = ttfa::rms_norm_bwd_parts(M, C);
+  return parts == 1 ? 0 : (long long)parts * C * (long long)sizeof(float);
+}
+
+int ttfa_rms_norm_bwd(const void *dy, const void *dh, const void *h, const float *w, void *dx, void *dr,
+                      float *dw, float *workspace, long long M, int C, int r_dtype, int y_dtype,
+                      double eps, void *hip_stream) {
+  int rc = check_norm(M, C, 8, r_dtype, r_dtype, y_dtype, eps);
+  if (rc) return rc;
+  const bool one = ttfa::rms_norm_bwd_parts(M, C) == 1;
+  const void *ptrs[] = {dy, h, w, dr, dw, dh ? dh : dr, dx ? dx : dr, workspace};
+  if ((rc = check_ptrs(ptrs, one ? 7 : 8))) return rc;
+  return static_cast<int>(ttfa::launch_rms_norm_bwd(dy, dh, h, w, dx, dr, dw, workspace, M, C, r_dtype,
+                                                    y_dtype, eps, static_cast<hipStream_t>(hip_stream)));
+}
+
+long long ttfa_swiglu_workspace_bytes(int M, int K, int N, int backward) {
+  if (check_swiglu(M, K, N)) return -1;
+  return backward ? 4ll * M * N : 0;
+}
+
+int ttfa_swiglu_fwd(const void *x, const void *w_gate, const void *w_up, void *a, void *workspace, int M,
+                    int K, int N, void *hip_stream) {
+  int rc = check_swiglu(M, K, N);
+  if (rc) return rc;
+  const void *ptrs[] = {x, w_gate, w_up, a, workspace};
+  if ((rc = check_ptrs(ptrs, ttfa_swiglu_workspace_bytes(M, K, N, 0) ? 5 : 4))) return rc;
+  return static_cast<int>(
+      ttfa::launch_swiglu_fwd(x, w_gate, w_up, a, M, K, N, static_cast<hipStream_t>(hip_stream)));
+}
+
+int ttfa_swiglu_bwd(const void *da, const void *x, const void *w_gate, const void *w_up, void *dx,
+                    void *dw_gate, void *dw_up, void *workspace, int M, int K, int N,
+                    void *hip_stream) {
+  int rc = check_swiglu(M, K, N);
+  if (rc) return rc;
+  if (!dx && !dw_gate) return TTFA_E_NULL;
+  if (!dw_gate != !dw_up) return TTFA_E_NULL;
+  const void *ptrs[] = {da, x, w_gate, w_up, workspace, dx ? dx : x, dw_gate ? dw_gate : x, dw_up ? dw_up : x};
+  if ((rc = check_ptrs(ptrs, 8))) return rc;
+  return static_cast<int>(ttfa::launch_swiglu_bwd(da, x, w_gate, w_up, dx, dw_gate, dw_up, workspace, M, K,
+                                                  N, static_cast<hipStream_t>(hip_stream)));
+}
+
+int ttfa_mx_quantize(const void *x, void *codes, void *scales, long long M, int K, int bits, int dtype,
+                     void *hip_stream) {
+  if (!is_dtype(dtype)) return TTFA_E_DTYPE;
+  if (bits != 4 && bits != 8) return TTFA_E_BITS;
+  int rc = check_rows(M, K, 32, kMostCols);
+  if (rc) return rc;
+  if (M > (((int64_t)1 << 34) - (1 << 13)) / K) return TTFA_E_SEQ;  // launches of fewer than 2^32 threads
+  const void *ptrs[] = {x, codes, scales};
+  if ((rc = check_ptrs(ptrs, 3))) return rc;
+  return static_cast<int>(ttfa::launch_mx_quantize(x, codes, scales, M * K, bits, dtype == TTFA_F32,
+                                                   static_cast<hipStream_t>(hip_stream)));
+}
+
+long long ttfa_linear_mx_workspace_bytes(int M, int K, int N, int bits, int x_quantised) {
+  (void)x_quantised;
+  return check_linear_mx(M, K, N, bits) ? -1 : 0;
+}
+
+int ttfa_linear_mx(const void *x, const void *x_scales, const void *codes, const void *scales, void *y,
+                   void *workspace, int M, int K, int N, int bits, void *hip_stream) {
+  int rc = check_linear_mx(M, K, N, bits);
+  if (rc) return rc;
+  const void *ptrs[] = {x, codes, scales, y, x_scales ? x_scales : x, workspace};
+  if ((rc = check_ptrs(ptrs, ttfa_linear_mx_workspace_bytes(M, K, N, bits, x_scales != nullptr) ? 6 : 5)))
+    return rc;
+  return static_cast<int>(ttfa::launch_linear_mx(x, x_scales, codes, scales, y, M, K, N, bits,
+                                                 static_cast<hipStream_t>(hip_stream)));
 }
 
 }  // extern "C"
