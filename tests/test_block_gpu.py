@@ -160,7 +160,8 @@ def test_norm_empty_and_other_ranks():
 # --------------------------------------------------------------------------------- swiglu
 
 SWIGLU_SHAPES = [(1, 8, 8), (1, 768, 2304), (5, 64, 72), (16, 104, 200), (33, 768, 328), (100, 40, 136), (128, 32, 128),
-                 (129, 200, 264), (300, 1000, 520), (1000, 136, 1032), (2051, 72, 128)]
+                 (129, 200, 264), (300, 1000, 520), (1000, 136, 1032), (2051, 72, 128),
+                 (4100, 520, 2056), (8197, 264, 2056), (20000, 136, 264), (5000, 2056, 776)]
 
 
 def _check_swiglu(M, K, N):

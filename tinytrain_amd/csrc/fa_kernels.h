@@ -115,7 +115,8 @@ hipError_t launch_rms_norm_bwd(const void *dy, const void *dh, const void *h, co
                                int y_dtype, double eps, hipStream_t stream);
 
 // a [M, N] = silu(x Wg^T) (x Wu^T), bf16, and its backward (swiglu.hip).  dx, or both weight
-// gradients, may be null.  workspace: 2 M N bf16.
+// gradients, may be null.  workspace: swiglu_bwd_workspace bytes.
+int64_t swiglu_bwd_workspace(int M, int K, int N);
 hipError_t launch_swiglu_fwd(const void *x, const void *w_gate, const void *w_up, void *a, int M, int K,
                              int N, hipStream_t stream);
 hipError_t launch_swiglu_bwd(const void *da, const void *x, const void *w_gate, const void *w_up, void *dx,

@@ -21,55 +21,81 @@
 
 namespace ttfa {
 
-// Rows of `ld` elements from p; `rows` of them.
-struct Operand {
-  const bf16 *p;
-  int64_t ld;
-  int64_t rows;
-};
-
-// Buffer resource over [p, end), at most 2^31 - 1 bytes of it.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_to(const bf16 *p, const bf16 *end) {
-  const int64_t left = (end - p) * 2;
-  return make_rsrc(p, left <= 0 ? 0u : left > 0x7fffffff ? 0x7fffffffu : (uint32_t)left);
+// The LDS reads of this wave, and all but its last N vector memory accesses, done; then the workgroup
+// meets.  Memory accesses stay on their side of it.
+template <int N>
+__device__ __forceinline__ void wait_and_meet() {
+  static_assert(N < 64, "six bits");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);  // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
-constexpr uint32_t kPastEnd = 0x80000000u;  // an offset that no resource covers
+// 16 bytes to byte_off of a buffer; past its end they are dropped (the instruction is issued all the same,
+// so what is counted by vmcnt does not depend on it).
+__device__ __forceinline__ void buf_store16(__amdgpu_buffer_rsrc_t r, uint32_t byte_off, u32x4 v) {
+  __builtin_amdgcn_raw_buffer_store_b128(v, r, byte_off, 0, 0);
+}
 
-// One operand's tile of T rows (of the m or n index) x BK, loaded by NT threads.
+constexpr uint32_t kPastEnd = 0x80000000u;  // an offset that no tile's buffer covers
+
+// One operand's tile of T rows (of the m or n index) x BK, loaded by NT threads, stage after stage along k.
 template <int T, int BK, bool TR, int NT>
 struct TileLoad {
   static constexpr int LOADS = T * BK * 2 / 16 / NT;
   static constexpr int CPR = TR ? T / 8 : BK / 8;  // 16-byte chunks of an LDS row
   static constexpr int BYTES = T * BK * 2;
   static_assert(T * BK * 2 % (16 * NT) == 0 && (!TR || T >= 128), "tile");
+  const char *base;  // of the next stage
+  uint32_t bytes;    // that the tile's rows have from there on
+  int64_t step;      // bytes to the stage after it
   uint32_t off[LOADS];
-  int chunk[LOADS];
 
   static __device__ __forceinline__ int swizzle(int row) {
     return TR ? (row & 3) << 2 : (row / (16 / CPR)) & (CPR - 1);
   }
-  // Rows from `half` on are row - half of a second source (dual tiles).
-  __device__ __forceinline__ void init(int64_t ld, int half = T) {
+
+  // The matrix at p, rows of ld elements: tile from row (TR: column) r0 of R on.
+  __device__ __forceinline__ void init(const bf16 *p, int64_t ld, int64_t r0, int64_t R) {
+    start(p, ld, r0, R);
+    step = TR ? ld * (BK * 2) : BK * 2;
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
-      const int e = j * NT + (int)threadIdx.x, row = e / CPR, ch = (e % CPR) ^ swizzle(row);
-      chunk[j] = ch;
-      off[j] = (uint32_t)((row >= half ? row - half : row) * ld * 2 + ch * 16);
+      const int e = j * NT + (int)threadIdx.x, row = e / CPR;
+      off[j] = (uint32_t)(row * ld * 2) + ((e % CPR) ^ swizzle(row)) * 16;
     }
   }
-  // Loads j0 .. j1 - 1 from the buffer r; `left`: the k's that rows along k still have.
-  template <int J0, int J1>
-  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, char *lds, int64_t left) const {
-    char *dst = lds + wave_id() * 1024;
-    if (TR || left >= BK) {
-#pragma unroll
-      for (int j = J0; j < J1; ++j) buf_load16_lds(r, off[j], dst + j * NT * 16);
+  // The same tile of another matrix of the same shape (k from 0 again).
+  __device__ __forceinline__ void start(const bf16 *p, int64_t ld, int64_t r0, int64_t R) {
+    base = reinterpret_cast<const char *>(p + (TR ? r0 : r0 * ld));
+    const int64_t rows = R - r0 < T ? R - r0 : T;
+    bytes = rows <= 0 ? 0u : (uint32_t)((TR ? BK * ld - r0 : rows * ld) * 2);
+  }
+  // Past the next n stages.
+  __device__ __forceinline__ void skip(int n) {
+    base += step * n;
+    if (!TR) bytes -= (uint32_t)(BK * 2) * n;
+  }
+  // A stage of `left` < BK k's, the last one: what lies past them loads as zeros.
+  __device__ __forceinline__ void shorten(int64_t ld, int left) {
+    if constexpr (TR) {
+      bytes -= (uint32_t)((BK - left) * ld * 2);
     } else {
 #pragma unroll
-      for (int j = J0; j < J1; ++j)
-        buf_load16_lds(r, 8 * chunk[j] < left ? off[j] : kPastEnd, dst + j * NT * 16);
+      for (int j = 0; j < LOADS; ++j) {
+        const int e = j * NT + (int)threadIdx.x, row = e / CPR;
+        if (8 * ((e % CPR) ^ swizzle(row)) >= left) off[j] = kPastEnd;
+      }
     }
+  }
+  __device__ __forceinline__ void load(char *lds) {
+    char *dst = lds + wave_id() * 1024;
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(base, bytes);
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) buf_load16_lds(r, off[j], dst + j * NT * 16);
+    base += step;
+    if (!TR) bytes -= (uint32_t)(BK * 2);
   }
 };
 
@@ -108,23 +134,55 @@ struct TileRead {
   }
 };
 
-// Registers of a 32 x 32 result block, rounded to bf16, as 16-byte pieces of rows: lane's piece p is
-// n = 16 p + 8 (lane / 32) .. + 7 of its column m.
-__device__ __forceinline__ u32x4 row_piece(const f32x16 &v, int p) {
-  const u32x2 a = __builtin_bit_cast(u32x2, pack4(v[8 * p], v[8 * p + 1], v[8 * p + 2], v[8 * p + 3]));
-  const u32x2 b = __builtin_bit_cast(u32x2, pack4(v[8 * p + 4], v[8 * p + 5], v[8 * p + 6], v[8 * p + 7]));
-  const auto x = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
-  const auto y = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
-  return u32x4{x[0], y[0], x[1], y[1]};
+// A 32 x 32 result block rounded to bf16, as two sets of 16-byte pieces of its rows: lane l holds, of set
+// q, n = 8 piece_of(l) .. + 7 of column m = 16 q + l % 16, so that a store writes 64 bytes of each of 16
+// rows.  (With 32 bytes of 32 rows, as the halves of the wave have them, stores took about twice the time.)
+__device__ __forceinline__ int piece_of(int lane) { return 2 * ((lane >> 4) & 1) + (lane >> 5); }
+
+__device__ __forceinline__ void swap_rows(u32x4 &a, u32x4 &b) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const auto x = __builtin_amdgcn_permlane16_swap(a[i], b[i], false, false);
+    a[i] = x[0];
+    b[i] = x[1];
+  }
 }
 
-// The inverse: registers 8p .. 8p + 7 of a block from piece p of bf16 rows.
-__device__ __forceinline__ void block_regs(u32x4 piece, f32x16 &v, int p) {
-  const auto x = __builtin_amdgcn_permlane32_swap(piece[0], piece[2], false, false);
-  const auto y = __builtin_amdgcn_permlane32_swap(piece[1], piece[3], false, false);
-  const bf16x8 b = __builtin_bit_cast(bf16x8, (u32x4{x[0], y[0], x[1], y[1]}));
+__device__ __forceinline__ void block_rows(const f32x16 &v, u32x4 (&set)[2]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[8 * p + i] = (float)b[i];
+  for (int p = 0; p < 2; ++p) {
+    const u32x2 a = __builtin_bit_cast(u32x2, pack4(v[8 * p], v[8 * p + 1], v[8 * p + 2], v[8 * p + 3]));
+    const u32x2 b = __builtin_bit_cast(u32x2, pack4(v[8 * p + 4], v[8 * p + 5], v[8 * p + 6], v[8 * p + 7]));
+    const auto x = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
+    const auto y = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
+    set[p] = u32x4{x[0], y[0], x[1], y[1]};
+  }
+  swap_rows(set[0], set[1]);
+}
+
+// The block in fp32: set 2 c + q holds, of rows 16 q + lane % 16, n = 16 c + 8 (lane / 16 % 2) + 4 (lane / 32) .. + 3.
+__device__ __forceinline__ void block_rows_f32(const f32x16 &v, u32x4 (&set)[4]) {
+#pragma unroll
+  for (int a = 0; a < 4; ++a)
+    set[a] = __builtin_bit_cast(u32x4, (f32x4{v[4 * a], v[4 * a + 1], v[4 * a + 2], v[4 * a + 3]}));
+  swap_rows(set[0], set[1]);
+  swap_rows(set[2], set[3]);
+}
+
+// The inverse: a block's registers from such pieces.
+__device__ __forceinline__ f32x16 block_regs(u32x4 a, u32x4 b) {
+  swap_rows(a, b);
+  f32x16 v;
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    const u32x4 c = p ? b : a;
+    const auto x = __builtin_amdgcn_permlane32_swap(c[0], c[2], false, false);
+    const auto y = __builtin_amdgcn_permlane32_swap(c[1], c[3], false, false);
+    const bf16x8 w = __builtin_bit_cast(bf16x8, (u32x4{x[0], y[0], x[1], y[1]}));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[8 * p + i] = (float)w[i];
+  }
+  return v;
 }
 
 }  // namespace ttfa

@@ -479,7 +479,7 @@ int ttfa_rms_norm_bwd(const void *dy, const void *dh, const void *h, const float
 
 long long ttfa_swiglu_workspace_bytes(int M, int K, int N, int backward) {
   if (check_swiglu(M, K, N)) return -1;
-  return backward ? 4ll * M * N : 0;
+  return backward ? ttfa::swiglu_bwd_workspace(M, K, N) : 0;
 }
 
 int ttfa_swiglu_fwd(const void *x, const void *w_gate, const void *w_up, void *a, void *workspace, int M,
