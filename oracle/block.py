@@ -53,8 +53,12 @@ def swiglu_grads(da, x, wg, wu):
 
 
 def linear_mx(x, x_scales, codes, scales):
-    """(y, sum of the products' magnitudes), fp64 on the CPU, from the values that the bytes stand for."""
+    """(y, sum of the products' magnitudes, sum over every eight consecutive products of the largest one), fp64 on
+    the CPU, from the values that the bytes stand for."""
     K = 32 * scales.shape[1]
     w = mx_cache.values(codes.cpu(), scales.cpu(), 8 * codes.shape[1] // K)
     x = x.cpu().double() if x_scales is None else mx_cache.values(x.cpu(), x_scales.cpu(), 8)
-    return x @ w.t(), x.abs() @ w.abs().t()
+    top = torch.zeros(x.shape[0], w.shape[0], dtype=torch.float64)
+    for k in range(0, K, 8):
+        top += (x[:, None, k:k + 8] * w[None, :, k:k + 8]).abs().amax(-1)
+    return x @ w.t(), x.abs() @ w.abs().t(), top

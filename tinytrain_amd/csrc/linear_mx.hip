@@ -2,13 +2,17 @@
 // power of two per 32 elements (kv_cache_mx.hip describes the format), x in bf16 or in 8 bits as the
 // norm's kernel gives it.  The reference has no counterpart (its linear layers are bf16 products).
 //
-// Every value of either format is a bf16 as it stands, and so the products are bf16 ones with fp32
-// sums: exact products, one rounding of y at the end.
+// Every value of either format is a bf16 as it stands, so with x in bf16 the products are bf16 ones with
+// fp32 sums.  With x in 8 bits the matrix unit takes both as they lie, with their scales
+// (v_mfma_scale_f32_16x16x128_f8f6f4, twice the rate, no conversions); of every eight consecutive
+// products it drops the bits below 2^-13 of the largest before it adds in fp32 (fa_decode_mx.hip), so a
+// sum is off by less than 2^-10 of those largest ones' sum, on random values by 2^-19 of sum |x w|, far
+// below the 2^-9 of y's own rounding.
 //
-// Few rows (up to kFewRows): bound by reading W once.  A workgroup takes 16 rows of W, its four waves
-// every fourth 128 columns; a lane loads 32 consecutive elements of its row with their scale, converts
-// them in registers, and multiplies them with the same 32 elements of 16 rows of x at a time
-// (v_mfma_f32_16x16x32_bf16, W as first operand: D[n][m]).  The waves' sums are joined through LDS.
+// Few rows: bound by reading W once.  A workgroup takes 16 NB rows of W, its eight waves every eighth 128
+// columns, two or four of these at once; a lane has, of its row, 32 consecutive elements with their scale (e4m3:
+// 16 and the 16 that are 64 further on, the matrix unit's layout).  The waves' sums are joined through
+// LDS.
 #include <type_traits>
 
 #include "fa_common.h"
@@ -20,21 +24,20 @@ namespace ttfa {
 
 namespace {
 
-// 32 consecutive elements of a row with their scale, as loaded; a lane past the row's end holds zeros.
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kRowWaves = 8;
+
+// 32 consecutive elements (a group) of a row of W, as bf16 for the product with x in bf16.
 template <int BITS>
-struct Mx32 {
+struct Group {
   u32x4 c[BITS / 4];
   uint32_t byte;
   __device__ __forceinline__ void load(const uint8_t *codes, const uint8_t *scales, int64_t group, bool ok) {
-    byte = 0;
+    byte = ok ? scales[group] : 0;
 #pragma unroll
-    for (int i = 0; i < BITS / 4; ++i) c[i] = u32x4{};
-    if (ok) {
-      byte = scales[group];
-#pragma unroll
-      for (int i = 0; i < BITS / 4; ++i)
-        c[i] = reinterpret_cast<const u32x4 *>(codes + group * (4 * BITS))[i];
-    }
+    for (int i = 0; i < BITS / 4; ++i)
+      c[i] = ok ? reinterpret_cast<const u32x4 *>(codes + group * (4 * BITS))[i] : u32x4{};
   }
   // elements 8 j .. 8 j + 7
   __device__ __forceinline__ bf16x8 values(int j) const {
@@ -53,69 +56,155 @@ struct Rows32 {
   __device__ __forceinline__ bf16x8 values(int j) const { return __builtin_bit_cast(bf16x8, c[j]); }
 };
 
-template <int BITS, bool XMX, int MB>
-__global__ __launch_bounds__(256) void linear_mx_rows_kernel(
+// A lane's part of 128 k's of a row as an operand of the scaled product: lane i + 16 q has the scale of
+// elements 32 q .. 32 q + 31 and those elements (BITS 4), or 16 q .. and 64 + 16 q .. (BITS 8).
+template <int BITS>
+struct Scaled {
+  u32x4 c[BITS / 4];
+  uint32_t byte;
+  // group0: the first of the row's four groups, `left` groups from there to the row's end
+  __device__ __forceinline__ void load(const uint8_t *codes, const uint8_t *scales, int64_t group0, int left, int q) {
+    byte = q < left ? scales[group0 + q] : 127;
+    if constexpr (BITS == 4) {
+      c[0] = q < left ? *reinterpret_cast<const u32x4 *>(codes + (group0 + q) * 16) : u32x4{};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        c[i] = 2 * i + q / 2 < left ? *reinterpret_cast<const u32x4 *>(codes + group0 * 32 + 64 * i + 16 * q) : u32x4{};
+    }
+  }
+  __device__ __forceinline__ i32x8 operand() const {
+    i32x8 v{};
+#pragma unroll
+    for (int i = 0; i < BITS; ++i) v[i] = (int)c[i / 4][i % 4];
+    return v;
+  }
+};
+
+template <int BITS, bool XMX, int MB, int NB>
+__global__ __launch_bounds__(64 * kRowWaves) void linear_mx_rows_kernel(
     const void *__restrict__ x, const uint8_t *__restrict__ x_scales, const uint8_t *__restrict__ codes,
     const uint8_t *__restrict__ scales, bf16 *__restrict__ y, int M, int K, int N) {
-  __shared__ f32x4 part[4][MB][64];
+  constexpr int U = XMX && MB <= 2 ? 4 : 2, STEP = 4 * kRowWaves;
+  __shared__ f32x4 part[kRowWaves][NB * MB][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, quarter = lane >> 4;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MB;
-  const int64_t groups = K / 32, wrow = (int64_t)min(n0 + row, N - 1) * groups;
-  int64_t xrow[MB];
+  const int n0 = blockIdx.x * 16 * NB, groups = K / 32;
+  int64_t wrow[NB], xrow[MB];  // rows past the end: the last one's, not stored
 #pragma unroll
-  for (int b = 0; b < MB; ++b) xrow[b] = (int64_t)min(m0 + 16 * b + row, M - 1) * groups;
-  f32x4 acc[MB] = {};
-  for (int k = 4 * wave + quarter; k - quarter < groups; k += 16) {
-    const bool ok = k < groups;
-    Mx32<BITS> w;
-    w.load(codes, scales, wrow + k, ok);
-    typename std::conditional<XMX, Mx32<8>, Rows32>::type v[MB];
+  for (int c = 0; c < NB; ++c) wrow[c] = (int64_t)min(n0 + 16 * c + row, N - 1) * groups;
 #pragma unroll
-    for (int b = 0; b < MB; ++b) {
-      if constexpr (XMX) v[b].load((const uint8_t *)x, x_scales, xrow[b] + k, ok);
-      else v[b].load((const bf16 *)x, xrow[b] + k, ok);
-    }
+  for (int b = 0; b < MB; ++b) xrow[b] = (int64_t)min(16 * b + row, M - 1) * groups;
+  f32x4 acc[NB][MB] = {};
+  for (int k = 4 * wave; k < groups; k += U * STEP) {
+    if constexpr (XMX) {
+      Scaled<BITS> w[U][NB];
+      Scaled<8> v[U][MB];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bf16x8 wv = w.values(j);
+      for (int u = 0; u < U; ++u) {
+        const int at = k + u * STEP, left = groups - at;
 #pragma unroll
-      for (int b = 0; b < MB; ++b)
-        acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, v[b].values(j), acc[b], 0, 0, 0);
+        for (int c = 0; c < NB; ++c) w[u][c].load(codes, scales, wrow[c] + at, left, quarter);
+#pragma unroll
+        for (int b = 0; b < MB; ++b) v[u][b].load((const uint8_t *)x, x_scales, xrow[b] + at, left, quarter);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int c = 0; c < NB; ++c)
+#pragma unroll
+          for (int b = 0; b < MB; ++b)
+            acc[c][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                w[u][c].operand(), v[u][b].operand(), acc[c][b], BITS == 4 ? 4 : 0, 0, 0, (int)w[u][c].byte, 0,
+                (int)v[u][b].byte);
+    } else {
+      Group<BITS> w[U][NB];
+      Rows32 v[U][MB];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int at = k + u * STEP + quarter;
+#pragma unroll
+        for (int c = 0; c < NB; ++c) w[u][c].load(codes, scales, wrow[c] + at, at < groups);
+#pragma unroll
+        for (int b = 0; b < MB; ++b) v[u][b].load((const bf16 *)x, xrow[b] + at, at < groups);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int c = 0; c < NB; ++c) {
+            const bf16x8 wv = w[u][c].values(j);
+#pragma unroll
+            for (int b = 0; b < MB; ++b)
+              acc[c][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, v[u][b].values(j), acc[c][b], 0, 0, 0);
+          }
     }
   }
 #pragma unroll
-  for (int b = 0; b < MB; ++b) part[wave][b][lane] = acc[b];
+  for (int c = 0; c < NB; ++c)
+#pragma unroll
+    for (int b = 0; b < MB; ++b) part[wave][c * MB + b][lane] = acc[c][b];
   __syncthreads();
-  for (int b = wave; b < MB; b += 4) {
-    const f32x4 t = (part[0][b][lane] + part[1][b][lane]) + (part[2][b][lane] + part[3][b][lane]);
-    const int m = m0 + 16 * b + row, n = n0 + 4 * quarter;
-    if (m < M && n < N) *reinterpret_cast<bf16x4 *>(y + (int64_t)m * N + n) = pack4(t[0], t[1], t[2], t[3]);
-  }
+  if (wave >= NB * MB) return;
+  f32x4 t{};
+#pragma unroll
+  for (int w = 0; w < kRowWaves; ++w) t += part[w][wave][lane];
+  const int m = 16 * (wave % MB) + row, n = n0 + 16 * (wave / MB) + 4 * quarter;
+  if (m < M && n < N) *reinterpret_cast<bf16x4 *>(y + (int64_t)m * N + n) = pack4(t[0], t[1], t[2], t[3]);
+}
+
+constexpr int kFewRows = 64;
+
+// f(bits, whether x is quantised) as compile-time values
+template <class F>
+hipError_t by_types(int bits, bool xmx, F f) {
+  using std::integral_constant;
+  if (bits == 4) return xmx ? f(integral_constant<int, 4>{}, std::true_type{}) : f(integral_constant<int, 4>{}, std::false_type{});
+  return xmx ? f(integral_constant<int, 8>{}, std::true_type{}) : f(integral_constant<int, 8>{}, std::false_type{});
+}
+
+// f(blocks of 16 rows of x, of 16 columns of W) for M rows: as many columns a workgroup as leave 256 of them,
+// up to eight blocks.
+template <class F>
+hipError_t by_blocks(int M, int N, F f) {
+  using std::integral_constant;
+  const int nb = (N + 16 * 256 - 1) / (16 * 256);
+  auto go = [&](auto m, auto most) {
+    constexpr int MOST = decltype(most)::value;
+    if (nb <= 1) return f(m, integral_constant<int, 1>{});
+    if (nb == 2 || MOST == 2) return f(m, integral_constant<int, 2>{});
+    if constexpr (MOST > 2) {
+      if (nb == 3) return f(m, integral_constant<int, 3>{});
+      return f(m, integral_constant<int, 4>{});
+    }
+    return hipErrorUnknown;
+  };
+  if (M <= 16) return go(integral_constant<int, 1>{}, integral_constant<int, 4>{});
+  if (M <= 32) return go(integral_constant<int, 2>{}, integral_constant<int, 4>{});
+  if (M <= 48) return go(integral_constant<int, 3>{}, integral_constant<int, 2>{});
+  return go(integral_constant<int, 4>{}, integral_constant<int, 2>{});
 }
 
 }  // namespace
 
 hipError_t launch_linear_mx(const void *x, const void *x_scales, const void *codes, const void *scales,
                             void *y, int M, int K, int N, int bits, hipStream_t stream) {
-  auto go = [&](auto bits_, auto xmx, auto mb) {
-    constexpr int MB = decltype(mb)::value;
-    linear_mx_rows_kernel<decltype(bits_)::value, decltype(xmx)::value, MB>
-        <<<dim3((N + 15) / 16, (M + 16 * MB - 1) / (16 * MB)), dim3(256), 0, stream>>>(
-            x, (const uint8_t *)x_scales, (const uint8_t *)codes, (const uint8_t *)scales, (bf16 *)y, M, K, N);
-  };
-  using std::integral_constant;
-  auto by_rows = [&](auto b, auto xmx) {
-    if (M <= 16) go(b, xmx, integral_constant<int, 1>{});
-    else if (M <= 32) go(b, xmx, integral_constant<int, 2>{});
-    else go(b, xmx, integral_constant<int, 4>{});
-  };
-  auto by_x = [&](auto b) {
-    if (x_scales) by_rows(b, std::true_type{});
-    else by_rows(b, std::false_type{});
-  };
-  if (bits == 4) by_x(integral_constant<int, 4>{});
-  else by_x(integral_constant<int, 8>{});
-  return hipGetLastError();
+  for (int m0 = 0; m0 < M; m0 += kFewRows) {
+    const int rows = M - m0 < kFewRows ? M - m0 : kFewRows;
+    const hipError_t e = by_types(bits, x_scales != nullptr, [&](auto b, auto xmx) {
+      return by_blocks(rows, N, [&](auto mb, auto nb) {
+        constexpr int NB = decltype(nb)::value;
+        const int64_t at = (int64_t)m0 * K;
+        linear_mx_rows_kernel<decltype(b)::value, decltype(xmx)::value, decltype(mb)::value, NB>
+            <<<dim3((N + 16 * NB - 1) / (16 * NB)), dim3(64 * kRowWaves), 0, stream>>>(
+                (const uint8_t *)x + (x_scales ? at : 2 * at), x_scales ? (const uint8_t *)x_scales + at / 32 : nullptr,
+                (const uint8_t *)codes, (const uint8_t *)scales, (bf16 *)y + (int64_t)m0 * N, rows, K, N);
+        return hipGetLastError();
+      });
+    });
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace ttfa
