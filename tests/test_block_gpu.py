@@ -268,7 +268,8 @@ def test_mx_quantize(shape, dtype, bits):
 
 
 LINEAR_SHAPES = [(1, 32, 8), (1, 4096, 520), (2, 96, 40), (7, 736, 104), (16, 128, 64), (17, 1024, 72), (32, 160, 136),
-                 (33, 512, 264), (64, 2048, 48), (65, 288, 128), (150, 640, 328), (520, 256, 392), (1027, 96, 136)]
+                 (33, 512, 264), (64, 2048, 48), (65, 288, 128), (150, 640, 328), (520, 256, 392), (1027, 96, 136),
+                 (66, 1152, 72), (300, 128, 1032), (900, 384, 264)]
 
 
 @pytest.mark.parametrize("bits", [4, 8])

@@ -97,8 +97,10 @@ hipError_t launch_mx_quantize(const void *x, void *codes, void *scales, int64_t 
                               bool f32, hipStream_t stream);
 
 // y [M, N] bf16 = x W^T: x [M, K] bf16 (x_scales null) or in 8 bits, W [N, K] in `bits` (linear_mx.hip).
+// workspace: linear_mx_workspace bytes.
+int64_t linear_mx_workspace(int M, int K, int N, int bits, bool x_quantised);
 hipError_t launch_linear_mx(const void *x, const void *x_scales, const void *codes, const void *scales,
-                            void *y, int M, int K, int N, int bits, hipStream_t stream);
+                            void *y, void *workspace, int M, int K, int N, int bits, hipStream_t stream);
 
 // RMSNorm of x + r over rows of C (rms_norm.hip); r and h null: of x.  Types by ttfa_dtype.
 hipError_t launch_rms_norm_fwd(const void *x, const void *r, const float *w, void *y, void *h,

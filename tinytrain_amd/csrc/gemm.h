@@ -195,6 +195,33 @@ __device__ __forceinline__ f32x16 block_regs(u32x4 a, u32x4 b) {
 
 namespace {
 
+// Work in tiles: `splits` parts of the contraction, z problems, tiles_m x tiles_n tiles of each.
+struct Tiles {
+  int splits, z, tiles_m, tiles_n;
+  __host__ __device__ int total() const { return splits * z * tiles_m * tiles_n; }
+};
+
+struct Tile {
+  int part, z, m, n;
+};
+
+// The i-th tile in the order of work.  Consecutive workgroup ids go to the 8 XCDs in turn, each with its own
+// L2, so each XCD gets a run of tiles; a run goes down bands of 8 rows of tiles before the next column:
+// those at work at one time share rows of X and of W.
+__device__ __forceinline__ Tile tile_at(const Tiles &g, int i) {
+  const int n = g.total(), x = i % 8, rem = n % 8;
+  int t = x * (n / 8) + (x < rem ? x : rem) + i / 8;
+  const int per = g.tiles_m * g.tiles_n, zs = t / per;
+  t -= zs * per;
+  const int band = 8 * g.tiles_n, b0 = t / band * 8, rows = min(8, g.tiles_m - b0), in = t - t / band * band;
+  return Tile{zs / g.z, zs % g.z, b0 + in % rows, in / rows};
+}
+
+// The first of `stages` stages that a part takes.
+__device__ __forceinline__ int first_stage(const Tiles &g, int stages, int part) {
+  return (int)((int64_t)stages * part / g.splits);
+}
+
 // kPartial: kStore's sums in fp32, one of `splits` parts of the contraction.
 enum Epilogue { kStore, kPartial, kGated, kGatedGrad };
 
@@ -206,18 +233,11 @@ struct GemmArgs {
   const bf16 *da;           // kGatedGrad
   bf16 *out[2];             // [M][N]
   float *part;              // kPartial: [splits][z][M][N]
-  int splits, tiles_m, tiles_n;
+  Tiles tiles;
 };
 
 __device__ __forceinline__ float sigmoid(float x) {
   return __builtin_amdgcn_rcpf(1.f + exp2f_fast(-x * kLog2e));
-}
-
-// The i-th of n tiles in the order of work -> tile.  Consecutive workgroup ids go to the 8 XCDs in turn,
-// each with its own L2, so each XCD gets a run of tiles.
-__device__ __forceinline__ int tile_of(int i, int n) {
-  const int per = n / 8, rem = n % 8, x = i % 8;
-  return x * per + (x < rem ? x : rem) + i / 8;
 }
 
 // Keeps a step's LDS reads among its first products, two to each, where the compiler would put them
@@ -246,22 +266,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   constexpr int STAGE = (TM + TN) * BK * 2;
   extern __shared__ __align__(1024) char lds[];
 
-  struct Tile {
-    int part, z;  // part of the contraction, problem
-    int64_t m0, n0;
-  };
-  const int per = g.tiles_m * g.tiles_n, total = g.splits * g.z * per;
+  const int total = g.tiles.total();
   const int per_seg = (int)((g.K + BK - 1) / BK), all_stages = per_seg * g.segs;
-  auto first_stage = [&](int part) { return E == kPartial ? (int)((int64_t)all_stages * part / g.splits) : part * all_stages; };
-  // Tiles go down bands of 8 rows of tiles before the next column: those at work at one time share rows
-  // of X and of W.
-  auto tile_at = [&](int i) {
-    int t = tile_of(i, total);
-    const int zs = t / per;
-    t -= zs * per;
-    const int band = 8 * g.tiles_n, b0 = t / band * 8, rows = min(8, g.tiles_m - b0), in = t - t / band * band;
-    return Tile{zs / g.z, zs % g.z, (int64_t)(b0 + in % rows) * TM, (int64_t)(in / rows) * WT};
-  };
 
   // Loads: a cursor over the stages of this workgroup's tiles.
   XL xl;
@@ -271,16 +277,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   Tile at;
   auto start = [&](int skip) {
     const int i = at.z + seg;
-    xl.init(g.x[i], g.ldx, at.m0, g.M);
-    wl.init(g.w[i], g.ldw, at.n0, g.N);
-    if constexpr (DUAL) ul.init(g.w[1], g.ldw, at.n0, g.N);
+    xl.init(g.x[i], g.ldx, (int64_t)at.m * TM, g.M);
+    wl.init(g.w[i], g.ldw, (int64_t)at.n * WT, g.N);
+    if constexpr (DUAL) ul.init(g.w[1], g.ldw, (int64_t)at.n * WT, g.N);
     if constexpr (E == kPartial) xl.skip(skip), wl.skip(skip);
     left = g.K - (int64_t)skip * BK;
   };
   auto next_tile = [&] {
-    at = tile_at(ahead);
-    const int first = first_stage(at.part);
-    to_do = first_stage(at.part + 1) - first;
+    at = tile_at(g.tiles, ahead);
+    const int first = first_stage(g.tiles, all_stages, at.part);
+    to_do = first_stage(g.tiles, all_stages, at.part + 1) - first;
     seg = first / per_seg;
     start(first - seg * per_seg);
   };
@@ -329,20 +335,21 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   read(0, 0, 0);
   int buf = 0;
   for (int i = blockIdx.x; i < total; i += gridDim.x) {
-    const Tile t = tile_at(i);
-    const int stages = first_stage(t.part + 1) - first_stage(t.part);
+    const Tile t = tile_at(g.tiles, i);
+    const int64_t m0 = (int64_t)t.m * TM, n0 = (int64_t)t.n * WT;
+    const int stages = first_stage(g.tiles, all_stages, t.part + 1) - first_stage(g.tiles, all_stages, t.part);
     f32x16 acc[MB][NB] = {};
     const int row = wm * (TM / WM) + (lane & 15), col = wn * (DUAL ? 32 : TN / WN) + 8 * piece_of(lane);
-    const uint32_t bytes = (uint32_t)((g.M - t.m0 < TM ? g.M - t.m0 : TM) * g.N * 2);
+    const uint32_t bytes = (uint32_t)((g.M - m0 < TM ? g.M - m0 : TM) * g.N * 2);
     // byte offset in the tile's rows of this lane's piece of set q of block (i, j)
     auto piece_at = [&](int i, int j, int q) {
-      const int64_t n = t.n0 + col + 32 * j;
+      const int64_t n = n0 + col + 32 * j;
       return n < g.N ? (uint32_t)((row + 32 * i + 16 * q) * g.N * 2 + n * 2) : kPastEnd;
     };
     u32x4 da[MB][2];
     for (int st = 0; st < stages; ++st) {
       if (E == kGatedGrad && st == 0) {  // a tile's time to arrive (in its last stage: 728 us for 713 at 16384 x 2048 x 6144)
-        const __amdgpu_buffer_rsrc_t r = make_rsrc(g.da + t.m0 * g.N, bytes);
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(g.da + m0 * g.N, bytes);
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
@@ -369,7 +376,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
     }
 
     if constexpr (E == kPartial) {
-      const __amdgpu_buffer_rsrc_t r = make_rsrc(g.part + ((int64_t)(t.part * g.z + t.z) * g.M + t.m0) * g.N, 2 * bytes);
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(g.part + ((int64_t)(t.part * g.z + t.z) * g.M + m0) * g.N, 2 * bytes);
 #pragma unroll
       for (int i = 0; i < MB; ++i)
 #pragma unroll
@@ -378,14 +385,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
           block_rows_f32(acc[i][j], set);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const int64_t n = t.n0 + wn * (TN / WN) + 32 * j + 16 * (q / 2) + 8 * ((lane >> 4) & 1) + 4 * (lane >> 5);
+            const int64_t n = n0 + wn * (TN / WN) + 32 * j + 16 * (q / 2) + 8 * ((lane >> 4) & 1) + 4 * (lane >> 5);
             buf_store16(r, n < g.N ? (uint32_t)((row + 32 * i + 16 * (q % 2)) * g.N * 4 + n * 4) : kPastEnd, set[q]);
           }
         }
       continue;
     }
-    const __amdgpu_buffer_rsrc_t r0 = make_rsrc(g.out[E == kStore ? t.z : 0] + t.m0 * g.N, bytes);
-    const __amdgpu_buffer_rsrc_t r1 = make_rsrc(g.out[1] + t.m0 * g.N, bytes);
+    const __amdgpu_buffer_rsrc_t r0 = make_rsrc(g.out[E == kStore ? t.z : 0] + m0 * g.N, bytes);
+    const __amdgpu_buffer_rsrc_t r1 = make_rsrc(g.out[1] + m0 * g.N, bytes);
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
       if constexpr (E == kStore) {
@@ -481,36 +488,38 @@ Cut cut_of(int64_t M, int64_t N, int64_t K, int segs, int z, bool dual) {
 int64_t part_bytes(const Cut &c, int64_t M, int64_t N, int z) { return c.splits > 1 ? 4 * c.splits * z * M * N : 0; }
 
 template <bool XTR, bool WTR, Epilogue E, int TM, int WM, int WN>
-hipError_t launch_tiles(GemmArgs g, hipStream_t stream) {
+hipError_t launch_tiles(GemmArgs g, int splits, hipStream_t stream) {
   constexpr int BK = 64, TN = TM, DUAL = E == kGated || E == kGatedGrad, WT = DUAL ? TN / 2 : TN;
   constexpr int lds = 2 * (TM + TN) * BK * 2;
   constexpr auto kernel = gemm_kernel<TM, TN, WM, WN, BK, XTR, WTR, E>;
-  g.tiles_m = (int)((g.M + TM - 1) / TM);
-  g.tiles_n = (int)((g.N + WT - 1) / WT);
+  g.tiles = Tiles{splits, g.z, (int)((g.M + TM - 1) / TM), (int)((g.N + WT - 1) / WT)};
   if constexpr (lds > 65536) {
     const hipError_t e = allow_lds<kernel>(lds);
     if (e != hipSuccess) return e;
   }
   const int slots = resident_slots<kernel>(64 * WM * WN, lds);
-  kernel<<<dim3(std::min(slots, g.splits * g.z * g.tiles_m * g.tiles_n)), dim3(64 * WM * WN), lds, stream>>>(g);
+  kernel<<<dim3(std::min(slots, g.tiles.total())), dim3(64 * WM * WN), lds, stream>>>(g);
+  return hipGetLastError();
+}
+
+hipError_t launch_sum_parts(const float *part, bf16 *out0, bf16 *out1, int splits, int64_t n0, int64_t n,
+                            hipStream_t stream) {
+  sum_parts_kernel<<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream>>>(part, out0, out1, splits, n0, n);
   return hipGetLastError();
 }
 
 template <bool XTR, bool WTR, Epilogue E>
 hipError_t launch_gemm(GemmArgs g, const Cut &c, hipStream_t stream) {
-  g.splits = c.splits;
   if constexpr (E == kStore) {
     if (c.splits > 1) {
-      const hipError_t e = c.wide ? launch_tiles<XTR, WTR, kPartial, 256, 2, 4>(g, stream)
-                                  : launch_tiles<XTR, WTR, kPartial, 128, 2, 2>(g, stream);
+      const hipError_t e = c.wide ? launch_tiles<XTR, WTR, kPartial, 256, 2, 4>(g, c.splits, stream)
+                                  : launch_tiles<XTR, WTR, kPartial, 128, 2, 2>(g, c.splits, stream);
       if (e != hipSuccess) return e;
-      const int64_t n0 = g.M * g.N / 8, n = g.z * n0;
-      sum_parts_kernel<<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream>>>(g.part, g.out[0], g.out[1],
-                                                                                   c.splits, n0, n);
-      return hipGetLastError();
+      return launch_sum_parts(g.part, g.out[0], g.out[1], c.splits, g.M * g.N / 8, g.z * g.M * g.N / 8, stream);
     }
   }
-  return c.wide ? launch_tiles<XTR, WTR, E, 256, 2, 4>(g, stream) : launch_tiles<XTR, WTR, E, 128, 2, 2>(g, stream);
+  return c.wide ? launch_tiles<XTR, WTR, E, 256, 2, 4>(g, 1, stream)
+                : launch_tiles<XTR, WTR, E, 128, 2, 2>(g, 1, stream);
 }
 
 }  // namespace

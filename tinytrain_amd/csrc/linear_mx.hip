@@ -17,6 +17,7 @@
 
 #include "fa_common.h"
 #include "fa_kernels.h"
+#include "gemm.h"
 #include "mx.h"
 #include "ttfa.h"
 
@@ -153,7 +154,187 @@ __global__ __launch_bounds__(64 * kRowWaves) void linear_mx_rows_kernel(
   if (m < M && n < N) *reinterpret_cast<bf16x4 *>(y + (int64_t)m * N + n) = pack4(t[0], t[1], t[2], t[3]);
 }
 
-constexpr int kFewRows = 64;
+// Many rows of x in 8 bits: tiles of TM x TN, stages of 128 k's, with the order of gemm_kernel (gemm.h): a
+// persistent workgroup, loads two stages ahead, operands read before they are needed.  128 k's of a row
+// of x are 128 bytes and of W 64 or 128, loaded as gemm.h's tiles of bf16 of that many bytes; the scales
+// of a stage, four bytes a row, go to LDS beside them.  A step is 16 rows of x by the wave's columns;
+// the operands of W stay in registers for a stage.  K is a multiple of 128.
+struct MxArgs {
+  const uint8_t *x, *x_scales, *codes, *scales;
+  bf16 *out;
+  float *part;  // PARTIAL: [splits][M][N]
+  int64_t M, N, K;
+  Tiles tiles;
+};
+
+// The scales of T rows, one dword each, into LDS: waves W0 .. W0 + T / 64 - 1 load one instruction each.
+template <int T, int W0>
+__device__ __forceinline__ void load_scales(const uint8_t *p, uint32_t bytes, int64_t ld, char *lds) {
+  const int w = wave_id() - W0;
+  if (w < 0 || w >= T / 64) return;
+  const __amdgpu_buffer_rsrc_t r = make_rsrc(p, bytes);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (TTFA_LDS void *)(lds + w * 256), 4,
+                                           (uint32_t)((w * 64 + (threadIdx.x & 63)) * ld), 0, 0, 0);
+}
+
+template <int TM, int TN, int WM, int WN, int BITS, bool PARTIAL>
+__global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs g) {
+  constexpr int NT = 64 * WM * WN, MB = TM / WM / 16, NB = TN / WN / 16, STORES = MB * NB / (PARTIAL ? 1 : 2);
+  constexpr int WK = BITS == 4 ? 32 : 64;  // bf16's as long as 128 elements of W
+  using XL = TileLoad<TM, 64, false, NT>;
+  using WL = TileLoad<TN, WK, false, NT>;
+  static_assert((TM + TN) / 64 <= NT / 64, "a wave loads scales once a stage");
+  constexpr int XS = XL::BYTES + WL::BYTES, WS = XS + 4 * TM, STAGE = WS + 4 * TN;
+  extern __shared__ __align__(1024) char lds[];
+  const int total = g.tiles.total(), all_stages = (int)(g.K / 128);
+  const int64_t sld = g.K / 32;
+
+  XL xl;
+  WL wl;
+  const uint8_t *xs, *ws;
+  uint32_t xs_bytes, ws_bytes;
+  int ahead = blockIdx.x, to_do;
+  auto next_tile = [&] {
+    const Tile at = tile_at(g.tiles, ahead);
+    const int first = first_stage(g.tiles, all_stages, at.part);
+    const int64_t m0 = (int64_t)at.m * TM, n0 = (int64_t)at.n * TN;
+    to_do = first_stage(g.tiles, all_stages, at.part + 1) - first;
+    xl.init(reinterpret_cast<const bf16 *>(g.x), g.K / 2, m0, g.M);
+    wl.init(reinterpret_cast<const bf16 *>(g.codes), g.K * BITS / 16, n0, g.N);
+    xl.skip(first);
+    wl.skip(first);
+    xs = g.x_scales + m0 * sld + 4 * first;
+    ws = g.scales + n0 * sld + 4 * first;
+    xs_bytes = (uint32_t)((g.M - m0 < TM ? g.M - m0 : TM) * sld) - 4 * first;
+    ws_bytes = (uint32_t)((g.N - n0 < TN ? g.N - n0 : TN) * sld) - 4 * first;
+  };
+  next_tile();
+  auto load = [&](int buf) {
+    if (ahead >= total) return;
+    char *dst = lds + buf * STAGE;
+    xl.load(dst);
+    wl.load(dst + XL::BYTES);
+    load_scales<TM, 0>(xs, xs_bytes, sld, dst + XS);
+    load_scales<TN, TM / 64>(ws, ws_bytes, sld, dst + WS);
+    xs += 4, ws += 4, xs_bytes -= 4, ws_bytes -= 4;
+    if (--to_do == 0) {
+      ahead += gridDim.x;
+      if (ahead < total) next_tile();
+    }
+  };
+
+  const int wave = wave_id(), wm = wave / WN, wn = wave % WN, lane = threadIdx.x & 63;
+  const int i16 = lane & 15, q = lane >> 4;
+  // offsets in a stage of this lane's pieces of block 0 (16 rows on: the same swizzle)
+  const int xrow = wm * (TM / WM) + i16, wrow = wn * (TN / WN) + i16;
+  const int x0 = xrow * 128 + ((q ^ XL::swizzle(xrow)) << 4), x1 = xrow * 128 + (((q + 4) ^ XL::swizzle(xrow)) << 4);
+  const int w0 = XL::BYTES + wrow * (2 * WK) + ((q ^ WL::swizzle(wrow)) << 4);
+  const int w1 = XL::BYTES + wrow * (2 * WK) + (((q + 4) ^ WL::swizzle(wrow)) << 4);  // BITS 8
+  u32x4 xf[2][2], wf[NB][BITS / 4];
+  uint32_t sx[2], sw[NB];
+  auto read_x = [&](int buf, int b, int into) {
+    const char *from = lds + buf * STAGE;
+    xf[into][0] = *reinterpret_cast<const u32x4 *>(from + x0 + b * 2048);
+    xf[into][1] = *reinterpret_cast<const u32x4 *>(from + x1 + b * 2048);
+    sx[into] = *reinterpret_cast<const uint8_t *>(from + XS + 4 * xrow + q + b * 64);
+  };
+  auto read_w = [&](int buf, int c) {
+    const char *from = lds + buf * STAGE;
+    wf[c][0] = *reinterpret_cast<const u32x4 *>(from + w0 + c * (32 * WK));
+    if constexpr (BITS == 8) wf[c][1] = *reinterpret_cast<const u32x4 *>(from + w1 + c * (32 * WK));
+    sw[c] = *reinterpret_cast<const uint8_t *>(from + WS + 4 * wrow + q + c * 64);
+  };
+  auto operand = [](const u32x4 *c, int n) {
+    i32x8 v{};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) v[i] = (int)c[i / 4][i % 4];
+    return v;
+  };
+
+  load(0);
+  wait_and_meet<0>();
+  load(1);
+#pragma unroll
+  for (int c = 0; c < NB; ++c) read_w(0, c);
+  read_x(0, 0, 0);
+  int buf = 0;
+  for (int i = blockIdx.x; i < total; i += gridDim.x) {
+    const Tile t = tile_at(g.tiles, i);
+    const int64_t m0 = (int64_t)t.m * TM, n0 = (int64_t)t.n * TN;
+    const int stages = first_stage(g.tiles, all_stages, t.part + 1) - first_stage(g.tiles, all_stages, t.part);
+    f32x4 acc[MB][NB] = {};
+    for (int st = 0; st < stages; ++st) {
+#pragma unroll
+      for (int b = 0; b < MB; ++b) {
+        if (b + 1 < MB) {
+          read_x(buf, b + 1, (b + 1) & 1);
+        } else {
+          if (st == 0 && i != (int)blockIdx.x) wait_and_meet<STORES>();
+          else wait_and_meet<0>();
+          load(buf);
+          read_x(buf ^ 1, 0, (b + 1) & 1);  // after the last stage: values that nothing uses
+        }
+#pragma unroll
+        for (int c = 0; c < NB; ++c) {
+          acc[b][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+              operand(wf[c], BITS), operand(xf[b & 1], 8), acc[b][c], BITS == 4 ? 4 : 0, 0, 0, (int)sw[c], 0,
+              (int)sx[b & 1]);
+          if (b + 1 == MB) {
+            read_w(buf ^ 1, c);  // into the registers that the product has read
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      buf ^= 1;
+    }
+
+    const int64_t rows = g.M - m0 < TM ? g.M - m0 : TM;
+    if constexpr (PARTIAL) {
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(g.part + ((int64_t)t.part * g.M + m0) * g.N, (uint32_t)(rows * g.N * 4));
+#pragma unroll
+      for (int b = 0; b < MB; ++b)
+#pragma unroll
+        for (int c = 0; c < NB; ++c) {
+          const int64_t n = n0 + wn * (TN / WN) + 16 * c + 4 * q;
+          buf_store16(r, n < g.N ? (uint32_t)((xrow + 16 * b) * g.N * 4 + n * 4) : kPastEnd,
+                      __builtin_bit_cast(u32x4, acc[b][c]));
+        }
+    } else {
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(g.out + m0 * g.N, (uint32_t)(rows * g.N * 2));
+#pragma unroll
+      for (int b = 0; b < MB; ++b)
+#pragma unroll
+        for (int c = 0; c < NB; c += 2) {
+          // lanes of odd q take the second block's halves: 16 bytes a lane, 64 of a row
+          const f32x4 u = acc[b][c], v = acc[b][c + 1];
+          const u32x2 e = __builtin_bit_cast(u32x2, pack4(u[0], u[1], u[2], u[3]));
+          const u32x2 f = __builtin_bit_cast(u32x2, pack4(v[0], v[1], v[2], v[3]));
+          const auto y0 = __builtin_amdgcn_permlane16_swap(e[0], f[0], false, false);
+          const auto y1 = __builtin_amdgcn_permlane16_swap(e[1], f[1], false, false);
+          const int64_t n = n0 + wn * (TN / WN) + 16 * c + 16 * (q & 1) + 8 * (q >> 1);
+          buf_store16(r, n < g.N ? (uint32_t)((xrow + 16 * b) * g.N * 2 + n * 2) : kPastEnd,
+                      u32x4{y0[0], y1[0], y0[1], y1[1]});
+        }
+    }
+  }
+}
+
+// Values of quantised rows in bf16, 8 a lane (for products of bf16 rows, and of K's that are no multiple of 128).
+template <int BITS>
+__global__ __launch_bounds__(256) void mx_values_kernel(const uint8_t *__restrict__ codes,
+                                                        const uint8_t *__restrict__ scales, bf16 *__restrict__ out,
+                                                        int64_t lanes) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= lanes) return;
+  u32x2 c{};
+  if constexpr (BITS == 4) c[0] = reinterpret_cast<const uint32_t *>(codes)[i];
+  else c = reinterpret_cast<const u32x2 *>(codes)[i];
+  reinterpret_cast<bf16x8 *>(out)[i] = mx_values8<BITS>(c, __uint_as_float((uint32_t)scales[i / 4] << 23));
+}
+
+constexpr int kFewRows = 64;  // of linear_mx_rows_kernel at most
 
 // f(bits, whether x is quantised) as compile-time values
 template <class F>
@@ -187,24 +368,95 @@ hipError_t by_blocks(int M, int N, F f) {
 
 }  // namespace
 
+namespace {
+
+// kRows: the kernel for few rows; kTiles: tiles of quantised operands; kValues: tiles of bf16 values, which are
+// written to the workspace first.  Measured at the borders, us: x in 8 bits, K 4096, N 12288, 64 rows: kRows 34.1,
+// kTiles 21.7, 32 rows 14.4; N 4096, 64 rows: 15.2, 14.9; K 768, N 2304: 4.1, 6.9.  x in bf16, N 12288, 64 rows:
+// kRows 41.6, kValues 47.8.
+enum Path { kRows, kTiles, kValues };
+
+Path path_of(int M, int K, int N, bool x_quantised) {
+  const bool tiles = x_quantised && K % 128 == 0;
+  if (M <= (tiles && N > 4096 ? 32 : kFewRows)) return kRows;
+  return tiles ? kTiles : kValues;
+}
+
+// 128 k's in 8 bits take the time of 64 in bf16.
+Cut mx_cut(int M, int K, int N) { return cut_of(M, N, K / 2, 1, 1, false); }
+
+template <int TM, int WM, int WN, int BITS, bool PARTIAL>
+hipError_t launch_mx_tiles(MxArgs g, int splits, hipStream_t stream) {
+  constexpr int lds = 2 * (TM * 128 + TM * 16 * BITS + 8 * TM);
+  constexpr auto kernel = linear_mx_tile_kernel<TM, TM, WM, WN, BITS, PARTIAL>;
+  g.tiles = Tiles{splits, 1, (int)((g.M + TM - 1) / TM), (int)((g.N + TM - 1) / TM)};
+  if constexpr (lds > 65536) {
+    const hipError_t e = allow_lds<kernel>(lds);
+    if (e != hipSuccess) return e;
+  }
+  const int slots = resident_slots<kernel>(64 * WM * WN, lds);
+  kernel<<<dim3(std::min(slots, g.tiles.total())), dim3(64 * WM * WN), lds, stream>>>(g);
+  return hipGetLastError();
+}
+
+template <int BITS>
+hipError_t launch_mx(const MxArgs &g, hipStream_t stream) {
+  const Cut c = mx_cut((int)g.M, (int)g.K, (int)g.N);
+  if (c.splits == 1)
+    return c.wide ? launch_mx_tiles<256, 2, 4, BITS, false>(g, 1, stream) : launch_mx_tiles<128, 2, 2, BITS, false>(g, 1, stream);
+  const hipError_t e = c.wide ? launch_mx_tiles<256, 2, 4, BITS, true>(g, c.splits, stream)
+                              : launch_mx_tiles<128, 2, 2, BITS, true>(g, c.splits, stream);
+  return e != hipSuccess ? e : launch_sum_parts(g.part, g.out, nullptr, c.splits, g.M * g.N / 8, g.M * g.N / 8, stream);
+}
+
+hipError_t launch_values(const void *codes, const void *scales, bf16 *out, int64_t elements, int bits,
+                         hipStream_t stream) {
+  const int64_t lanes = elements / 8;
+  const dim3 grid((unsigned)((lanes + 255) / 256)), block(256);
+  const uint8_t *c = (const uint8_t *)codes, *s = (const uint8_t *)scales;
+  if (bits == 4) mx_values_kernel<4><<<grid, block, 0, stream>>>(c, s, out, lanes);
+  else mx_values_kernel<8><<<grid, block, 0, stream>>>(c, s, out, lanes);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+int64_t linear_mx_workspace(int M, int K, int N, int bits, bool x_quantised) {
+  (void)bits;
+  switch (path_of(M, K, N, x_quantised)) {
+    case kRows: return 0;
+    case kTiles: return part_bytes(mx_cut(M, K, N), M, N, 1);
+    default:
+      return 2 * ((int64_t)N * K + (x_quantised ? (int64_t)M * K : 0)) + part_bytes(cut_of(M, N, K, 1, 1, false), M, N, 1);
+  }
+}
+
 hipError_t launch_linear_mx(const void *x, const void *x_scales, const void *codes, const void *scales,
-                            void *y, int M, int K, int N, int bits, hipStream_t stream) {
-  for (int m0 = 0; m0 < M; m0 += kFewRows) {
-    const int rows = M - m0 < kFewRows ? M - m0 : kFewRows;
-    const hipError_t e = by_types(bits, x_scales != nullptr, [&](auto b, auto xmx) {
-      return by_blocks(rows, N, [&](auto mb, auto nb) {
+                            void *y, void *workspace, int M, int K, int N, int bits, hipStream_t stream) {
+  const Path path = path_of(M, K, N, x_scales != nullptr);
+  if (path == kRows)
+    return by_types(bits, x_scales != nullptr, [&](auto b, auto xmx) {
+      return by_blocks(M, N, [&](auto mb, auto nb) {
         constexpr int NB = decltype(nb)::value;
-        const int64_t at = (int64_t)m0 * K;
         linear_mx_rows_kernel<decltype(b)::value, decltype(xmx)::value, decltype(mb)::value, NB>
             <<<dim3((N + 16 * NB - 1) / (16 * NB)), dim3(64 * kRowWaves), 0, stream>>>(
-                (const uint8_t *)x + (x_scales ? at : 2 * at), x_scales ? (const uint8_t *)x_scales + at / 32 : nullptr,
-                (const uint8_t *)codes, (const uint8_t *)scales, (bf16 *)y + (int64_t)m0 * N, rows, K, N);
+                x, (const uint8_t *)x_scales, (const uint8_t *)codes, (const uint8_t *)scales, (bf16 *)y, M, K, N);
         return hipGetLastError();
       });
     });
-    if (e != hipSuccess) return e;
+  if (path == kTiles) {
+    const MxArgs g{(const uint8_t *)x, (const uint8_t *)x_scales, (const uint8_t *)codes, (const uint8_t *)scales,
+                   (bf16 *)y, (float *)workspace, M, N, K, {}};
+    return bits == 4 ? launch_mx<4>(g, stream) : launch_mx<8>(g, stream);
   }
-  return hipSuccess;
+  bf16 *w = (bf16 *)workspace, *xv = w + (int64_t)N * K;
+  float *part = (float *)(xv + (x_scales ? (int64_t)M * K : 0));
+  hipError_t e = launch_values(codes, scales, w, (int64_t)N * K, bits, stream);
+  if (e == hipSuccess && x_scales) e = launch_values(x, x_scales, xv, (int64_t)M * K, 8, stream);
+  if (e != hipSuccess) return e;
+  const bf16 *xp = x_scales ? xv : (const bf16 *)x;
+  GemmArgs g{{xp, xp}, {w, w}, K, K, M, N, K, 1, 1, nullptr, {(bf16 *)y, nullptr}, part, {}};
+  return launch_gemm<false, false, kStore>(g, cut_of(M, N, K, 1, 1, false), stream);
 }
 
 }  // namespace ttfa

@@ -519,8 +519,7 @@ int ttfa_mx_quantize(const void *x, void *codes, void *scales, long long M, int 
 }
 
 long long ttfa_linear_mx_workspace_bytes(int M, int K, int N, int bits, int x_quantised) {
-  (void)x_quantised;
-  return check_linear_mx(M, K, N, bits) ? -1 : 0;
+  return check_linear_mx(M, K, N, bits) ? -1 : ttfa::linear_mx_workspace(M, K, N, bits, x_quantised != 0);
 }
 
 int ttfa_linear_mx(const void *x, const void *x_scales, const void *codes, const void *scales, void *y,
@@ -530,7 +529,7 @@ int ttfa_linear_mx(const void *x, const void *x_scales, const void *codes, const
   const void *ptrs[] = {x, codes, scales, y, x_scales ? x_scales : x, workspace};
   if ((rc = check_ptrs(ptrs, ttfa_linear_mx_workspace_bytes(M, K, N, bits, x_scales != nullptr) ? 6 : 5)))
     return rc;
-  return static_cast<int>(ttfa::launch_linear_mx(x, x_scales, codes, scales, y, M, K, N, bits,
+  return static_cast<int>(ttfa::launch_linear_mx(x, x_scales, codes, scales, y, workspace, M, K, N, bits,
                                                  static_cast<hipStream_t>(hip_stream)));
 }
 
