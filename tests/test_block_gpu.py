@@ -6,7 +6,7 @@ Tolerances count roundings.  u = 2^-24 for fp32, and half a step of the result's
 * Norm: a lane adds at most 64 squares and the rows' lanes are joined in at most 8 steps, so the mean is off
   by at most 72 u, its root by half of that, and five more roundings follow: 48 u with room.  Gradients:
   two such sums and ten roundings on the terms: 160 u of the terms' sizes.  dw adds at most 5 rows a lane
-  (1024 workgroups), 32 lane groups and 64 + 16 partials, each term off by 48 u: 170 u with the sizes of
+  (512 workgroups), 32 lane groups and 8 + 16 partials, each term off by 48 u: 170 u with the sizes of
   these tests.
 * Products: n terms in fp32, each addition off by at most 2 u (the matrix unit may cut instead of round):
   2 n u of the sum of magnitudes.  The activation (an exponential and a reciprocal of one step each, the

@@ -26,18 +26,29 @@ struct F8 {
   float v[8];
 };
 
-__device__ __forceinline__ F8 load8(const bf16 *p) {
-  const bf16x8 b = *reinterpret_cast<const bf16x8 *>(p);
+__device__ __forceinline__ bf16x8 raw8(const bf16 *p) { return *reinterpret_cast<const bf16x8 *>(p); }
+
+__device__ __forceinline__ F8 raw8(const float *p) {
+  const f32x4 a = reinterpret_cast<const f32x4 *>(p)[0], b = reinterpret_cast<const f32x4 *>(p)[1];
+  return F8{{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
+}
+
+// Eight elements as they lie in memory.
+__device__ __forceinline__ F8 floats(const bf16x8 &b) {
   F8 f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) f.v[i] = (float)b[i];
   return f;
 }
+__device__ __forceinline__ F8 floats(const F8 &f) { return f; }
 
-__device__ __forceinline__ F8 load8(const float *p) {
-  const f32x4 a = reinterpret_cast<const f32x4 *>(p)[0], b = reinterpret_cast<const f32x4 *>(p)[1];
-  return F8{{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
+template <class T>
+__device__ __forceinline__ F8 load8(const T *p) {
+  return floats(raw8(p));
 }
+
+template <class T>
+using Raw8 = typename std::conditional<std::is_same<T, float>::value, F8, bf16x8>::type;
 
 __device__ __forceinline__ void store8(bf16 *p, const F8 &f) {
   bf16x8 b;
@@ -56,26 +67,30 @@ __device__ __forceinline__ float rounded(float x) {
   return (float)(T)x;
 }
 
-// The lanes of a row: L = 2^log2 of a wave, or all 256 threads of the workgroup (WIDE).
+// The lanes of a row: L = 2^log2 of a wave, or all WT threads of the workgroup.
+template <int WT>
 struct Lanes {
+  static constexpr int THREADS = WT ? WT : 256;
   int log2;
-  __device__ __forceinline__ int lane() const { return threadIdx.x & ((1 << log2) - 1); }
-  __device__ __forceinline__ int group() const { return threadIdx.x >> log2; }
-  __device__ __forceinline__ int groups() const { return 256 >> log2; }
+  __device__ __forceinline__ int count() const { return WT ? WT : 1 << log2; }
+  __device__ __forceinline__ int lane() const { return WT ? threadIdx.x : threadIdx.x & ((1 << log2) - 1); }
+  __device__ __forceinline__ int group() const { return WT ? 0 : threadIdx.x >> log2; }
+  __device__ __forceinline__ int groups() const { return WT ? 1 : 256 >> log2; }
 };
 
 // Sum over the row's lanes; every lane gets it, from the same order of additions.  `shared` holds a
-// value per wave for WIDE rows and is free again at the next call's barrier pair.
-template <bool WIDE, class T>
-__device__ __forceinline__ T row_sum(T x, const Lanes &ln, T *shared) {
+// value per wave of a workgroup's row and is free again at the next call's barrier pair.
+template <int WT, class T>
+__device__ __forceinline__ T row_sum(T x, const Lanes<WT> &ln, T *shared) {
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1)
-    if (WIDE || m < (1 << ln.log2)) x += __shfl_xor(x, m);
-  if constexpr (WIDE) {
+    if (WT || m < (1 << ln.log2)) x += __shfl_xor(x, m);
+  if constexpr (WT != 0) {
     __syncthreads();
     if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = x;
     __syncthreads();
     x = (shared[0] + shared[1]) + (shared[2] + shared[3]);
+    if constexpr (WT == 512) x += (shared[4] + shared[5]) + (shared[6] + shared[7]);
   }
   return x;
 }
@@ -101,15 +116,15 @@ __device__ __forceinline__ void load_h(F8 (&v)[CH], const TX *x, const TR *r, TR
   }
 }
 
-template <class TX, class TR, class TY, bool RES, int CH, bool WIDE>
-__global__ __launch_bounds__(256) void rms_norm_fwd_kernel(const TX *__restrict__ x,
+template <class TX, class TR, class TY, bool RES, int CH, int WT>
+__global__ __launch_bounds__(Lanes<WT>::THREADS) void rms_norm_fwd_kernel(const TX *__restrict__ x,
                                                            const TR *__restrict__ r,
                                                            const float *__restrict__ w,
                                                            TY *__restrict__ y, TR *__restrict__ h,
-                                                           int64_t M, int nch, Lanes lanes,
+                                                           int64_t M, int nch, Lanes<WT> lanes,
                                                            float inv_c, float eps) {
-  __shared__ float shared[4];
-  const int ln = lanes.lane(), L = 1 << lanes.log2;
+  __shared__ float shared[8];
+  const int ln = lanes.lane(), L = lanes.count();
   const int64_t step = (int64_t)gridDim.x * lanes.groups();
   for (int64_t row = (int64_t)blockIdx.x * lanes.groups() + lanes.group(); row < M; row += step) {
     const int64_t at = row * nch * 8;
@@ -120,7 +135,7 @@ __global__ __launch_bounds__(256) void rms_norm_fwd_kernel(const TX *__restrict_
     for (int i = 0; i < CH; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum = fmaf(v[i].v[e], v[i].v[e], sum);
-    const float s = 1.f / sqrtf(row_sum<WIDE>(sum, lanes, shared) * inv_c + eps);
+    const float s = 1.f / sqrtf(row_sum(sum, lanes, shared) * inv_c + eps);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int c = ln + i * L;
@@ -150,16 +165,16 @@ __device__ __forceinline__ float sticky(double d) {
 // The forward with y in 8 bits: 32 elements (four lanes) share a power of two, as in the quantised
 // KV cache.  Norm and product in fp64, then one rounding, so codes do not depend on how the sum is
 // split over lanes (to about 2^-26 of a step in fp32 one value in 10^6 went to its other neighbour).
-template <class TX, class TR, bool RES, int CH, bool WIDE>
-__global__ __launch_bounds__(256) void rms_norm_mx_kernel(const TX *__restrict__ x,
+template <class TX, class TR, bool RES, int CH, int WT>
+__global__ __launch_bounds__(Lanes<WT>::THREADS) void rms_norm_mx_kernel(const TX *__restrict__ x,
                                                           const TR *__restrict__ r,
                                                           const float *__restrict__ w,
                                                           uint8_t *__restrict__ codes,
                                                           uint8_t *__restrict__ scales,
                                                           TR *__restrict__ h, int64_t M, int nch,
-                                                          Lanes lanes, double eps) {
-  __shared__ double shared[4];
-  const int ln = lanes.lane(), L = 1 << lanes.log2;
+                                                          Lanes<WT> lanes, double eps) {
+  __shared__ double shared[8];
+  const int ln = lanes.lane(), L = lanes.count();
   const int64_t step = (int64_t)gridDim.x * lanes.groups();
   for (int64_t row = (int64_t)blockIdx.x * lanes.groups() + lanes.group(); row < M; row += step) {
     const int64_t at = row * nch * 8;
@@ -170,7 +185,7 @@ __global__ __launch_bounds__(256) void rms_norm_mx_kernel(const TX *__restrict__
     for (int i = 0; i < CH; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum = fma((double)v[i].v[e], (double)v[i].v[e], sum);
-    const double s = 1.0 / sqrt(row_sum<WIDE>(sum, lanes, shared) / (double)(8 * nch) + eps);
+    const double s = 1.0 / sqrt(row_sum(sum, lanes, shared) / (double)(8 * nch) + eps);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int c = ln + i * L;
@@ -199,59 +214,75 @@ __global__ __launch_bounds__(256) void rms_norm_mx_kernel(const TX *__restrict__
 // Backward.  Workgroups walk the rows and keep dw of their rows in registers: lane groups are added
 // through LDS, the workgroup's sum goes to part[blockIdx.x] (to dw itself where it is the only one).
 // TX is the type of dx where that is another than TR (dx null: d is the gradient of both).
-template <class TX, class TR, class TY, int CH, bool WIDE>
-__global__ __launch_bounds__(256) void rms_norm_bwd_kernel(
+template <class TX, class TR, class TY, int CH, int WT>
+__global__ __launch_bounds__(Lanes<WT>::THREADS) void rms_norm_bwd_kernel(
     const TY *__restrict__ dy, const TR *__restrict__ dh, const TR *__restrict__ h,
     const float *__restrict__ w, TX *__restrict__ dx, TR *__restrict__ dr, float *__restrict__ part,
-    int64_t M, int nch, Lanes lanes, float inv_c, float eps) {
+    int64_t M, int nch, Lanes<WT> lanes, float inv_c, float eps) {
   extern __shared__ float acc_lds[];
-  __shared__ float shared[4];
-  const int ln = lanes.lane(), L = 1 << lanes.log2;
+  __shared__ float shared[8];
+  const int ln = lanes.lane(), L = lanes.count();
   const int64_t step = (int64_t)gridDim.x * lanes.groups();
   F8 acc[CH], k[CH];
+  auto load_w = [&] {
 #pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    acc[i] = F8{};
-    const int c = ln + i * L;
-    k[i] = c < nch ? load8(w + 8 * c) : F8{};
-  }
-  for (int64_t row = (int64_t)blockIdx.x * lanes.groups() + lanes.group(); row < M; row += step) {
-    const int64_t at = row * nch * 8;
-    F8 v[CH], g[CH];
-    float sq = 0.f, dot = 0.f;
+    for (int i = 0; i < CH; ++i) k[i] = ln + i * L < nch ? load8(w + 8 * (ln + i * L)) : F8{};
+  };
+#pragma unroll
+  for (int i = 0; i < CH; ++i) acc[i] = F8{};
+  // The widest rows leave no registers for w, nor for the next row on its way during a row.
+  constexpr bool AHEAD = WT != 512;
+  if (AHEAD) load_w();
+  Raw8<TR> nh[CH], nd[CH];
+  Raw8<TY> ng[CH];
+  auto load = [&](int64_t row) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int c = ln + i * L;
-      v[i] = c < nch ? load8(h + at + 8 * c) : F8{};
-      g[i] = c < nch ? load8(dy + at + 8 * c) : F8{};
+      const bool ok = row < M && c < nch;
+      const int64_t at = row * nch * 8 + 8 * c;
+      nh[i] = ok ? raw8(h + at) : Raw8<TR>{};
+      ng[i] = ok ? raw8(dy + at) : Raw8<TY>{};
+      nd[i] = ok && dh ? raw8(dh + at) : Raw8<TR>{};
+    }
+  };
+  int64_t row = (int64_t)blockIdx.x * lanes.groups() + lanes.group();
+  if (AHEAD) load(row);
+  for (; row < M; row += step) {
+    if (!AHEAD) load(row);
+    const int64_t at = row * nch * 8;
+    F8 v[CH], g[CH], d[CH];
+    float sq = 0.f, dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) v[i] = floats(nh[i]), g[i] = floats(ng[i]), d[i] = floats(nd[i]);
+    if (AHEAD) load(row + step);
+    else load_w();
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         sq = fmaf(v[i].v[e], v[i].v[e], sq);
         dot = fmaf(v[i].v[e], g[i].v[e] * k[i].v[e], dot);
       }
-    }
-    const float s = 1.f / sqrtf(row_sum<WIDE>(sq, lanes, shared) * inv_c + eps);
-    const float b = row_sum<WIDE>(dot, lanes, shared) * inv_c * s * s;
+    const float s = 1.f / sqrtf(row_sum(sq, lanes, shared) * inv_c + eps);
+    const float b = row_sum(dot, lanes, shared) * inv_c * s * s;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int c = ln + i * L;
       if (c < nch) {
-        F8 d;
-        if (dh) d = load8(dh + at + 8 * c);
-        else d = F8{};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          d.v[e] += s * (g[i].v[e] * k[i].v[e] - v[i].v[e] * b);
+          d[i].v[e] += s * (g[i].v[e] * k[i].v[e] - v[i].v[e] * b);
           acc[i].v[e] = fmaf(g[i].v[e], v[i].v[e] * s, acc[i].v[e]);
         }
-        store8(dr + at + 8 * c, d);
+        store8(dr + at + 8 * c, d[i]);
         if constexpr (!std::is_same<TX, TR>::value)
-          if (dx) store8(dx + at + 8 * c, d);
+          if (dx) store8(dx + at + 8 * c, d[i]);
       }
     }
   }
   float *out = part + (int64_t)blockIdx.x * nch * 8;
-  if constexpr (WIDE) {
+  if constexpr (WT != 0) {
 #pragma unroll
     for (int i = 0; i < CH; ++i)
       if (ln + i * L < nch) store8(out + 8 * (ln + i * L), acc[i]);
@@ -269,54 +300,65 @@ __global__ __launch_bounds__(256) void rms_norm_bwd_kernel(
   }
 }
 
-// dw = sum of n partials [n][C], in a fixed order: 16 lanes a workgroup's 64 columns, 16 rows at once.
+// dw = sum of n partials [n][C], in a fixed order: a workgroup takes 16 columns, 64 partials at once.  (With 64
+// columns and 16 partials at once 512 partials of 768 columns took 10 us, so 4.)
 __global__ __launch_bounds__(256) void rms_norm_dw_kernel(const float *__restrict__ part,
                                                           float *__restrict__ dw, int n, int nq) {
-  __shared__ f32x4 shared[16][16];
-  const int col = blockIdx.x * 16 + (threadIdx.x & 15), row = threadIdx.x >> 4;
+  __shared__ f32x4 shared[64][4];
+  const int col = blockIdx.x * 4 + (threadIdx.x & 3), row = threadIdx.x >> 2;
   f32x4 t{};
   if (col < nq)
-    for (int i = row; i < n; i += 16) t += reinterpret_cast<const f32x4 *>(part)[(int64_t)i * nq + col];
-  shared[row][threadIdx.x & 15] = t;
+#pragma unroll 8
+    for (int i = row; i < n; i += 64) t += reinterpret_cast<const f32x4 *>(part)[(int64_t)i * nq + col];
+  shared[row][threadIdx.x & 3] = t;
+  __syncthreads();
+  if (row < 8) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) t += shared[row + 8 * i][threadIdx.x & 3];
+    shared[row][threadIdx.x & 3] = t;
+  }
   __syncthreads();
   if (row == 0 && col < nq) {
-    for (int i = 1; i < 16; ++i) t += shared[i][threadIdx.x];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) t += shared[i][threadIdx.x];
     reinterpret_cast<f32x4 *>(dw)[col] = t;
   }
 }
 
-// How a row of nch chunks is spread: lanes (log2), chunks a lane.
+// How a row of nch chunks is spread: lanes (log2; 8, 9: the workgroup's), chunks a lane.
 struct Spread {
   int log2, ch;
-  bool wide() const { return log2 == 8; }
+  int threads() const { return log2 == 9 ? 512 : 256; }
 };
 
-Spread spread_of(int nch) {
+// Up to four chunks a lane, fewer where the rows would not give 512 workgroups.
+Spread spread_of(int nch, int64_t M) {
   for (int l = 3; l <= 6; ++l)
-    if (nch <= 4 << l) {
-      const int ch = (nch + (1 << l) - 1) >> l;
-      return {l, ch};
+    if (nch <= 3 << l) {
+      while (l < 6 && nch > 1 << l && M >> (8 - l) < 512) ++l;
+      return {l, (nch + (1 << l) - 1) >> l};
     }
-  const int ch = (nch + 255) / 256;
-  return {8, ch <= 2 ? 2 : ch <= 4 ? 4 : 8};
+  return nch <= 256 ? Spread{8, 1} : nch <= 512 ? Spread{8, 2} : nch <= 1024 ? Spread{8, 4} : Spread{9, 4};
 }
 
-// f(chunks a lane, wide) as compile-time values
+// f(chunks a lane, threads of a workgroup's row or 0) as compile-time values
 template <class F>
 void by_spread(const Spread &s, F f) {
   using std::integral_constant;
-  auto go = [&](auto ch, auto wide) { f(ch, wide); };
-  if (s.wide()) {
-    if (s.ch == 2) go(integral_constant<int, 2>{}, std::true_type{});
-    else if (s.ch == 4) go(integral_constant<int, 4>{}, std::true_type{});
-    else go(integral_constant<int, 8>{}, std::true_type{});
-  } else {
-    if (s.ch == 1) go(integral_constant<int, 1>{}, std::false_type{});
-    else if (s.ch == 2) go(integral_constant<int, 2>{}, std::false_type{});
-    else if (s.ch == 3) go(integral_constant<int, 3>{}, std::false_type{});
-    else go(integral_constant<int, 4>{}, std::false_type{});
-  }
+  using One = integral_constant<int, 1>;
+  using Two = integral_constant<int, 2>;
+  using Three = integral_constant<int, 3>;
+  using Four = integral_constant<int, 4>;
+  if (s.log2 == 9) return f(Four{}, integral_constant<int, 512>{});
+  if (s.log2 == 8 && s.ch == 1) return f(One{}, integral_constant<int, 256>{});
+  if (s.log2 == 8) return s.ch == 2 ? f(Two{}, integral_constant<int, 256>{}) : f(Four{}, integral_constant<int, 256>{});
+  using InWave = integral_constant<int, 0>;
+  if (s.ch == 1) return f(One{}, InWave{});
+  if (s.ch == 2) return f(Two{}, InWave{});
+  return f(Three{}, InWave{});
 }
+
+int64_t rows_of_workgroup(const Spread &s) { return s.log2 >= 8 ? 1 : 256 >> s.log2; }
 
 // f(value of the type that dt names)
 template <class F>
@@ -327,23 +369,25 @@ void by_type(int dt, F f) {
 
 // Workgroups of a forward: one pass over the rows up to 2^20 workgroups, then each takes several.
 unsigned fwd_grid(int64_t M, const Spread &s) {
-  const int64_t per = 256 >> s.log2, n = (M + per - 1) / per;
+  const int64_t per = rows_of_workgroup(s), n = (M + per - 1) / per;
   return (unsigned)(n < 1 << 20 ? n : 1 << 20);
 }
 
 }  // namespace
 
+constexpr int kMostParts = 512;  // workgroups of a backward: what is resident at once, two a CU
+
 int rms_norm_bwd_parts(int64_t M, int C) {
-  const Spread s = spread_of(C / 8);
-  const int64_t per = 256 >> s.log2, n = (M + per - 1) / per;
-  return (int)(n < 1024 ? n : 1024);
+  const Spread s = spread_of(C / 8, M);
+  const int64_t per = rows_of_workgroup(s), n = (M + per - 1) / per;
+  return (int)(n < kMostParts ? n : kMostParts);
 }
 
 hipError_t launch_rms_norm_fwd(const void *x, const void *r, const float *w, void *y, void *h,
                                int64_t M, int C, int x_dtype, int r_dtype, int y_dtype, double eps,
                                hipStream_t stream) {
   const int nch = C / 8;
-  const Spread sp = spread_of(nch);
+  const Spread sp = spread_of(nch, M);
   const dim3 grid(fwd_grid(M, sp));
   by_spread(sp, [&](auto ch, auto wide) {
     by_type(x_dtype, [&](auto tx) {
@@ -351,17 +395,17 @@ hipError_t launch_rms_norm_fwd(const void *x, const void *r, const float *w, voi
         using TX = decltype(tx);
         using TY = decltype(ty);
         constexpr int CH = decltype(ch)::value;
-        constexpr bool W = decltype(wide)::value;
+        constexpr int W = decltype(wide)::value;
         if (r)
           by_type(r_dtype, [&](auto tr) {
             using TR = decltype(tr);
-            rms_norm_fwd_kernel<TX, TR, TY, true, CH, W><<<grid, dim3(256), 0, stream>>>(
-                (const TX *)x, (const TR *)r, w, (TY *)y, (TR *)h, M, nch, Lanes{sp.log2}, 1.f / C,
+            rms_norm_fwd_kernel<TX, TR, TY, true, CH, W><<<grid, dim3(sp.threads()), 0, stream>>>(
+                (const TX *)x, (const TR *)r, w, (TY *)y, (TR *)h, M, nch, Lanes<W>{sp.log2}, 1.f / C,
                 (float)eps);
           });
         else
-          rms_norm_fwd_kernel<TX, TX, TY, false, CH, W><<<grid, dim3(256), 0, stream>>>(
-              (const TX *)x, nullptr, w, (TY *)y, nullptr, M, nch, Lanes{sp.log2}, 1.f / C, (float)eps);
+          rms_norm_fwd_kernel<TX, TX, TY, false, CH, W><<<grid, dim3(sp.threads()), 0, stream>>>(
+              (const TX *)x, nullptr, w, (TY *)y, nullptr, M, nch, Lanes<W>{sp.log2}, 1.f / C, (float)eps);
       });
     });
   });
@@ -372,24 +416,24 @@ hipError_t launch_rms_norm_mx(const void *x, const void *r, const float *w, void
                               void *h, int64_t M, int C, int x_dtype, int r_dtype, double eps,
                               hipStream_t stream) {
   const int nch = C / 8;
-  const Spread sp = spread_of(nch);
+  const Spread sp = spread_of(nch, M);
   const dim3 grid(fwd_grid(M, sp));
   by_spread(sp, [&](auto ch, auto wide) {
     by_type(x_dtype, [&](auto tx) {
       using TX = decltype(tx);
       constexpr int CH = decltype(ch)::value;
-      constexpr bool W = decltype(wide)::value;
+      constexpr int W = decltype(wide)::value;
       if (r)
         by_type(r_dtype, [&](auto tr) {
           using TR = decltype(tr);
-          rms_norm_mx_kernel<TX, TR, true, CH, W><<<grid, dim3(256), 0, stream>>>(
+          rms_norm_mx_kernel<TX, TR, true, CH, W><<<grid, dim3(sp.threads()), 0, stream>>>(
               (const TX *)x, (const TR *)r, w, (uint8_t *)codes, (uint8_t *)scales, (TR *)h, M, nch,
-              Lanes{sp.log2}, eps);
+              Lanes<W>{sp.log2}, eps);
         });
       else
-        rms_norm_mx_kernel<TX, TX, false, CH, W><<<grid, dim3(256), 0, stream>>>(
+        rms_norm_mx_kernel<TX, TX, false, CH, W><<<grid, dim3(sp.threads()), 0, stream>>>(
             (const TX *)x, nullptr, w, (uint8_t *)codes, (uint8_t *)scales, nullptr, M, nch,
-            Lanes{sp.log2}, eps);
+            Lanes<W>{sp.log2}, eps);
     });
   });
   return hipGetLastError();
@@ -399,7 +443,7 @@ hipError_t launch_rms_norm_bwd(const void *dy, const void *dh, const void *h, co
                                void *dr, float *dw, float *part, int64_t M, int C, int r_dtype,
                                int y_dtype, double eps, hipStream_t stream) {
   const int nch = C / 8, parts = rms_norm_bwd_parts(M, C);
-  const Spread sp = spread_of(nch);
+  const Spread sp = spread_of(nch, M);
   float *out = parts == 1 ? dw : part;
   by_spread(sp, [&](auto ch, auto wide) {
     by_type(r_dtype, [&](auto tr) {
@@ -407,16 +451,16 @@ hipError_t launch_rms_norm_bwd(const void *dy, const void *dh, const void *h, co
         using TR = decltype(tr);
         using TY = decltype(ty);
         using TX = typename std::conditional<std::is_same<TR, float>::value, bf16, float>::type;
-        constexpr bool W = decltype(wide)::value;
-        const size_t lds = W ? 0 : (size_t)(256 >> sp.log2) * C * sizeof(float);
-        rms_norm_bwd_kernel<TX, TR, TY, decltype(ch)::value, W><<<dim3(parts), dim3(256), lds, stream>>>(
+        constexpr int W = decltype(wide)::value;
+        const size_t lds = W != 0 ? 0 : (size_t)(256 >> sp.log2) * C * sizeof(float);
+        rms_norm_bwd_kernel<TX, TR, TY, decltype(ch)::value, W><<<dim3(parts), dim3(sp.threads()), lds, stream>>>(
             (const TY *)dy, (const TR *)dh, (const TR *)h, w, (TX *)dx, (TR *)dr, out, M, nch,
-            Lanes{sp.log2}, 1.f / C, (float)eps);
+            Lanes<W>{sp.log2}, 1.f / C, (float)eps);
       });
     });
   });
   if (parts > 1)
-    rms_norm_dw_kernel<<<dim3((C / 4 + 15) / 16), dim3(256), 0, stream>>>(part, dw, parts, C / 4);
+    rms_norm_dw_kernel<<<dim3((C / 4 + 3) / 4), dim3(256), 0, stream>>>(part, dw, parts, C / 4);
   return hipGetLastError();
 }
 
