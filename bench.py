@@ -869,7 +869,8 @@ def _decode_bench(dev, steps: int, warmup: int, settle_ms: float = 0.0) -> int:
 def _model_bench(dev, steps: int, warmup: int, batch: int) -> int:
     """Whole-model training step (forward, backward, AdamW) of the reference's 112M shape
     under torch.compile, with attn_impl "sdpa" (enable_gqa, the reference's
-    "compile + GQA" row, docs/results.md:178) vs "hip" vs "hip" + fused prologue; plus
+    "compile + GQA" row, docs/results.md:178) vs "hip" vs "hip" + fused prologue vs that with
+    the block's other operators (norms with the residual additions, gated feed-forward); plus
     the logits of the same weights and tokens under each implementation."""
     import torch
 
@@ -887,23 +888,30 @@ def _model_bench(dev, steps: int, warmup: int, batch: int) -> int:
         opt_name = "AdamW (foreach)"
     tok = torch.randint(0, c.vocab_size, (batch, T + 1), device=dev)
     inp, tgt = tok[:, :-1].contiguous(), tok[:, 1:].contiguous()
-    impls = [("sdpa", False, True), ("hip", False, False), ("hip", True, False)]
+    # attn_impl, fused prologue, enable_gqa, block_impl
+    impls = [("sdpa", False, True, "eager"), ("hip", False, False, "eager"), ("hip", True, False, "eager"),
+             ("hip", True, False, "hip")]
+
+    def select(name, fused, gqa, block):
+        model.set_attn_impl(name, fused_prologue=fused, enable_gqa=gqa)
+        model.set_block_impl(block)
+        return name + ("+fused_prologue" if fused else "") + ("+hip_block" if block == "hip" else "")
 
     # logits of one set of weights under each implementation (eager, no grad)
     logits = {}
     with torch.no_grad(), torch.autocast(device_type="cuda", dtype=torch.bfloat16):
-        for name, fused, gqa in impls:
-            model.set_attn_impl(name, fused_prologue=fused, enable_gqa=gqa)
-            logits[(name, fused)] = model(inp[:4])[0].float()
-    ref = logits[("sdpa", False)]
-    parity = {f"{n}{'+fused_prologue' if f else ''}": {
+        for impl in impls:
+            key = select(*impl)
+            logits[key] = model(inp[:4])[0].float()
+    ref = logits["sdpa"]
+    parity = {key: {
         "max_abs_vs_sdpa": round((l - ref).abs().max().item(), 5),
         "mean_abs_vs_sdpa": round((l - ref).abs().mean().item(), 6)}
-        for (n, f), l in logits.items() if (n, f) != ("sdpa", False)}
+        for key, l in logits.items() if key != "sdpa"}
 
     res = {}
-    for name, fused, gqa in impls:
-        model.set_attn_impl(name, fused_prologue=fused, enable_gqa=gqa)
+    for impl in impls:
+        key = select(*impl)
         torch._dynamo.reset()
         cm = torch.compile(model)
 
@@ -916,7 +924,6 @@ def _model_bench(dev, steps: int, warmup: int, batch: int) -> int:
 
         ms = _ev_time(step, steps, warmup)
         tps = batch * T / (ms * 1e-3)
-        key = f"{name}{'+fused_prologue' if fused else ''}"
         res[key] = {"ms_per_step": round(ms, 3), "tokens_per_s": round(tps, 1),
                     "model_tflops": round(c.train_flop_per_token(T) * tps / 1e12, 1)}
         print(f"[model] {key}: {ms:.2f} ms/step, {tps:.0f} tok/s", file=sys.stderr, flush=True)

@@ -6,7 +6,9 @@ Structure and defaults follow the reference's model.py: ``ModelConfig`` (:9-21, 
 112M pretrain shape: hidden 768, 12 layers, 8 query / 2 KV heads of 128, SwiGLU 2304,
 T <= 512, RoPE base 1e6, tied embeddings), pre-norm blocks (:128-139), final RMSNorm and
 a tied LM head with mean cross-entropy (:143-212), normal(0, 0.02) init (:183-186).
-Attention, RMSNorm and RoPE come from ``tinytrain_amd.attention``.  Chunked
+Attention, RMSNorm and RoPE come from ``tinytrain_amd.attention``.  ``set_block_impl("hip")`` runs
+the rest of a block as HIP operators: the residual additions with the norms behind them
+(``add_rms_norm``) and the MLP's two projections with their activation (``swiglu``).  Chunked
 cross-entropy and activation checkpointing (reference training options) are not part of
 this benchmark model.
 """
@@ -15,10 +17,27 @@ from __future__ import annotations
 
 from dataclasses import dataclass
 
+import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
 from .attention import Attention, RMSNorm, precompute_rope, validate_attn_impl
+from .kernels.rms_norm import add_rms_norm, rms_norm
+from .kernels.swiglu import swiglu
+
+BLOCK_IMPLS = ("eager", "hip")
+
+
+def validate_block_impl(name: str) -> str:
+    """Reject anything but a known implementation name, as validate_attn_impl does."""
+    if name not in BLOCK_IMPLS:
+        raise ValueError(f"block_impl must be one of {BLOCK_IMPLS}, got {name!r}")
+    return name
+
+
+def _compute_dtype(x: torch.Tensor) -> torch.dtype:
+    """What a linear layer computes in: autocast's type where that is on."""
+    return torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
 
 
 @dataclass
@@ -65,8 +84,13 @@ class MLP(nn.Module):
         self.gate_proj = nn.Linear(c.hidden_size, c.intermediate_size, bias=False)
         self.up_proj = nn.Linear(c.hidden_size, c.intermediate_size, bias=False)
         self.down_proj = nn.Linear(c.intermediate_size, c.hidden_size, bias=False)
+        self.block_impl = "eager"
 
     def forward(self, x):
+        if self.block_impl == "hip":
+            dt = _compute_dtype(x)
+            a = swiglu(x.to(dt), self.gate_proj.weight.to(dt), self.up_proj.weight.to(dt))
+            return self.down_proj(a)
         return self.down_proj(F.silu(self.gate_proj(x)) * self.up_proj(x))
 
 
@@ -96,6 +120,7 @@ class ModelForCausalLM(nn.Module):
         self.layers = nn.ModuleList(Block(c) for _ in range(c.num_hidden_layers))
         self.norm = RMSNorm(c.hidden_size, c.rms_norm_eps)
         self.lm_head = nn.Linear(c.hidden_size, c.vocab_size, bias=False)
+        self.block_impl = "eager"
         cos, sin = precompute_rope(c.head_dim, c.max_seq_len, c.rope_theta)
         self.register_buffer("cos", cos, persistent=False)
         self.register_buffer("sin", sin, persistent=False)
@@ -116,15 +141,43 @@ class ModelForCausalLM(nn.Module):
                 mod.fused_prologue = fused_prologue
                 mod.enable_gqa = enable_gqa
 
+    def set_block_impl(self, block_impl: str) -> None:
+        """Select how the norms, residual additions and gate and up projections of every block run:
+        ``"eager"`` expressions, or ``"hip"`` operators (bf16 compute: under autocast, or bf16 weights)."""
+        self.block_impl = validate_block_impl(block_impl)
+        for blk in self.layers:
+            blk.mlp.block_impl = block_impl
+
+    def _hip_blocks(self, h, cos, sin):
+        """The blocks and the final norm with every residual addition in the norm behind it: h is the residual
+        stream, x the newest branch's output that is not added to it yet."""
+        dt, x = _compute_dtype(h), None
+
+        def norm(n):
+            nonlocal h
+            if x is None:
+                return rms_norm(h, n.weight, n.eps, dt)
+            y, h = add_rms_norm(x, h, n.weight, n.eps, dt)
+            return y
+
+        for blk in self.layers:
+            x = blk.self_attn(norm(blk.input_layernorm), cos, sin)
+            x = blk.mlp(norm(blk.post_attention_layernorm))
+        return norm(self.norm)
+
     def forward(self, input_ids, targets=None):
         B, T = input_ids.shape
         if T > self.config.max_seq_len:
             raise ValueError(f"T={T} exceeds max_seq_len={self.config.max_seq_len}")
         x = self.embed_tokens(input_ids)
         cos, sin = self.cos[:T], self.sin[:T]
-        for blk in self.layers:
-            x = blk(x, cos, sin)
-        logits = self.lm_head(self.norm(x))
+        if self.block_impl == "hip":
+            x = self._hip_blocks(x, cos, sin)
+        else:
+            for blk in self.layers:
+                x = blk(x, cos, sin)
+            x = self.norm(x)
+        logits = self.lm_head(x)
         loss = None
         if targets is not None:
             loss = F.cross_entropy(logits.view(B * T, -1), targets.view(B * T))
