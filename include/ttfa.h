@@ -380,18 +380,22 @@ int ttfa_rms_norm_bwd(const void *dy, const void *dh, const void *h, const float
 /*
  * Gated feed-forward input (model.py:111-125), bf16 with fp32 sums:
  *   a = silu(x w_gate^T) * (x w_up^T):  x [M, K], w_gate and w_up [N, K], a [M, N]
- * ttfa_swiglu_bwd: da [M, N] -> dx [M, K], dw_gate and dw_up [N, K]; dx, or both weight gradients, may be
- * NULL (not computed).  The products are formed again, nothing of the forward is kept but its inputs.
- * K and N multiples of 8, up to 2^20.  workspace: ttfa_swiglu_workspace_bytes of the pass (backward 0 or
- * 1), or NULL where that is 0.
+ * saved, if not NULL, gets ttfa_swiglu_saved_bytes for the backward: both products in 20 bits (12
+ * significant ones), 5 bytes an element.
+ * ttfa_swiglu_bwd: da [M, N] and saved -> dx [M, K], dw_gate and dw_up [N, K]; dx, or both weight
+ * gradients, may be NULL (not computed).  workspace: ttfa_swiglu_workspace_bytes.  Two to five launches;
+ * sums in a fixed order.
+ * K and N multiples of 8, up to 2^20.
  */
-long long ttfa_swiglu_workspace_bytes(int M, int K, int N, int backward);
+long long ttfa_swiglu_saved_bytes(int M, int N);
 
-int ttfa_swiglu_fwd(const void *x, const void *w_gate, const void *w_up, void *a, void *workspace, int M,
-                    int K, int N, void *hip_stream);
+int ttfa_swiglu_fwd(const void *x, const void *w_gate, const void *w_up, void *a, void *saved, int M, int K,
+                    int N, void *hip_stream);
 
-int ttfa_swiglu_bwd(const void *da, const void *x, const void *w_gate, const void *w_up, void *dx,
-                    void *dw_gate, void *dw_up, void *workspace, int M, int K, int N,
+long long ttfa_swiglu_workspace_bytes(int M, int K, int N);
+
+int ttfa_swiglu_bwd(const void *da, const void *saved, const void *x, const void *w_gate, const void *w_up,
+                    void *dx, void *dw_gate, void *dw_up, void *workspace, int M, int K, int N,
                     void *hip_stream);
 
 /*

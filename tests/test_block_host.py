@@ -12,7 +12,7 @@ from oracle import block
 from tinytrain_amd import _lib
 from tinytrain_amd.kernels.linear_mx import linear_mx, mx_quantize
 from tinytrain_amd.kernels.rms_norm import BlockInputError, add_rms_norm, add_rms_norm_mx, rms_norm, rms_norm_bwd
-from tinytrain_amd.kernels.swiglu import swiglu, swiglu_bwd
+from tinytrain_amd.kernels.swiglu import swiglu, swiglu_bwd, swiglu_fwd
 
 BF, F32, U8 = torch.bfloat16, torch.float32, torch.uint8
 needs_lib = pytest.mark.skipif(not _lib.LIB_PATH.exists(),
@@ -83,7 +83,7 @@ def _swiglu_fwd(p=P, M=64, K=64, N=64):
 
 
 def _swiglu_bwd(p=P, M=64, K=64, N=64):
-    return _lib.load().ttfa_swiglu_bwd(*p[:8], M, K, N, None)
+    return _lib.load().ttfa_swiglu_bwd(*p[:9], M, K, N, None)
 
 
 def _quantize(p=P, M=4, K=64, bits=4, dt=0):
@@ -116,7 +116,7 @@ def test_argument_errors_return_codes(entry, kw, code):
 @needs_lib
 @pytest.mark.parametrize("entry, required, n", [
     (_norm, (0, 2, 3), 5), (_norm_mx, (0, 2, 3, 4), 6), (_norm_bwd, (0, 2, 3, 5, 6, 7), 8),
-    (_swiglu_fwd, (0, 1, 2, 3), 4), (_swiglu_bwd, (0, 1, 2, 3, 7), 8), (_quantize, (0, 1, 2), 3),
+    (_swiglu_fwd, (0, 1, 2, 3), 5), (_swiglu_bwd, (0, 1, 2, 3, 4, 8), 9), (_quantize, (0, 1, 2), 3),
     (_linear, (0, 2, 3, 4), 5)])
 def test_null_and_misaligned_pointers(entry, required, n):
     for i in range(n):
@@ -131,13 +131,13 @@ def test_null_and_misaligned_pointers(entry, required, n):
 @needs_lib
 def test_pointers_that_come_together():
     """A residual and its sum; the two weight gradients; at least one gradient."""
-    for entry, pair in ((_norm, (1, 4)), (_norm_mx, (1, 5)), (_swiglu_bwd, (5, 6))):
+    for entry, pair in ((_norm, (1, 4)), (_norm_mx, (1, 5)), (_swiglu_bwd, (6, 7))):
         for i in pair:
             bad = list(P)
             bad[i] = None
             assert entry(bad) == _lib.E_NULL
     bad = list(P)
-    bad[4] = bad[5] = bad[6] = None
+    bad[5] = bad[6] = bad[7] = None
     assert _swiglu_bwd(bad) == _lib.E_NULL
 
 
@@ -147,8 +147,9 @@ def test_workspace_sizes():
     assert lib.ttfa_rms_norm_workspace_bytes(0, 64) == lib.ttfa_rms_norm_workspace_bytes(4, 60) == -1
     assert lib.ttfa_rms_norm_workspace_bytes(1, 64) == 0
     assert lib.ttfa_rms_norm_workspace_bytes(1 << 20, 64) % (64 * 4) == 0
-    assert lib.ttfa_swiglu_workspace_bytes(4, 64, 60, 0) == -1
-    assert lib.ttfa_swiglu_workspace_bytes(1 << 20, 64, 1 << 14, 1) >= 4 << 34   # past 32 bits
+    assert lib.ttfa_swiglu_workspace_bytes(4, 64, 60) == lib.ttfa_swiglu_saved_bytes(4, 60) == -1
+    assert lib.ttfa_swiglu_workspace_bytes(1 << 20, 64, 1 << 14) >= 4 << 34   # past 32 bits
+    assert lib.ttfa_swiglu_saved_bytes(1 << 20, 1 << 14) == 5 << 34
     assert lib.ttfa_linear_mx_workspace_bytes(4, 64, 64, 5, 0) == -1
     assert lib.ttfa_linear_mx_workspace_bytes(1, 64, 64, 4, 0) >= 0
 
@@ -258,9 +259,11 @@ def test_fake_shapes():
         wg, wu = _e(48, 64), _e(48, 64)
         a = swiglu(x, wg, wu)
         assert a.shape == (3, 5, 48)
-        dx, dg, du = swiglu_bwd(a, x, wg, wu, True, False)
+        kept = swiglu_fwd(x, wg, wu, True)[1]
+        assert kept.shape == (5 * 15 * 48,) and swiglu_fwd(x, wg, wu, False)[1].numel() == 0
+        dx, dg, du = swiglu_bwd(a, kept, x, wg, wu, True, False)
         assert dx.shape == x.shape and dg.numel() == du.numel() == 0
-        assert swiglu_bwd(a, x, wg, wu, False, True)[1].shape == wg.shape
+        assert swiglu_bwd(a, kept, x, wg, wu, False, True)[1].shape == wg.shape
         codes, scales, h = add_rms_norm_mx(x, None, w)
         assert codes.shape == (3, 5, 64) and scales.shape == (3, 5, 2) and h.shape == x.shape
         wc, ws = mx_quantize(_e(48, 64), 4)

@@ -35,7 +35,8 @@ EXPORTED = ("ttfa_abi_version", "ttfa_strerror", "ttfa_fwd", "ttfa_bwd", "ttfa_b
             "ttfa_bwd_workspace_bytes", "ttfa_bwd_ws", "ttfa_kv_append", "ttfa_kv_read",
             "ttfa_decode_mx_workspace_bytes", "ttfa_decode_mx_fwd", "ttfa_rms_norm_fwd",
             "ttfa_rms_norm_mx", "ttfa_rms_norm_workspace_bytes", "ttfa_rms_norm_bwd",
-            "ttfa_swiglu_workspace_bytes", "ttfa_swiglu_fwd", "ttfa_swiglu_bwd", "ttfa_mx_quantize",
+            "ttfa_swiglu_saved_bytes", "ttfa_swiglu_workspace_bytes", "ttfa_swiglu_fwd", "ttfa_swiglu_bwd",
+            "ttfa_mx_quantize",
             "ttfa_linear_mx_workspace_bytes", "ttfa_linear_mx")
 
 
@@ -84,9 +85,10 @@ _SIGS = {
     "ttfa_rms_norm_mx": ([_vp] * 6 + [_ll] + [_i] * 3 + [_d, _vp], _i),
     "ttfa_rms_norm_workspace_bytes": ([_ll, _i], _ll),
     "ttfa_rms_norm_bwd": ([_vp] * 8 + [_ll] + [_i] * 3 + [_d, _vp], _i),
-    "ttfa_swiglu_workspace_bytes": ([_i] * 4, _ll),
+    "ttfa_swiglu_saved_bytes": ([_i] * 2, _ll),
+    "ttfa_swiglu_workspace_bytes": ([_i] * 3, _ll),
     "ttfa_swiglu_fwd": ([_vp] * 5 + [_i] * 3 + [_vp], _i),
-    "ttfa_swiglu_bwd": ([_vp] * 8 + [_i] * 3 + [_vp], _i),
+    "ttfa_swiglu_bwd": ([_vp] * 9 + [_i] * 3 + [_vp], _i),
     "ttfa_mx_quantize": ([_vp] * 3 + [_ll] + [_i] * 3 + [_vp], _i),
     "ttfa_linear_mx_workspace_bytes": ([_i] * 5, _ll),
     "ttfa_linear_mx": ([_vp] * 6 + [_i] * 4 + [_vp], _i),

@@ -116,14 +116,15 @@ hipError_t launch_rms_norm_bwd(const void *dy, const void *dh, const void *h, co
                                void *dr, float *dw, float *part, int64_t M, int C, int r_dtype,
                                int y_dtype, double eps, hipStream_t stream);
 
-// a [M, N] = silu(x Wg^T) (x Wu^T), bf16, and its backward (swiglu.hip).  dx, or both weight
-// gradients, may be null.  workspace: swiglu_bwd_workspace bytes.
+// a [M, N] = silu(x Wg^T) (x Wu^T), bf16, and its backward (swiglu.hip).  saved: swiglu_saved_bytes for the
+// backward, may be null.  dx, or both weight gradients, may be null.  workspace: swiglu_bwd_workspace bytes.
+int64_t swiglu_saved_bytes(int M, int N);
+hipError_t launch_swiglu_fwd(const void *x, const void *w_gate, const void *w_up, void *a, void *saved, int M,
+                             int K, int N, hipStream_t stream);
 int64_t swiglu_bwd_workspace(int M, int K, int N);
-hipError_t launch_swiglu_fwd(const void *x, const void *w_gate, const void *w_up, void *a, int M, int K,
-                             int N, hipStream_t stream);
-hipError_t launch_swiglu_bwd(const void *da, const void *x, const void *w_gate, const void *w_up, void *dx,
-                             void *dw_gate, void *dw_up, void *workspace, int M, int K, int N,
-                             hipStream_t stream);
+hipError_t launch_swiglu_bwd(const void *da, const void *saved, const void *x, const void *w_gate,
+                             const void *w_up, void *dx, void *dw_gate, void *dw_up, void *workspace, int M,
+                             int K, int N, hipStream_t stream);
 
 hipError_t launch_fwd_f32(const void *q, const void *k, const void *v, void *o, float *lse,
                           int B, int Hq, int Hkv, int T, int D, float scale, hipStream_t stream);

@@ -46,6 +46,10 @@ __device__ __forceinline__ void buf_store16(__amdgpu_buffer_rsrc_t r, uint32_t b
   __builtin_amdgcn_raw_buffer_store_b128(v, r, byte_off, 0, 0);
 }
 
+__device__ __forceinline__ void buf_store8(__amdgpu_buffer_rsrc_t r, uint32_t byte_off, u32x2 v) {
+  __builtin_amdgcn_raw_buffer_store_b64(v, r, byte_off, 0, 0);
+}
+
 constexpr uint32_t kPastEnd = 0x80000000u;  // an offset that no tile's buffer covers
 
 // One operand's tile of T rows (of the m or n index) x BK, loaded by NT threads, stage after stage along k.
@@ -156,16 +160,39 @@ __device__ __forceinline__ void swap_rows(u32x4 &a, u32x4 &b) {
   }
 }
 
-__device__ __forceinline__ void block_rows(const f32x16 &v, u32x4 (&set)[2]) {
+// From the block's registers in pairs: w[k] holds elements 2k and 2k + 1.
+__device__ __forceinline__ void block_rows(const uint32_t (&w)[8], u32x4 (&set)[2]) {
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
-    const u32x2 a = __builtin_bit_cast(u32x2, pack4(v[8 * p], v[8 * p + 1], v[8 * p + 2], v[8 * p + 3]));
-    const u32x2 b = __builtin_bit_cast(u32x2, pack4(v[8 * p + 4], v[8 * p + 5], v[8 * p + 6], v[8 * p + 7]));
-    const auto x = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
-    const auto y = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
+    const auto x = __builtin_amdgcn_permlane32_swap(w[4 * p], w[4 * p + 2], false, false);
+    const auto y = __builtin_amdgcn_permlane32_swap(w[4 * p + 1], w[4 * p + 3], false, false);
     set[p] = u32x4{x[0], y[0], x[1], y[1]};
   }
   swap_rows(set[0], set[1]);
+}
+
+__device__ __forceinline__ void block_rows(const f32x16 &v, u32x4 (&set)[2]) {
+  uint32_t w[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    w[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[2 * k], v[2 * k + 1]}), bf16x2));
+  block_rows(w, set);
+}
+
+// The same of a block of bytes, four to a word: pieces of eight.
+__device__ __forceinline__ void block_rows_u8(const uint32_t (&w)[4], u32x2 (&set)[2]) {
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    const auto x = __builtin_amdgcn_permlane32_swap(w[2 * p], w[2 * p + 1], false, false);
+    set[p] = u32x2{x[0], x[1]};
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t u = set[0][i], v = set[1][i];
+    const auto x = __builtin_amdgcn_permlane16_swap(u, v, false, false);
+    set[0][i] = x[0];
+    set[1][i] = x[1];
+  }
 }
 
 // The block in fp32: set 2 c + q holds, of rows 16 q + lane % 16, n = 16 c + 8 (lane / 16 % 2) + 4 (lane / 32) .. + 3.
@@ -177,20 +204,23 @@ __device__ __forceinline__ void block_rows_f32(const f32x16 &v, u32x4 (&set)[4])
   swap_rows(set[2], set[3]);
 }
 
-// The inverse: a block's registers from such pieces.
-__device__ __forceinline__ f32x16 block_regs(u32x4 a, u32x4 b) {
-  swap_rows(a, b);
-  f32x16 v;
-#pragma unroll
-  for (int p = 0; p < 2; ++p) {
-    const u32x4 c = p ? b : a;
-    const auto x = __builtin_amdgcn_permlane32_swap(c[0], c[2], false, false);
-    const auto y = __builtin_amdgcn_permlane32_swap(c[1], c[3], false, false);
-    const bf16x8 w = __builtin_bit_cast(bf16x8, (u32x4{x[0], y[0], x[1], y[1]}));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[8 * p + i] = (float)w[i];
-  }
-  return v;
+// Both sums of M N elements as the backward reads them: 20 bits each, fp32 rounded to 12 significant bits,
+// the high halves as two matrices of bf16 and the low four bits of both in a byte.
+struct SavedSums {
+  bf16 *high[2];
+  uint8_t *low;
+  __host__ __device__ SavedSums(uint8_t *p, int64_t n)
+      : high{reinterpret_cast<bf16 *>(p), reinterpret_cast<bf16 *>(p) + n}, low(p + 4 * n) {}
+};
+
+// To nearest; a NaN or infinity as it is.
+__device__ __forceinline__ uint32_t saved_bits(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return (b & 0x7f800000u) == 0x7f800000u ? b : b + 0x800u;
+}
+
+__device__ __forceinline__ float sigmoid(float x) {
+  return __builtin_amdgcn_rcpf(1.f + exp2f_fast(-x * kLog2e));
 }
 
 namespace {
@@ -223,22 +253,19 @@ __device__ __forceinline__ int first_stage(const Tiles &g, int stages, int part)
 }
 
 // kPartial: kStore's sums in fp32, one of `splits` parts of the contraction.
-enum Epilogue { kStore, kPartial, kGated, kGatedGrad };
+// kGatedSave: kGated, and both sums for the backward.
+enum Epilogue { kStore, kPartial, kGated, kGatedSave };
 
 struct GemmArgs {
   const bf16 *x[2], *w[2];  // kStore, kPartial: segments of the sum (segs) or problems (z)
   int64_t ldx, ldw;
   int64_t M, N, K;          // K of one segment
   int segs, z;
-  const bf16 *da;           // kGatedGrad
   bf16 *out[2];             // [M][N]
   float *part;              // kPartial: [splits][z][M][N]
+  uint8_t *saved;           // kGatedSave: SavedSums of M N elements
   Tiles tiles;
 };
-
-__device__ __forceinline__ float sigmoid(float x) {
-  return __builtin_amdgcn_rcpf(1.f + exp2f_fast(-x * kLog2e));
-}
 
 // Keeps a step's LDS reads among its first products, two to each, where the compiler would put them
 // right before their use; nothing moves across.
@@ -257,10 +284,10 @@ __device__ __forceinline__ void interleave() {
 template <int TM, int TN, int WM, int WN, int BK, bool XTR, bool WTR, Epilogue E>
 __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   constexpr int NT = 64 * WM * WN, MB = TM / WM / 32, NB = TN / WN / 32, STEPS = BK / 16;
-  constexpr bool DUAL = E == kGated || E == kGatedGrad;
+  constexpr bool DUAL = E == kGated || E == kGatedSave;
   static_assert(!DUAL || (NB == 2 && !WTR), "a wave has 32 columns of both sums");
   static_assert(STEPS % 2 == 0, "operands alternate between two sets of registers");
-  constexpr int WT = DUAL ? TN / 2 : TN, STORES = MB * (E == kGated ? 2 : E == kPartial ? 4 * NB : 4);
+  constexpr int WT = DUAL ? TN / 2 : TN, STORES = MB * (E == kGated ? 2 : E == kGatedSave ? 8 : E == kPartial ? 4 * NB : 2 * NB);
   using XL = TileLoad<TM, BK, XTR, NT>;
   using WL = TileLoad<WT, BK, WTR, NT>;
   constexpr int STAGE = (TM + TN) * BK * 2;
@@ -346,15 +373,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
       const int64_t n = n0 + col + 32 * j;
       return n < g.N ? (uint32_t)((row + 32 * i + 16 * q) * g.N * 2 + n * 2) : kPastEnd;
     };
-    u32x4 da[MB][2];
     for (int st = 0; st < stages; ++st) {
-      if (E == kGatedGrad && st == 0) {  // a tile's time to arrive (in its last stage: 728 us for 713 at 16384 x 2048 x 6144)
-        const __amdgpu_buffer_rsrc_t r = make_rsrc(g.da + m0 * g.N, bytes);
-#pragma unroll
-        for (int i = 0; i < MB; ++i)
-#pragma unroll
-          for (int p = 0; p < 2; ++p) da[i][p] = buf_load16(r, piece_at(i, 0, p));
-      }
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
         if (s + 1 < STEPS) {
@@ -392,7 +411,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
       continue;
     }
     const __amdgpu_buffer_rsrc_t r0 = make_rsrc(g.out[E == kStore ? t.z : 0] + m0 * g.N, bytes);
-    const __amdgpu_buffer_rsrc_t r1 = make_rsrc(g.out[1] + m0 * g.N, bytes);
+    const SavedSums saved(g.saved, g.M * g.N);
+    const __amdgpu_buffer_rsrc_t rg = make_rsrc(saved.high[0] + m0 * g.N, bytes);
+    const __amdgpu_buffer_rsrc_t ru = make_rsrc(saved.high[1] + m0 * g.N, bytes);
+    const __amdgpu_buffer_rsrc_t rl = make_rsrc(saved.low + m0 * g.N, bytes / 2);
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
       if constexpr (E == kStore) {
@@ -404,27 +426,32 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
           buf_store16(r0, piece_at(i, j, 1), set[1]);
         }
       } else {
-        f32x16 d, v0, v1;
-        if constexpr (E == kGatedGrad) d = block_regs(da[i][0], da[i][1]);
+        f32x16 v;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float gate = acc[i][0][e], up = acc[i][1][e];
-          const float sig = sigmoid(gate);
-          if constexpr (E == kGated) {
-            v0[e] = gate * sig * up;
-          } else {
-            v0[e] = d[e] * up * sig * fmaf(gate, 1.f - sig, 1.f);
-            v1[e] = d[e] * gate * sig;
-          }
-        }
+        for (int e = 0; e < 16; ++e) v[e] = acc[i][0][e] * sigmoid(acc[i][0][e]) * acc[i][1][e];
         u32x4 set[2];
-        block_rows(v0, set);
+        block_rows(v, set);
         buf_store16(r0, piece_at(i, 0, 0), set[0]);
         buf_store16(r0, piece_at(i, 0, 1), set[1]);
-        if constexpr (E == kGatedGrad) {
-          block_rows(v1, set);
-          buf_store16(r1, piece_at(i, 0, 0), set[0]);
-          buf_store16(r1, piece_at(i, 0, 1), set[1]);
+        if constexpr (E == kGatedSave) {
+          uint32_t high[2][8], low[4] = {};
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint32_t x = saved_bits(acc[i][0][e]), y = saved_bits(acc[i][1][e]);
+            if (e % 2 == 0) high[0][e / 2] = x >> 16, high[1][e / 2] = y >> 16;
+            else high[0][e / 2] |= x & 0xffff0000u, high[1][e / 2] |= y & 0xffff0000u;
+            low[e / 4] |= ((x >> 12 & 15) | (y >> 8 & 0xf0)) << (8 * (e % 4));
+          }
+          block_rows(high[0], set);
+          buf_store16(rg, piece_at(i, 0, 0), set[0]);
+          buf_store16(rg, piece_at(i, 0, 1), set[1]);
+          block_rows(high[1], set);
+          buf_store16(ru, piece_at(i, 0, 0), set[0]);
+          buf_store16(ru, piece_at(i, 0, 1), set[1]);
+          u32x2 bytes8[2];
+          block_rows_u8(low, bytes8);
+          buf_store8(rl, piece_at(i, 0, 0) / 2, bytes8[0]);
+          buf_store8(rl, piece_at(i, 0, 1) / 2, bytes8[1]);
         }
       }
     }
@@ -489,7 +516,7 @@ int64_t part_bytes(const Cut &c, int64_t M, int64_t N, int z) { return c.splits 
 
 template <bool XTR, bool WTR, Epilogue E, int TM, int WM, int WN>
 hipError_t launch_tiles(GemmArgs g, int splits, hipStream_t stream) {
-  constexpr int BK = 64, TN = TM, DUAL = E == kGated || E == kGatedGrad, WT = DUAL ? TN / 2 : TN;
+  constexpr int BK = 64, TN = TM, DUAL = E == kGated || E == kGatedSave, WT = DUAL ? TN / 2 : TN;
   constexpr int lds = 2 * (TM + TN) * BK * 2;
   constexpr auto kernel = gemm_kernel<TM, TN, WM, WN, BK, XTR, WTR, E>;
   g.tiles = Tiles{splits, g.z, (int)((g.M + TM - 1) / TM), (int)((g.N + WT - 1) / WT)};

@@ -455,7 +455,7 @@ hipError_t launch_linear_mx(const void *x, const void *x_scales, const void *cod
   if (e == hipSuccess && x_scales) e = launch_values(x, x_scales, xv, (int64_t)M * K, 8, stream);
   if (e != hipSuccess) return e;
   const bf16 *xp = x_scales ? xv : (const bf16 *)x;
-  GemmArgs g{{xp, xp}, {w, w}, K, K, M, N, K, 1, 1, nullptr, {(bf16 *)y, nullptr}, part, {}};
+  GemmArgs g{{xp, xp}, {w, w}, K, K, M, N, K, 1, 1, {(bf16 *)y, nullptr}, part, nullptr, {}};
   return launch_gemm<false, false, kStore>(g, cut_of(M, N, K, 1, 1, false), stream);
 }
 

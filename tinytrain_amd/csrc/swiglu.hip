@@ -5,11 +5,12 @@
 //   du = da silu(g), dg = da u sig(g) (1 + g (1 - sig(g)))
 //   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x
 //
-// g and u never leave the registers in fp32: a workgroup's W tile holds rows of Wg and the same rows
-// of Wu, so a wave has both sums of an element.  The backward forms them again (4MNK more operations
-// on top of 8MNK): kept in fp32 they would be written and read back at 8 bytes an element each way,
-// which takes as long and as much memory; kept in bf16 they would round every gradient once more.
-// dg and du are rounded to bf16 once, as operands of the last two products.
+// a is formed from both sums in fp32 registers: a workgroup's W tile holds rows of Wg and the same rows of
+// Wu, so a wave has both sums of an element.  For the backward they are written as well, in 20 bits each: 12
+// significant bits, an error of 2^-13 against the 2^-9 that every gradient has from its own rounding and
+// from that of dg and du, as bf16 operands of the last two products (in bf16 they would add as much
+// again).  That is 5 bytes an element; to form them again instead of reading them was 713 us at
+// 16384 x 2048 x 6144, four times as long as the kernel that reads them (swiglu_grad_kernel).
 #include "fa_kernels.h"
 #include "gemm.h"
 
@@ -41,7 +42,9 @@ template <int MB, int NB>
 __global__ __launch_bounds__(64 * kRowWaves) void swiglu_rows_kernel(const bf16 *__restrict__ x,
                                                                      const bf16 *__restrict__ w_gate,
                                                                      const bf16 *__restrict__ w_up,
-                                                                     bf16 *__restrict__ a, int M, int K, int N) {
+                                                                     bf16 *__restrict__ a,
+                                                                     uint8_t *__restrict__ saved, int M, int K,
+                                                                     int N) {
   __shared__ f32x4 part[kRowWaves][2 * NB * MB][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, quarter = lane >> 4;
   const int n0 = blockIdx.x * 16 * NB;
@@ -88,7 +91,47 @@ __global__ __launch_bounds__(64 * kRowWaves) void swiglu_rows_kernel(const bf16 
 #pragma unroll
   for (int e = 0; e < 4; ++e) r[e] = g[e] * sigmoid(g[e]) * u[e];
   const int m = 16 * (wave % MB) + row, n = n0 + 16 * (wave / MB) + 4 * quarter;
-  if (m < M && n < N) *reinterpret_cast<bf16x4 *>(a + (int64_t)m * N + n) = pack4(r[0], r[1], r[2], r[3]);
+  if (m >= M || n >= N) return;
+  const int64_t at = (int64_t)m * N + n;
+  *reinterpret_cast<bf16x4 *>(a + at) = pack4(r[0], r[1], r[2], r[3]);
+  if (!saved) return;
+  const SavedSums s(saved, (int64_t)M * N);
+  u32x2 high[2] = {};
+  uint32_t low = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t p = saved_bits(g[e]), q = saved_bits(u[e]);
+    high[0][e / 2] |= (p >> 16) << (16 * (e % 2));
+    high[1][e / 2] |= (q >> 16) << (16 * (e % 2));
+    low |= ((p >> 12 & 15) | (q >> 8 & 0xf0)) << (8 * e);
+  }
+  *reinterpret_cast<u32x2 *>(s.high[0] + at) = high[0];
+  *reinterpret_cast<u32x2 *>(s.high[1] + at) = high[1];
+  *reinterpret_cast<uint32_t *>(s.low + at) = low;
+}
+
+// dg and du from da and the saved sums, eight elements a lane.  Bound by memory: 11 bytes an element.
+__global__ __launch_bounds__(256) void swiglu_grad_kernel(const bf16 *__restrict__ da, const uint8_t *saved_at,
+                                                          bf16 *__restrict__ dg, bf16 *__restrict__ du,
+                                                          int64_t lanes) {
+  const SavedSums s(const_cast<uint8_t *>(saved_at), 8 * lanes);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < lanes; i += (int64_t)gridDim.x * 256) {
+    const bf16x8 d = reinterpret_cast<const bf16x8 *>(da)[i];
+    const u32x4 gh = reinterpret_cast<const u32x4 *>(s.high[0])[i], uh = reinterpret_cast<const u32x4 *>(s.high[1])[i];
+    const u32x2 low = reinterpret_cast<const u32x2 *>(s.low)[i];
+    bf16x8 x, y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t l = low[e / 4] >> (8 * (e % 4));
+      const float g = __uint_as_float((e % 2 ? gh[e / 2] & 0xffff0000u : gh[e / 2] << 16) | (l & 15) << 12);
+      const float u = __uint_as_float((e % 2 ? uh[e / 2] & 0xffff0000u : uh[e / 2] << 16) | (l >> 4 & 15) << 12);
+      const float sig = sigmoid(g), t = (float)d[e] * sig;
+      x[e] = (bf16)(t * u * fmaf(g, 1.f - sig, 1.f));
+      y[e] = (bf16)(t * g);
+    }
+    reinterpret_cast<bf16x8 *>(dg)[i] = x;
+    reinterpret_cast<bf16x8 *>(du)[i] = y;
+  }
 }
 
 // Rows of x up to which the kernel above is faster than a tile of 128 x 64 (K 768, N 2304, M 64: 6.8 us, tiles
@@ -99,12 +142,14 @@ const bf16 *in(const void *p) { return static_cast<const bf16 *>(p); }
 
 }  // namespace
 
-hipError_t launch_swiglu_fwd(const void *x, const void *w_gate, const void *w_up, void *a, int M, int K,
-                             int N, hipStream_t stream) {
+int64_t swiglu_saved_bytes(int M, int N) { return 5ll * M * N; }
+
+hipError_t launch_swiglu_fwd(const void *x, const void *w_gate, const void *w_up, void *a, void *saved, int M,
+                             int K, int N, hipStream_t stream) {
   if (few_rows(M, N)) {
     auto go = [&](auto kernel, int columns) {
       kernel<<<dim3((N + columns - 1) / columns), dim3(64 * kRowWaves), 0, stream>>>(
-          in(x), in(w_gate), in(w_up), (bf16 *)a, M, K, N);
+          in(x), in(w_gate), in(w_up), (bf16 *)a, (uint8_t *)saved, M, K, N);
       return hipGetLastError();
     };
     // 32 columns a workgroup where 16 would give some CUs two workgroups and others one.
@@ -118,8 +163,10 @@ hipError_t launch_swiglu_fwd(const void *x, const void *w_gate, const void *w_up
            : M <= 48 ? go(swiglu_rows_kernel<3, 1>, 16)
                      : go(swiglu_rows_kernel<4, 1>, 16);
   }
-  GemmArgs g{{in(x), in(x)}, {in(w_gate), in(w_up)}, K, K, M, N, K, 1, 1, nullptr, {(bf16 *)a, nullptr}, nullptr};
-  return launch_gemm<false, false, kGated>(g, cut_of(M, N, K, 1, 1, true), stream);
+  GemmArgs g{{in(x), in(x)}, {in(w_gate), in(w_up)}, K, K, M, N, K, 1, 1, {(bf16 *)a, nullptr}, nullptr,
+             (uint8_t *)saved, {}};
+  const Cut c = cut_of(M, N, K, 1, 1, true);
+  return saved ? launch_gemm<false, false, kGatedSave>(g, c, stream) : launch_gemm<false, false, kGated>(g, c, stream);
 }
 
 int64_t swiglu_bwd_workspace(int M, int K, int N) {
@@ -128,19 +175,21 @@ int64_t swiglu_bwd_workspace(int M, int K, int N) {
   return 4ll * M * N + std::max(dx, dw);
 }
 
-hipError_t launch_swiglu_bwd(const void *da, const void *x, const void *w_gate, const void *w_up, void *dx,
-                             void *dw_gate, void *dw_up, void *workspace, int M, int K, int N,
-                             hipStream_t stream) {
+hipError_t launch_swiglu_bwd(const void *da, const void *saved, const void *x, const void *w_gate,
+                             const void *w_up, void *dx, void *dw_gate, void *dw_up, void *workspace, int M,
+                             int K, int N, hipStream_t stream) {
   bf16 *dg = static_cast<bf16 *>(workspace), *du = dg + (int64_t)M * N;
   float *part = reinterpret_cast<float *>(du + (int64_t)M * N);
-  GemmArgs g{{in(x), in(x)}, {in(w_gate), in(w_up)}, K, K, M, N, K, 1, 1, in(da), {dg, du}, nullptr};
-  hipError_t e = launch_gemm<false, false, kGatedGrad>(g, cut_of(M, N, K, 1, 1, true), stream);
+  const int64_t lanes = (int64_t)M * N / 8;
+  swiglu_grad_kernel<<<dim3((unsigned)std::min<int64_t>((lanes + 255) / 256, 1 << 20)), dim3(256), 0, stream>>>(
+      in(da), static_cast<const uint8_t *>(saved), dg, du, lanes);
+  hipError_t e = hipGetLastError();
   if (e == hipSuccess && dx) {
-    GemmArgs d{{dg, du}, {in(w_gate), in(w_up)}, N, K, M, K, N, 2, 1, nullptr, {(bf16 *)dx, nullptr}, part};
+    GemmArgs d{{dg, du}, {in(w_gate), in(w_up)}, N, K, M, K, N, 2, 1, {(bf16 *)dx, nullptr}, part, nullptr, {}};
     e = launch_gemm<false, true, kStore>(d, cut_of(M, K, N, 2, 1, false), stream);
   }
   if (e == hipSuccess && dw_gate) {
-    GemmArgs d{{dg, du}, {in(x), in(x)}, N, K, N, K, M, 1, 2, nullptr, {(bf16 *)dw_gate, (bf16 *)dw_up}, part};
+    GemmArgs d{{dg, du}, {in(x), in(x)}, N, K, N, K, M, 1, 2, {(bf16 *)dw_gate, (bf16 *)dw_up}, part, nullptr, {}};
     e = launch_gemm<true, true, kStore>(d, cut_of(N, K, M, 1, 2, false), stream);
   }
   return e;

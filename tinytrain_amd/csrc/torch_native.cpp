@@ -605,18 +605,19 @@ struct SwigluIn {
   }
 };
 
-Tensor swiglu_fwd(const SwigluIn &i) {
+// {a, the saved products (undefined unless asked for)}
+std::pair<Tensor, Tensor> swiglu_fwd(const SwigluIn &i, bool save) {
   RECORD_FUNCTION("tinytrain::swiglu_fwd", c10::ArrayRef<const c10::IValue>());
   const c10::DeviceGuard on(i.x.device());
   const int M = (int)i.M(), K = (int)i.K(), N = (int)i.N();
-  Tensor a = at::empty(i.out_sizes(), i.x.options());
-  Tensor ws = workspace(i.x, ttfa_swiglu_workspace_bytes(M, K, N, 0));
+  Tensor a = at::empty(i.out_sizes(), i.x.options()), saved;
+  if (save) saved = workspace(i.x, ttfa_swiglu_saved_bytes(M, N));
   check(ttfa_swiglu_fwd(i.x.const_data_ptr(), i.wg.const_data_ptr(), i.wu.const_data_ptr(),
-                        a.mutable_data_ptr(), ptr(ws), M, K, N, stream_of(i.x)));
-  return a;
+                        a.mutable_data_ptr(), ptr(saved), M, K, N, stream_of(i.x)));
+  return {a, saved};
 }
 
-Grads3 swiglu_bwd(const Tensor &da, const SwigluIn &i, bool need_dx, bool need_dw) {
+Grads3 swiglu_bwd(const Tensor &da, const Tensor &saved, const SwigluIn &i, bool need_dx, bool need_dw) {
   RECORD_FUNCTION("tinytrain::swiglu_bwd", c10::ArrayRef<const c10::IValue>());
   const c10::DeviceGuard on(i.x.device());
   const Tensor g = da.contiguous();
@@ -624,8 +625,8 @@ Grads3 swiglu_bwd(const Tensor &da, const SwigluIn &i, bool need_dx, bool need_d
   Tensor dx, dwg, dwu;
   if (need_dx) dx = same(i.x);
   if (need_dw) dwg = same(i.wg), dwu = same(i.wu);
-  Tensor ws = workspace(i.x, ttfa_swiglu_workspace_bytes(M, K, N, 1));
-  check(ttfa_swiglu_bwd(g.const_data_ptr(), i.x.const_data_ptr(), i.wg.const_data_ptr(),
+  Tensor ws = workspace(i.x, ttfa_swiglu_workspace_bytes(M, K, N));
+  check(ttfa_swiglu_bwd(g.const_data_ptr(), saved.const_data_ptr(), i.x.const_data_ptr(), i.wg.const_data_ptr(),
                         i.wu.const_data_ptr(), ptr(dx), ptr(dwg), ptr(dwu), ptr(ws), M, K, N, stream_of(i.x)));
   return {dx, dwg, dwu};
 }
@@ -634,20 +635,22 @@ struct Swiglu : torch::autograd::Function<Swiglu> {
   static constexpr bool is_traceable = true;
 
   static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &wg, const Tensor &wu) {
-    ctx->save_for_backward({x, wg, wu});
-    return swiglu_fwd({x, wg, wu});
+    auto [a, saved] = swiglu_fwd({x, wg, wu}, true);
+    ctx->save_for_backward({x, wg, wu, saved});
+    return a;
   }
 
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
     const SwigluIn i{s[0], s[1], s[2]};
-    const Tensor &g = grads[0];
+    const Tensor &g = grads[0], &saved = s[3];
     const bool nx = ctx->needs_input_grad(0), ng = ctx->needs_input_grad(1), nu = ctx->needs_input_grad(2);
-    const bool native = plain_backward() && i.takes() && grad_of(g, s[0], i.out_sizes(), at::kBFloat16);
-    Grads3 d = native ? swiglu_bwd(g, i, nx, ng || nu)
-                      : op<Grads3(const Tensor &, const Tensor &, const Tensor &, const Tensor &, bool, bool)>(
-                            "tinytrain::swiglu_bwd")
-                            .call(g, s[0], s[1], s[2], nx, ng || nu);
+    const bool native = plain_backward() && i.takes() && grad_of(g, s[0], i.out_sizes(), at::kBFloat16) &&
+                        saved_as(saved, s[0], {ttfa_swiglu_saved_bytes((int)i.M(), (int)i.N())}, at::kByte);
+    Grads3 d = native ? swiglu_bwd(g, saved, i, nx, ng || nu)
+                      : op<Grads3(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &,
+                                  bool, bool)>("tinytrain::swiglu_bwd")
+                            .call(g, saved, s[0], s[1], s[2], nx, ng || nu);
     return {nx ? std::get<0>(d) : Tensor(), ng ? std::get<1>(d) : Tensor(), nu ? std::get<2>(d) : Tensor()};
   }
 };
@@ -900,7 +903,8 @@ PyObject *py_swiglu(PyObject *, PyObject *const *args, Py_ssize_t n) {
   if (!unpack(args, t) || !plain_mode()) Py_RETURN_NONE;
   const SwigluIn in{t[0], t[1], t[2]};
   if (!in.takes()) Py_RETURN_NONE;
-  return THPVariable_Wrap(recorded({&t[0], &t[1], &t[2]}) ? Swiglu::apply(t[0], t[1], t[2]) : swiglu_fwd(in));
+  return THPVariable_Wrap(recorded({&t[0], &t[1], &t[2]}) ? Swiglu::apply(t[0], t[1], t[2])
+                                                               : swiglu_fwd(in, false).first);
   END_HANDLE_TH_ERRORS
 }
 

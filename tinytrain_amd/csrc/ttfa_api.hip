@@ -477,32 +477,35 @@ int ttfa_rms_norm_bwd(const void *dy, const void *dh, const void *h, const float
                                                     y_dtype, eps, static_cast<hipStream_t>(hip_stream)));
 }
 
-long long ttfa_swiglu_workspace_bytes(int M, int K, int N, int backward) {
-  if (check_swiglu(M, K, N)) return -1;
-  return backward ? ttfa::swiglu_bwd_workspace(M, K, N) : 0;
+long long ttfa_swiglu_saved_bytes(int M, int N) {
+  return check_swiglu(M, 8, N) ? -1 : ttfa::swiglu_saved_bytes(M, N);
 }
 
-int ttfa_swiglu_fwd(const void *x, const void *w_gate, const void *w_up, void *a, void *workspace, int M,
-                    int K, int N, void *hip_stream) {
+int ttfa_swiglu_fwd(const void *x, const void *w_gate, const void *w_up, void *a, void *saved, int M, int K,
+                    int N, void *hip_stream) {
   int rc = check_swiglu(M, K, N);
   if (rc) return rc;
-  const void *ptrs[] = {x, w_gate, w_up, a, workspace};
-  if ((rc = check_ptrs(ptrs, ttfa_swiglu_workspace_bytes(M, K, N, 0) ? 5 : 4))) return rc;
+  const void *ptrs[] = {x, w_gate, w_up, a, saved ? saved : a};
+  if ((rc = check_ptrs(ptrs, 5))) return rc;
   return static_cast<int>(
-      ttfa::launch_swiglu_fwd(x, w_gate, w_up, a, M, K, N, static_cast<hipStream_t>(hip_stream)));
+      ttfa::launch_swiglu_fwd(x, w_gate, w_up, a, saved, M, K, N, static_cast<hipStream_t>(hip_stream)));
 }
 
-int ttfa_swiglu_bwd(const void *da, const void *x, const void *w_gate, const void *w_up, void *dx,
-                    void *dw_gate, void *dw_up, void *workspace, int M, int K, int N,
+long long ttfa_swiglu_workspace_bytes(int M, int K, int N) {
+  return check_swiglu(M, K, N) ? -1 : ttfa::swiglu_bwd_workspace(M, K, N);
+}
+
+int ttfa_swiglu_bwd(const void *da, const void *saved, const void *x, const void *w_gate, const void *w_up,
+                    void *dx, void *dw_gate, void *dw_up, void *workspace, int M, int K, int N,
                     void *hip_stream) {
   int rc = check_swiglu(M, K, N);
   if (rc) return rc;
   if (!dx && !dw_gate) return TTFA_E_NULL;
   if (!dw_gate != !dw_up) return TTFA_E_NULL;
-  const void *ptrs[] = {da, x, w_gate, w_up, workspace, dx ? dx : x, dw_gate ? dw_gate : x, dw_up ? dw_up : x};
-  if ((rc = check_ptrs(ptrs, 8))) return rc;
-  return static_cast<int>(ttfa::launch_swiglu_bwd(da, x, w_gate, w_up, dx, dw_gate, dw_up, workspace, M, K,
-                                                  N, static_cast<hipStream_t>(hip_stream)));
+  const void *ptrs[] = {da, saved, x, w_gate, w_up, workspace, dx ? dx : x, dw_gate ? dw_gate : x, dw_up ? dw_up : x};
+  if ((rc = check_ptrs(ptrs, 9))) return rc;
+  return static_cast<int>(ttfa::launch_swiglu_bwd(da, saved, x, w_gate, w_up, dx, dw_gate, dw_up, workspace, M,
+                                                  K, N, static_cast<hipStream_t>(hip_stream)));
 }
 
 int ttfa_mx_quantize(const void *x, void *codes, void *scales, long long M, int K, int bits, int dtype,

@@ -6,8 +6,9 @@ what the reference's MLP (model.py:111-125) does before its down projection, as 
 products stay in fp32 registers, and a is rounded to bf16 once.
 
 ``swiglu(x, w_gate, w_up)``: x [..., K], w_gate and w_up [N, K], bf16, contiguous; a [..., N].  Gradients
-flow to all three.  The backward keeps nothing but the inputs: it forms the products again, and rounds
-the gradients of both to bf16 once, as operands of the products that give dx and the weights' gradients.
+flow to all three.  Where one is needed, the forward keeps both products for it, in 20 bits each (12
+significant: 5 bytes an element of a); the backward rounds the gradients of both to bf16 once, as operands
+of the products that give dx and the weights' gradients.
 Where x or both weights need no gradient, theirs is not computed.  Sums have a fixed order: results are
 bitwise reproducible.
 
@@ -45,54 +46,60 @@ def _check(x, w_gate, w_up):
     return M, x.shape[-1], N
 
 
-def _workspace(lib, M, K, N, backward, device):
-    nbytes = lib.ttfa_swiglu_workspace_bytes(M, K, N, backward)
-    if nbytes < 0:
+def _bytes(n, device):
+    if n < 0:
         _lib.check(_lib.E_SEQ)
-    return torch.empty((nbytes,), device=device, dtype=torch.uint8) if nbytes else None
+    return torch.empty((n,), device=device, dtype=torch.uint8)
 
 
 @torch.library.custom_op("tinytrain::swiglu_fwd", mutates_args=())
-def swiglu_fwd(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor) -> torch.Tensor:
+def swiglu_fwd(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, save: bool
+               ) -> tuple[torch.Tensor, torch.Tensor]:
+    """(a, what the backward needs, or empty)."""
     M, K, N = _check(x, w_gate, w_up)
     a = x.new_empty((*x.shape[:-1], N))
+    lib = _lib.load()
+    saved = _bytes(lib.ttfa_swiglu_saved_bytes(M, N) if save and M else 0, x.device)
     if M:
-        lib = _lib.load()
-        ws = _workspace(lib, M, K, N, 0, x.device)
         with torch.cuda.device(x.device):
             _lib.check(lib.ttfa_swiglu_fwd(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), a.data_ptr(),
-                                           _ptr(ws), M, K, N, _stream(x.device)))
-    return a
+                                           saved.data_ptr() if save else None, M, K, N, _stream(x.device)))
+    return a, saved
 
 
 @swiglu_fwd.register_fake
-def _(x, w_gate, w_up):
-    return x.new_empty((*x.shape[:-1], w_gate.shape[0]))
+def _(x, w_gate, w_up, save):
+    M, N = x.numel() // x.shape[-1], w_gate.shape[0]
+    return x.new_empty((*x.shape[:-1], N)), x.new_empty(5 * M * N if save else 0, dtype=torch.uint8)
 
 
 @torch.library.custom_op("tinytrain::swiglu_bwd", mutates_args=())
-def swiglu_bwd(da: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, need_dx: bool,
-               need_dw: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+def swiglu_bwd(da: torch.Tensor, saved: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
+               need_dx: bool, need_dw: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dx, dw_gate, dw_up); what is not needed is empty."""
     M, K, N = _check(x, w_gate, w_up)
     if da.shape != (*x.shape[:-1], N) or da.dtype != x.dtype or da.device != x.device:
         raise BlockInputError(f"da must be bfloat16 {(*x.shape[:-1], N)} beside x")
+    if saved.numel() == 0 and M:  # a forward that kept nothing
+        saved = swiglu_fwd(x, w_gate, w_up, True)[1]
+    if saved.shape != (5 * M * N,) or saved.dtype != torch.uint8 or saved.device != x.device:
+        raise BlockInputError(f"saved must be the forward's {5 * M * N} bytes beside x")
     dx = torch.empty_like(x) if need_dx else x.new_empty(0)
     make = torch.empty_like if M else torch.zeros_like
     dwg, dwu = (make(w_gate), make(w_up)) if need_dw else (x.new_empty(0), x.new_empty(0))
     if M and (need_dx or need_dw):
-        da, lib = da.contiguous(), _lib.load()
-        ws = _workspace(lib, M, K, N, 1, x.device)
+        da, saved, lib = da.contiguous(), saved.contiguous(), _lib.load()
+        ws = _bytes(lib.ttfa_swiglu_workspace_bytes(M, K, N), x.device)
         with torch.cuda.device(x.device):
             _lib.check(lib.ttfa_swiglu_bwd(
-                da.data_ptr(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
+                da.data_ptr(), saved.data_ptr(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
                 dx.data_ptr() if need_dx else None, dwg.data_ptr() if need_dw else None,
-                dwu.data_ptr() if need_dw else None, _ptr(ws), M, K, N, _stream(x.device)))
+                dwu.data_ptr() if need_dw else None, ws.data_ptr(), M, K, N, _stream(x.device)))
     return dx, dwg, dwu
 
 
 @swiglu_bwd.register_fake
-def _(da, x, w_gate, w_up, need_dx, need_dw):
+def _(da, saved, x, w_gate, w_up, need_dx, need_dw):
     none = x.new_empty(0)
     return (torch.empty_like(x) if need_dx else none,
             torch.empty_like(w_gate) if need_dw else x.new_empty(0),
@@ -100,14 +107,15 @@ def _(da, x, w_gate, w_up, need_dx, need_dw):
 
 
 def _setup_context(ctx, inputs, output):
-    ctx.save_for_backward(*inputs)
+    ctx.save_for_backward(*inputs[:3], output[1])
+    ctx.mark_non_differentiable(output[1])
 
 
-def _backward_fn(ctx, da):
-    x, w_gate, w_up = ctx.saved_tensors
-    need_x, need_g, need_u = ctx.needs_input_grad
-    dx, dwg, dwu = swiglu_bwd(da, x, w_gate, w_up, need_x, need_g or need_u)
-    return dx if need_x else None, dwg if need_g else None, dwu if need_u else None
+def _backward_fn(ctx, da, _):
+    x, w_gate, w_up, saved = ctx.saved_tensors
+    need_x, need_g, need_u, _ = ctx.needs_input_grad
+    dx, dwg, dwu = swiglu_bwd(da, saved, x, w_gate, w_up, need_x, need_g or need_u)
+    return dx if need_x else None, dwg if need_g else None, dwu if need_u else None, None
 
 
 swiglu_fwd.register_autograd(_backward_fn, setup_context=_setup_context)
@@ -120,4 +128,5 @@ def swiglu(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor) -> torch.T
         a = _lib.native().swiglu(x, w_gate, w_up)
         if a is not None:
             return a
-    return swiglu_fwd(x, w_gate, w_up)
+    save = torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad)
+    return swiglu_fwd(x, w_gate, w_up, save)[0]
