@@ -402,7 +402,11 @@ int ttfa_swiglu_bwd(const void *da, const void *saved, const void *x, const void
  * Products with a quantised weight: y [M, N] bf16 = x W^T with W [N, K] in 4 or 8 bits, codes
  * [N, K * bits / 8] and scales [N, K / 32] (uint8), the format of the quantised KV cache, and x [M, K]
  * in bf16 (x_scales NULL) or in 8 bits (codes [M, K] and x_scales [M, K / 32], what ttfa_rms_norm_mx
- * gives).  Exact products, fp32 sums.  K a multiple of 32 and N of 8, up to 2^20.
+ * gives).  fp32 sums, rounded once; of exact products with x in bf16.  With x in 8 bits the matrix unit drops, of
+ * every eight consecutive products, the bits below 2^-13 of the largest: a sum is within 2^-10 of those largest
+ * ones' sum (on random values 2^-19 of sum |x w|).  Which instructions a call uses goes by M, K and N alone.
+ * K a multiple of 32 and N of 8, up to 2^20.  workspace: ttfa_linear_mx_workspace_bytes, or NULL where that
+ * is 0.  One to four launches.
  * ttfa_mx_quantize rounds rows x [M, K], `dtype`, into that format.
  */
 int ttfa_mx_quantize(const void *x, void *codes, void *scales, long long M, int K, int bits, int dtype,

@@ -26,7 +26,7 @@ from helpers import announce
 from oracle import block, mx_cache
 from tinytrain_amd import _lib
 from tinytrain_amd.kernels.linear_mx import linear_mx, mx_quantize
-from tinytrain_amd.kernels.rms_norm import add_rms_norm, add_rms_norm_mx, rms_norm, rms_norm_fwd
+from tinytrain_amd.kernels.rms_norm import add_rms_norm, add_rms_norm_mx, rms_norm, rms_norm_bwd, rms_norm_fwd
 from tinytrain_amd.kernels.swiglu import swiglu, swiglu_fwd
 
 pytestmark = pytest.mark.gpu
@@ -319,6 +319,49 @@ def test_linear_mx_keeps_nan_in_place_and_takes_odd_scales(M):
                 sb[1, 0] = 255
                 got = linear_mx(xx, codes, scales, sb)
             assert torch.isnan(got[1]).all() and torch.equal(got[rows], y[rows])
+
+
+# --------------------------------------------------------------------------- large calls
+
+def test_calls_past_2_31_elements():
+    """The last rows of tensors of more than 2^31 elements, against calls on those rows alone."""
+    M, C = 2**31 // 4096 + 200, 4096
+    announce(f"add_rms_norm {M} x {C}")
+    x = torch.zeros(M, C, device="cuda", dtype=BF)
+    r = torch.zeros(M, C, device="cuda", dtype=BF)
+    x[-200:], r[-200:] = _rand(200, C, seed=1, dtype=BF), _rand(200, C, seed=2, dtype=BF)
+    w = _rand(C, seed=3)
+    y, h = add_rms_norm(x, r, w)
+    want = add_rms_norm(x[-200:].clone(), r[-200:].clone(), w)
+    assert torch.equal(y[-200:], want[0]) and torch.equal(h[-200:], want[1]) and not y[:-200].any()
+    dr, _, _ = rms_norm_bwd(y, h, h, w, 1e-6, BF)
+    assert torch.equal(dr[-200:], rms_norm_bwd(want[0], want[1], want[1], w, 1e-6, BF)[0])
+    del y, dr, r
+    codes, scales, _ = add_rms_norm_mx(h, None, w)
+    wc, ws, _ = add_rms_norm_mx(h[-200:].clone(), None, w)
+    assert torch.equal(codes[-200:], wc) and torch.equal(scales[-200:], ws)
+    weight = mx_quantize(_rand(72, C, seed=4), 4)
+    got = linear_mx(codes, *weight, scales)
+    want, size, top = block.linear_mx(wc, ws, *weight)
+    _within("y", got[-200:].cpu(), want, 2.0**-10 * top + 2 * C * U * size)
+    del x, h, codes, scales, got
+    M, K, N = 2**31 // 8192 + 300, 64, 8192
+    announce(f"swiglu {M} x {K} x {N}")
+    x = torch.zeros(M, K, device="cuda", dtype=BF)
+    x[-300:] = _rand(300, K, seed=5, dtype=BF)
+    wg, wu = _rand(N, K, seed=6, dtype=BF, scale=1 / 8), _rand(N, K, seed=7, dtype=BF, scale=1 / 8)
+    t = [v.requires_grad_() for v in (x, wg, wu)]
+    a = swiglu(*t)
+    da = torch.zeros(M, N, device="cuda", dtype=BF)
+    da[-300:] = _rand(300, N, seed=8, dtype=BF)
+    dx, dwg, dwu = torch.autograd.grad(a, t, da)
+    tail = x[-300:].detach()
+    want, unit = block.swiglu(tail, wg.detach(), wu.detach())
+    _within("a", a.detach()[-300:], want, 2 * K * U * unit + 2.0**-20 * want.abs())
+    for g, (name, (want, size, unit)) in zip((dx[-300:], dwg, dwu), block.swiglu_grads(da[-300:], tail, wg.detach(), wu.detach()).items()):
+        # the rows of zeros add nothing to a sum
+        _within(name, g, want, (2.0**-8 + 2.0**-20 + 4 * N * U) * size + (2 * K * U * 1.01 + 2.0**-13) * unit)
+    assert not a.detach()[:-300].any() and not dx[:-300].any()
 
 
 # ------------------------------------------------------------------- paths, streams, graphs

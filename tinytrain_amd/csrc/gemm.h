@@ -281,7 +281,7 @@ __device__ __forceinline__ void interleave() {
 
 // Workgroups take tiles in turn, and load the next one's first stages during the last steps of the one
 // before, so that its results are rounded and stored while those are on their way.
-template <int TM, int TN, int WM, int WN, int BK, bool XTR, bool WTR, Epilogue E>
+template <int TM, int TN, int WM, int WN, int BK, int S, bool XTR, bool WTR, Epilogue E>
 __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   constexpr int NT = 64 * WM * WN, MB = TM / WM / 32, NB = TN / WN / 32, STEPS = BK / 16;
   constexpr bool DUAL = E == kGated || E == kGatedSave;
@@ -354,11 +354,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   };
 
   // Operands of a step are read during the step before it.  All reads of a stage are so done before its
-  // last step: there the workgroup meets, the stage's buffer takes the loads of the stage after next,
-  // and the next stage, whose loads had a whole stage's time, is read from.
-  load(0);
-  wait_and_meet<0>();
-  load(1);
+  // last step: there the workgroup meets, the stage's buffer takes the loads of the stage that is S
+  // further on, and the next stage is read from.  Loads that were issued after the next stage's may still
+  // be on their way, and so may a tile's stores, if they are younger than those.
+  constexpr int LOADS = XL::LOADS + WL::LOADS * (DUAL ? 2 : 1);
+#pragma unroll
+  for (int b = 0; b < S; ++b) load(b);
+  if (ahead < total) wait_and_meet<(S - 1) * LOADS>();
+  else wait_and_meet<0>();
   read(0, 0, 0);
   int buf = 0;
   for (int i = blockIdx.x; i < total; i += gridDim.x) {
@@ -379,11 +382,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
         if (s + 1 < STEPS) {
           read(buf, s + 1, (s + 1) & 1);
         } else {
-          // After a tile's results were stored: its stores are younger than the loads waited for.
-          if (st == 0 && i != (int)blockIdx.x) wait_and_meet<STORES>();
-          else wait_and_meet<0>();
+          if (ahead >= total) wait_and_meet<0>();
+          else if (st <= S - 2 && i != (int)blockIdx.x) wait_and_meet<(S - 2) * LOADS + STORES>();
+          else wait_and_meet<(S - 2) * LOADS>();
           load(buf);
-          read(buf ^ 1, 0, (s + 1) & 1);  // after the last stage: values that nothing uses
+          buf = buf + 1 == S ? 0 : buf + 1;
+          read(buf, 0, (s + 1) & 1);  // after the last stage: values that nothing uses
         }
 #pragma unroll
         for (int i = 0; i < MB; ++i)
@@ -391,7 +395,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
           for (int j = 0; j < NB; ++j) acc[i][j] = mfma32(wf[s & 1][j], xf[s & 1][i], acc[i][j]);
         interleave<MB * NB>();
       }
-      buf ^= 1;
     }
 
     if constexpr (E == kPartial) {
@@ -474,11 +477,12 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(const float *__restrict_
       bf16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
 }
 
-// How a product is cut: tiles of 256 x 256 (one workgroup a CU) or 128 x 128 (two), and parts of the
-// contraction that sum_parts_kernel joins.
+// How a product is cut: tiles of 256 x 256 (one workgroup a CU) or 128 x 128 (two, or one with four stages
+// in LDS where there are no more than CUs: deep), and parts of the contraction that sum_parts_kernel joins.
 struct Cut {
   bool wide;
   int splits;
+  bool deep;
 };
 
 int64_t tiles_of(int64_t M, int64_t N, int tm, int tn) { return (M + tm - 1) / tm * ((N + tn - 1) / tn); }
@@ -490,7 +494,7 @@ constexpr double kMostPartFloats = 1 << 26;  // 256 MB, what the last-level cach
 // start and end; parts go out and in at 4 TB/s, with a launch of 4 us.
 Cut cut_of(int64_t M, int64_t N, int64_t K, int segs, int z, bool dual) {
   const int64_t stages = (K + 63) / 64 * segs;
-  Cut best{true, 1};
+  Cut best{true, 1, false};
   double least = 1e30;
   for (int wide = 1; wide >= 0; --wide) {
     const int64_t tiles = z * (wide ? tiles_of(M, N, 256, dual ? 128 : 256) : tiles_of(M, N, 128, dual ? 64 : 128));
@@ -498,15 +502,10 @@ Cut cut_of(int64_t M, int64_t N, int64_t K, int segs, int z, bool dual) {
       if (s > 1 && (double)s * z * M * N > kMostPartFloats) break;
       const int64_t n = tiles * s;
       const double len = (double)((stages + s - 1) / s) + 3;
-      double t;
-      if (wide) {
-        t = (double)((n + 255) / 256) * len * 1.5;
-      } else {
-        const int64_t full = n / 512, rest = n % 512;
-        t = ((double)full * 1.0 + (rest == 0 ? 0 : rest <= 256 ? 0.6 : 1.0)) * len;
-      }
+      const bool deep = !wide && n <= 256;
+      double t = len * (wide ? (double)((n + 255) / 256) * 1.5 : deep ? 0.6 : (double)((n + 511) / 512) * 1.0);
       if (s > 1) t += 4 + (double)s * z * M * N * 8 / 4e6;
-      if (t < least) least = t, best = Cut{wide != 0, s};
+      if (t < least) least = t, best = Cut{wide != 0, s, deep};
     }
   }
   return best;
@@ -514,11 +513,11 @@ Cut cut_of(int64_t M, int64_t N, int64_t K, int segs, int z, bool dual) {
 
 int64_t part_bytes(const Cut &c, int64_t M, int64_t N, int z) { return c.splits > 1 ? 4 * c.splits * z * M * N : 0; }
 
-template <bool XTR, bool WTR, Epilogue E, int TM, int WM, int WN>
+template <bool XTR, bool WTR, Epilogue E, int TM, int WM, int WN, int S>
 hipError_t launch_tiles(GemmArgs g, int splits, hipStream_t stream) {
   constexpr int BK = 64, TN = TM, DUAL = E == kGated || E == kGatedSave, WT = DUAL ? TN / 2 : TN;
-  constexpr int lds = 2 * (TM + TN) * BK * 2;
-  constexpr auto kernel = gemm_kernel<TM, TN, WM, WN, BK, XTR, WTR, E>;
+  constexpr int lds = S * (TM + TN) * BK * 2;
+  constexpr auto kernel = gemm_kernel<TM, TN, WM, WN, BK, S, XTR, WTR, E>;
   g.tiles = Tiles{splits, g.z, (int)((g.M + TM - 1) / TM), (int)((g.N + WT - 1) / WT)};
   if constexpr (lds > 65536) {
     const hipError_t e = allow_lds<kernel>(lds);
@@ -536,17 +535,22 @@ hipError_t launch_sum_parts(const float *part, bf16 *out0, bf16 *out1, int split
 }
 
 template <bool XTR, bool WTR, Epilogue E>
-hipError_t launch_gemm(GemmArgs g, const Cut &c, hipStream_t stream) {
+hipError_t launch_cut(const GemmArgs &g, const Cut &c, hipStream_t stream) {
+  if (c.wide) return launch_tiles<XTR, WTR, E, 256, 2, 4, 2>(g, c.splits, stream);
+  return c.deep ? launch_tiles<XTR, WTR, E, 128, 4, 2, 4>(g, c.splits, stream)
+                : launch_tiles<XTR, WTR, E, 128, 2, 2, 2>(g, c.splits, stream);
+}
+
+template <bool XTR, bool WTR, Epilogue E>
+hipError_t launch_gemm(const GemmArgs &g, const Cut &c, hipStream_t stream) {
   if constexpr (E == kStore) {
     if (c.splits > 1) {
-      const hipError_t e = c.wide ? launch_tiles<XTR, WTR, kPartial, 256, 2, 4>(g, c.splits, stream)
-                                  : launch_tiles<XTR, WTR, kPartial, 128, 2, 2>(g, c.splits, stream);
+      const hipError_t e = launch_cut<XTR, WTR, kPartial>(g, c, stream);
       if (e != hipSuccess) return e;
       return launch_sum_parts(g.part, g.out[0], g.out[1], c.splits, g.M * g.N / 8, g.z * g.M * g.N / 8, stream);
     }
   }
-  return c.wide ? launch_tiles<XTR, WTR, E, 256, 2, 4>(g, 1, stream)
-                : launch_tiles<XTR, WTR, E, 128, 2, 2>(g, 1, stream);
+  return launch_cut<XTR, WTR, E>(g, c, stream);
 }
 
 }  // namespace

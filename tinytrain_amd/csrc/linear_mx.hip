@@ -177,7 +177,7 @@ __device__ __forceinline__ void load_scales(const uint8_t *p, uint32_t bytes, in
                                            (uint32_t)((w * 64 + (threadIdx.x & 63)) * ld), 0, 0, 0);
 }
 
-template <int TM, int TN, int WM, int WN, int BITS, bool PARTIAL>
+template <int TM, int TN, int WM, int WN, int S, int BITS, bool PARTIAL>
 __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs g) {
   constexpr int NT = 64 * WM * WN, MB = TM / WM / 16, NB = TN / WN / 16, STORES = MB * NB / (PARTIAL ? 1 : 2);
   constexpr int WK = BITS == 4 ? 32 : 64;  // bf16's as long as 128 elements of W
@@ -252,9 +252,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
     return v;
   };
 
-  load(0);
-  wait_and_meet<0>();
-  load(1);
+  constexpr int LOADS = XL::LOADS + WL::LOADS;  // and one of scales in some waves: not counted
+#pragma unroll
+  for (int b = 0; b < S; ++b) load(b);
+  if (ahead < total) wait_and_meet<(S - 1) * LOADS>();
+  else wait_and_meet<0>();
 #pragma unroll
   for (int c = 0; c < NB; ++c) read_w(0, c);
   read_x(0, 0, 0);
@@ -270,10 +272,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
         if (b + 1 < MB) {
           read_x(buf, b + 1, (b + 1) & 1);
         } else {
-          if (st == 0 && i != (int)blockIdx.x) wait_and_meet<STORES>();
-          else wait_and_meet<0>();
+          if (ahead >= total) wait_and_meet<0>();
+          else if (st <= S - 2 && i != (int)blockIdx.x) wait_and_meet<(S - 2) * LOADS + STORES>();
+          else wait_and_meet<(S - 2) * LOADS>();
           load(buf);
-          read_x(buf ^ 1, 0, (b + 1) & 1);  // after the last stage: values that nothing uses
+          buf = buf + 1 == S ? 0 : buf + 1;
+          read_x(buf, 0, (b + 1) & 1);  // after the last stage: values that nothing uses
         }
 #pragma unroll
         for (int c = 0; c < NB; ++c) {
@@ -281,13 +285,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
               operand(wf[c], BITS), operand(xf[b & 1], 8), acc[b][c], BITS == 4 ? 4 : 0, 0, 0, (int)sw[c], 0,
               (int)sx[b & 1]);
           if (b + 1 == MB) {
-            read_w(buf ^ 1, c);  // into the registers that the product has read
+            read_w(buf, c);  // into the registers that the product has read
             __builtin_amdgcn_sched_barrier(0);
           }
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      buf ^= 1;
     }
 
     const int64_t rows = g.M - m0 < TM ? g.M - m0 : TM;
@@ -326,12 +329,12 @@ template <int BITS>
 __global__ __launch_bounds__(256) void mx_values_kernel(const uint8_t *__restrict__ codes,
                                                         const uint8_t *__restrict__ scales, bf16 *__restrict__ out,
                                                         int64_t lanes) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= lanes) return;
-  u32x2 c{};
-  if constexpr (BITS == 4) c[0] = reinterpret_cast<const uint32_t *>(codes)[i];
-  else c = reinterpret_cast<const u32x2 *>(codes)[i];
-  reinterpret_cast<bf16x8 *>(out)[i] = mx_values8<BITS>(c, __uint_as_float((uint32_t)scales[i / 4] << 23));
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < lanes; i += (int64_t)gridDim.x * 256) {
+    u32x2 c{};
+    if constexpr (BITS == 4) c[0] = reinterpret_cast<const uint32_t *>(codes)[i];
+    else c = reinterpret_cast<const u32x2 *>(codes)[i];
+    reinterpret_cast<bf16x8 *>(out)[i] = mx_values8<BITS>(c, __uint_as_float((uint32_t)scales[i / 4] << 23));
+  }
 }
 
 constexpr int kFewRows = 64;  // of linear_mx_rows_kernel at most
@@ -385,10 +388,10 @@ Path path_of(int M, int K, int N, bool x_quantised) {
 // 128 k's in 8 bits take the time of 64 in bf16.
 Cut mx_cut(int M, int K, int N) { return cut_of(M, N, K / 2, 1, 1, false); }
 
-template <int TM, int WM, int WN, int BITS, bool PARTIAL>
+template <int TM, int WM, int WN, int S, int BITS, bool PARTIAL>
 hipError_t launch_mx_tiles(MxArgs g, int splits, hipStream_t stream) {
-  constexpr int lds = 2 * (TM * 128 + TM * 16 * BITS + 8 * TM);
-  constexpr auto kernel = linear_mx_tile_kernel<TM, TM, WM, WN, BITS, PARTIAL>;
+  constexpr int lds = S * (TM * 128 + TM * 16 * BITS + 8 * TM);
+  constexpr auto kernel = linear_mx_tile_kernel<TM, TM, WM, WN, S, BITS, PARTIAL>;
   g.tiles = Tiles{splits, 1, (int)((g.M + TM - 1) / TM), (int)((g.N + TM - 1) / TM)};
   if constexpr (lds > 65536) {
     const hipError_t e = allow_lds<kernel>(lds);
@@ -399,20 +402,25 @@ hipError_t launch_mx_tiles(MxArgs g, int splits, hipStream_t stream) {
   return hipGetLastError();
 }
 
+template <int BITS, bool PARTIAL>
+hipError_t launch_mx_cut(const MxArgs &g, const Cut &c, hipStream_t stream) {
+  if (c.wide) return launch_mx_tiles<256, 2, 4, 2, BITS, PARTIAL>(g, c.splits, stream);
+  return c.deep ? launch_mx_tiles<128, 4, 2, 4, BITS, PARTIAL>(g, c.splits, stream)
+                : launch_mx_tiles<128, 2, 2, 2, BITS, PARTIAL>(g, c.splits, stream);
+}
+
 template <int BITS>
 hipError_t launch_mx(const MxArgs &g, hipStream_t stream) {
   const Cut c = mx_cut((int)g.M, (int)g.K, (int)g.N);
-  if (c.splits == 1)
-    return c.wide ? launch_mx_tiles<256, 2, 4, BITS, false>(g, 1, stream) : launch_mx_tiles<128, 2, 2, BITS, false>(g, 1, stream);
-  const hipError_t e = c.wide ? launch_mx_tiles<256, 2, 4, BITS, true>(g, c.splits, stream)
-                              : launch_mx_tiles<128, 2, 2, BITS, true>(g, c.splits, stream);
+  if (c.splits == 1) return launch_mx_cut<BITS, false>(g, c, stream);
+  const hipError_t e = launch_mx_cut<BITS, true>(g, c, stream);
   return e != hipSuccess ? e : launch_sum_parts(g.part, g.out, nullptr, c.splits, g.M * g.N / 8, g.M * g.N / 8, stream);
 }
 
 hipError_t launch_values(const void *codes, const void *scales, bf16 *out, int64_t elements, int bits,
                          hipStream_t stream) {
   const int64_t lanes = elements / 8;
-  const dim3 grid((unsigned)((lanes + 255) / 256)), block(256);
+  const dim3 grid((unsigned)std::min<int64_t>((lanes + 255) / 256, 1 << 20)), block(256);
   const uint8_t *c = (const uint8_t *)codes, *s = (const uint8_t *)scales;
   if (bits == 4) mx_values_kernel<4><<<grid, block, 0, stream>>>(c, s, out, lanes);
   else mx_values_kernel<8><<<grid, block, 0, stream>>>(c, s, out, lanes);

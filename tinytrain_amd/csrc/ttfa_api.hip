@@ -160,7 +160,7 @@ int check_residual(const void *const *ptrs, int n, const void *residual, const v
 
 constexpr int kMostCols = 1 << 20;  // of a product: a tile's byte offsets stay within 31 bits
 
-// Tiles of tm x tn of a result: workgroups of 256 threads, 2^32 in all.
+// Tiles of tm x tn of a result: their number fits an int with room for its parts.
 int check_tiles(int64_t M, int64_t N, int tm, int tn) {
   return (M + tm - 1) / tm * ((N + tn - 1) / tn) < 1 << 23 ? TTFA_OK : TTFA_E_SEQ;
 }
@@ -176,7 +176,7 @@ int check_linear_mx(int M, int K, int N, int bits) {
   if (bits != 4 && bits != 8) return TTFA_E_BITS;
   int rc = check_rows(M, K, 32, kMostCols);
   if (rc || (rc = check_rows(M, N, 8, kMostCols))) return rc;
-  return check_tiles(M, N, 64, 16);
+  return check_tiles(M, N, 128, 128);
 }
 
 // The workspace of ttfa_bwd_ws: Delta rows, padded to 16 bytes, then the dK/dV partials.
