@@ -27,7 +27,7 @@ from oracle import block, mx_cache
 from tinytrain_amd import _lib
 from tinytrain_amd.kernels.linear_mx import linear_mx, mx_quantize
 from tinytrain_amd.kernels.rms_norm import add_rms_norm, add_rms_norm_mx, rms_norm, rms_norm_bwd, rms_norm_fwd
-from tinytrain_amd.kernels.swiglu import swiglu, swiglu_fwd
+from tinytrain_amd.kernels.swiglu import swiglu, swiglu_bwd, swiglu_fwd
 
 pytestmark = pytest.mark.gpu
 BF, F32 = torch.bfloat16, torch.float32
@@ -163,7 +163,9 @@ def test_norm_empty_and_other_ranks():
 
 SWIGLU_SHAPES = [(1, 8, 8), (1, 768, 2304), (5, 64, 72), (16, 104, 200), (33, 768, 328), (100, 40, 136), (128, 32, 128),
                  (129, 200, 264), (300, 1000, 520), (1000, 136, 1032), (2051, 72, 128),
-                 (4100, 520, 2056), (8197, 264, 2056), (20000, 136, 264), (5000, 2056, 776)]
+                 (4100, 520, 2056), (8197, 264, 2056), (20000, 136, 264), (5000, 2056, 776),
+                 (3, 136, 4104), (31, 72, 4360), (48, 1160, 4104), (64, 40, 8192), (65, 40, 8192), (16, 264, 8200),
+                 (17, 264, 8200)]
 
 
 def _check_swiglu(M, K, N):
@@ -269,7 +271,9 @@ def test_mx_quantize(shape, dtype, bits):
 
 LINEAR_SHAPES = [(1, 32, 8), (1, 4096, 520), (2, 96, 40), (7, 736, 104), (16, 128, 64), (17, 1024, 72), (32, 160, 136),
                  (33, 512, 264), (64, 2048, 48), (65, 288, 128), (150, 640, 328), (520, 256, 392), (1027, 96, 136),
-                 (66, 1152, 72), (300, 128, 1032), (900, 384, 264)]
+                 (66, 1152, 72), (300, 128, 1032), (900, 384, 264),
+                 (3, 128, 4104), (30, 288, 4360), (48, 96, 8192), (64, 1152, 8192), (1, 256, 8200), (32, 128, 8200),
+                 (33, 128, 8200), (15, 2080, 12296), (18, 288, 12296), (16, 160, 16392), (17, 256, 16392)]
 
 
 @pytest.mark.parametrize("bits", [4, 8])
@@ -502,3 +506,121 @@ def test_serving_step_as_used():
     want, _ = block.add_rms_norm((a @ W[2].t()).float(), h.cpu().float(), w.cpu(), 1e-6)
     # four roundings to bf16 on the branch and two on the way out, each 2^-8 at most
     assert (out.cpu().double() - want).norm() <= 6 * 2.0**-8 * want.norm()
+
+
+def test_one_tensor_twice():
+    """The same tensor as input and residual, and as both weights: gradients are the sums of both uses'."""
+    x, w, wg = (v.requires_grad_() for v in (_rand(37, 96, seed=1, dtype=BF), _rand(96, seed=3),
+                                             _rand(72, 96, seed=4, dtype=BF)))
+    r, wu = x.detach().clone().requires_grad_(), wg.detach().clone().requires_grad_()
+    dy, dh, da = _rand(37, 96, seed=5, dtype=BF), _rand(37, 96, seed=6, dtype=BF), _rand(37, 72, seed=7, dtype=BF)
+    one = torch.autograd.grad(add_rms_norm(x, x, w), (x, w), (dy, dh))
+    two = torch.autograd.grad(add_rms_norm(x, r, w), (x, r, w), (dy, dh))
+    assert torch.equal(one[0], two[0] + two[1]) and torch.equal(one[1], two[2])
+    one = torch.autograd.grad(swiglu(x, wg, wg), (x, wg), da)
+    two = torch.autograd.grad(swiglu(x, wg, wu), (x, wg, wu), da)
+    assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1] + two[2])
+
+
+@pytest.mark.parametrize("leaf", range(3))
+def test_norm_with_one_leaf(leaf):
+    """Only one of x, residual and weight takes part in autograd: its gradient is the same."""
+    ts = [_rand(37, 96, seed=1, dtype=BF), _rand(37, 96, seed=2), _rand(96, seed=3)]
+    grads = (_rand(37, 96, seed=4, dtype=BF), _rand(37, 96, seed=5))
+    every = [t.clone().requires_grad_() for t in ts]
+    want = torch.autograd.grad(add_rms_norm(*every), every, grads)[leaf]
+    ts[leaf].requires_grad_()
+    y, h = add_rms_norm(*ts)
+    assert torch.equal(torch.autograd.grad((y, h), ts[leaf], grads)[0], want)
+
+
+def test_two_streams_at_once():
+    """Training steps on two streams at the same time, with the same weights and rows of other numbers: bitwise
+    what each gives alone.  2600 rows split the contraction of both backward products."""
+    w, wg, wu = (_rand(768, seed=3).requires_grad_(), _rand(1040, 768, seed=4, dtype=BF).requires_grad_(),
+                 _rand(1040, 768, seed=5, dtype=BF).requires_grad_())
+    q = mx_quantize(wg.detach(), 4)
+
+    def step(M):
+        x, r = _rand(M, 768, seed=1, dtype=BF).requires_grad_(), _rand(M, 768, seed=2).requires_grad_()
+        torch.cuda.current_stream().synchronize()
+        for _ in range(5):
+            y, h = add_rms_norm(x, r, w)
+            a = swiglu(y, wg, wu)
+            out = (a.detach(), h.detach(), *torch.autograd.grad((a, h), (x, r, w, wg, wu),
+                                                                (torch.ones_like(a), torch.ones_like(h))),
+                   linear_mx(y.detach(), *q))
+        return out
+    want = [step(M) for M in (2600, 300)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for s, M in zip(streams, (2600, 300)):
+        with torch.cuda.stream(s):
+            got.append(step(M))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_two_graphs_in_turn():
+    """Two graphs whose calls need workspaces, captured one after the other and replayed in turn."""
+    wg, wu = _rand(1040, 768, seed=4, dtype=BF), _rand(1040, 768, seed=5, dtype=BF)
+    weight = mx_quantize(wg, 8)
+    xs = [_rand(M, 768, seed=M, dtype=BF) for M in (200, 520)]
+
+    def step(x):
+        a, saved = swiglu_fwd(x, wg, wu, True)
+        return (a, *swiglu_bwd(torch.ones_like(a), saved, x, wg, wu, True, True), linear_mx(x, *weight))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for x in xs:
+            step(x)
+    torch.cuda.current_stream().wait_stream(s)
+    graphs, held = [torch.cuda.CUDAGraph() for _ in xs], []
+    for g, x in zip(graphs, xs):
+        with torch.cuda.graph(g):
+            held.append(step(x))
+    for i in range(3):
+        for k, x in enumerate(xs):
+            x.copy_(_rand(*x.shape, seed=100 * i + k, dtype=BF))
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for k, x in enumerate(xs):
+            assert all(torch.equal(a, b) for a, b in zip(held[k], step(x)))
+
+
+def test_ops_hold_to_their_schemas():
+    x, r, w = _rand(37, 96, seed=1, dtype=BF), _rand(37, 96, seed=2), _rand(96, seed=3)
+    wg, wu, da = _rand(72, 96, seed=4, dtype=BF), _rand(72, 96, seed=5, dtype=BF), _rand(37, 72, seed=6, dtype=BF)
+    saved, (codes, scales) = swiglu_fwd(x, wg, wu, True)[1], mx_quantize(wg, 4)
+    ops = torch.ops.tinytrain
+    for op, args in ((ops.rms_norm_bwd, (x, r, r, w, 1e-6, BF)), (ops.rms_norm_bwd, (x, None, x, w, 1e-6, BF)),
+                     (ops.swiglu_bwd, (da, saved, x, wg, wu, True, False)), (ops.rms_norm_mx, (x, r, w, 1e-6)),
+                     (ops.rms_norm_mx, (x, None, w, 1e-6)), (ops.mx_quantize, (r, 4)),
+                     (ops.linear_mx, (x, codes, scales, None))):
+        torch.library.opcheck(op, args)
+
+
+def test_function_transforms():
+    """Under vmap the operators are loops of their calls; tangents of recorded inputs and second derivatives,
+    which have no formula, raise."""
+    import torch.autograd.forward_ad as fw
+
+    xs, r, w = _rand(3, 9, 96, seed=1, dtype=BF), _rand(9, 96, seed=2), _rand(96, seed=3)
+    wg, wu = _rand(72, 96, seed=4, dtype=BF), _rand(72, 96, seed=5, dtype=BF)
+    q = mx_quantize(wg, 4)
+    for f in (lambda x: add_rms_norm(x, r, w), lambda x: (swiglu(x, wg, wu),), lambda x: add_rms_norm_mx(x, r, w),
+              lambda x: (linear_mx(x, *q),), lambda x: mx_quantize(x, 8)):
+        got = torch.vmap(f)(xs)
+        for i, x in enumerate(xs):
+            assert all(torch.equal(a[i], b) for a, b in zip(got, f(x)))
+    for f in (lambda x: add_rms_norm(x, r, w)[0], lambda x: swiglu(x, wg, wu)):
+        with fw.dual_level(), pytest.raises(NotImplementedError, match="forward mode AD"):
+            f(fw.make_dual(xs[0].clone().requires_grad_(), torch.ones_like(xs[0])))
+        x = xs[0].clone().requires_grad_()
+        y = f(x)
+        with pytest.raises(RuntimeError):
+            g, = torch.autograd.grad(y, x, torch.ones_like(y).requires_grad_(), create_graph=True)
+            torch.autograd.grad(g.sum(), x)

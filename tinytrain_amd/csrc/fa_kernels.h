@@ -98,7 +98,7 @@ hipError_t launch_mx_quantize(const void *x, void *codes, void *scales, int64_t 
 
 // y [M, N] bf16 = x W^T: x [M, K] bf16 (x_scales null) or in 8 bits, W [N, K] in `bits` (linear_mx.hip).
 // workspace: linear_mx_workspace bytes.
-int64_t linear_mx_workspace(int M, int K, int N, int bits, bool x_quantised);
+int64_t linear_mx_workspace(int M, int K, int N, bool x_quantised);
 hipError_t launch_linear_mx(const void *x, const void *x_scales, const void *codes, const void *scales,
                             void *y, void *workspace, int M, int K, int N, int bits, hipStream_t stream);
 

@@ -3,7 +3,7 @@
 //
 // An operand is read as it lies in memory: rows along k (row m holds its k's), or rows along the
 // other index (row k holds its m's; TR), so no product needs a transposed copy.  Tiles go straight
-// to LDS (16 bytes a lane, double-buffered: the next stage's loads run during this stage's products)
+// to LDS (16 bytes a lane, S stages: the next ones' loads run during this stage's products)
 // and come back as operand registers of v_mfma_f32_32x32x16_bf16, TR ones through
 // ds_read_b64_tr_b16.  LDS rows are swizzled in 16-byte chunks so that both reads are free of
 // conflicts (fa_common.h: 16 rows at one chunk; 4 rows x 4 chunks).
@@ -58,11 +58,14 @@ struct TileLoad {
   static constexpr int LOADS = T * BK * 2 / 16 / NT;
   static constexpr int CPR = TR ? T / 8 : BK / 8;  // 16-byte chunks of an LDS row
   static constexpr int BYTES = T * BK * 2;
+  static constexpr int ROWS = NT / CPR;  // of one load of all threads
   static_assert(T * BK * 2 % (16 * NT) == 0 && (!TR || T >= 128), "tile");
+  static_assert(NT % CPR == 0 && ROWS % 16 == 0, "a thread's loads have one swizzle");
   const char *base;  // of the next stage
   uint32_t bytes;    // that the tile's rows have from there on
   int64_t step;      // bytes to the stage after it
-  uint32_t off[LOADS];
+  uint32_t off;   // this thread's first load in the stage, the others `rows` bytes further on each
+  uint32_t rows;
 
   static __device__ __forceinline__ int swizzle(int row) {
     return TR ? (row & 3) << 2 : (row / (16 / CPR)) & (CPR - 1);
@@ -72,17 +75,15 @@ struct TileLoad {
   __device__ __forceinline__ void init(const bf16 *p, int64_t ld, int64_t r0, int64_t R) {
     start(p, ld, r0, R);
     step = TR ? ld * (BK * 2) : BK * 2;
-#pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      const int e = j * NT + (int)threadIdx.x, row = e / CPR;
-      off[j] = (uint32_t)(row * ld * 2) + ((e % CPR) ^ swizzle(row)) * 16;
-    }
+    const int row = (int)threadIdx.x / CPR;
+    off = (uint32_t)(row * ld * 2) + (((int)threadIdx.x % CPR) ^ swizzle(row)) * 16;
+    rows = (uint32_t)(ROWS * ld * 2);
   }
   // The same tile of another matrix of the same shape (k from 0 again).
   __device__ __forceinline__ void start(const bf16 *p, int64_t ld, int64_t r0, int64_t R) {
     base = reinterpret_cast<const char *>(p + (TR ? r0 : r0 * ld));
-    const int64_t rows = R - r0 < T ? R - r0 : T;
-    bytes = rows <= 0 ? 0u : (uint32_t)((TR ? BK * ld - r0 : rows * ld) * 2);
+    const int64_t n = R - r0 < T ? R - r0 : T;
+    bytes = n <= 0 ? 0u : (uint32_t)((TR ? BK * ld - r0 : n * ld) * 2);
   }
   // Past the next n stages.
   __device__ __forceinline__ void skip(int n) {
@@ -94,18 +95,18 @@ struct TileLoad {
     if constexpr (TR) {
       bytes -= (uint32_t)((BK - left) * ld * 2);
     } else {
-#pragma unroll
-      for (int j = 0; j < LOADS; ++j) {
-        const int e = j * NT + (int)threadIdx.x, row = e / CPR;
-        if (8 * ((e % CPR) ^ swizzle(row)) >= left) off[j] = kPastEnd;
-      }
+      if (8 * (((int)threadIdx.x % CPR) ^ swizzle((int)threadIdx.x / CPR)) >= left) off = kPastEnd;
     }
   }
-  __device__ __forceinline__ void load(char *lds) {
+  // The stage, of the matrix that lies `beside` bytes further on.
+  __device__ __forceinline__ void load_beside(int64_t beside, char *lds) const {
     char *dst = lds + wave_id() * 1024;
-    const __amdgpu_buffer_rsrc_t r = make_rsrc(base, bytes);
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(base + beside, bytes);
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) buf_load16_lds(r, off[j], dst + j * NT * 16);
+    for (int j = 0; j < LOADS; ++j) buf_load16_lds(r, off + j * rows, dst + j * NT * 16);
+  }
+  __device__ __forceinline__ void load(char *lds) {
+    load_beside(0, lds);
     base += step;
     if (!TR) bytes -= (uint32_t)(BK * 2);
   }
@@ -247,9 +248,9 @@ __device__ __forceinline__ Tile tile_at(const Tiles &g, int i) {
   return Tile{zs / g.z, zs % g.z, b0 + in % rows, in / rows};
 }
 
-// The first of `stages` stages that a part takes.
+// The first of `stages` (at most 2^25: 64 of 2^31 rows each) stages that a part, of at most 32, takes.
 __device__ __forceinline__ int first_stage(const Tiles &g, int stages, int part) {
-  return (int)((int64_t)stages * part / g.splits);
+  return (int)((uint32_t)(stages * part) / (uint32_t)g.splits);
 }
 
 // kPartial: kStore's sums in fp32, one of `splits` parts of the contraction.
@@ -298,7 +299,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
 
   // Loads: a cursor over the stages of this workgroup's tiles.
   XL xl;
-  WL wl, ul;  // ul: the second weight's rows of a dual tile
+  WL wl;  // of a dual tile both weights' rows
+  const int64_t beside = DUAL ? reinterpret_cast<const char *>(g.w[1]) - reinterpret_cast<const char *>(g.w[0]) : 0;
   int ahead = blockIdx.x, seg, to_do;  // stages of the tile at `at`
   int64_t left;
   Tile at;
@@ -306,7 +308,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
     const int i = at.z + seg;
     xl.init(g.x[i], g.ldx, (int64_t)at.m * TM, g.M);
     wl.init(g.w[i], g.ldw, (int64_t)at.n * WT, g.N);
-    if constexpr (DUAL) ul.init(g.w[1], g.ldw, (int64_t)at.n * WT, g.N);
     if constexpr (E == kPartial) xl.skip(skip), wl.skip(skip);
     left = g.K - (int64_t)skip * BK;
   };
@@ -324,11 +325,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
     if (left < BK) {
       xl.shorten(g.ldx, (int)left);
       wl.shorten(g.ldw, (int)left);
-      if constexpr (DUAL) ul.shorten(g.ldw, (int)left);
     }
     xl.load(dst);
+    if constexpr (DUAL) wl.load_beside(beside, dst + XL::BYTES + WL::BYTES);
     wl.load(dst + XL::BYTES);
-    if constexpr (DUAL) ul.load(dst + XL::BYTES + WL::BYTES);
     left -= BK;
     if (--to_do == 0) {
       ahead += gridDim.x;

@@ -10,7 +10,7 @@
 // below the 2^-9 of y's own rounding.
 //
 // Few rows: bound by reading W once.  A workgroup takes 16 NB rows of W, its eight waves every eighth 128
-// columns, two or four of these at once; a lane has, of its row, 32 consecutive elements with their scale (e4m3:
+// columns, two or four of these at once (as many as registers hold); a lane has, of its row, 32 consecutive elements with their scale (e4m3:
 // 16 and the 16 that are 64 further on, the matrix unit's layout).  The waves' sums are joined through
 // LDS.
 #include <type_traits>
@@ -86,7 +86,7 @@ template <int BITS, bool XMX, int MB, int NB>
 __global__ __launch_bounds__(64 * kRowWaves) void linear_mx_rows_kernel(
     const void *__restrict__ x, const uint8_t *__restrict__ x_scales, const uint8_t *__restrict__ codes,
     const uint8_t *__restrict__ scales, bf16 *__restrict__ y, int M, int K, int N) {
-  constexpr int U = XMX && MB <= 2 ? 4 : 2, STEP = 4 * kRowWaves;
+  constexpr int U = XMX && MB <= 2 && NB * BITS / 4 + 2 * MB <= 10 ? 4 : 2, STEP = 4 * kRowWaves;
   __shared__ f32x4 part[kRowWaves][NB * MB][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, quarter = lane >> 4;
   const int n0 = blockIdx.x * 16 * NB, groups = K / 32;
@@ -169,12 +169,12 @@ struct MxArgs {
 
 // The scales of T rows, one dword each, into LDS: waves W0 .. W0 + T / 64 - 1 load one instruction each.
 template <int T, int W0>
-__device__ __forceinline__ void load_scales(const uint8_t *p, uint32_t bytes, int64_t ld, char *lds) {
+__device__ __forceinline__ void load_scales(const uint8_t *p, uint32_t bytes, uint32_t ld, char *lds) {
   const int w = wave_id() - W0;
   if (w < 0 || w >= T / 64) return;
   const __amdgpu_buffer_rsrc_t r = make_rsrc(p, bytes);
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (TTFA_LDS void *)(lds + w * 256), 4,
-                                           (uint32_t)((w * 64 + (threadIdx.x & 63)) * ld), 0, 0, 0);
+                                           (w * 64 + (threadIdx.x & 63)) * ld, 0, 0, 0);
 }
 
 template <int TM, int TN, int WM, int WN, int S, int BITS, bool PARTIAL>
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
   constexpr int XS = XL::BYTES + WL::BYTES, WS = XS + 4 * TM, STAGE = WS + 4 * TN;
   extern __shared__ __align__(1024) char lds[];
   const int total = g.tiles.total(), all_stages = (int)(g.K / 128);
-  const int64_t sld = g.K / 32;
+  const uint32_t sld = (uint32_t)(g.K / 32);
 
   XL xl;
   WL wl;
@@ -227,21 +227,21 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
   const int i16 = lane & 15, q = lane >> 4;
   // offsets in a stage of this lane's pieces of block 0 (16 rows on: the same swizzle)
   const int xrow = wm * (TM / WM) + i16, wrow = wn * (TN / WN) + i16;
-  const int x0 = xrow * 128 + ((q ^ XL::swizzle(xrow)) << 4), x1 = xrow * 128 + (((q + 4) ^ XL::swizzle(xrow)) << 4);
+  // the second piece, four chunks on: that bit flipped
+  const int x0 = xrow * 128 + ((q ^ XL::swizzle(xrow)) << 4);
   const int w0 = XL::BYTES + wrow * (2 * WK) + ((q ^ WL::swizzle(wrow)) << 4);
-  const int w1 = XL::BYTES + wrow * (2 * WK) + (((q + 4) ^ WL::swizzle(wrow)) << 4);  // BITS 8
   u32x4 xf[2][2], wf[NB][BITS / 4];
   uint32_t sx[2], sw[NB];
   auto read_x = [&](int buf, int b, int into) {
     const char *from = lds + buf * STAGE;
     xf[into][0] = *reinterpret_cast<const u32x4 *>(from + x0 + b * 2048);
-    xf[into][1] = *reinterpret_cast<const u32x4 *>(from + x1 + b * 2048);
+    xf[into][1] = *reinterpret_cast<const u32x4 *>(from + (x0 ^ 64) + b * 2048);
     sx[into] = *reinterpret_cast<const uint8_t *>(from + XS + 4 * xrow + q + b * 64);
   };
   auto read_w = [&](int buf, int c) {
     const char *from = lds + buf * STAGE;
     wf[c][0] = *reinterpret_cast<const u32x4 *>(from + w0 + c * (32 * WK));
-    if constexpr (BITS == 8) wf[c][1] = *reinterpret_cast<const u32x4 *>(from + w1 + c * (32 * WK));
+    if constexpr (BITS == 8) wf[c][1] = *reinterpret_cast<const u32x4 *>(from + (w0 ^ 64) + c * (32 * WK));
     sw[c] = *reinterpret_cast<const uint8_t *>(from + WS + 4 * wrow + q + c * 64);
   };
   auto operand = [](const u32x4 *c, int n) {
@@ -293,21 +293,27 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
       }
     }
 
+    // Byte offsets of rows, a step further for each block.  The lane's part is formed here, not kept over the
+    // stages, whose registers it would spill.
     const int64_t rows = g.M - m0 < TM ? g.M - m0 : TM;
+    const uint32_t row_bytes = (uint32_t)g.N * (PARTIAL ? 4 : 2);
+    int l = threadIdx.x & 63;
+    asm volatile("" : "+v"(l));
+    const int lq = l >> 4;
+    uint32_t to = (wm * (TM / WM) + (l & 15)) * row_bytes;
     if constexpr (PARTIAL) {
       const __amdgpu_buffer_rsrc_t r = make_rsrc(g.part + ((int64_t)t.part * g.M + m0) * g.N, (uint32_t)(rows * g.N * 4));
 #pragma unroll
-      for (int b = 0; b < MB; ++b)
+      for (int b = 0; b < MB; ++b, to += 16 * row_bytes)
 #pragma unroll
         for (int c = 0; c < NB; ++c) {
-          const int64_t n = n0 + wn * (TN / WN) + 16 * c + 4 * q;
-          buf_store16(r, n < g.N ? (uint32_t)((xrow + 16 * b) * g.N * 4 + n * 4) : kPastEnd,
-                      __builtin_bit_cast(u32x4, acc[b][c]));
+          const int n = (int)n0 + wn * (TN / WN) + 16 * c + 4 * lq;
+          buf_store16(r, n < g.N ? to + 4 * n : kPastEnd, __builtin_bit_cast(u32x4, acc[b][c]));
         }
     } else {
       const __amdgpu_buffer_rsrc_t r = make_rsrc(g.out + m0 * g.N, (uint32_t)(rows * g.N * 2));
 #pragma unroll
-      for (int b = 0; b < MB; ++b)
+      for (int b = 0; b < MB; ++b, to += 16 * row_bytes)
 #pragma unroll
         for (int c = 0; c < NB; c += 2) {
           // lanes of odd q take the second block's halves: 16 bytes a lane, 64 of a row
@@ -316,9 +322,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
           const u32x2 f = __builtin_bit_cast(u32x2, pack4(v[0], v[1], v[2], v[3]));
           const auto y0 = __builtin_amdgcn_permlane16_swap(e[0], f[0], false, false);
           const auto y1 = __builtin_amdgcn_permlane16_swap(e[1], f[1], false, false);
-          const int64_t n = n0 + wn * (TN / WN) + 16 * c + 16 * (q & 1) + 8 * (q >> 1);
-          buf_store16(r, n < g.N ? (uint32_t)((xrow + 16 * b) * g.N * 2 + n * 2) : kPastEnd,
-                      u32x4{y0[0], y1[0], y0[1], y1[1]});
+          const int n = (int)n0 + wn * (TN / WN) + 16 * c + 16 * (lq & 1) + 8 * (lq >> 1);
+          buf_store16(r, n < g.N ? to + 2 * n : kPastEnd, u32x4{y0[0], y1[0], y0[1], y1[1]});
         }
     }
   }
@@ -356,12 +361,11 @@ hipError_t by_blocks(int M, int N, F f) {
   auto go = [&](auto m, auto most) {
     constexpr int MOST = decltype(most)::value;
     if (nb <= 1) return f(m, integral_constant<int, 1>{});
-    if (nb == 2 || MOST == 2) return f(m, integral_constant<int, 2>{});
     if constexpr (MOST > 2) {
       if (nb == 3) return f(m, integral_constant<int, 3>{});
-      return f(m, integral_constant<int, 4>{});
+      if (nb > 3) return f(m, integral_constant<int, 4>{});
     }
-    return hipErrorUnknown;
+    return f(m, integral_constant<int, 2>{});
   };
   if (M <= 16) return go(integral_constant<int, 1>{}, integral_constant<int, 4>{});
   if (M <= 32) return go(integral_constant<int, 2>{}, integral_constant<int, 4>{});
@@ -374,14 +378,14 @@ hipError_t by_blocks(int M, int N, F f) {
 namespace {
 
 // kRows: the kernel for few rows; kTiles: tiles of quantised operands; kValues: tiles of bf16 values, which are
-// written to the workspace first.  Measured at the borders, us: x in 8 bits, K 4096, N 12288, 64 rows: kRows 34.1,
-// kTiles 21.7, 32 rows 14.4; N 4096, 64 rows: 15.2, 14.9; K 768, N 2304: 4.1, 6.9.  x in bf16, N 12288, 64 rows:
-// kRows 41.6, kValues 47.8.
+// written to the workspace first.  Measured at the borders, us, W in 4 bits: x in 8 bits, K 4096, N 12288, 32 rows:
+// kRows 14.0, kTiles 19.1; 48 rows: 28.4, 20.3; N 24576, 16 rows: 23.4, 24.3; 24 rows: 28.1, 24.8; N 8192, 64
+// rows: 18.0, 18.5; K 768, N 2304: 4.2, 7.0.  x in bf16, N 12288, 64 rows: kRows 41.6, kValues 47.9.
 enum Path { kRows, kTiles, kValues };
 
 Path path_of(int M, int K, int N, bool x_quantised) {
   const bool tiles = x_quantised && K % 128 == 0;
-  if (M <= (tiles && N > 4096 ? 32 : kFewRows)) return kRows;
+  if (M <= (!tiles || N <= 8192 ? kFewRows : N <= 16384 ? 32 : 16)) return kRows;
   return tiles ? kTiles : kValues;
 }
 
@@ -429,8 +433,7 @@ hipError_t launch_values(const void *codes, const void *scales, bf16 *out, int64
 
 }  // namespace
 
-int64_t linear_mx_workspace(int M, int K, int N, int bits, bool x_quantised) {
-  (void)bits;
+int64_t linear_mx_workspace(int M, int K, int N, bool x_quantised) {
   switch (path_of(M, K, N, x_quantised)) {
     case kRows: return 0;
     case kTiles: return part_bytes(mx_cut(M, K, N), M, N, 1);

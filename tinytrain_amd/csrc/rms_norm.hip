@@ -8,7 +8,7 @@
 // y is computed from the rounded h, so the backward, which reads h again, differentiates what the
 // forward computed; s is computed again there from the same h, which costs no bytes.
 //
-// A row belongs to L lanes (8 to 64 of a wave, or the 256 of a workgroup), 8 elements at a time:
+// A row belongs to L lanes (8 to 64 of a wave, or the 256 or 512 of a workgroup), 8 elements at a time:
 // lane l holds chunks l, l + L, ... in registers, so every tensor is read and written once.  Sums
 // are fp32 over the lanes (fp64 for the 8-bit output, whose codes are defined to the bit).
 #include <type_traits>
@@ -163,8 +163,8 @@ __device__ __forceinline__ float sticky(double d) {
 }
 
 // The forward with y in 8 bits: 32 elements (four lanes) share a power of two, as in the quantised
-// KV cache.  Norm and product in fp64, then one rounding, so codes do not depend on how the sum is
-// split over lanes (to about 2^-26 of a step in fp32 one value in 10^6 went to its other neighbour).
+// KV cache.  Norm and product in fp64, then one rounding: in fp32 a value within 2^-20 of the middle
+// between two codes could go to either, by how the sum is split over lanes.
 template <class TX, class TR, bool RES, int CH, int WT>
 __global__ __launch_bounds__(Lanes<WT>::THREADS) void rms_norm_mx_kernel(const TX *__restrict__ x,
                                                           const TR *__restrict__ r,
@@ -300,8 +300,8 @@ __global__ __launch_bounds__(Lanes<WT>::THREADS) void rms_norm_bwd_kernel(
   }
 }
 
-// dw = sum of n partials [n][C], in a fixed order: a workgroup takes 16 columns, 64 partials at once.  (With 64
-// columns and 16 partials at once 512 partials of 768 columns took 10 us, so 4.)
+// dw = sum of n partials [n][C], in a fixed order: a workgroup takes 16 columns, 64 partials at once.  (512 partials
+// of 768 columns: 4.0 us.  With 64 columns a workgroup, 12 of them, 1024 partials took 20.7.)
 __global__ __launch_bounds__(256) void rms_norm_dw_kernel(const float *__restrict__ part,
                                                           float *__restrict__ dw, int n, int nq) {
   __shared__ f32x4 shared[64][4];
@@ -331,7 +331,7 @@ struct Spread {
   int threads() const { return log2 == 9 ? 512 : 256; }
 };
 
-// Up to four chunks a lane, fewer where the rows would not give 512 workgroups.
+// Up to three chunks a lane, fewer where the rows would not give 512 workgroups (rows past a wave's: the workgroup's).
 Spread spread_of(int nch, int64_t M) {
   for (int l = 3; l <= 6; ++l)
     if (nch <= 3 << l) {

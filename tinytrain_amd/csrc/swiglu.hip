@@ -134,9 +134,11 @@ __global__ __launch_bounds__(256) void swiglu_grad_kernel(const bf16 *__restrict
   }
 }
 
-// Rows of x up to which the kernel above is faster than a tile of 128 x 64 (K 768, N 2304, M 64: 6.8 us, tiles
-// 11.6; K 2048, N 6144: 21.0, 32.6), but for many columns (K 4096, N 12288: 74, 68; M 48: 62, 66).
-bool few_rows(int M, int N) { return M <= (N <= 8192 ? 64 : 48); }
+// Rows of x up to which the kernel above is faster than tiles (us, K x N: rows, tiles).  768 x 2304, 64 rows: 7.2,
+// 11.2; 2048 x 6144: 20.7, 22.0; 4096 x 8192: 39.6, 39.2.  More columns give a tile to each CU, and reading x again
+// for every 16 of them counts: 4096 x 12288, 1 row: 36.7, 41.1; 16: 45.3, 42.0; 32: 52.7, 44.5; 2048 x 12288, 16:
+// 23.9, 24.0.
+bool few_rows(int M, int N) { return M <= (N <= 8192 ? 64 : 16); }
 
 const bf16 *in(const void *p) { return static_cast<const bf16 *>(p); }
 

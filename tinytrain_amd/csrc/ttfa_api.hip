@@ -522,7 +522,7 @@ int ttfa_mx_quantize(const void *x, void *codes, void *scales, long long M, int 
 }
 
 long long ttfa_linear_mx_workspace_bytes(int M, int K, int N, int bits, int x_quantised) {
-  return check_linear_mx(M, K, N, bits) ? -1 : ttfa::linear_mx_workspace(M, K, N, bits, x_quantised != 0);
+  return check_linear_mx(M, K, N, bits) ? -1 : ttfa::linear_mx_workspace(M, K, N, x_quantised != 0);
 }
 
 int ttfa_linear_mx(const void *x, const void *x_scales, const void *codes, const void *scales, void *y,
