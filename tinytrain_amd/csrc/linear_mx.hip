@@ -9,10 +9,12 @@
 // sum is off by less than 2^-10 of those largest ones' sum, on random values by 2^-19 of sum |x w|, far
 // below the 2^-9 of y's own rounding.
 //
-// Few rows: bound by reading W once.  A workgroup takes 16 NB rows of W, its eight waves every eighth 128
-// columns, two or four of these at once (as many as registers hold); a lane has, of its row, 32 consecutive elements with their scale (e4m3:
-// 16 and the 16 that are 64 further on, the matrix unit's layout).  The waves' sums are joined through
-// LDS.
+// Few rows: bound by reading W once, and by the cache lines that its loads touch.  A workgroup takes 16 NB rows
+// of W and each of its eight waves an eighth of the columns, in blocks of 128, two or four of these at once (as
+// many as registers hold).  A lane has, of its row, 32 consecutive elements of a block (e4m3 with x in 8 bits: 16
+// and the 16 that are 64 further on, the matrix unit's layout).  The waves' sums are joined through LDS.  4096 x
+// 12288 in 4 bits, us: one row 8.0 (3.3 TB/s, of which a launch and one round of loads are half), 32 rows 11.3;
+// with every eighth block to a wave, and so a load for each scale, 8.8 and 14.0.
 #include <type_traits>
 
 #include "fa_common.h"
@@ -29,19 +31,37 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kRowWaves = 8;
 
+// Scale bytes of a lane's row in U blocks of four groups, of group q of each: the row's bytes lie together, so one
+// load of 4 U of them where the row has as many left, and not U of one byte each.
+template <int U>
+struct Scales {
+  uint32_t w[U];
+  int shift;
+  // at: the first block's first byte, `left` groups from there to the row's end
+  __device__ __forceinline__ void load(const uint8_t *at, int left, int q) {
+    if (left >= 4 * U) {
+      __builtin_memcpy(w, at, 4 * U);
+      shift = 8 * q;
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) w[u] = 4 * u + q < left ? at[4 * u + q] : 127;
+      shift = 0;
+    }
+  }
+  __device__ __forceinline__ uint32_t byte(int u) const { return w[u] >> shift & 255; }
+};
+
 // 32 consecutive elements (a group) of a row of W, as bf16 for the product with x in bf16.
 template <int BITS>
 struct Group {
   u32x4 c[BITS / 4];
-  uint32_t byte;
-  __device__ __forceinline__ void load(const uint8_t *codes, const uint8_t *scales, int64_t group, bool ok) {
-    byte = ok ? scales[group] : 0;
+  __device__ __forceinline__ void load(const uint8_t *codes, int64_t group, bool ok) {
 #pragma unroll
     for (int i = 0; i < BITS / 4; ++i)
       c[i] = ok ? reinterpret_cast<const u32x4 *>(codes + group * (4 * BITS))[i] : u32x4{};
   }
   // elements 8 j .. 8 j + 7
-  __device__ __forceinline__ bf16x8 values(int j) const {
+  __device__ __forceinline__ bf16x8 values(int j, uint32_t byte) const {
     const float scale = __uint_as_float(byte << 23);
     if constexpr (BITS == 4) return mx_values8<4>(u32x2{c[0][j], 0u}, scale);
     else return mx_values8<8>(u32x2{c[j / 2][2 * (j % 2)], c[j / 2][2 * (j % 2) + 1]}, scale);
@@ -62,10 +82,8 @@ struct Rows32 {
 template <int BITS>
 struct Scaled {
   u32x4 c[BITS / 4];
-  uint32_t byte;
   // group0: the first of the row's four groups, `left` groups from there to the row's end
-  __device__ __forceinline__ void load(const uint8_t *codes, const uint8_t *scales, int64_t group0, int left, int q) {
-    byte = q < left ? scales[group0 + q] : 127;
+  __device__ __forceinline__ void load(const uint8_t *codes, int64_t group0, int left, int q) {
     if constexpr (BITS == 4) {
       c[0] = q < left ? *reinterpret_cast<const u32x4 *>(codes + (group0 + q) * 16) : u32x4{};
     } else {
@@ -86,27 +104,35 @@ template <int BITS, bool XMX, int MB, int NB>
 __global__ __launch_bounds__(64 * kRowWaves) void linear_mx_rows_kernel(
     const void *__restrict__ x, const uint8_t *__restrict__ x_scales, const uint8_t *__restrict__ codes,
     const uint8_t *__restrict__ scales, bf16 *__restrict__ y, int M, int K, int N) {
-  constexpr int U = XMX && MB <= 2 && NB * BITS / 4 + 2 * MB <= 10 ? 4 : 2, STEP = 4 * kRowWaves;
+  constexpr int U = XMX && MB <= 2 && NB * BITS / 4 + 2 * MB <= 10 ? 4 : 2;
   __shared__ f32x4 part[kRowWaves][NB * MB][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, quarter = lane >> 4;
-  const int n0 = blockIdx.x * 16 * NB, groups = K / 32;
+  const int lane = threadIdx.x & 63, wave = wave_id(), row = lane & 15, quarter = lane >> 4;
+  const int n0 = blockIdx.x * 16 * NB, groups = K / 32, blocks = (groups + 3) / 4;
+  const int each = (blocks + kRowWaves - 1) / kRowWaves, end = min(blocks, each * (wave + 1));
   int64_t wrow[NB], xrow[MB];  // rows past the end: the last one's, not stored
 #pragma unroll
   for (int c = 0; c < NB; ++c) wrow[c] = (int64_t)min(n0 + 16 * c + row, N - 1) * groups;
 #pragma unroll
   for (int b = 0; b < MB; ++b) xrow[b] = (int64_t)min(16 * b + row, M - 1) * groups;
   f32x4 acc[NB][MB] = {};
-  for (int k = 4 * wave; k < groups; k += U * STEP) {
+  for (int k = each * wave; k < end; k += U) {
+    const int left = groups - 4 * k;  // to the row's end
+    Scales<U> ws[NB];
+#pragma unroll
+    for (int c = 0; c < NB; ++c) ws[c].load(scales + wrow[c] + 4 * k, left, quarter);
     if constexpr (XMX) {
       Scaled<BITS> w[U][NB];
       Scaled<8> v[U][MB];
+      Scales<U> xs[MB];
+#pragma unroll
+      for (int b = 0; b < MB; ++b) xs[b].load(x_scales + xrow[b] + 4 * k, left, quarter);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int at = k + u * STEP, left = groups - at;
+        const int at = 4 * (k + u), of = k + u < end ? groups - at : 0;
 #pragma unroll
-        for (int c = 0; c < NB; ++c) w[u][c].load(codes, scales, wrow[c] + at, left, quarter);
+        for (int c = 0; c < NB; ++c) w[u][c].load(codes, wrow[c] + at, of, quarter);
 #pragma unroll
-        for (int b = 0; b < MB; ++b) v[u][b].load((const uint8_t *)x, x_scales, xrow[b] + at, left, quarter);
+        for (int b = 0; b < MB; ++b) v[u][b].load((const uint8_t *)x, xrow[b] + at, of, quarter);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -115,18 +141,19 @@ __global__ __launch_bounds__(64 * kRowWaves) void linear_mx_rows_kernel(
 #pragma unroll
           for (int b = 0; b < MB; ++b)
             acc[c][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                w[u][c].operand(), v[u][b].operand(), acc[c][b], BITS == 4 ? 4 : 0, 0, 0, (int)w[u][c].byte, 0,
-                (int)v[u][b].byte);
+                w[u][c].operand(), v[u][b].operand(), acc[c][b], BITS == 4 ? 4 : 0, 0, 0, (int)ws[c].byte(u), 0,
+                (int)xs[b].byte(u));
     } else {
       Group<BITS> w[U][NB];
       Rows32 v[U][MB];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int at = k + u * STEP + quarter;
+        const int at = 4 * (k + u) + quarter;
+        const bool ok = k + u < end && at < groups;
 #pragma unroll
-        for (int c = 0; c < NB; ++c) w[u][c].load(codes, scales, wrow[c] + at, at < groups);
+        for (int c = 0; c < NB; ++c) w[u][c].load(codes, wrow[c] + at, ok);
 #pragma unroll
-        for (int b = 0; b < MB; ++b) v[u][b].load((const bf16 *)x, xrow[b] + at, at < groups);
+        for (int b = 0; b < MB; ++b) v[u][b].load((const bf16 *)x, xrow[b] + at, ok);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -134,7 +161,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void linear_mx_rows_kernel(
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int c = 0; c < NB; ++c) {
-            const bf16x8 wv = w[u][c].values(j);
+            const bf16x8 wv = w[u][c].values(j, ws[c].byte(u));
 #pragma unroll
             for (int b = 0; b < MB; ++b)
               acc[c][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, v[u][b].values(j), acc[c][b], 0, 0, 0);
@@ -378,9 +405,10 @@ hipError_t by_blocks(int M, int N, F f) {
 namespace {
 
 // kRows: the kernel for few rows; kTiles: tiles of quantised operands; kValues: tiles of bf16 values, which are
-// written to the workspace first.  Measured at the borders, us, W in 4 bits: x in 8 bits, K 4096, N 12288, 32 rows:
-// kRows 14.0, kTiles 19.1; 48 rows: 28.4, 20.3; N 24576, 16 rows: 23.4, 24.3; 24 rows: 28.1, 24.8; N 8192, 64
-// rows: 18.0, 18.5; K 768, N 2304: 4.2, 7.0.  x in bf16, N 12288, 64 rows: kRows 41.6, kValues 47.9.
+// written to the workspace first.  Measured at the borders, us, x in 8 bits, W in 4 (8): K 4096, N 8192, 64 rows:
+// kRows 15.1 (18.0), kTiles 18.2 (17.3); N 12288, 32 rows: 11.3 (15.6), 18.6 (20.6); 48 rows: 21.8 (28.1), 20.0
+// (21.8); N 20480, 16 rows: 19.5 (29.4), 20.9 (25.9); 24 rows: 22.7 (33.9), 21.6 (26.8).  x in bf16, N 12288, 64
+// rows: kRows 40.9, kValues 47.9.
 enum Path { kRows, kTiles, kValues };
 
 Path path_of(int M, int K, int N, bool x_quantised) {
