@@ -316,6 +316,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
             __builtin_amdgcn_sched_barrier(0);
           }
         }
+        // The products of the step before are done in this one: without a use they would all be moved behind the
+        // last step's wait, and every operand of the stage be held until then.
+        if (b > 0)
+#pragma unroll
+          for (int c = 0; c < NB; ++c) asm volatile("" : "+v"(acc[b - 1][c]));
         __builtin_amdgcn_sched_barrier(0);
       }
     }
