@@ -214,10 +214,23 @@ struct SavedSums {
       : high{reinterpret_cast<bf16 *>(p), reinterpret_cast<bf16 *>(p) + n}, low(p + 4 * n) {}
 };
 
-// To nearest; a NaN or infinity as it is.
-__device__ __forceinline__ uint32_t saved_bits(float x) {
-  const uint32_t b = __float_as_uint(x);
-  return (b & 0x7f800000u) == 0x7f800000u ? b : b + 0x800u;
+// Four elements of both: their high halves in pairs, and a byte of low bits each, g's below u's.  Half a step is
+// added and the bits past the twelfth are left out, so an infinity stays one, and a NaN does: its low bits are zero (an
+// operand's, which has 16 bits) or it is the matrix unit's own.
+__device__ __forceinline__ void saved_four(const float (&g)[4], const float (&u)[4], uint32_t *gh, uint32_t *uh,
+                                           uint32_t &low) {
+  uint32_t x[4], y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = __float_as_uint(g[e]) + 0x800u, y[e] = __float_as_uint(u[e]) + 0x800u;
+#pragma unroll
+  for (int e = 0; e < 4; e += 2) {
+    gh[e / 2] = __builtin_amdgcn_perm(x[e + 1], x[e], 0x07060302u);
+    uh[e / 2] = __builtin_amdgcn_perm(y[e + 1], y[e], 0x07060302u);
+  }
+  // the second byte of each, whose upper half is wanted (0x0c: zero)
+  const uint32_t p = __builtin_amdgcn_perm(x[1], x[0], 0x0c0c0501u) | __builtin_amdgcn_perm(x[3], x[2], 0x05010c0cu);
+  const uint32_t q = __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0501u) | __builtin_amdgcn_perm(y[3], y[2], 0x05010c0cu);
+  low = (p >> 4 & 0x0f0f0f0fu) | (q & 0xf0f0f0f0u);
 }
 
 __device__ __forceinline__ float sigmoid(float x) {
@@ -370,12 +383,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
     const int stages = first_stage(g.tiles, all_stages, t.part + 1) - first_stage(g.tiles, all_stages, t.part);
     f32x16 acc[MB][NB] = {};
     const int row = wm * (TM / WM) + (lane & 15), col = wn * (DUAL ? 32 : TN / WN) + 8 * piece_of(lane);
-    const uint32_t bytes = (uint32_t)((g.M - m0 < TM ? g.M - m0 : TM) * g.N * 2);
-    // byte offset in the tile's rows of this lane's piece of set q of block (i, j)
-    auto piece_at = [&](int i, int j, int q) {
-      const int64_t n = n0 + col + 32 * j;
-      return n < g.N ? (uint32_t)((row + 32 * i + 16 * q) * g.N * 2 + n * 2) : kPastEnd;
-    };
+    const uint32_t row_bytes = (uint32_t)g.N * (E == kPartial ? 4 : 2);
+    const uint32_t bytes = (uint32_t)(g.M - m0 < TM ? g.M - m0 : TM) * row_bytes;
+    // byte offset in the tile's rows of this lane's piece of set q of block (i, j): past the end with its column
+    uint32_t piece0[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int n = (int)n0 + col + 32 * j;
+      piece0[j] = n < (int)g.N ? row * row_bytes + 2 * n : kPastEnd;
+    }
+    auto piece_at = [&](int i, int j, int q) { return piece0[j] + (32 * i + 16 * q) * row_bytes; };
     for (int st = 0; st < stages; ++st) {
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
@@ -398,7 +415,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
     }
 
     if constexpr (E == kPartial) {
-      const __amdgpu_buffer_rsrc_t r = make_rsrc(g.part + ((int64_t)(t.part * g.z + t.z) * g.M + m0) * g.N, 2 * bytes);
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(g.part + ((int64_t)(t.part * g.z + t.z) * g.M + m0) * g.N, bytes);
 #pragma unroll
       for (int i = 0; i < MB; ++i)
 #pragma unroll
@@ -407,8 +424,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
           block_rows_f32(acc[i][j], set);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const int64_t n = n0 + wn * (TN / WN) + 32 * j + 16 * (q / 2) + 8 * ((lane >> 4) & 1) + 4 * (lane >> 5);
-            buf_store16(r, n < g.N ? (uint32_t)((row + 32 * i + 16 * (q % 2)) * g.N * 4 + n * 4) : kPastEnd, set[q]);
+            const int n = (int)n0 + wn * (TN / WN) + 32 * j + 16 * (q / 2) + 8 * ((lane >> 4) & 1) + 4 * (lane >> 5);
+            const uint32_t to = n < (int)g.N ? row * row_bytes + 4 * n : kPastEnd;
+            buf_store16(r, to + (32 * i + 16 * (q % 2)) * row_bytes, set[q]);
           }
         }
       continue;
@@ -437,13 +455,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
         buf_store16(r0, piece_at(i, 0, 0), set[0]);
         buf_store16(r0, piece_at(i, 0, 1), set[1]);
         if constexpr (E == kGatedSave) {
-          uint32_t high[2][8], low[4] = {};
+          uint32_t high[2][8], low[4];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const uint32_t x = saved_bits(acc[i][0][e]), y = saved_bits(acc[i][1][e]);
-            if (e % 2 == 0) high[0][e / 2] = x >> 16, high[1][e / 2] = y >> 16;
-            else high[0][e / 2] |= x & 0xffff0000u, high[1][e / 2] |= y & 0xffff0000u;
-            low[e / 4] |= ((x >> 12 & 15) | (y >> 8 & 0xf0)) << (8 * (e % 4));
+          for (int a = 0; a < 4; ++a) {
+            const f32x16 &g4 = acc[i][0], &u4 = acc[i][1];
+            saved_four({g4[4 * a], g4[4 * a + 1], g4[4 * a + 2], g4[4 * a + 3]},
+                       {u4[4 * a], u4[4 * a + 1], u4[4 * a + 2], u4[4 * a + 3]}, &high[0][2 * a], &high[1][2 * a], low[a]);
           }
           block_rows(high[0], set);
           buf_store16(rg, piece_at(i, 0, 0), set[0]);

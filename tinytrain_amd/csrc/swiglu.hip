@@ -10,7 +10,7 @@
 // significant bits, an error of 2^-13 against the 2^-9 that every gradient has from its own rounding and
 // from that of dg and du, as bf16 operands of the last two products (in bf16 they would add as much
 // again).  That is 5 bytes an element; to form them again instead of reading them was 713 us at
-// 16384 x 2048 x 6144, four times as long as the kernel that reads them (swiglu_grad_kernel).
+// 16384 x 2048 x 6144, against 190 to 225 of the kernel that reads them (swiglu_grad_kernel).
 #include "fa_kernels.h"
 #include "gemm.h"
 
@@ -23,9 +23,9 @@ namespace {
 // them with up to 16 MB rows of x (v_mfma_f32_16x16x32_bf16, W as first operand: D[n][m]).  A lane takes
 // eight k's of every 32, so that a load instruction reads 64 consecutive bytes of each of 16 rows (with 32
 // consecutive k's a lane, four pieces of 16 bytes of each: 50 MB of weights 16.5 us, 13.3 so).  The waves'
-// sums are joined through LDS.  200 MB of weights and one row: 36 us, 5.6 TB/s; 7 MB 3.9 us, of which a
+// sums are joined through LDS.  200 MB of weights and one row: 36.7 us, 5.5 TB/s; 7 MB 4.1 us, of which a
 // launch and the latency of one round of loads are most.  More rows take longer by reading x again for
-// every 16 NB columns (32 rows: 16.8 us at 50 MB).
+// every 16 NB columns (32 rows: 15.6 us at 50 MB).
 struct K32 {
   u32x4 c[4];
   __device__ __forceinline__ void load(const bf16 *row, int k, int K) {
@@ -96,17 +96,10 @@ __global__ __launch_bounds__(64 * kRowWaves) void swiglu_rows_kernel(const bf16 
   *reinterpret_cast<bf16x4 *>(a + at) = pack4(r[0], r[1], r[2], r[3]);
   if (!saved) return;
   const SavedSums s(saved, (int64_t)M * N);
-  u32x2 high[2] = {};
-  uint32_t low = 0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint32_t p = saved_bits(g[e]), q = saved_bits(u[e]);
-    high[0][e / 2] |= (p >> 16) << (16 * (e % 2));
-    high[1][e / 2] |= (q >> 16) << (16 * (e % 2));
-    low |= ((p >> 12 & 15) | (q >> 8 & 0xf0)) << (8 * e);
-  }
-  *reinterpret_cast<u32x2 *>(s.high[0] + at) = high[0];
-  *reinterpret_cast<u32x2 *>(s.high[1] + at) = high[1];
+  uint32_t gh[2], uh[2], low;
+  saved_four({g[0], g[1], g[2], g[3]}, {u[0], u[1], u[2], u[3]}, gh, uh, low);
+  *reinterpret_cast<u32x2 *>(s.high[0] + at) = u32x2{gh[0], gh[1]};
+  *reinterpret_cast<u32x2 *>(s.high[1] + at) = u32x2{uh[0], uh[1]};
   *reinterpret_cast<uint32_t *>(s.low + at) = low;
 }
 
