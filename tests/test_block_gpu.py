@@ -273,7 +273,8 @@ LINEAR_SHAPES = [(1, 32, 8), (1, 4096, 520), (2, 96, 40), (7, 736, 104), (16, 12
                  (33, 512, 264), (64, 2048, 48), (65, 288, 128), (150, 640, 328), (520, 256, 392), (1027, 96, 136),
                  (66, 1152, 72), (300, 128, 1032), (900, 384, 264),
                  (3, 128, 4104), (30, 288, 4360), (48, 96, 8192), (64, 1152, 8192), (1, 256, 8200), (32, 128, 8200),
-                 (33, 128, 8200), (15, 2080, 12296), (18, 288, 12296), (16, 160, 16392), (17, 256, 16392)]
+                 (33, 128, 8200), (15, 2080, 12296), (18, 288, 12296), (16, 160, 16392), (17, 256, 16392),
+                 (300, 416, 264), (700, 32, 520), (129, 4128, 136), (1100, 1056, 776), (513, 2080, 264)]
 
 
 @pytest.mark.parametrize("bits", [4, 8])

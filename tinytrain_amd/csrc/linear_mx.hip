@@ -185,14 +185,33 @@ __global__ __launch_bounds__(64 * kRowWaves) void linear_mx_rows_kernel(
 // persistent workgroup, loads two stages ahead, operands read before they are needed.  128 k's of a row
 // of x are 128 bytes and of W 64 or 128, loaded as gemm.h's tiles of bf16 of that many bytes; the scales
 // of a stage, four bytes a row, go to LDS beside them.  A step is 16 rows of x by the wave's columns;
-// the operands of W stay in registers for a stage.  K is a multiple of 128.
+// the operands of W stay in registers for a stage.  What a last stage has past K loads as zeros; rows of scales
+// that are no whole dwords are laid out anew first (pad_scales_kernel).
 struct MxArgs {
   const uint8_t *x, *x_scales, *codes, *scales;
   bf16 *out;
   float *part;  // PARTIAL: [splits][M][N]
   int64_t M, N, K;
+  int sld;      // bytes of a row of scales
   Tiles tiles;
 };
+
+// Rows of K / 32 scales of x (rows 0 .. m - 1) and W as rows of whole dwords, the bytes behind them a scale of one.
+__global__ __launch_bounds__(256) void pad_scales_kernel(const uint8_t *__restrict__ x_scales,
+                                                         const uint8_t *__restrict__ scales, uint32_t *__restrict__ x_out,
+                                                         uint32_t *__restrict__ out, int groups, int dwords, int64_t m,
+                                                         int64_t rows) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * dwords; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / dwords;
+    const int g = 4 * (int)(i - row * dwords);
+    const uint8_t *from = row < m ? x_scales + row * groups : scales + (row - m) * groups;
+    uint32_t w = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) w |= (g + b < groups ? from[g + b] : 127u) << (8 * b);
+    if (row < m) x_out[i] = w;
+    else out[i - m * dwords] = w;
+  }
+}
 
 // The scales of T rows, one dword each, into LDS: waves W0 .. W0 + T / 64 - 1 load one instruction each.
 template <int T, int W0>
@@ -213,14 +232,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
   static_assert((TM + TN) / 64 <= NT / 64, "a wave loads scales once a stage");
   constexpr int XS = XL::BYTES + WL::BYTES, WS = XS + 4 * TM, STAGE = WS + 4 * TN;
   extern __shared__ __align__(1024) char lds[];
-  const int total = g.tiles.total(), all_stages = (int)(g.K / 128);
-  const uint32_t sld = (uint32_t)(g.K / 32);
+  const int total = g.tiles.total(), all_stages = (int)((g.K + 127) / 128);
+  const uint32_t sld = (uint32_t)g.sld;
 
   XL xl;
   WL wl;
   const uint8_t *xs, *ws;
   uint32_t xs_bytes, ws_bytes;
-  int ahead = blockIdx.x, to_do;
+  int ahead = blockIdx.x, to_do, left;
   auto next_tile = [&] {
     const Tile at = tile_at(g.tiles, ahead);
     const int first = first_stage(g.tiles, all_stages, at.part);
@@ -230,6 +249,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
     wl.init(reinterpret_cast<const bf16 *>(g.codes), g.K * BITS / 16, n0, g.N);
     xl.skip(first);
     wl.skip(first);
+    left = (int)g.K - 128 * first;
     xs = g.x_scales + m0 * sld + 4 * first;
     ws = g.scales + n0 * sld + 4 * first;
     xs_bytes = (uint32_t)((g.M - m0 < TM ? g.M - m0 : TM) * sld) - 4 * first;
@@ -239,6 +259,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
   auto load = [&](int buf) {
     if (ahead >= total) return;
     char *dst = lds + buf * STAGE;
+    if (left < 128) {
+      xl.shorten(0, left / 2);
+      wl.shorten(0, left * BITS / 16);
+    }
+    left -= 128;
     xl.load(dst);
     wl.load(dst + XL::BYTES);
     load_scales<TM, 0>(xs, xs_bytes, sld, dst + XS);
@@ -361,7 +386,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
   }
 }
 
-// Values of quantised rows in bf16, 8 a lane (for products of bf16 rows, and of K's that are no multiple of 128).
+// Values of quantised rows in bf16, 8 a lane.
 template <int BITS>
 __global__ __launch_bounds__(256) void mx_values_kernel(const uint8_t *__restrict__ codes,
                                                         const uint8_t *__restrict__ scales, bf16 *__restrict__ out,
@@ -417,13 +442,15 @@ namespace {
 enum Path { kRows, kTiles, kValues };
 
 Path path_of(int M, int K, int N, bool x_quantised) {
-  const bool tiles = x_quantised && K % 128 == 0;
-  if (M <= (!tiles || N <= 8192 ? kFewRows : N <= 16384 ? 32 : 16)) return kRows;
-  return tiles ? kTiles : kValues;
+  if (M <= (!x_quantised || N <= 8192 ? kFewRows : N <= 16384 ? 32 : 16)) return kRows;
+  return x_quantised ? kTiles : kValues;
 }
 
 // 128 k's in 8 bits take the time of 64 in bf16.
 Cut mx_cut(int M, int K, int N) { return cut_of(M, N, K / 2, 1, 1, false); }
+
+// Bytes of the scales of `rows` rows in whole dwords, to where the next piece of a workspace begins.
+int64_t padded_scales(int64_t rows, int K) { return (rows * ((K + 127) / 128 * 4) + 15) / 16 * 16; }
 
 template <int TM, int WM, int WN, int S, int BITS, bool PARTIAL>
 hipError_t launch_mx_tiles(MxArgs g, int splits, hipStream_t stream) {
@@ -469,9 +496,9 @@ hipError_t launch_values(const void *codes, const void *scales, bf16 *out, int64
 int64_t linear_mx_workspace(int M, int K, int N, bool x_quantised) {
   switch (path_of(M, K, N, x_quantised)) {
     case kRows: return 0;
-    case kTiles: return part_bytes(mx_cut(M, K, N), M, N, 1);
-    default:
-      return 2 * ((int64_t)N * K + (x_quantised ? (int64_t)M * K : 0)) + part_bytes(cut_of(M, N, K, 1, 1, false), M, N, 1);
+    case kTiles:
+      return (K % 128 ? padded_scales(M, K) + padded_scales(N, K) : 0) + part_bytes(mx_cut(M, K, N), M, N, 1);
+    default: return 2 * (int64_t)N * K + part_bytes(cut_of(M, N, K, 1, 1, false), M, N, 1);
   }
 }
 
@@ -489,16 +516,25 @@ hipError_t launch_linear_mx(const void *x, const void *x_scales, const void *cod
       });
     });
   if (path == kTiles) {
-    const MxArgs g{(const uint8_t *)x, (const uint8_t *)x_scales, (const uint8_t *)codes, (const uint8_t *)scales,
-                   (bf16 *)y, (float *)workspace, M, N, K, {}};
+    MxArgs g{(const uint8_t *)x, (const uint8_t *)x_scales, (const uint8_t *)codes, (const uint8_t *)scales,
+             (bf16 *)y, (float *)workspace, M, N, K, K / 32, {}};
+    if (K % 128) {
+      uint8_t *xp = (uint8_t *)workspace, *wp = xp + padded_scales(M, K);
+      const int dwords = (K + 127) / 128;
+      const int64_t rows = (int64_t)M + N, blocks = (rows * dwords + 255) / 256;
+      pad_scales_kernel<<<dim3((unsigned)std::min<int64_t>(blocks, 1 << 20)), dim3(256), 0, stream>>>(
+          g.x_scales, g.scales, (uint32_t *)xp, (uint32_t *)wp, K / 32, dwords, M, rows);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+      g.x_scales = xp, g.scales = wp, g.sld = 4 * dwords, g.part = (float *)(wp + padded_scales(N, K));
+    }
     return bits == 4 ? launch_mx<4>(g, stream) : launch_mx<8>(g, stream);
   }
-  bf16 *w = (bf16 *)workspace, *xv = w + (int64_t)N * K;
-  float *part = (float *)(xv + (x_scales ? (int64_t)M * K : 0));
-  hipError_t e = launch_values(codes, scales, w, (int64_t)N * K, bits, stream);
-  if (e == hipSuccess && x_scales) e = launch_values(x, x_scales, xv, (int64_t)M * K, 8, stream);
+  bf16 *w = (bf16 *)workspace;
+  float *part = (float *)(w + (int64_t)N * K);
+  const hipError_t e = launch_values(codes, scales, w, (int64_t)N * K, bits, stream);
   if (e != hipSuccess) return e;
-  const bf16 *xp = x_scales ? xv : (const bf16 *)x;
+  const bf16 *xp = (const bf16 *)x;
   GemmArgs g{{xp, xp}, {w, w}, K, K, M, N, K, 1, 1, {(bf16 *)y, nullptr}, part, nullptr, {}};
   return launch_gemm<false, false, kStore>(g, cut_of(M, N, K, 1, 1, false), stream);
 }
