@@ -406,7 +406,7 @@ int ttfa_swiglu_bwd(const void *da, const void *saved, const void *x, const void
  * every eight consecutive products, the bits below 2^-13 of the largest: a sum is within 2^-10 of those largest
  * ones' sum (on random values 2^-19 of sum |x w|).  Which instructions a call uses goes by M, K and N alone.
  * K a multiple of 32 and N of 8, up to 2^20.  workspace: ttfa_linear_mx_workspace_bytes, or NULL where that
- * is 0.  One to four launches.
+ * is 0.  One to three launches.
  * ttfa_mx_quantize rounds rows x [M, K], `dtype`, into that format.
  */
 int ttfa_mx_quantize(const void *x, void *codes, void *scales, long long M, int K, int bits, int dtype,

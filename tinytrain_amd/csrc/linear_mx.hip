@@ -3,8 +3,8 @@
 // norm's kernel gives it.  The reference has no counterpart (its linear layers are bf16 products).
 //
 // Every value of either format is a bf16 as it stands, so with x in bf16 the products are bf16 ones with
-// fp32 sums.  With x in 8 bits the matrix unit takes both as they lie, with their scales
-// (v_mfma_scale_f32_16x16x128_f8f6f4, twice the rate, no conversions); of every eight consecutive
+// fp32 sums, of values that are formed in registers.  With x in 8 bits the matrix unit takes both as they lie, with
+// their scales (v_mfma_scale_f32_16x16x128_f8f6f4, twice the rate, no conversions); of every eight consecutive
 // products it drops the bits below 2^-13 of the largest before it adds in fp32 (fa_decode_mx.hip), so a
 // sum is off by less than 2^-10 of those largest ones' sum, on random values by 2^-19 of sum |x w|, far
 // below the 2^-9 of y's own rounding.
@@ -181,12 +181,15 @@ __global__ __launch_bounds__(64 * kRowWaves) void linear_mx_rows_kernel(
   if (m < M && n < N) *reinterpret_cast<bf16x4 *>(y + (int64_t)m * N + n) = pack4(t[0], t[1], t[2], t[3]);
 }
 
-// Many rows of x in 8 bits: tiles of TM x TN, stages of 128 k's, with the order of gemm_kernel (gemm.h): a
-// persistent workgroup, loads two stages ahead, operands read before they are needed.  128 k's of a row
-// of x are 128 bytes and of W 64 or 128, loaded as gemm.h's tiles of bf16 of that many bytes; the scales
-// of a stage, four bytes a row, go to LDS beside them.  A step is 16 rows of x by the wave's columns;
-// the operands of W stay in registers for a stage.  What a last stage has past K loads as zeros; rows of scales
-// that are no whole dwords are laid out anew first (pad_scales_kernel).
+// Many rows: tiles of TM x TN, stages of 128 k's, with the order of gemm_kernel (gemm.h): a persistent
+// workgroup, loads S stages ahead, operands read before they are needed.  128 k's of a row of x are 128 or 256
+// bytes and of W 64 or 128, loaded as gemm.h's tiles of bf16 of that many bytes; the scales of a stage, four bytes a
+// row, go to LDS beside them.  With x in 8 bits a step is 16 rows of x by the wave's columns, whose operands stay in
+// registers for a stage.  With x in bf16 it is a quarter of the stage's k's, eight of each group, for which the
+// wave's columns become bf16.  What a last stage has past K loads as zeros; rows of scales that are no whole dwords
+// are laid out anew first (pad_scales_kernel).
+// 4096 x 4096 x 12288 in 4 bits: x in 8 bits 169 us (2440 TFLOP/s), x in bf16 336 (1230); 128 rows: 25 and 29.
+// With W written out in bf16 first and tiles of that, x in bf16 took 346 and 52, and 2 N K bytes of workspace.
 struct MxArgs {
   const uint8_t *x, *x_scales, *codes, *scales;
   bf16 *out;
@@ -223,14 +226,14 @@ __device__ __forceinline__ void load_scales(const uint8_t *p, uint32_t bytes, ui
                                            (w * 64 + (threadIdx.x & 63)) * ld, 0, 0, 0);
 }
 
-template <int TM, int TN, int WM, int WN, int S, int BITS, bool PARTIAL>
+template <int TM, int TN, int WM, int WN, int S, int BITS, bool XMX, bool PARTIAL>
 __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs g) {
   constexpr int NT = 64 * WM * WN, MB = TM / WM / 16, NB = TN / WN / 16, STORES = MB * NB / (PARTIAL ? 1 : 2);
-  constexpr int WK = BITS == 4 ? 32 : 64;  // bf16's as long as 128 elements of W
-  using XL = TileLoad<TM, 64, false, NT>;
+  constexpr int XK = XMX ? 64 : 128, WK = BITS == 4 ? 32 : 64;  // bf16's as long as 128 elements of x, W
+  using XL = TileLoad<TM, XK, false, NT>;
   using WL = TileLoad<TN, WK, false, NT>;
-  static_assert((TM + TN) / 64 <= NT / 64, "a wave loads scales once a stage");
-  constexpr int XS = XL::BYTES + WL::BYTES, WS = XS + 4 * TM, STAGE = WS + 4 * TN;
+  static_assert(((XMX ? TM : 0) + TN) / 64 <= NT / 64, "a wave loads scales once a stage");
+  constexpr int XS = XL::BYTES + WL::BYTES, WS = XS + (XMX ? 4 * TM : 0), STAGE = WS + 4 * TN;
   extern __shared__ __align__(1024) char lds[];
   const int total = g.tiles.total(), all_stages = (int)((g.K + 127) / 128);
   const uint32_t sld = (uint32_t)g.sld;
@@ -245,14 +248,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
     const int first = first_stage(g.tiles, all_stages, at.part);
     const int64_t m0 = (int64_t)at.m * TM, n0 = (int64_t)at.n * TN;
     to_do = first_stage(g.tiles, all_stages, at.part + 1) - first;
-    xl.init(reinterpret_cast<const bf16 *>(g.x), g.K / 2, m0, g.M);
+    xl.init(reinterpret_cast<const bf16 *>(g.x), XMX ? g.K / 2 : g.K, m0, g.M);
     wl.init(reinterpret_cast<const bf16 *>(g.codes), g.K * BITS / 16, n0, g.N);
     xl.skip(first);
     wl.skip(first);
     left = (int)g.K - 128 * first;
-    xs = g.x_scales + m0 * sld + 4 * first;
+    if constexpr (XMX) {
+      xs = g.x_scales + m0 * sld + 4 * first;
+      xs_bytes = (uint32_t)((g.M - m0 < TM ? g.M - m0 : TM) * sld) - 4 * first;
+    }
     ws = g.scales + n0 * sld + 4 * first;
-    xs_bytes = (uint32_t)((g.M - m0 < TM ? g.M - m0 : TM) * sld) - 4 * first;
     ws_bytes = (uint32_t)((g.N - n0 < TN ? g.N - n0 : TN) * sld) - 4 * first;
   };
   next_tile();
@@ -260,15 +265,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
     if (ahead >= total) return;
     char *dst = lds + buf * STAGE;
     if (left < 128) {
-      xl.shorten(0, left / 2);
+      xl.shorten(0, XMX ? left / 2 : left);
       wl.shorten(0, left * BITS / 16);
     }
     left -= 128;
     xl.load(dst);
     wl.load(dst + XL::BYTES);
-    load_scales<TM, 0>(xs, xs_bytes, sld, dst + XS);
-    load_scales<TN, TM / 64>(ws, ws_bytes, sld, dst + WS);
-    xs += 4, ws += 4, xs_bytes -= 4, ws_bytes -= 4;
+    if constexpr (XMX) {
+      load_scales<TM, 0>(xs, xs_bytes, sld, dst + XS);
+      xs += 4, xs_bytes -= 4;
+    }
+    load_scales<TN, XMX ? TM / 64 : 0>(ws, ws_bytes, sld, dst + WS);
+    ws += 4, ws_bytes -= 4;
     if (--to_do == 0) {
       ahead += gridDim.x;
       if (ahead < total) next_tile();
@@ -277,23 +285,30 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
 
   const int wave = wave_id(), wm = wave / WN, wn = wave % WN, lane = threadIdx.x & 63;
   const int i16 = lane & 15, q = lane >> 4;
-  // offsets in a stage of this lane's pieces of block 0 (16 rows on: the same swizzle)
+  // Offsets in a stage of this lane's pieces of block 0 (16 rows on: the same swizzle).  With x in 8 bits a second
+  // piece is four chunks on: that bit flipped.  With x in bf16 lane q has group q of W (e4m3: its second half in the
+  // next chunk), and of x the same 32 elements, four chunks.
   const int xrow = wm * (TM / WM) + i16, wrow = wn * (TN / WN) + i16;
-  // the second piece, four chunks on: that bit flipped
-  const int x0 = xrow * 128 + ((q ^ XL::swizzle(xrow)) << 4);
-  const int w0 = XL::BYTES + wrow * (2 * WK) + ((q ^ WL::swizzle(wrow)) << 4);
-  u32x4 xf[2][2], wf[NB][BITS / 4];
+  const int x0 = xrow * (2 * XK) + (((XMX ? q : 4 * q) ^ XL::swizzle(xrow)) << 4);
+  const int w0 = XL::BYTES + wrow * (2 * WK) + (((XMX || BITS == 4 ? q : 2 * q) ^ WL::swizzle(wrow)) << 4);
+  u32x4 xf[2][XMX ? 2 : MB], wf[NB][BITS / 4];
   uint32_t sx[2], sw[NB];
+  // block b (x in bf16: chunk b of all blocks)
   auto read_x = [&](int buf, int b, int into) {
     const char *from = lds + buf * STAGE;
-    xf[into][0] = *reinterpret_cast<const u32x4 *>(from + x0 + b * 2048);
-    xf[into][1] = *reinterpret_cast<const u32x4 *>(from + (x0 ^ 64) + b * 2048);
-    sx[into] = *reinterpret_cast<const uint8_t *>(from + XS + 4 * xrow + q + b * 64);
+    if constexpr (XMX) {
+      xf[into][0] = *reinterpret_cast<const u32x4 *>(from + x0 + b * 2048);
+      xf[into][1] = *reinterpret_cast<const u32x4 *>(from + (x0 ^ 64) + b * 2048);
+      sx[into] = *reinterpret_cast<const uint8_t *>(from + XS + 4 * xrow + q + b * 64);
+    } else {
+#pragma unroll
+      for (int i = 0; i < MB; ++i) xf[into][i] = *reinterpret_cast<const u32x4 *>(from + (x0 ^ (b << 4)) + i * 4096);
+    }
   };
   auto read_w = [&](int buf, int c) {
     const char *from = lds + buf * STAGE;
     wf[c][0] = *reinterpret_cast<const u32x4 *>(from + w0 + c * (32 * WK));
-    if constexpr (BITS == 8) wf[c][1] = *reinterpret_cast<const u32x4 *>(from + (w0 ^ 64) + c * (32 * WK));
+    if constexpr (BITS == 8) wf[c][1] = *reinterpret_cast<const u32x4 *>(from + (w0 ^ (XMX ? 64 : 16)) + c * (32 * WK));
     sw[c] = *reinterpret_cast<const uint8_t *>(from + WS + 4 * wrow + q + c * 64);
   };
   auto operand = [](const u32x4 *c, int n) {
@@ -303,6 +318,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
       if (i < n) v[i] = (int)c[i / 4][i % 4];
     return v;
   };
+  // x in bf16: elements 8 j .. 8 j + 7 of the lane's group of block c
+  auto values = [&](int c, int j) {
+    const u32x4 &v = wf[c][BITS == 4 ? 0 : j / 2];
+    const u32x2 codes = BITS == 4 ? u32x2{v[j], 0u} : u32x2{v[2 * (j % 2)], v[2 * (j % 2) + 1]};
+    return mx_values8<BITS>(codes, __uint_as_float(sw[c] << 23));
+  };
+  constexpr int XSTEPS = XMX ? MB : 4;  // of a stage: blocks of rows, or chunks of k's
 
   constexpr int LOADS = XL::LOADS + WL::LOADS;  // and one of scales in some waves: not counted
 #pragma unroll
@@ -313,6 +335,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
   for (int c = 0; c < NB; ++c) read_w(0, c);
   read_x(0, 0, 0);
   int buf = 0;
+  bf16x8 wv[NB];
   for (int i = blockIdx.x; i < total; i += gridDim.x) {
     const Tile t = tile_at(g.tiles, i);
     const int64_t m0 = (int64_t)t.m * TM, n0 = (int64_t)t.n * TN;
@@ -320,8 +343,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
     f32x4 acc[MB][NB] = {};
     for (int st = 0; st < stages; ++st) {
 #pragma unroll
-      for (int b = 0; b < MB; ++b) {
-        if (b + 1 < MB) {
+      for (int b = 0; b < XSTEPS; ++b) {
+        if constexpr (!XMX)
+#pragma unroll
+          for (int c = 0; c < NB; ++c) wv[c] = values(c, b);
+        if (b + 1 < XSTEPS) {
           read_x(buf, b + 1, (b + 1) & 1);
         } else {
           if (ahead >= total) wait_and_meet<0>();
@@ -331,21 +357,39 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
           buf = buf + 1 == S ? 0 : buf + 1;
           read_x(buf, 0, (b + 1) & 1);  // after the last stage: values that nothing uses
         }
+        if constexpr (XMX) {
 #pragma unroll
-        for (int c = 0; c < NB; ++c) {
-          acc[b][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-              operand(wf[c], BITS), operand(xf[b & 1], 8), acc[b][c], BITS == 4 ? 4 : 0, 0, 0, (int)sw[c], 0,
-              (int)sx[b & 1]);
-          if (b + 1 == MB) {
-            read_w(buf, c);  // into the registers that the product has read
-            __builtin_amdgcn_sched_barrier(0);
+          for (int c = 0; c < NB; ++c) {
+            acc[b][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                operand(wf[c], BITS), operand(xf[b & 1], 8), acc[b][c], BITS == 4 ? 4 : 0, 0, 0, (int)sw[c], 0,
+                (int)sx[b & 1]);
+            if (b + 1 == XSTEPS) {
+              read_w(buf, c);  // into the registers that the product has read
+              __builtin_amdgcn_sched_barrier(0);
+            }
           }
-        }
-        // The products of the step before are done in this one: without a use they would all be moved behind the
-        // last step's wait, and every operand of the stage be held until then.
-        if (b > 0)
+        } else {
+          if (b + 1 == XSTEPS)
 #pragma unroll
-          for (int c = 0; c < NB; ++c) asm volatile("" : "+v"(acc[b - 1][c]));
+            for (int c = 0; c < NB; ++c) read_w(buf, c);
+#pragma unroll
+          for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int c = 0; c < NB; ++c)
+              acc[i][c] = mfma16(wv[c], __builtin_bit_cast(bf16x8, xf[b & 1][i]), acc[i][c]);
+        }
+        // The products of the step before (of this one, with x in bf16) are done here: without a use they would all
+        // be moved behind the last step's wait, and every operand of the stage be held until then.
+        if constexpr (XMX) {
+          if (b > 0)
+#pragma unroll
+            for (int c = 0; c < NB; ++c) asm volatile("" : "+v"(acc[b - 1][c]));
+        } else if (b + 1 < XSTEPS) {
+#pragma unroll
+          for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int c = 0; c < NB; ++c) asm volatile("" : "+v"(acc[i][c]));
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -386,21 +430,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_mx_tile_kernel(MxArgs 
   }
 }
 
-// Values of quantised rows in bf16, 8 a lane.
-template <int BITS>
-__global__ __launch_bounds__(256) void mx_values_kernel(const uint8_t *__restrict__ codes,
-                                                        const uint8_t *__restrict__ scales, bf16 *__restrict__ out,
-                                                        int64_t lanes) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < lanes; i += (int64_t)gridDim.x * 256) {
-    u32x2 c{};
-    if constexpr (BITS == 4) c[0] = reinterpret_cast<const uint32_t *>(codes)[i];
-    else c = reinterpret_cast<const u32x2 *>(codes)[i];
-    reinterpret_cast<bf16x8 *>(out)[i] = mx_values8<BITS>(c, __uint_as_float((uint32_t)scales[i / 4] << 23));
-  }
-}
-
-constexpr int kFewRows = 64;  // of linear_mx_rows_kernel at most
-
 // f(bits, whether x is quantised) as compile-time values
 template <class F>
 hipError_t by_types(int bits, bool xmx, F f) {
@@ -409,8 +438,8 @@ hipError_t by_types(int bits, bool xmx, F f) {
   return xmx ? f(integral_constant<int, 8>{}, std::true_type{}) : f(integral_constant<int, 8>{}, std::false_type{});
 }
 
-// f(blocks of 16 rows of x, of 16 columns of W) for M rows: as many columns a workgroup as leave 256 of them,
-// up to eight blocks.
+// f(blocks of 16 rows of x, of 16 columns of W) for M rows: as many columns a workgroup as leave 256 of them
+// (more than 32 rows come with at most 8192 columns: few_rows).
 template <class F>
 hipError_t by_blocks(int M, int N, F f) {
   using std::integral_constant;
@@ -430,33 +459,38 @@ hipError_t by_blocks(int M, int N, F f) {
   return go(integral_constant<int, 4>{}, integral_constant<int, 2>{});
 }
 
-}  // namespace
+// Whether a call takes the kernel for few rows.  Measured at the borders, us (rows, tiles), K 4096, x and W in 8 and 4
+// bits: N 8192, 64 rows: 15.1, 18.2; N 12288, 32 rows: 11.3, 18.6; 48 rows: 21.8, 20.0; N 20480, 16 rows: 19.5, 20.9;
+// 24 rows: 22.7, 21.6.  x in bf16: 21.4, 20.5; 16.3, 23.6; 33.3, 24.5; 23.8, 27.0; 32 rows: 33.8, 28.1; 768 x 2304, 64
+// rows: 5.4, 9.1.  W in 8 bits, x in 8: 18.0, 17.3; 15.6, 20.6; 28.1, 21.8; 29.4, 25.9.
+bool few_rows(int M, int N) { return M <= (N <= 8192 ? 64 : N <= 16384 ? 32 : 16); }
 
-namespace {
-
-// kRows: the kernel for few rows; kTiles: tiles of quantised operands; kValues: tiles of bf16 values, which are
-// written to the workspace first.  Measured at the borders, us, x in 8 bits, W in 4 (8): K 4096, N 8192, 64 rows:
-// kRows 15.1 (18.0), kTiles 18.2 (17.3); N 12288, 32 rows: 11.3 (15.6), 18.6 (20.6); 48 rows: 21.8 (28.1), 20.0
-// (21.8); N 20480, 16 rows: 19.5 (29.4), 20.9 (25.9); 24 rows: 22.7 (33.9), 21.6 (26.8).  x in bf16, N 12288, 64
-// rows: kRows 40.9, kValues 47.9.
-enum Path { kRows, kTiles, kValues };
-
-Path path_of(int M, int K, int N, bool x_quantised) {
-  if (M <= (!x_quantised || N <= 8192 ? kFewRows : N <= 16384 ? 32 : 16)) return kRows;
-  return x_quantised ? kTiles : kValues;
+// With x in 8 bits 128 k's take the time of 64 in bf16.  With x in bf16 (tiles of 128 x 256: wide, or 128 x 128) they
+// take 1.6 and 0.95 us.
+Cut mx_cut(int M, int K, int N, bool x_quantised) {
+  if (x_quantised) return cut_of(M, N, K / 2, 1, 1, false);
+  const int64_t stages = (K + 127) / 128;
+  Cut best{true, 1, false};
+  double least = 1e30;
+  for (int wide = 1; wide >= 0; --wide)
+    for (int s = 1; s <= 32 && s <= stages; ++s) {
+      if (s > 1 && (double)s * M * N > kMostPartFloats) break;
+      const int64_t n = tiles_of(M, N, 128, wide ? 256 : 128) * s;
+      double t = (double)((n + 255) / 256) * (wide ? 1.6 : 0.95) * (double)((stages + s - 1) / s + 3);
+      if (s > 1) t += 4 + (double)s * M * N * 8 / 4e6;
+      if (t < least) least = t, best = Cut{wide != 0, s, false};
+    }
+  return best;
 }
-
-// 128 k's in 8 bits take the time of 64 in bf16.
-Cut mx_cut(int M, int K, int N) { return cut_of(M, N, K / 2, 1, 1, false); }
 
 // Bytes of the scales of `rows` rows in whole dwords, to where the next piece of a workspace begins.
 int64_t padded_scales(int64_t rows, int K) { return (rows * ((K + 127) / 128 * 4) + 15) / 16 * 16; }
 
-template <int TM, int WM, int WN, int S, int BITS, bool PARTIAL>
+template <int TM, int TN, int WM, int WN, int S, int BITS, bool XMX, bool PARTIAL>
 hipError_t launch_mx_tiles(MxArgs g, int splits, hipStream_t stream) {
-  constexpr int lds = S * (TM * 128 + TM * 16 * BITS + 8 * TM);
-  constexpr auto kernel = linear_mx_tile_kernel<TM, TM, WM, WN, S, BITS, PARTIAL>;
-  g.tiles = Tiles{splits, 1, (int)((g.M + TM - 1) / TM), (int)((g.N + TM - 1) / TM)};
+  constexpr int lds = S * (TM * (XMX ? 132 : 256) + TN * (16 * BITS + 4));
+  constexpr auto kernel = linear_mx_tile_kernel<TM, TN, WM, WN, S, BITS, XMX, PARTIAL>;
+  g.tiles = Tiles{splits, 1, (int)((g.M + TM - 1) / TM), (int)((g.N + TN - 1) / TN)};
   if constexpr (lds > 65536) {
     const hipError_t e = allow_lds<kernel>(lds);
     if (e != hipSuccess) return e;
@@ -466,77 +500,60 @@ hipError_t launch_mx_tiles(MxArgs g, int splits, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <int BITS, bool PARTIAL>
+template <int BITS, bool XMX, bool PARTIAL>
 hipError_t launch_mx_cut(const MxArgs &g, const Cut &c, hipStream_t stream) {
-  if (c.wide) return launch_mx_tiles<256, 2, 4, 2, BITS, PARTIAL>(g, c.splits, stream);
-  return c.deep ? launch_mx_tiles<128, 4, 2, 4, BITS, PARTIAL>(g, c.splits, stream)
-                : launch_mx_tiles<128, 2, 2, 2, BITS, PARTIAL>(g, c.splits, stream);
+  if constexpr (!XMX)
+    return c.wide ? launch_mx_tiles<128, 256, 2, 4, BITS == 4 ? 3 : 2, BITS, false, PARTIAL>(g, c.splits, stream)
+                  : launch_mx_tiles<128, 128, 4, 2, 3, BITS, false, PARTIAL>(g, c.splits, stream);
+  else if (c.wide) return launch_mx_tiles<256, 256, 2, 4, 2, BITS, true, PARTIAL>(g, c.splits, stream);
+  else if (c.deep) return launch_mx_tiles<128, 128, 4, 2, 4, BITS, true, PARTIAL>(g, c.splits, stream);
+  else return launch_mx_tiles<128, 128, 2, 2, 2, BITS, true, PARTIAL>(g, c.splits, stream);
 }
 
-template <int BITS>
+template <int BITS, bool XMX>
 hipError_t launch_mx(const MxArgs &g, hipStream_t stream) {
-  const Cut c = mx_cut((int)g.M, (int)g.K, (int)g.N);
-  if (c.splits == 1) return launch_mx_cut<BITS, false>(g, c, stream);
-  const hipError_t e = launch_mx_cut<BITS, true>(g, c, stream);
+  const Cut c = mx_cut((int)g.M, (int)g.K, (int)g.N, XMX);
+  if (c.splits == 1) return launch_mx_cut<BITS, XMX, false>(g, c, stream);
+  const hipError_t e = launch_mx_cut<BITS, XMX, true>(g, c, stream);
   return e != hipSuccess ? e : launch_sum_parts(g.part, g.out, nullptr, c.splits, g.M * g.N / 8, g.M * g.N / 8, stream);
-}
-
-hipError_t launch_values(const void *codes, const void *scales, bf16 *out, int64_t elements, int bits,
-                         hipStream_t stream) {
-  const int64_t lanes = elements / 8;
-  const dim3 grid((unsigned)std::min<int64_t>((lanes + 255) / 256, 1 << 20)), block(256);
-  const uint8_t *c = (const uint8_t *)codes, *s = (const uint8_t *)scales;
-  if (bits == 4) mx_values_kernel<4><<<grid, block, 0, stream>>>(c, s, out, lanes);
-  else mx_values_kernel<8><<<grid, block, 0, stream>>>(c, s, out, lanes);
-  return hipGetLastError();
 }
 
 }  // namespace
 
 int64_t linear_mx_workspace(int M, int K, int N, bool x_quantised) {
-  switch (path_of(M, K, N, x_quantised)) {
-    case kRows: return 0;
-    case kTiles:
-      return (K % 128 ? padded_scales(M, K) + padded_scales(N, K) : 0) + part_bytes(mx_cut(M, K, N), M, N, 1);
-    default: return 2 * (int64_t)N * K + part_bytes(cut_of(M, N, K, 1, 1, false), M, N, 1);
-  }
+  if (few_rows(M, N)) return 0;
+  return (K % 128 ? padded_scales(x_quantised ? M : 0, K) + padded_scales(N, K) : 0) +
+         part_bytes(mx_cut(M, K, N, x_quantised), M, N, 1);
 }
 
 hipError_t launch_linear_mx(const void *x, const void *x_scales, const void *codes, const void *scales,
                             void *y, void *workspace, int M, int K, int N, int bits, hipStream_t stream) {
-  const Path path = path_of(M, K, N, x_scales != nullptr);
-  if (path == kRows)
+  MxArgs g{(const uint8_t *)x, (const uint8_t *)x_scales, (const uint8_t *)codes, (const uint8_t *)scales,
+           (bf16 *)y, (float *)workspace, M, N, K, K / 32, {}};
+  if (few_rows(M, N))
     return by_types(bits, x_scales != nullptr, [&](auto b, auto xmx) {
       return by_blocks(M, N, [&](auto mb, auto nb) {
         constexpr int NB = decltype(nb)::value;
         linear_mx_rows_kernel<decltype(b)::value, decltype(xmx)::value, decltype(mb)::value, NB>
             <<<dim3((N + 16 * NB - 1) / (16 * NB)), dim3(64 * kRowWaves), 0, stream>>>(
-                x, (const uint8_t *)x_scales, (const uint8_t *)codes, (const uint8_t *)scales, (bf16 *)y, M, K, N);
+                x, g.x_scales, g.codes, g.scales, g.out, M, K, N);
         return hipGetLastError();
       });
     });
-  if (path == kTiles) {
-    MxArgs g{(const uint8_t *)x, (const uint8_t *)x_scales, (const uint8_t *)codes, (const uint8_t *)scales,
-             (bf16 *)y, (float *)workspace, M, N, K, K / 32, {}};
-    if (K % 128) {
-      uint8_t *xp = (uint8_t *)workspace, *wp = xp + padded_scales(M, K);
-      const int dwords = (K + 127) / 128;
-      const int64_t rows = (int64_t)M + N, blocks = (rows * dwords + 255) / 256;
-      pad_scales_kernel<<<dim3((unsigned)std::min<int64_t>(blocks, 1 << 20)), dim3(256), 0, stream>>>(
-          g.x_scales, g.scales, (uint32_t *)xp, (uint32_t *)wp, K / 32, dwords, M, rows);
-      const hipError_t e = hipGetLastError();
-      if (e != hipSuccess) return e;
-      g.x_scales = xp, g.scales = wp, g.sld = 4 * dwords, g.part = (float *)(wp + padded_scales(N, K));
-    }
-    return bits == 4 ? launch_mx<4>(g, stream) : launch_mx<8>(g, stream);
+  if (K % 128) {
+    const int64_t x_rows = x_scales ? M : 0, rows = x_rows + N;
+    uint8_t *xp = (uint8_t *)workspace, *wp = xp + padded_scales(x_rows, K);
+    const int dwords = (K + 127) / 128;
+    const int64_t blocks = (rows * dwords + 255) / 256;
+    pad_scales_kernel<<<dim3((unsigned)std::min<int64_t>(blocks, 1 << 20)), dim3(256), 0, stream>>>(
+        g.x_scales, g.scales, (uint32_t *)xp, (uint32_t *)wp, K / 32, dwords, x_rows, rows);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    g.x_scales = xp, g.scales = wp, g.sld = 4 * dwords, g.part = (float *)(wp + padded_scales(N, K));
   }
-  bf16 *w = (bf16 *)workspace;
-  float *part = (float *)(w + (int64_t)N * K);
-  const hipError_t e = launch_values(codes, scales, w, (int64_t)N * K, bits, stream);
-  if (e != hipSuccess) return e;
-  const bf16 *xp = (const bf16 *)x;
-  GemmArgs g{{xp, xp}, {w, w}, K, K, M, N, K, 1, 1, {(bf16 *)y, nullptr}, part, nullptr, {}};
-  return launch_gemm<false, false, kStore>(g, cut_of(M, N, K, 1, 1, false), stream);
+  return by_types(bits, x_scales != nullptr, [&](auto b, auto xmx) {
+    return launch_mx<decltype(b)::value, decltype(xmx)::value>(g, stream);
+  });
 }
 
 }  // namespace ttfa
