@@ -506,7 +506,8 @@ hipError_t launch_mx_cut(const MxArgs &g, const Cut &c, hipStream_t stream) {
     return c.wide ? launch_mx_tiles<128, 256, 2, 4, BITS == 4 ? 3 : 2, BITS, false, PARTIAL>(g, c.splits, stream)
                   : launch_mx_tiles<128, 128, 4, 2, 3, BITS, false, PARTIAL>(g, c.splits, stream);
   else if (c.wide) return launch_mx_tiles<256, 256, 2, 4, 2, BITS, true, PARTIAL>(g, c.splits, stream);
-  else if (c.deep) return launch_mx_tiles<128, 128, 4, 2, 4, BITS, true, PARTIAL>(g, c.splits, stream);
+  else if (c.deep)  // eight waves: 256 x 4096 x 12288 in 4 bits 28.7 us, four 26.5
+    return launch_mx_tiles<128, 128, 2, 2, 4, BITS, true, PARTIAL>(g, c.splits, stream);
   else return launch_mx_tiles<128, 128, 2, 2, 2, BITS, true, PARTIAL>(g, c.splits, stream);
 }
 
