@@ -625,3 +625,40 @@ def test_function_transforms():
         with pytest.raises(RuntimeError):
             g, = torch.autograd.grad(y, x, torch.ones_like(y).requires_grad_(), create_graph=True)
             torch.autograd.grad(g.sum(), x)
+
+
+@pytest.mark.parametrize("x8", [False, True])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("M, K, N", [(70, 160, 264), (300, 1152, 520), (129, 4128, 136), (65, 2080, 776)])
+def test_linear_mx_workspace_ends_where_it_says(M, K, N, bits, x8):
+    """Through the C ABI with exactly the workspace that is asked for: nothing behind it, nor behind y, is written."""
+    lib = _lib.load()
+    x, xs = _rand(M, K, seed=1, dtype=BF), None
+    codes, scales = mx_quantize(_rand(N, K, seed=2, scale=1 / math.sqrt(K)), bits)
+    if x8:
+        x, xs = mx_quantize(x, 8)
+    n = lib.ttfa_linear_mx_workspace_bytes(M, K, N, bits, int(x8))
+    ws = torch.full((n + 4096,), 7, dtype=torch.uint8, device="cuda")
+    y = torch.full((M + 3, N), 7.0, dtype=BF, device="cuda")
+    _lib.check(lib.ttfa_linear_mx(x.data_ptr(), None if xs is None else xs.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+                                  y.data_ptr(), ws.data_ptr(), M, K, N, bits, torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert (ws[n:] == 7).all() and (y[M:] == 7).all()
+    assert torch.equal(y[:M], linear_mx(x, codes, scales, xs))
+
+
+@pytest.mark.parametrize("M, K, N", [(70, 160, 264), (2600, 768, 1040), (999, 1000, 2600), (100, 2056, 72)])
+def test_swiglu_workspace_ends_where_it_says(M, K, N):
+    lib, stream = _lib.load(), torch.cuda.current_stream().cuda_stream
+    x, wg, wu = _rand(M, K, seed=1, dtype=BF), _rand(N, K, seed=2, dtype=BF), _rand(N, K, seed=3, dtype=BF)
+    da = _rand(M, N, seed=4, dtype=BF)
+    a, saved = swiglu_fwd(x, wg, wu, True)
+    n = lib.ttfa_swiglu_workspace_bytes(M, K, N)
+    ws = torch.full((n + 4096,), 7, dtype=torch.uint8, device="cuda")
+    dx, dg, du = torch.empty_like(x), torch.empty_like(wg), torch.empty_like(wu)
+    _lib.check(lib.ttfa_swiglu_bwd(da.data_ptr(), saved.data_ptr(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), dx.data_ptr(),
+                                   dg.data_ptr(), du.data_ptr(), ws.data_ptr(), M, K, N, stream))
+    torch.cuda.synchronize()
+    assert (ws[n:] == 7).all()
+    for p, q in zip((dx, dg, du), swiglu_bwd(da, saved, x, wg, wu, True, True)):
+        assert torch.equal(p, q)
