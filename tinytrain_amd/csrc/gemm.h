@@ -507,8 +507,10 @@ int64_t tiles_of(int64_t M, int64_t N, int tm, int tn) { return (M + tm - 1) / t
 constexpr double kMostPartFloats = 1 << 26;  // 256 MB, what the last-level cache holds
 
 // The cut that is estimated to take least time, in microseconds on 256 CUs: a stage of 64 k's of a wide
-// tile takes 1.5, of a narrow one 0.6 alone on its CU and 1.0 beside another; 3 stages more for a tile's
-// start and end; parts go out and in at 4 TB/s, with a launch of 4 us.
+// tile takes 1.5, of a narrow one 0.6 alone on its CU and 0.97 beside another; 3 stages more for a tile's
+// start and end; parts go out and in at 4 TB/s, with a launch of 4 us.  (Whole rounds of narrow tiles take 0.9 to
+// 1.06 a stage; 0.97 decides the near draws as they were measured: forward 2048 x 2048 x 6144 wide 110, narrow 101;
+// 4096 x 1024 x 2816: 58, 52; dx of 4096 x 2048 x 6144: wide in two parts 232 with the kernel before it, narrow 262.)
 Cut cut_of(int64_t M, int64_t N, int64_t K, int segs, int z, bool dual) {
   const int64_t stages = (K + 63) / 64 * segs;
   Cut best{true, 1, false};
@@ -520,7 +522,7 @@ Cut cut_of(int64_t M, int64_t N, int64_t K, int segs, int z, bool dual) {
       const int64_t n = tiles * s;
       const double len = (double)((stages + s - 1) / s) + 3;
       const bool deep = !wide && n <= 256;
-      double t = len * (wide ? (double)((n + 255) / 256) * 1.5 : deep ? 0.6 : (double)((n + 511) / 512) * 1.0);
+      double t = len * (wide ? (double)((n + 255) / 256) * 1.5 : deep ? 0.6 : (double)((n + 511) / 512) * 0.97);
       if (s > 1) t += 4 + (double)s * z * M * N * 8 / 4e6;
       if (t < least) least = t, best = Cut{wide != 0, s, deep};
     }
