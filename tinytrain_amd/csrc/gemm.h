@@ -21,6 +21,7 @@
 
 #include "fa_bwd.h"  // allow_lds
 #include "fa_common.h"
+#include "product_cut.h"
 
 namespace ttfa {
 
@@ -493,44 +494,6 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(const float *__restrict_
   reinterpret_cast<bf16x8 *>(i < n0 ? out0 : out1)[i < n0 ? i : i - n0] =
       bf16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
 }
-
-// How a product is cut: tiles of 256 x 256 (one workgroup a CU) or 128 x 128 (two, or one with four stages
-// in LDS where there are no more than CUs: deep), and parts of the contraction that sum_parts_kernel joins.
-struct Cut {
-  bool wide;
-  int splits;
-  bool deep;
-};
-
-int64_t tiles_of(int64_t M, int64_t N, int tm, int tn) { return (M + tm - 1) / tm * ((N + tn - 1) / tn); }
-
-constexpr double kMostPartFloats = 1 << 26;  // 256 MB, what the last-level cache holds
-
-// The cut that is estimated to take least time, in microseconds on 256 CUs: a stage of 64 k's of a wide
-// tile takes 1.5, of a narrow one 0.6 alone on its CU and 0.97 beside another; 3 stages more for a tile's
-// start and end; parts go out and in at 4 TB/s, with a launch of 4 us.  (Whole rounds of narrow tiles take 0.9 to
-// 1.06 a stage; 0.97 decides the near draws as they were measured: forward 2048 x 2048 x 6144 wide 110, narrow 101;
-// 4096 x 1024 x 2816: 58, 52; dx of 4096 x 2048 x 6144: wide in two parts 232 with the kernel before it, narrow 262.)
-Cut cut_of(int64_t M, int64_t N, int64_t K, int segs, int z, bool dual) {
-  const int64_t stages = (K + 63) / 64 * segs;
-  Cut best{true, 1, false};
-  double least = 1e30;
-  for (int wide = 1; wide >= 0; --wide) {
-    const int64_t tiles = z * (wide ? tiles_of(M, N, 256, dual ? 128 : 256) : tiles_of(M, N, 128, dual ? 64 : 128));
-    for (int s = 1; s <= (dual ? 1 : 32) && s <= stages; ++s) {
-      if (s > 1 && (double)s * z * M * N > kMostPartFloats) break;
-      const int64_t n = tiles * s;
-      const double len = (double)((stages + s - 1) / s) + 3;
-      const bool deep = !wide && n <= 256;
-      double t = len * (wide ? (double)((n + 255) / 256) * 1.5 : deep ? 0.6 : (double)((n + 511) / 512) * 0.97);
-      if (s > 1) t += 4 + (double)s * z * M * N * 8 / 4e6;
-      if (t < least) least = t, best = Cut{wide != 0, s, deep};
-    }
-  }
-  return best;
-}
-
-int64_t part_bytes(const Cut &c, int64_t M, int64_t N, int z) { return c.splits > 1 ? 4 * c.splits * z * M * N : 0; }
 
 template <bool XTR, bool WTR, Epilogue E, int TM, int WM, int WN, int S>
 hipError_t launch_tiles(GemmArgs g, int splits, hipStream_t stream) {

@@ -439,7 +439,7 @@ hipError_t by_types(int bits, bool xmx, F f) {
 }
 
 // f(blocks of 16 rows of x, of 16 columns of W) for M rows: as many columns a workgroup as leave 256 of them
-// (more than 32 rows come with at most 8192 columns: few_rows).
+// (more than 32 rows come with at most 8192 columns: linear_mx_few_rows).
 template <class F>
 hipError_t by_blocks(int M, int N, F f) {
   using std::integral_constant;
@@ -457,30 +457,6 @@ hipError_t by_blocks(int M, int N, F f) {
   if (M <= 32) return go(integral_constant<int, 2>{}, integral_constant<int, 4>{});
   if (M <= 48) return go(integral_constant<int, 3>{}, integral_constant<int, 2>{});
   return go(integral_constant<int, 4>{}, integral_constant<int, 2>{});
-}
-
-// Whether a call takes the kernel for few rows.  Measured at the borders, us (rows, tiles), K 4096, x and W in 8 and 4
-// bits: N 8192, 64 rows: 15.1, 18.2; N 12288, 32 rows: 11.3, 18.6; 48 rows: 21.8, 20.0; N 20480, 16 rows: 19.5, 20.9;
-// 24 rows: 22.7, 21.6.  x in bf16: 21.4, 20.5; 16.3, 23.6; 33.3, 24.5; 23.8, 27.0; 32 rows: 33.8, 28.1; 768 x 2304, 64
-// rows: 5.4, 9.1.  W in 8 bits, x in 8: 18.0, 17.3; 15.6, 20.6; 28.1, 21.8; 29.4, 25.9.
-bool few_rows(int M, int N) { return M <= (N <= 8192 ? 64 : N <= 16384 ? 32 : 16); }
-
-// With x in 8 bits 128 k's take the time of 64 in bf16.  With x in bf16 (tiles of 128 x 256: wide, or 128 x 128) they
-// take 1.6 and 0.95 us.
-Cut mx_cut(int M, int K, int N, bool x_quantised) {
-  if (x_quantised) return cut_of(M, N, K / 2, 1, 1, false);
-  const int64_t stages = (K + 127) / 128;
-  Cut best{true, 1, false};
-  double least = 1e30;
-  for (int wide = 1; wide >= 0; --wide)
-    for (int s = 1; s <= 32 && s <= stages; ++s) {
-      if (s > 1 && (double)s * M * N > kMostPartFloats) break;
-      const int64_t n = tiles_of(M, N, 128, wide ? 256 : 128) * s;
-      double t = (double)((n + 255) / 256) * (wide ? 1.6 : 0.95) * (double)((stages + s - 1) / s + 3);
-      if (s > 1) t += 4 + (double)s * M * N * 8 / 4e6;
-      if (t < least) least = t, best = Cut{wide != 0, s, false};
-    }
-  return best;
 }
 
 // Bytes of the scales of `rows` rows in whole dwords, to where the next piece of a workspace begins.
@@ -522,7 +498,7 @@ hipError_t launch_mx(const MxArgs &g, hipStream_t stream) {
 }  // namespace
 
 int64_t linear_mx_workspace(int M, int K, int N, bool x_quantised) {
-  if (few_rows(M, N)) return 0;
+  if (linear_mx_few_rows(M, N)) return 0;
   return (K % 128 ? padded_scales(x_quantised ? M : 0, K) + padded_scales(N, K) : 0) +
          part_bytes(mx_cut(M, K, N, x_quantised), M, N, 1);
 }
@@ -531,7 +507,7 @@ hipError_t launch_linear_mx(const void *x, const void *x_scales, const void *cod
                             void *y, void *workspace, int M, int K, int N, int bits, hipStream_t stream) {
   MxArgs g{(const uint8_t *)x, (const uint8_t *)x_scales, (const uint8_t *)codes, (const uint8_t *)scales,
            (bf16 *)y, (float *)workspace, M, N, K, K / 32, {}};
-  if (few_rows(M, N))
+  if (linear_mx_few_rows(M, N))
     return by_types(bits, x_scales != nullptr, [&](auto b, auto xmx) {
       return by_blocks(M, N, [&](auto mb, auto nb) {
         constexpr int NB = decltype(nb)::value;

@@ -127,12 +127,6 @@ __global__ __launch_bounds__(256) void swiglu_grad_kernel(const bf16 *__restrict
   }
 }
 
-// Rows of x up to which the kernel above is faster than tiles (us, K x N: rows, tiles).  768 x 2304, 64 rows: 7.2,
-// 11.2; 2048 x 6144: 20.7, 22.0; 4096 x 8192: 39.6, 39.2.  More columns give a tile to each CU, and reading x again
-// for every 16 of them counts: 4096 x 12288, 1 row: 36.7, 41.1; 16: 45.3, 42.0; 32: 52.7, 44.5; 2048 x 12288, 16:
-// 23.9, 24.0.
-bool few_rows(int M, int N) { return M <= (N <= 8192 ? 64 : 16); }
-
 const bf16 *in(const void *p) { return static_cast<const bf16 *>(p); }
 
 }  // namespace
@@ -141,7 +135,7 @@ int64_t swiglu_saved_bytes(int M, int N) { return 5ll * M * N; }
 
 hipError_t launch_swiglu_fwd(const void *x, const void *w_gate, const void *w_up, void *a, void *saved, int M,
                              int K, int N, hipStream_t stream) {
-  if (few_rows(M, N)) {
+  if (swiglu_few_rows(M, N)) {
     auto go = [&](auto kernel, int columns) {
       kernel<<<dim3((N + columns - 1) / columns), dim3(64 * kRowWaves), 0, stream>>>(
           in(x), in(w_gate), in(w_up), (bf16 *)a, (uint8_t *)saved, M, K, N);
