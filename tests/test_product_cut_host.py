@@ -8,6 +8,7 @@ import subprocess
 import pytest
 
 import test_linear_mx_tiles_gpu as linear
+import test_swiglu_tiles_gpu as swiglu
 from tinytrain_amd import build as B
 
 SOURCE = """
@@ -16,6 +17,11 @@ extern "C" void mx_cut(int M, int K, int N, int x_quantised, int *out) {
   const ttfa::Cut c = ttfa::mx_cut(M, K, N, x_quantised != 0);
   out[0] = c.wide, out[1] = c.splits, out[2] = c.deep, out[3] = ttfa::linear_mx_few_rows(M, N);
 }
+extern "C" void cut_of(int M, int N, int K, int segs, int z, int dual, int *out) {
+  const ttfa::Cut c = ttfa::cut_of(M, N, K, segs, z, dual != 0);
+  out[0] = c.wide, out[1] = c.splits, out[2] = c.deep;
+}
+extern "C" int swiglu_few_rows(int M, int N) { return ttfa::swiglu_few_rows(M, N); }
 """
 
 
@@ -59,4 +65,31 @@ def test_linear_mx_sizes_take_the_tiles_that_they_name(rules):
     assert _kinds(bf) == {k + p for k in ("wide", "narrow") for p in ("", "/")}
     for found, slots in ((x8, {"wide": 256, "two": 512}), (bf, {"wide": 256, "narrow": 256})):
         for kind, n in slots.items():
+            assert any(name.startswith(kind) and items > n for name, items in found), kind
+
+
+def _product(rules, M, N, K, segs, z, dual):
+    c = (ctypes.c_int * 3)()
+    rules.cut_of(M, N, K, segs, z, int(dual), c)
+    wide, splits, deep = c
+    t = 256 if wide else 128
+    return _named("wide" if wide else "deep" if deep else "two", t, t // 2 if dual else t, M, N, splits, z)
+
+
+def _swiglu(rules, M, K, N):
+    """Tiles of the forward, of dx and of the weights' gradients."""
+    assert not rules.swiglu_few_rows(M, N)
+    return (_product(rules, M, N, K, 1, 1, True), _product(rules, M, K, N, 2, 1, False),
+            _product(rules, N, K, M, 1, 2, False))
+
+
+def test_swiglu_sizes_take_the_tiles_that_they_name(rules):
+    for size, want in swiglu.CASES.items():
+        assert _swiglu(rules, *size) == want, size
+    forward, dx, dw = zip(*swiglu.CASES.values())
+    assert _kinds(forward) == {"wide", "two", "deep"}
+    for found in (dx, dw):
+        assert _kinds(found) == {k + p for k in ("wide", "two", "deep") for p in ("", "/")}
+    for found in (forward, dx, dw):
+        for kind, n in (("wide", 256), ("two", 512)):
             assert any(name.startswith(kind) and items > n for name, items in found), kind
