@@ -93,3 +93,8 @@ def test_swiglu_sizes_take_the_tiles_that_they_name(rules):
     for found in (forward, dx, dw):
         for kind, n in (("wide", 256), ("two", 512)):
             assert any(name.startswith(kind) and items > n for name, items in found), kind
+
+
+def test_swiglu_sizes_on_two_streams_are_in_parts(rules):
+    for size in swiglu.STREAMS:
+        assert all("/" in name for name, _ in _swiglu(rules, *size)[1:]), size

@@ -85,3 +85,32 @@ def test_nan_stays_in_place(M, K, N):
     keep = torch.ones(N, dtype=torch.bool, device="cuda")
     keep[cols] = False
     assert torch.isnan(a[:, cols]).all() and torch.equal(a[:, keep], a0[:, keep])
+
+
+STREAMS = [(1000, 136, 1032), (1300, 136, 1032)]  # both products of the backward in parts
+
+
+def test_two_streams_with_parts():
+    """Backward passes on two streams at the same time, each with parts of both products in its workspace: bitwise what
+    each gives alone."""
+    announce(f"swiglu on two streams {STREAMS}")
+    wg, wu = (t.requires_grad_() for t in _inputs(*STREAMS[0])[1:])
+
+    def step(M, K, N):
+        x, da = _rand(M, K, seed=M, dtype=BF).requires_grad_(), _rand(M, N, seed=M + 1, dtype=BF)
+        torch.cuda.current_stream().synchronize()
+        out = []
+        for _ in range(10):
+            a = swiglu(x, wg, wu)
+            out.append((a.detach(), *torch.autograd.grad(a, (x, wg, wu), da)))
+        return out
+    want = [step(*size)[-1] for size in STREAMS]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in STREAMS], []
+    for s, size in zip(streams, STREAMS):
+        with torch.cuda.stream(s):
+            got.append(step(*size))
+    torch.cuda.synchronize()
+    for w, runs in zip(want, got):
+        for g in runs:
+            assert all(torch.equal(p, q) for p, q in zip(w, g))
