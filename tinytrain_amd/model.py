@@ -8,7 +8,8 @@ T <= 512, RoPE base 1e6, tied embeddings), pre-norm blocks (:128-139), final RMS
 a tied LM head with mean cross-entropy (:143-212), normal(0, 0.02) init (:183-186).
 Attention, RMSNorm and RoPE come from ``tinytrain_amd.attention``.  ``set_block_impl("hip")`` runs
 the rest of a block as HIP operators: the residual additions with the norms behind them
-(``add_rms_norm``) and the MLP's two projections with their activation (``swiglu``).  Chunked
+(``add_rms_norm``) and the MLP's two projections with their activation (``swiglu``); modules that are not
+as this file builds them (hooks, other classes in their place) are called as ever.  Chunked
 cross-entropy and activation checkpointing (reference training options) are not part of
 this benchmark model.
 """
@@ -33,6 +34,15 @@ def validate_block_impl(name: str) -> str:
     if name not in BLOCK_IMPLS:
         raise ValueError(f"block_impl must be one of {BLOCK_IMPLS}, got {name!r}")
     return name
+
+
+def _as_built(mod: nn.Module, kind: type) -> bool:
+    """Whether a call of mod is its class's forward and nothing else, so that an operator may compute it from its
+    weights: no class in kind's place (an adapter, a parametrization), no hooks on it or on all modules, no
+    forward of its own."""
+    return type(mod) is kind and not (
+        mod._forward_pre_hooks or mod._forward_hooks or mod._backward_pre_hooks or mod._backward_hooks
+        or "forward" in mod.__dict__ or nn.modules.module._has_any_global_hook())
 
 
 def _compute_dtype(x: torch.Tensor) -> torch.dtype:
@@ -87,11 +97,11 @@ class MLP(nn.Module):
         self.block_impl = "eager"
 
     def forward(self, x):
-        if self.block_impl == "hip":
+        gate, up = self.gate_proj, self.up_proj
+        if self.block_impl == "hip" and all(_as_built(m, nn.Linear) and m.bias is None for m in (gate, up)):
             dt = _compute_dtype(x)
-            a = swiglu(x.to(dt), self.gate_proj.weight.to(dt), self.up_proj.weight.to(dt))
-            return self.down_proj(a)
-        return self.down_proj(F.silu(self.gate_proj(x)) * self.up_proj(x))
+            return self.down_proj(swiglu(x.to(dt), gate.weight.to(dt), up.weight.to(dt)))
+        return self.down_proj(F.silu(gate(x)) * up(x))
 
 
 class Block(nn.Module):
@@ -143,7 +153,10 @@ class ModelForCausalLM(nn.Module):
 
     def set_block_impl(self, block_impl: str) -> None:
         """Select how the norms, residual additions and gate and up projections of every block run:
-        ``"eager"`` expressions, or ``"hip"`` operators (bf16 compute: under autocast, or bf16 weights)."""
+        ``"eager"`` expressions, or ``"hip"`` operators (bf16 compute: under autocast, or bf16 weights).  The
+        operators read the weights of ``Block``, ``RMSNorm`` and the two ``nn.Linear`` without calling these
+        modules; one that has hooks, a bias or another class (an adapter in its place) is called, as with
+        ``"eager"``, and the operators run around it."""
         self.block_impl = validate_block_impl(block_impl)
         for blk in self.layers:
             blk.mlp.block_impl = block_impl
@@ -153,16 +166,25 @@ class ModelForCausalLM(nn.Module):
         stream, x the newest branch's output that is not added to it yet."""
         dt, x = _compute_dtype(h), None
 
+        def added():
+            return h if x is None else h + x
+
         def norm(n):
             nonlocal h
+            if not _as_built(n, RMSNorm):
+                h = added()
+                return n(h)
             if x is None:
                 return rms_norm(h, n.weight, n.eps, dt)
             y, h = add_rms_norm(x, h, n.weight, n.eps, dt)
             return y
 
         for blk in self.layers:
-            x = blk.self_attn(norm(blk.input_layernorm), cos, sin)
-            x = blk.mlp(norm(blk.post_attention_layernorm))
+            if _as_built(blk, Block):
+                x = blk.self_attn(norm(blk.input_layernorm), cos, sin)
+                x = blk.mlp(norm(blk.post_attention_layernorm))
+            else:
+                h, x = blk(added(), cos, sin), None
         return norm(self.norm)
 
     def forward(self, input_ids, targets=None):
