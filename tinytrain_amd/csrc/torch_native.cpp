@@ -532,7 +532,9 @@ Grads3 norm_grads(AutogradContext *ctx, const variable_list &grads) {
   const auto x_type = (at::ScalarType)ctx->saved_data["x_type"].toInt();
   const auto y_type = (at::ScalarType)ctx->saved_data["y_type"].toInt();
   const Tensor dh = grads.size() > 1 ? grads[1] : Tensor();
-  const Tensor dy = grads[0].defined() ? grads[0] : at::zeros(h.sizes(), h.options().dtype(y_type));
+  const Tensor &dy = grads[0];
+  // h alone was read: the sum's gradient (zeros through the norm would make NaN rows' NaN)
+  if (!dy.defined()) return {dh, dh.defined() ? dh.to(x_type) : dh, Tensor()};
   if (plain_backward() && NormIn{h, {}, w}.takes(8) && grad_of(dy, h, h.sizes(), y_type) &&
       (!dh.defined() || grad_of(dh, h, h.sizes(), h.scalar_type())))
     return norm_bwd(dy, dh, h, w, eps, x_type);

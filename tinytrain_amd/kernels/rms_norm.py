@@ -144,14 +144,16 @@ def _(dy, dh, h, weight, eps, dtype):
 
 def _setup_context(ctx, inputs, output):
     x, residual, weight, eps, _ = inputs
+    ctx.set_materialize_grads(False)
     ctx.save_for_backward(x if residual is None else output[1], weight)
-    ctx.eps, ctx.x_dtype, ctx.added, ctx.y_dtype = eps, x.dtype, residual is not None, output[0].dtype
+    ctx.eps, ctx.x_dtype, ctx.added = eps, x.dtype, residual is not None
 
 
 def _backward_fn(ctx, dy, dh):
     h, weight = ctx.saved_tensors
-    if dy is None:
-        dy = torch.zeros_like(h, dtype=ctx.y_dtype)
+    if dy is None:  # h alone was read: the sum's gradient (zeros through the norm would make NaN rows' NaN)
+        dh = dh if ctx.added else None
+        return None if dh is None else dh.to(ctx.x_dtype), dh, None, None, None
     dr, dx, dw = rms_norm_bwd(dy, dh if ctx.added else None, h, weight, ctx.eps, ctx.x_dtype)
     return dr if ctx.x_dtype == h.dtype else dx, dr if ctx.added else None, dw, None, None
 
