@@ -478,6 +478,13 @@ Tensor workspace(const Tensor &like, long long bytes) {
   return bytes ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
 
+// A gradient as the library takes it: contiguous, and from a multiple of 16 bytes on, which a piece of a longer
+// tensor's gradient need not be.
+Tensor laid_out(const Tensor &g) {
+  const Tensor c = g.contiguous();
+  return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 ? c.clone() : c;
+}
+
 void *ptr(const Tensor &t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 const void *cptr(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 
@@ -514,7 +521,7 @@ Grads3 norm_bwd(const Tensor &gy, const Tensor &gh, const Tensor &h, const Tenso
                 at::ScalarType x_type) {
   RECORD_FUNCTION("tinytrain::rms_norm_bwd", c10::ArrayRef<const c10::IValue>());
   const c10::DeviceGuard on(h.device());
-  const Tensor dy = gy.contiguous(), dh = gh.defined() ? gh.contiguous() : gh, w = weight(w0);
+  const Tensor dy = laid_out(gy), dh = gh.defined() ? laid_out(gh) : gh, w = weight(w0);
   const int64_t C = h.size(-1), M = h.numel() / C;
   Tensor dr = same(h), dx, dw = f32(h, {C});
   if (x_type != h.scalar_type()) dx = at::empty(h.sizes(), h.options().dtype(x_type));
@@ -622,7 +629,7 @@ std::pair<Tensor, Tensor> swiglu_fwd(const SwigluIn &i, bool save) {
 Grads3 swiglu_bwd(const Tensor &da, const Tensor &saved, const SwigluIn &i, bool need_dx, bool need_dw) {
   RECORD_FUNCTION("tinytrain::swiglu_bwd", c10::ArrayRef<const c10::IValue>());
   const c10::DeviceGuard on(i.x.device());
-  const Tensor g = da.contiguous();
+  const Tensor g = laid_out(da);
   const int M = (int)i.M(), K = (int)i.K(), N = (int)i.N();
   Tensor dx, dwg, dwu;
   if (need_dx) dx = same(i.x);

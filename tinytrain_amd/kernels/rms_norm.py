@@ -15,7 +15,7 @@ x and residual [..., C], each bf16 or fp32, contiguous; weight [C].  h has resid
 formed in fp32 and rounded to it, and y is computed from that h in fp32 and rounded to ``dtype`` (x's if
 not given), so a residual stream in fp32 with branches in bf16, as under autocast, is one call.
 
-Gradients flow to x, residual and weight, through y and h.  They are those of the formula at the h that
+Gradients flow to x, residual and weight, through y and h; they may come in any strides.  They are those of the formula at the h that
 was returned; dx and dresidual are one tensor where their types are.  The weight's is summed in a fixed
 order.  (codes, scales) is the format of the quantised KV cache: 32 elements share a power of two, e4m3
 elements rounded once from a 64-bit y; a group with a NaN or an infinity reads as NaN.
@@ -73,6 +73,13 @@ def _check(x, residual, weight, unit):
     _check_device(x, weight, *(() if residual is None else (residual,)))
 
 
+def _laid_out(g: torch.Tensor) -> torch.Tensor:
+    """A gradient as the library takes it: contiguous, and from a multiple of 16 bytes on, which a piece of a
+    longer tensor's gradient need not be."""
+    g = g.contiguous()
+    return g.clone() if g.data_ptr() % 16 else g
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -122,7 +129,7 @@ def rms_norm_bwd(dy: torch.Tensor, dh: Optional[torch.Tensor], h: torch.Tensor, 
     dw = torch.zeros_like(weight, dtype=torch.float32) if h.numel() == 0 \
         else torch.empty(weight.shape, dtype=torch.float32, device=h.device)
     if h.numel():
-        dy, dh = dy.contiguous(), None if dh is None else dh.contiguous()
+        dy, dh = _laid_out(dy), None if dh is None else _laid_out(dh)
         w, M, C, lib = weight.float().contiguous(), h.numel() // h.shape[-1], h.shape[-1], _lib.load()
         nbytes = lib.ttfa_rms_norm_workspace_bytes(M, C)
         if nbytes < 0:

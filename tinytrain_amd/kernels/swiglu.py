@@ -21,7 +21,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from .rms_norm import BlockInputError, _check_device, _check_rows, _ptr, _stream
+from .rms_norm import BlockInputError, _check_device, _check_rows, _laid_out, _ptr, _stream
 
 __all__ = ["swiglu", "swiglu_fwd", "swiglu_bwd"]
 
@@ -88,7 +88,7 @@ def swiglu_bwd(da: torch.Tensor, saved: torch.Tensor, x: torch.Tensor, w_gate: t
     make = torch.empty_like if M else torch.zeros_like
     dwg, dwu = (make(w_gate), make(w_up)) if need_dw else (x.new_empty(0), x.new_empty(0))
     if M and (need_dx or need_dw):
-        da, saved, lib = da.contiguous(), saved.contiguous(), _lib.load()
+        da, saved, lib = _laid_out(da), _laid_out(saved), _lib.load()
         ws = _bytes(lib.ttfa_swiglu_workspace_bytes(M, K, N), x.device)
         with torch.cuda.device(x.device):
             _lib.check(lib.ttfa_swiglu_bwd(
