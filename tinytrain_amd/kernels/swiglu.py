@@ -21,7 +21,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from .rms_norm import BlockInputError, _check_device, _check_rows, _laid_out, _ptr, _stream
+from .rms_norm import BlockInputError, _check_device, _check_rows, _laid_out, _stream
 
 __all__ = ["swiglu", "swiglu_fwd", "swiglu_bwd"]
 
