@@ -15,8 +15,9 @@ A step of generation beside that cache:
     codes, scales, h = add_rms_norm_mx(x, h, norm_weight)
     q = linear_mx(codes, *w_q, scales)
 
-Supported: K a multiple of 32 and N of 8, both up to 2^20, any number of rows (none among them);
-contiguous tensors that start at a multiple of 16 bytes.
+Supported: K a multiple of 32 and N of 8, both up to 2^20; any number of rows M, none among them, for which y has
+fewer than 2^23 tiles of 128 x 128 (M < 2^30, and less from N of 256 on: 2^17 - 128 at 2^20) and, in
+``mx_quantize``, x no more than 2^34 - 2^13 elements; contiguous tensors that start at a multiple of 16 bytes.
 """
 
 from __future__ import annotations

@@ -20,8 +20,8 @@ was returned; dx and dresidual are one tensor where their types are.  The weight
 order.  (codes, scales) is the format of the quantised KV cache: 32 elements share a power of two, e4m3
 elements rounded once from a 64-bit y; a group with a NaN or an infinity reads as NaN.
 
-Supported: C a multiple of 8 (32 for ``add_rms_norm_mx``) up to 16384, any number of rows, none among
-them; tensors that start at a multiple of 16 bytes; eps in [0, 1).
+Supported: C a multiple of 8 (32 for ``add_rms_norm_mx``) up to 16384; any number of rows, none among
+them, up to 2^40 elements; tensors that start at a multiple of 16 bytes, gradients anywhere; eps in [0, 1).
 """
 
 from __future__ import annotations

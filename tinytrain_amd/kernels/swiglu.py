@@ -12,8 +12,9 @@ of the products that give dx and the weights' gradients.
 Where x or both weights need no gradient, theirs is not computed.  Sums have a fixed order: results are
 bitwise reproducible.
 
-Supported: K and N multiples of 8 up to 2^20, any number of rows (none among them); tensors that start
-at a multiple of 16 bytes.
+Supported: K and N multiples of 8 up to 2^20; any number of rows M, none among them, for which each of a, dx and
+the two weights' gradients together has fewer than 2^23 tiles of 128 x 128 (M < 2^30, and less from N or K of
+256 on: 2^17 - 128 at 2^20); tensors that start at a multiple of 16 bytes, gradients anywhere.
 """
 
 from __future__ import annotations
