@@ -188,7 +188,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void linear_mx_rows_kernel(
 // registers for a stage.  With x in bf16 it is a quarter of the stage's k's, eight of each group, for which the
 // wave's columns become bf16.  What a last stage has past K loads as zeros; rows of scales that are no whole dwords
 // are laid out anew first (pad_scales_kernel).
-// 4096 x 4096 x 12288 in 4 bits: x in 8 bits 169 us (2440 TFLOP/s), x in bf16 336 (1230); 128 rows: 25 and 29.
+// 4096 x 4096 x 12288 in 4 bits: x in 8 bits 166 to 173 us (2480 to 2380 TFLOP/s), x in bf16 332 (1240); 128 rows: 25
+// and 29.  W in 8 bits: 194 and 368.
 // With W written out in bf16 first and tiles of that, x in bf16 took 346 and 52, and 2 N K bytes of workspace.
 struct MxArgs {
   const uint8_t *x, *x_scales, *codes, *scales;

@@ -21,7 +21,8 @@ constexpr double kMostPartFloats = 1 << 26;  // 256 MB, what the last-level cach
 
 // The cut that is estimated to take least time, in microseconds on 256 CUs: a stage of 64 k's of a wide
 // tile takes 1.5, of a narrow one 0.6 alone on its CU and 0.97 beside another; 3 stages more for a tile's
-// start and end; parts go out and in at 4 TB/s, with a launch of 4 us.  (Whole rounds of narrow tiles take 0.9 to
+// start and end; parts go out and in at 4 TB/s, with a launch of 4 us.  What a forward keeps for its backward is the
+// same for every cut and not counted.  (Whole rounds of narrow tiles take 0.9 to
 // 1.06 a stage; 0.97 decides the near draws as they were measured: forward 2048 x 2048 x 6144 wide 110, narrow 101;
 // 4096 x 1024 x 2816: 58, 52; dx of 4096 x 2048 x 6144: wide in two parts 232 with the kernel before it, narrow 262.)
 inline Cut cut_of(int64_t M, int64_t N, int64_t K, int segs, int z, bool dual) {

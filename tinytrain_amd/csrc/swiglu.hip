@@ -10,7 +10,7 @@
 // significant bits, an error of 2^-13 against the 2^-9 that every gradient has from its own rounding and
 // from that of dg and du, as bf16 operands of the last two products (in bf16 they would add as much
 // again).  That is 5 bytes an element; to form them again instead of reading them was 713 us at
-// 16384 x 2048 x 6144, against 190 to 225 of the kernel that reads them (swiglu_grad_kernel).
+// 16384 x 2048 x 6144, against 227 of the kernel that reads them (swiglu_grad_kernel).
 #include "fa_kernels.h"
 #include "gemm.h"
 
